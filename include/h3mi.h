@@ -216,6 +216,95 @@ int h3mi_rms_rope_split_half_bf16(uint16_t* q, uint16_t* k, const uint16_t* tab,
                                   int64_t rot, float eps, int rsqrt_mode, float* rstd_out,
                                   void* stream);
 
+/* ------------------------------------------------------------------ 8-bit key/value cache
+ * No counterpart in the reference, whose attention is the host program's own
+ * (comfyui_nodes/minimax-h3-sp/minimax_sp/sp_forward.py:276-318): keys and values
+ * that outlive a call, held in 8 bits with a scale for each block of
+ * H3MI_KV_BLOCK tokens and head, and the attention that reads them.
+ *
+ * A cache is a pool of pages, one block of tokens a page.  A sequence's block b is
+ * page tables[b]; pages of different sequences need not be distinct for reading.
+ * A page index outside [0, pages) is a block that is not there: writes to it are
+ * dropped, reads of it give zeros, attention and selection pass over it. */
+#define H3MI_KV_BLOCK 64   /* tokens of a block */
+#define H3MI_KV_TILE 128   /* query rows that share a selection of blocks */
+
+typedef struct h3mi_kv_cache {
+    int8_t* k;       /* [pages, heads, 64, dim] */
+    int8_t* v;       /* [pages, heads, dim, 64]: each block's values transposed */
+    float* k_scale;  /* [pages, heads] */
+    float* v_scale;  /* [pages, heads] */
+    int16_t* k_sum;  /* [pages, heads, dim]: sum of the block's 8-bit keys */
+    int64_t pages, heads, dim;
+} h3mi_kv_cache;
+
+/* The sequences of a call.  A call's rows of sequence i are its last counts[i]
+ * tokens: row r is token lens[i] - counts[i] + r.  counts is taken as at most the
+ * call's rows, both as at least 0.  Tokens before 0 and from 64 * blocks on are not
+ * there: not written, not read, seen by no query. */
+typedef struct h3mi_kv_seqs {
+    const int32_t* tables;  /* [n, blocks] pages */
+    const int32_t* lens;    /* [n] tokens of each sequence, the call's own among them */
+    const int32_t* counts;  /* [n] rows of each sequence that are its own (NULL: all) */
+    int64_t n, blocks;
+} h3mi_kv_seqs;
+
+/* Quantizes k and v (bf16 [n, rows, heads, dim], heads contiguous, strides in
+ * elements: ld_* from token to token, bs_* from sequence to sequence, multiples of
+ * 8) into the cache.  Per block and head, with a = fl(max |x| * fl(1 / 127)) of the
+ * tokens written now and s the scale the block had:
+ *   first token of the block written now, or s = 0:  s' = a
+ *   s not finite:                                    s' = s
+ *   else r = a / s:  r <= 1: s' = s;  r <= 256: s' = s 2^k, the least k with
+ *   2^k >= r;  else s' = a
+ *   q = clamp(rne(x / s'), -127, 127), and the tokens the block held before become
+ *   rne(q 2^-k) (0 where s' starts anew); 0 everywhere where s' is 0 or not finite.
+ * A value's error is at most one step s' (half of one if its scale never grew).
+ * A block with a NaN or an infinity reads back as NaN.  Tokens of a written block
+ * behind the sequence's end become 0; other blocks are left as they were.  k_sum is
+ * renewed.  The pages that a call writes have to be distinct.  dim 64, 128 or 256. */
+int h3mi_kv_write_i8(const uint16_t* k, const uint16_t* v, int64_t rows, int64_t ld_k, int64_t bs_k,
+                     int64_t ld_v, int64_t bs_v, const h3mi_kv_cache* cache, const h3mi_kv_seqs* seqs,
+                     void* stream);
+
+/* k, v (bf16 [n, length, heads, dim], contiguous) <- bf16(q s) of the tokens
+ * starts[i] .. starts[i] + length - 1 of each sequence (starts NULL: 0 ..); zeros
+ * where a sequence has no such token.  counts is not read. */
+int h3mi_kv_read_bf16(uint16_t* k, uint16_t* v, const int32_t* starts, int64_t length,
+                      const h3mi_kv_cache* cache, const h3mi_kv_seqs* seqs, void* stream);
+
+/* blocks (int32 [n, ceil(rows / 128), kv heads, top]) <- the blocks that each tile
+ * of 128 query rows selects, ascending, -1 behind the last.  q bf16 [n, rows, heads,
+ * dim] as k above; heads a multiple of the cache's.  Per tile and kv head:
+ *   P = sum of the query rows of the tile and of the heads that share the kv head
+ *   (64-bit), qi = rne(1023 P / max |P|)  (0 where max |P| is 0 or not finite),
+ *   score_b = f32(sum_d qi[d] k_sum_b[d]) * (k_scale_b / tokens of block b),
+ * the mean key's product with the mean query but for a factor that is the tile's.
+ * It is a whole number's rounding, so no order of summing changes a selection.
+ * causal: the blocks with the tile's own tokens come first, later ones are not
+ * seen.  Equal scores: the lowest block first; NaN scores come last.  A tile with no
+ * rows of its own selects nothing.  top in [1, 32768], seqs->blocks <= 32768. */
+int h3mi_kv_select(const uint16_t* q, int64_t rows, int64_t heads, int64_t ld_q, int64_t bs_q,
+                   const h3mi_kv_cache* cache, const h3mi_kv_seqs* seqs, int64_t top, int causal,
+                   int32_t* blocks, void* stream);
+
+/* out (bf16 [n, rows, heads, dim], contiguous) <- softmax(scale q k^T) v over the
+ * tokens of each sequence; query head h reads kv head h / (heads / kv heads).
+ * causal: row r sees tokens up to its own.  blocks (NULL: all) as h3mi_kv_select
+ * gives them: a row sees the tokens of its tile's blocks alone; entries outside the
+ * sequence are passed over, and a tile's entries have to be distinct.  Rows that
+ * see no token, and rows behind counts, are 0.  Sums and statistics are fp32, the
+ * products' operands bf16 (8-bit keys and values are exact in it, probabilities
+ * are rounded to it).
+ * workspace: h3mi_kv_attention_workspace bytes of device memory, 16-byte aligned
+ * (NULL where that is 0), for this call alone until it has run. */
+int64_t h3mi_kv_attention_workspace(int64_t n, int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim,
+                                    int64_t blocks, int64_t top);
+int h3mi_kv_attention_bf16(const uint16_t* q, int64_t rows, int64_t heads, int64_t ld_q, int64_t bs_q,
+                           const h3mi_kv_cache* cache, const h3mi_kv_seqs* seqs, float scale, int causal,
+                           const int32_t* blocks, int64_t top, uint16_t* out, void* workspace,
+                           int64_t workspace_bytes, void* stream);
+
 /* (numx, vec, warp) of an order; returns H3MI_EINVAL for an unknown order. */
 int h3mi_norm_order_info(int order, int* numx, int* vec, int* warp);
 

@@ -1,0 +1,239 @@
+// Selecting a sequence's blocks of keys for tiles of queries.
+//
+// A tile's score of a block is a product of whole numbers (the pooled queries as 11-bit
+// integers, the sum of the block's 8-bit keys as 16-bit ones), exact in int32: |qi| <=
+// 1023, |k_sum| <= 64 * 127 and dim <= 256 keep it below 2^31.  The pooled queries are
+// summed in 64 bits, where bf16 values within a factor of 2^30 of each other add
+// exactly.  So neither the order of a sum nor the split of the work changes a selection.
+//
+// A workgroup takes one tile of one kv head: it pools the queries, scores every block
+// (dim / 8 lanes a block, 16 bytes of k_sum each, v_dot2_i32_i16), keeps the scores as
+// ordered 32-bit keys in LDS, finds the last selected key by four passes over 8 bits of
+// it, and writes the selected blocks in order.
+#include "kv.h"
+
+namespace h3mi {
+namespace {
+
+constexpr int kMaxSelect = 32768;  // blocks: their keys fill 128 KiB of LDS
+constexpr int kSelThreads = 512;
+constexpr int kSelWaves = kSelThreads / 64;
+
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+
+// Keys ordered as scores: 0 is kept for blocks that are not there.  NaN becomes the
+// lowest key of a block, and -0 (a negative product times a zero scale) is 0.
+__device__ __forceinline__ uint32_t key_of(float s) {
+    if (__builtin_isnan(s)) return 1u;
+    const uint32_t b = __float_as_uint(s + 0.0f);
+    const uint32_t k = (b & 0x80000000u) ? ~b : b | 0x80000000u;
+    return k < 2u ? 2u : k;
+}
+
+template <int D>
+__global__ __launch_bounds__(kSelThreads) void kv_select_kernel(const uint16_t* __restrict__ q, int64_t ld, int64_t bs, KvCache c,
+                                                                KvSeqs s, int rows, int heads, int top, int causal, int tiles,
+                                                                int32_t* __restrict__ out) {
+    constexpr int CH = D / 8;
+    constexpr int GROUPS = kSelThreads / CH;  // row groups while pooling, blocks at once while scoring
+    extern __shared__ uint32_t keys[];
+    __shared__ double part[kSelWaves][D];
+    __shared__ double pool[D];
+    __shared__ __align__(16) int16_t qi[D];
+    __shared__ uint32_t hist[256];
+    __shared__ uint32_t pick[2];
+    __shared__ int wsum[2][kSelWaves];
+    __shared__ double wmax[kSelWaves];
+
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const int h = blockIdx.x % c.heads;
+    const int item = blockIdx.x / c.heads;
+    const int i = item / tiles, tile = item % tiles;
+    int32_t* const to = out + (static_cast<int64_t>(item) * c.heads + h) * top;
+    const int len = s.len(i), count = s.count(i, rows), group = heads / c.heads;
+    const int r0 = tile * kKvTile, live = count - r0 < kKvTile ? count - r0 : kKvTile;
+    // the tile's own tokens, and the blocks it sees
+    const int first = s.end(i) - count + r0, last = first + live - 1;
+    int seen = (len + kKvBlock - 1) / kKvBlock;
+    if (causal && last < len) seen = last < 0 ? 0 : block_of(last) + 1;
+    if (live <= 0) seen = 0;
+    if (seen == 0) {
+        for (int j = t; j < top; j += kSelThreads) to[j] = -1;
+        return;
+    }
+
+    const int ch = t % CH, grp = t / CH;
+    {
+        double p[8] = {};
+        for (int x = grp; x < live * group; x += GROUPS) {
+            const int64_t r = r0 + x / group;
+            const int hq = h * group + x % group;
+            const uint4 w = *reinterpret_cast<const uint4*>(q + i * bs + r * ld + static_cast<int64_t>(hq) * D + ch * 8);
+            const uint32_t a[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                p[2 * j] += bf16_lo(a[j]);
+                p[2 * j + 1] += bf16_hi(a[j]);
+            }
+        }
+        // the row groups of a wave, then the waves through LDS
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+#pragma unroll
+            for (int m = 32; m >= CH; m >>= 1) p[j] += __shfl_xor(p[j], m);
+            if (lane < CH) part[wave][ch * 8 + j] = p[j];
+        }
+    }
+    __syncthreads();
+    if (t < D) {
+        double p = 0.0;
+#pragma unroll
+        for (int w = 0; w < kSelWaves; ++w) p += part[w][t];
+        pool[t] = p;
+    }
+    __syncthreads();
+    double m = t < D ? fabs(pool[t]) : 0.0;
+    bool bad = !(m < __builtin_inf());  // a NaN or an infinity
+#pragma unroll
+    for (int x = 32; x; x >>= 1) m = fmax(m, __shfl_xor(m, x));
+    bad = __any(bad);
+    if (lane == 0) wmax[wave] = bad ? __builtin_inf() : m;
+    __syncthreads();
+    m = 0.0;
+#pragma unroll
+    for (int w = 0; w < kSelWaves; ++w) m = fmax(m, wmax[w]);
+    if (t < D) qi[t] = m > 0.0 && m < __builtin_inf() ? static_cast<int16_t>(rint(pool[t] * 1023.0 / m)) : int16_t{0};
+    __syncthreads();
+
+    const uint4 qw = *reinterpret_cast<const uint4*>(qi + ch * 8);
+    const int own = first < 0 ? 0 : block_of(first);
+    const int blocks_up = (seen + GROUPS - 1) / GROUPS * GROUPS;  // whole groups, so that every lane takes part
+    for (int b = grp; b < blocks_up; b += GROUPS) {
+        const int page = b < seen ? s.page(i, b, c.pages) : -1;
+        int dot = 0;
+        const int64_t at = static_cast<int64_t>(page < 0 ? 0 : page) * c.heads + h;
+        if (page >= 0) {
+            const uint4 k = *reinterpret_cast<const uint4*>(c.ksum + at * D + ch * 8);
+            dot = __builtin_amdgcn_sdot2(__builtin_bit_cast(s16x2, qw.x), __builtin_bit_cast(s16x2, k.x), dot, false);
+            dot = __builtin_amdgcn_sdot2(__builtin_bit_cast(s16x2, qw.y), __builtin_bit_cast(s16x2, k.y), dot, false);
+            dot = __builtin_amdgcn_sdot2(__builtin_bit_cast(s16x2, qw.z), __builtin_bit_cast(s16x2, k.z), dot, false);
+            dot = __builtin_amdgcn_sdot2(__builtin_bit_cast(s16x2, qw.w), __builtin_bit_cast(s16x2, k.w), dot, false);
+        }
+#pragma unroll
+        for (int x = CH / 2; x; x >>= 1) dot += __shfl_xor(dot, x);
+        if (ch == 0 && b < seen) {
+            uint32_t key = 0;
+            if (page >= 0) {
+                const int held = len - b * kKvBlock < kKvBlock ? len - b * kKvBlock : kKvBlock;
+                key = causal && b >= own ? 0xFFFFFFFFu : key_of(static_cast<float>(dot) * (c.ks[at] / static_cast<float>(held)));
+            }
+            keys[b] = key;
+        }
+    }
+    __syncthreads();
+
+    // The least key taken (thr), and how many of the blocks that have it (need).
+    uint32_t thr = 1u;
+    int need = top;
+    if (seen > top) {
+        uint32_t prefix = 0, have = 0;
+        int want = top;
+        for (int shift = 24; shift >= 0; shift -= 8) {
+            for (int x = t; x < 256; x += kSelThreads) hist[x] = 0;
+            __syncthreads();
+            for (int b = t; b < seen; b += kSelThreads)
+                if (shift == 24 || (keys[b] >> (shift + 8)) == prefix) atomicAdd(&hist[(keys[b] >> shift) & 255u], 1u);
+            __syncthreads();
+            if (wave == 0) {
+                // suffix sums of four bins a lane: the highest bin at which `want` blocks are reached
+                uint32_t n[4], sum = 0;
+#pragma unroll
+                for (int j = 3; j >= 0; --j) n[j] = hist[255 - (4 * lane + 3 - j)];
+                // lane 0 holds the highest four bins, n[3] the highest of them
+                sum = n[0] + n[1] + n[2] + n[3];
+                uint32_t before = sum;
+#pragma unroll
+                for (int x = 1; x < 64; x <<= 1) {
+                    const uint32_t o = __shfl_up(before, x);
+                    if (lane >= x) before += o;
+                }
+                before -= sum;  // blocks in higher bins than this lane's
+                const uint32_t w = static_cast<uint32_t>(want);
+                if (before < w && before + sum >= w) {
+                    uint32_t run = before;
+                    int bin = 255 - 4 * lane;
+#pragma unroll
+                    for (int j = 3; j >= 0; --j, --bin) {
+                        if (run + n[j] >= w) break;
+                        run += n[j];
+                    }
+                    pick[0] = static_cast<uint32_t>(bin);
+                    pick[1] = run;
+                }
+            }
+            __syncthreads();
+            prefix = (prefix << 8) | pick[0];
+            have = pick[1];
+            want -= static_cast<int>(have);
+            __syncthreads();
+        }
+        thr = prefix;
+        need = want;
+        if (thr == 0) thr = 1u, need = top;  // fewer blocks are there than wanted: all of them
+    }
+
+    // In order: blocks above thr, and the first `need` at it.
+    int done = 0, ties = 0;
+    for (int b0 = 0; b0 < seen; b0 += kSelThreads) {
+        const int b = b0 + t;
+        const uint32_t key = b < seen ? keys[b] : 0u;
+        const bool over = key > thr, tie = key == thr;
+        const uint64_t mo = __ballot(over), mt = __ballot(tie), below = (uint64_t{1} << lane) - 1;
+        if (lane == 0) wsum[0][wave] = __popcll(mo), wsum[1][wave] = __popcll(mt);
+        __syncthreads();
+        int o = __popcll(mo & below), e = ties + __popcll(mt & below), all_o = 0, all_e = 0;
+#pragma unroll
+        for (int w = 0; w < kSelWaves; ++w) {
+            if (w < wave) o += wsum[0][w], e += wsum[1][w];
+            all_o += wsum[0][w];
+            all_e += wsum[1][w];
+        }
+        // blocks taken before this one: those above thr, and the ties before it that were taken
+        const int t0 = ties < need ? ties : need, te = e < need ? e : need;
+        if (over || (tie && e < need)) to[done + o + te - t0] = b;
+        const int t1 = ties + all_e < need ? ties + all_e : need;
+        done += all_o + t1 - t0;
+        ties += all_e;
+        __syncthreads();
+    }
+    for (int j = done + t; j < top; j += kSelThreads) to[j] = -1;
+}
+
+}  // namespace
+}  // namespace h3mi
+
+using namespace h3mi;
+
+extern "C" int h3mi_kv_select(const uint16_t* q, int64_t rows, int64_t heads, int64_t ld_q, int64_t bs_q,
+                              const h3mi_kv_cache* cache, const h3mi_kv_seqs* seqs, int64_t top, int causal, int32_t* blocks,
+                              void* stream) {
+    if (int e = kv_check("kv_select", cache, seqs)) return e;
+    if (heads <= 0 || heads > 65536 || heads % cache->heads)
+        return fail(H3MI_EINVAL, "kv_select: heads=%lld must be a multiple of the cache's %lld", (long long)heads, (long long)cache->heads);
+    if (int e = kv_check_rows("kv_select", "q", q, rows, heads, cache->dim, seqs->n, ld_q, bs_q)) return e;
+    if (top < 1 || top > kMaxSelect) return fail(H3MI_EINVAL, "kv_select: top=%lld must be in [1, %d]", (long long)top, kMaxSelect);
+    if (seqs->blocks > kMaxSelect)
+        return fail(H3MI_EINVAL, "kv_select: %lld blocks a sequence, at most %d", (long long)seqs->blocks, kMaxSelect);
+    if (seqs->n == 0 || rows == 0) return ok();
+    if (!blocks) return fail(H3MI_EINVAL, "kv_select: null blocks");
+    if (!aligned(blocks, 4)) return fail(H3MI_EALIGN, "kv_select: blocks must be 4-byte aligned");
+    const int64_t tiles = (rows + kKvTile - 1) / kKvTile;
+    int64_t groups;
+    if (!launchable(seqs->n, tiles, cache->heads, kSelThreads, &groups)) return fail(H3MI_EINVAL, "kv_select: too many rows for one call");
+    const int D = static_cast<int>(cache->dim);
+    const auto fn = D == 64 ? kv_select_kernel<64> : D == 128 ? kv_select_kernel<128> : kv_select_kernel<256>;
+    hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(groups)), dim3(kSelThreads), static_cast<unsigned>(seqs->blocks * 4),
+                       as_stream(stream), q, ld_q, bs_q, kv_cache(*cache), kv_seqs(*seqs), static_cast<int>(rows),
+                       static_cast<int>(heads), static_cast<int>(top), causal, static_cast<int>(tiles), blocks);
+    return check_launch("kv_select");
+}

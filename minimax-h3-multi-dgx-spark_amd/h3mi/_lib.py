@@ -28,6 +28,20 @@ _I = ctypes.c_int64
 _F = ctypes.c_float
 _C = ctypes.c_int
 
+
+
+class KvCacheC(ctypes.Structure):
+    """h3mi_kv_cache"""
+    _fields_ = [("k", _P), ("v", _P), ("k_scale", _P), ("v_scale", _P), ("k_sum", _P), ("pages", _I), ("heads", _I), ("dim", _I)]
+
+
+class KvSeqsC(ctypes.Structure):
+    """h3mi_kv_seqs"""
+    _fields_ = [("tables", _P), ("lens", _P), ("counts", _P), ("n", _I), ("blocks", _I)]
+
+
+_KC, _KS = ctypes.POINTER(KvCacheC), ctypes.POINTER(KvSeqsC)
+
 # name -> argtypes (restype int unless listed in _RESTYPE)
 SIGNATURES = {
     "h3mi_abi_version": [],
@@ -48,12 +62,17 @@ SIGNATURES = {
     "h3mi_gate_norm_mod_bf16_ex": [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _F, _C, _C, _P, _P, _P],
     "h3mi_norm_mod_quant_i8": [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _F, _P],
     "h3mi_gate_norm_mod_quant_i8": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _F, _P],
+    "h3mi_kv_write_i8": [_P, _P, _I, _I, _I, _I, _I, _KC, _KS, _P],
+    "h3mi_kv_read_bf16": [_P, _P, _P, _I, _KC, _KS, _P],
+    "h3mi_kv_select": [_P, _I, _I, _I, _I, _KC, _KS, _I, _C, _P, _P],
+    "h3mi_kv_attention_workspace": [_I, _I, _I, _I, _I, _I, _I],
+    "h3mi_kv_attention_bf16": [_P, _I, _I, _I, _I, _KC, _KS, _F, _C, _P, _I, _P, _P, _I, _P],
     "h3mi_norm_order_info": [_C, ctypes.POINTER(_C), ctypes.POINTER(_C), ctypes.POINTER(_C)],
     "h3mi_debug_rsqrt_f32": [_P, _P, _I, _C, _P],
     "h3mi_debug_bf16_rne": [_P, _P, _I, _P],
     "h3mi_debug_buffer_lds_load": [_P, _I, _P, ctypes.c_int32, ctypes.c_int32, _P, _P],
 }
-_RESTYPE = {"h3mi_last_error": ctypes.c_char_p}
+_RESTYPE = {"h3mi_last_error": ctypes.c_char_p, "h3mi_kv_attention_workspace": _I}
 
 
 class H3miError(RuntimeError):

@@ -1,0 +1,528 @@
+"""The 8-bit key/value cache against plain forms on the CPU: written bytes are pinned, reading is exact, selections are
+equal, attention is within the bounds that kv_ref.bound derives."""
+import numpy as np
+import pytest
+import torch
+
+import kv_ref as R
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def _h():
+    import h3mi
+    return h3mi
+
+
+def _bf(a):
+    """float32 array of bf16 values -> bf16 GPU tensor"""
+    return torch.from_numpy(np.ascontiguousarray(a, np.float32)).to(torch.bfloat16).to(DEV)
+
+
+def _np(t):
+    return t.detach().float().cpu().numpy()
+
+
+def _round(a):
+    return torch.from_numpy(np.asarray(a, np.float32)).to(torch.bfloat16).float().numpy()
+
+
+def _i32(a):
+    return torch.tensor(np.asarray(a), dtype=torch.int32, device=DEV)
+
+
+def _tables(rng, n, blocks, spare=2):
+    return rng.permutation(n * blocks + spare)[:n * blocks].reshape(n, blocks).astype(np.int32)
+
+
+# ------------------------------------------------------------------ writing and reading
+
+
+@pytest.mark.parametrize("heads,dim", [(3, 64), (2, 128), (5, 256)])
+@pytest.mark.parametrize("steps", [
+    [(100, 100)], [(64, 64), (1, 65), (1, 66), (70, 136)], [(1, 1), (62, 63), (1, 64), (1, 65)], [(130, 130), (3, 100), (200, 256)],
+])
+def test_write_is_pinned(heads, dim, steps):
+    """A chain of writes (rows, length after it), every row in use; the tokens grow so that scales do."""
+    h = _h()
+    rng = np.random.default_rng(len(steps) * dim)
+    blocks = 4
+    ref = R.Cache(2 * blocks + 2, heads, dim, seed=1)
+    cache, tables = ref.to(), _tables(rng, 2, blocks)
+    for x, (rows, end) in enumerate(steps):
+        k = _round(rng.standard_normal((2, rows, heads, dim)) * 3.0 ** x)
+        v = _round(rng.standard_normal((2, rows, heads, dim)) * 1.5 ** x)
+        lens = np.array([end, max(end - 5, 0)])
+        counts = np.array([rows, max(rows - 5, 0)])
+        R.write(ref, k, v, tables, lens, counts)
+        assert h.kv_write_(cache, _bf(k), _bf(v), _i32(tables), _i32(lens), counts=_i32(counts)) is cache
+        assert ref.same(cache) == []
+
+
+def test_write_of_views_and_without_counts():
+    h = _h()
+    rng = np.random.default_rng(5)
+    heads, dim, rows = 3, 128, 77
+    qkv = _round(rng.standard_normal((2, rows, 3, heads, dim)))
+    ref = R.Cache(6, heads, dim, seed=2)
+    cache, tables, lens = ref.to(), _tables(rng, 2, 2), np.array([77, 100])
+    t = _bf(qkv)
+    h.kv_write_(cache, t[:, :, 1], t[:, :, 2], _i32(tables), _i32(lens))
+    R.write(ref, qkv[:, :, 1], qkv[:, :, 2], tables, lens, [rows, rows])
+    assert ref.same(cache) == []
+
+
+@pytest.mark.parametrize("first,second", [
+    (1.0, 1.0), (1.0, 0.25), (1.0, 2.0), (1.0, 2.0078125), (1.0, 255.0), (1.0, 256.0), (1.0, 258.0), (1.0, 1e30), (0.0, 3.0),
+    (3.0, 0.0), (1e-38, 1e-38), (1e-38, 3e-38), (9.2e-41, 1.0), (1e-40, 3e-40), (3e38, 3e38), (1e-3, 3e38),
+    (1.0, np.inf), (np.inf, 1.0), (np.nan, 1.0), (1.0, np.nan), (1.0, -np.inf),
+])
+def test_scale_growth(first, second):
+    """The second write of a block against its first, at the edges of every rule."""
+    h = _h()
+    rng = np.random.default_rng(9)
+    heads, dim = 2, 64
+    ref = R.Cache(2, heads, dim, seed=3)
+    cache, tables = ref.to(), np.array([[1]], np.int32)
+    for end, rows, top in ((20, 20, first), (21, 1, second), (40, 19, 1.0 if np.isfinite(first) else first)):
+        x = rng.uniform(-1, 1, (2, 1, rows, heads, dim))
+        x[:, :, 0, :, 3] = 1.0  # the largest is `top` itself
+        with np.errstate(invalid="ignore"):
+            x = _round(x * top)
+        R.write(ref, x[0], x[1], tables, [end], [rows])
+        h.kv_write_(cache, _bf(x[0]), _bf(x[1]), _i32(tables), _i32([end]))
+        assert ref.same(cache) == [], (end, first, second)
+
+
+def test_write_drops_what_has_no_place():
+    """Lengths past the table, rows before token 0, negative counts and lengths, pages outside the pool, no rows."""
+    h = _h()
+    rng = np.random.default_rng(11)
+    heads, dim, rows = 2, 64, 90
+    ref = R.Cache(9, heads, dim, seed=4)
+    cache = ref.to()
+    tables = np.array([[0, 1], [2, 9], [3, 4], [-1, 5], [6, 7], [8, 2147483647]], np.int32)
+    lens, counts = np.array([140, 128, 30, 128, -5, 100]), np.array([90, 90, 90, 200, 20, -3])
+    k, v = (_round(rng.standard_normal((6, rows, heads, dim))) for _ in range(2))
+    R.write(ref, k, v, tables, lens, counts)
+    h.kv_write_(cache, _bf(k), _bf(v), _i32(tables), _i32(lens), counts=_i32(counts))
+    assert ref.same(cache) == []
+    h.kv_write_(cache, _bf(k[:, :0]), _bf(v[:, :0]), _i32(tables), _i32(lens))
+    h.kv_write_(cache, _bf(k[:0]), _bf(v[:0]), _i32(tables[:0]), _i32(lens[:0]))
+    assert ref.same(cache) == []
+
+
+@pytest.mark.parametrize("heads,dim", [(3, 64), (2, 128), (5, 256)])
+@pytest.mark.parametrize("length,starts", [(1, None), (64, None), (200, None), (65, [3, 64, 127]), (130, [-10, 60, 1000]),
+                                           (10, [-100, 2147483640, -2147483648])])
+def test_read(heads, dim, length, starts):
+    h = _h()
+    rng = np.random.default_rng(13)
+    ref = R.Cache(11, heads, dim, seed=5)
+    tables, lens = _tables(rng, 3, 3), np.array([192, 70, 0])
+    tables[0, 1] = 11  # a page outside the pool
+    k, v = h.kv_read(ref.to(), _i32(tables), _i32(lens), length, starts=None if starts is None else _i32(starts))
+    for i in range(3):
+        a, b, _ = R.tokens(ref, tables[i], int(lens[i]))
+        first = 0 if starts is None else starts[i]
+        for got, want in ((k, a), (v, b)):
+            full = np.zeros((length, heads, dim))
+            for r in range(length):
+                if 0 <= first + r < lens[i]:
+                    full[r] = want[first + r]
+            # one rounding of an fp32 product of an 8-bit value and a scale
+            want_bits = torch.from_numpy(full).float().to(torch.bfloat16)
+            assert torch.equal(got[i].cpu(), want_bits)
+
+
+def test_round_trip_error():
+    """Tokens written one by one: every value within a step of its block's last scale, the newest within half of one."""
+    h = _h()
+    rng = np.random.default_rng(17)
+    heads, dim, n = 2, 128, 150
+    x = _round(rng.standard_normal((2, 1, n, heads, dim)) * np.geomspace(0.01, 30, n)[None, None, :, None, None])
+    cache, tables = h.kv_cache(4, heads, dim), np.array([[2, 0, 3]], np.int32)
+    for t in range(n):
+        h.kv_write_(cache, _bf(x[0][:, t:t + 1]), _bf(x[1][:, t:t + 1]), _i32(tables), _i32([t + 1]))
+    step = np.repeat(_np(cache.k_scale)[tables[0]], 64, 0)[:n, :, None]
+    got = (_np(cache.k)[tables[0]].swapaxes(1, 2).reshape(-1, heads, dim)[:n] * step)
+    off = np.abs(got - x[0][0]) / step
+    assert off.max() <= 1 + 1e-5 and off[-1].max() <= 0.5 + 1e-5
+
+
+# ------------------------------------------------------------------ attention
+
+
+def _case(rng, heads, kv, dim, n, rows, blocks, seed):
+    ref = R.Cache(n * blocks + 2, kv, dim, seed=seed)
+    tables = _tables(rng, n, blocks)
+    q = _round(rng.standard_normal((n, rows, heads, dim)))
+    return ref, tables, q
+
+
+def _check(ref, q, tables, lens, counts, causal, scale=None, blocks=None, view=None):
+    h = _h()
+    out = h.kv_attention(_bf(q) if view is None else view, ref.to(), _i32(tables), _i32(lens), causal=causal,
+                         counts=None if counts is None else _i32(counts), scale=scale, blocks=None if blocks is None else _i32(blocks))
+    if counts is None:
+        counts = [q.shape[1]] * q.shape[0]
+    want, mag, top = R.attention(ref, q.astype(np.float64), tables, lens, counts, causal, scale, blocks)
+    got = out.double().cpu().numpy()
+    assert got.shape == want.shape and np.isfinite(got).all()
+    off = np.abs(got - want) / R.bound(want, mag, top, q.shape[3])
+    assert off.max(initial=0.0) <= 1, (off.max(), np.unravel_index(off.argmax(), off.shape))
+    assert (got[mag == 0] == 0).all()
+    return out
+
+
+HEADS = [(3, 3, 64), (2, 2, 128), (3, 3, 256), (10, 2, 128), (8, 1, 64), (6, 2, 256), (20, 1, 128)]
+
+
+@pytest.mark.parametrize("heads,kv,dim", HEADS)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("rows,lens,counts", [
+    (1, [1, 64, 65], None), (1, [700, 0, 333], None), (3, [3, 200, 130], [3, 2, 0]), (16, [16, 500, 61], [16, 15, 9]),
+    (17, [400, 17, 40], None), (64, [64, 129, 700], None), (65, [65, 90, 640], [65, 1, 33]), (130, [130, 2, 600], [130, 2, 129]),
+    (300, [300, 700, 299], [300, 280, 299]),
+])
+def test_attention(heads, kv, dim, causal, rows, lens, counts):
+    rng = np.random.default_rng(rows * dim + heads)
+    ref, tables, q = _case(rng, heads, kv, dim, 3, rows, 11, seed=rows)
+    _check(ref, q, tables, lens, counts, causal)
+
+
+@pytest.mark.parametrize("rows", [1, 5, 40, 200])
+def test_attention_rows_that_see_nothing(rows):
+    """No tokens, rows before token 0 (more rows than tokens), lengths past the table, pages outside the pool."""
+    rng = np.random.default_rng(rows)
+    ref, tables, q = _case(rng, 4, 2, 128, 5, rows, 3, seed=rows)
+    tables[1, :] = -1
+    tables[2, 1] = 10 ** 6
+    tables[3] = tables[0]  # a shared prefix
+    for causal in (False, True):
+        _check(ref, q, tables, [0, 150, 192, rows // 2, 500], None, causal)
+
+
+@pytest.mark.parametrize("rows", [1, 30, 200])
+def test_attention_does_not_read_behind_the_end(rows):
+    """NaN and infinite scales in pages that no sequence has, and 8-bit values behind the last token."""
+    rng = np.random.default_rng(3 * rows)
+    ref, tables, q = _case(rng, 4, 4, 64, 2, rows, 4, seed=1)
+    free = np.setdiff1d(np.arange(10), tables[:, :3])
+    ref.ks[free], ref.vs[free] = np.nan, np.inf
+    _check(ref, q, tables, [192, 140], None, False)
+    _check(ref, q, tables, [192, 140], None, True)
+
+
+def test_attention_poisoned_block():
+    """A NaN scale reaches the rows that see its block, and no others."""
+    h = _h()
+    rng = np.random.default_rng(2)
+    for rows in (4, 300):
+        ref, tables, q = _case(rng, 2, 2, 128, 1, rows, 6, seed=2)
+        ref.ks[tables[0, 3], 1] = np.nan
+        out = _np(h.kv_attention(_bf(q), ref.to(), _i32(tables), _i32([384]), causal=True))
+        at = 384 - rows + np.arange(rows)
+        assert np.isfinite(out[0, :, 0]).all() and np.isfinite(out[0, at < 192, 1]).all() and np.isnan(out[0, at >= 192, 1]).all()
+
+
+@pytest.mark.parametrize("scale", [0.0, 1.0, -0.3, 30.0])
+@pytest.mark.parametrize("rows", [2, 150])
+def test_attention_scales(scale, rows):
+    """Steep and negative scales; a scale of 0 is the mean of the values."""
+    rng = np.random.default_rng(4)
+    ref, tables, q = _case(rng, 2, 2, 64, 1, rows, 5, seed=4)
+    ref.ks *= 0.2
+    _check(ref, q, tables, [300], None, False, scale=scale)
+
+
+@pytest.mark.parametrize("rows", [1, 200])
+def test_attention_zero_and_tiny_scales(rows):
+    """Blocks of zero keys or values, and scales at the ends of fp32."""
+    rng = np.random.default_rng(6)
+    ref, tables, q = _case(rng, 2, 2, 128, 1, rows, 6, seed=6)
+    ref.ks[tables[0, 0]] = 0
+    ref.k[tables[0, 0]] = 0
+    ref.vs[tables[0, 1]] = 0
+    ref.v[tables[0, 1]] = 0
+    ref.vs[tables[0, 2]] = 1e-39
+    ref.ks[tables[0, 3]] = 1e-40
+    _check(ref, q, tables, [384], None, False)
+    ref.vs[:] = 1e-38
+    h = _h()
+    out = h.kv_attention(_bf(q), ref.to(), _i32(tables), _i32([384]))
+    assert np.isfinite(_np(out)).all()
+
+
+@pytest.mark.parametrize("rows", [1, 3, 129])
+def test_attention_of_views(rows):
+    """q as a view of a projection's output."""
+    rng = np.random.default_rng(8)
+    ref, tables, _ = _case(rng, 4, 2, 128, 2, rows, 5, seed=8)
+    qkv = _round(rng.standard_normal((2, rows, 3, 4, 128)))
+    _check(ref, qkv[:, :, 1], tables, [300, 250], None, True, view=_bf(qkv)[:, :, 1])
+
+
+@pytest.mark.parametrize("rows,n,heads,kv,tokens", [(1, 1, 4, 4, 20000), (1, 3, 10, 2, 9000), (24, 1, 2, 2, 12000), (200, 1, 2, 2, 9001)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_long(rows, n, heads, kv, tokens, causal):
+    """Few rows over long caches: the work is split over the tokens and joined."""
+    rng = np.random.default_rng(tokens)
+    blocks = -(-tokens // 64)
+    ref, tables, q = _case(rng, heads, kv, 128, n, rows, blocks, seed=7)
+    lens = [tokens] + [tokens // 3, 100][:n - 1]
+    _check(ref, q, tables, lens, None, causal)
+
+
+def test_offsets_past_32_bits():
+    """Pages whose bytes lie past 2^31 and whose elements past 2^32 in the pool, and rows past 2^31 elements."""
+    h = _h()
+    rng = np.random.default_rng(21)
+    heads, dim = 64, 256
+    pages = 4200  # 4200 * 64 * 64 * 256 = 4.4e9
+    cache = h.kv_cache(pages, heads, dim)
+    tables = np.array([[pages - 1, 1, pages - 2]], np.int32)
+    small = R.Cache(3, heads, dim)
+    k, v = (_round(rng.standard_normal((1, 150, heads, dim))) for _ in range(2))
+    R.write(small, k, v, np.array([[0, 1, 2]]), [150], [150])
+    h.kv_write_(cache, _bf(k), _bf(v), _i32(tables), _i32([150]))
+    part = h.KVCache(*(t[tables[0].tolist()].contiguous() for t in cache))
+    assert small.same(part) == []
+    for rows in (1, 60):
+        q = _round(rng.standard_normal((1, rows, heads, dim)))
+        want, mag, top = R.attention(small, q.astype(np.float64), np.array([[0, 1, 2]]), [150], [rows], True)
+        got = h.kv_attention(_bf(q), cache, _i32(tables), _i32([150]), causal=True).double().cpu().numpy()
+        assert (np.abs(got - want) <= R.bound(want, mag, top, dim)).all()
+        pick = h.kv_select(_bf(q), cache, _i32(tables), _i32([150]), 2).cpu().numpy()
+        assert np.array_equal(pick, R.select(small, q.astype(np.float64), np.array([[0, 1, 2]]), [150], [rows], 2, False))
+    rk, _ = h.kv_read(cache, _i32(tables), _i32([150]), 150)
+    want = torch.from_numpy(R.tokens(small, [0, 1, 2], 150)[0]).float().to(torch.bfloat16)
+    assert torch.equal(rk[0].cpu(), want)
+    # a token stride that takes the last row past 2^31 elements
+    wide = torch.empty(150 * 16_000_000, dtype=torch.bfloat16, device=DEV).as_strided((1, 150, heads, dim), (0, 15_999_904, dim, 1))
+    wide.copy_(_bf(k))
+    again = h.kv_cache(3, heads, dim)
+    h.kv_write_(again, wide, _bf(v), _i32([[0, 1, 2]]), _i32([150]))
+    assert small.same(again) == []
+
+
+# ------------------------------------------------------------------ selection
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(3, 3, 64), (10, 2, 128), (4, 2, 256)])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("rows,lens,counts,top", [
+    (1, [1, 64, 700], None, 1), (1, [2000, 0, 1337], None, 7), (5, [2048, 500, 3], [5, 0, 4], 12), (128, [128, 2000, 640], None, 3),
+    (300, [300, 2048, 1000], [300, 129, 1], 5), (130, [2048, 5000, 100], None, 40), (200, [100, 150, 2048], None, 4),
+])
+def test_select(heads, kv, dim, causal, rows, lens, counts, top):
+    rng = np.random.default_rng(rows + top + dim)
+    ref, tables, q = _case(rng, heads, kv, dim, 3, rows, 32, seed=top)
+    tables[2, 5] = -4
+    got = _h().kv_select(_bf(q), ref.to(), _i32(tables), _i32(lens), top, causal=causal, counts=None if counts is None else _i32(counts))
+    want = R.select(ref, q.astype(np.float64), tables, lens, counts or [rows] * 3, top, causal)
+    assert np.array_equal(got.cpu().numpy(), want)
+
+
+def test_select_ties_and_specials():
+    """Equal scores take the lowest blocks; NaN scales come last; a query of zeros, NaN or infinities scores all alike."""
+    rng = np.random.default_rng(31)
+    ref, tables, q = _case(rng, 2, 2, 64, 1, 1, 200, seed=31)
+    ref.ksum[tables[0, 3:150]] = ref.ksum[tables[0, 3]]
+    ref.ks[tables[0, 3:150]] = 0.01
+    ref.ks[tables[0, 170:180]] = np.nan
+    ref.ks[tables[0, 180:190]] = np.inf
+    ref.ks[tables[0, 190:195]] = 0
+    for scale in (1.0, -1.0, 0.0, np.nan, np.inf):
+        with np.errstate(invalid="ignore"):
+            x = _round(q * scale)
+        for top in (1, 20, 100, 195, 200, 250):
+            got = _h().kv_select(_bf(x), ref.to(), _i32(tables), _i32([200 * 64]), top)
+            with np.errstate(invalid="ignore"):
+                want = R.select(ref, x.astype(np.float64), tables, [200 * 64], [1], top, False)
+            assert np.array_equal(got.cpu().numpy(), want), (scale, top)
+
+
+def test_select_long():
+    """The longest table, and one page under many blocks: all scores equal but one."""
+    ref = R.Cache(3, 1, 64, seed=32)
+    ref.ksum[0], ref.ks[:] = 1, 0.01
+    ref.ksum[1] = 2
+    tables = np.zeros((1, 32768), np.int32)
+    tables[0, 30001] = 1
+    q = np.ones((1, 1, 1, 64), np.float32)
+    got = _h().kv_select(_bf(q), ref.to(), _i32(tables), _i32([32768 * 64]), 100).cpu().numpy().reshape(-1)
+    assert got.tolist() == list(range(99)) + [30001]
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(3, 3, 64), (10, 2, 128), (6, 2, 256), (20, 1, 64)])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("rows,top", [(1, 4), (2, 9), (128, 5), (300, 6), (140, 30)])
+def test_sparse_attention(heads, kv, dim, causal, rows, top):
+    """select, then attention over what it took."""
+    h = _h()
+    rng = np.random.default_rng(rows * top + dim)
+    ref, tables, q = _case(rng, heads, kv, dim, 2, rows, 20, seed=rows)
+    lens = [1270, 700]
+    blocks = h.kv_select(_bf(q), ref.to(), _i32(tables), _i32(lens), top, causal=causal).cpu().numpy()
+    assert np.array_equal(blocks, R.select(ref, q.astype(np.float64), tables, lens, [rows] * 2, top, causal))
+    _check(ref, q, tables, lens, None, causal, blocks=blocks)
+
+
+@pytest.mark.parametrize("rows", [1, 130])
+def test_sparse_attention_any_lists(rows):
+    """Lists in any order, with holes, blocks past the end and outside the table; empty lists give zeros."""
+    rng = np.random.default_rng(41)
+    ref, tables, q = _case(rng, 4, 2, 128, 2, rows, 12, seed=41)
+    tiles = -(-rows // 128)
+    blocks = np.full((2, tiles, 2, 9), -1, np.int32)
+    blocks[0, :, 0] = [7, -1, 2, 11, 10, -7, 0, 12, 2147483647]
+    blocks[0, :, 1] = [-1, -1, 3, -1, -1, 4, -1, -1, -2147483648]
+    blocks[1, :, 0] = [5, 9, 8, 7, 6, 4, 3, 2, 1]
+    for causal in (False, True):
+        _check(ref, q, tables, [700, 320], None, causal, blocks=blocks)
+
+
+def test_sparse_with_every_block_is_dense():
+    h = _h()
+    rng = np.random.default_rng(43)
+    for rows in (1, 7, 260):
+        ref, tables, q = _case(rng, 4, 2, 128, 2, rows, 9, seed=43)
+        c, t, lens = ref.to(), _i32(tables), _i32([570, 301])
+        blocks = h.kv_select(_bf(q), c, t, lens, 9, causal=True)
+        a, b = h.kv_attention(_bf(q), c, t, lens, causal=True), h.kv_attention(_bf(q), c, t, lens, causal=True, blocks=blocks)
+        want, mag, top = R.attention(ref, q.astype(np.float64), tables, [570, 301], [rows] * 2, True)
+        for x in (a, b):
+            assert (np.abs(x.double().cpu().numpy() - want) <= R.bound(want, mag, top, 128)).all()
+
+
+# ------------------------------------------------------------------ together, streams, graphs
+
+
+def _step(h, st):
+    """A step of a block's attention: norm and rotate q and k, write, select, attend (all and selected), read back."""
+    H, D, S = 4, 128, st["qkv"].shape[0]
+    st["work"].copy_(st["qkv"])
+    q, k, v = (st["work"][:, i * H * D:(i + 1) * H * D].view(1, S, H, D) for i in range(3))
+    h.rms_rope_split_half_(q, k, st["tab"], st["qw"], st["qw"], epsilon=1e-6)
+    h.kv_write_(st["cache"], k, v, st["tables"], st["lens"])
+    blocks = h.kv_select(q, st["cache"], st["tables"], st["lens"], 4, causal=True)
+    dense = h.kv_attention(q, st["cache"], st["tables"], st["lens"], causal=True)
+    sparse = h.kv_attention(q, st["cache"], st["tables"], st["lens"], causal=True, blocks=blocks)
+    rk, rv = h.kv_read(st["cache"], st["tables"], st["lens"], 100, starts=st["lens"] - 50)
+    return [dense, sparse, blocks, rk, rv] + [t.clone() for t in st["cache"]]
+
+
+def _state(h, S, seed):
+    g = torch.Generator().manual_seed(seed)
+    H, D = 4, 128
+    ang = 6.28 * torch.rand(S, D // 2, generator=g)
+    tab = torch.stack([ang.cos(), -ang.sin(), ang.sin(), ang.cos()], -1).reshape(1, S, D // 2, 2, 2)
+    return {"qkv": torch.randn(S, 3 * H * D, generator=g).to(torch.bfloat16).to(DEV), "work": torch.empty(S, 3 * H * D, dtype=torch.bfloat16, device=DEV),
+            "tab": tab.to(torch.bfloat16).to(DEV), "qw": torch.ones(D, dtype=torch.bfloat16, device=DEV),
+            "cache": h.kv_cache(40, H, D), "tables": torch.randperm(40, generator=g).to(torch.int32)[None].to(DEV),
+            "lens": torch.tensor([S], dtype=torch.int32, device=DEV)}
+
+
+@pytest.mark.parametrize("S", [1, 20, 150])
+def test_steps_captured_and_replayed(S):
+    """Steps that extend a sequence, each replayed from one graph against the same step run eagerly."""
+    h = _h()
+    eager, st = _state(h, S, 1), _state(h, S, 1)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        _step(h, st)
+    torch.cuda.synchronize()
+    for t in st["cache"]:
+        t.zero_()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = _step(h, st)
+    for r in range(5):
+        fresh = torch.randn(S, 3 * 512, generator=torch.Generator().manual_seed(r)).to(torch.bfloat16).to(DEV)
+        for x in (eager, st):
+            x["qkv"].copy_(fresh)
+            x["lens"].fill_((r + 1) * S)
+        want = _step(h, eager)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), r
+
+
+def test_two_graphs_share_no_workspace():
+    """Two captured calls that split their work, replayed on two streams at once."""
+    h = _h()
+    rng = np.random.default_rng(51)
+    ref, tables, q = _case(rng, 4, 4, 128, 1, 1, 150, seed=51)
+    c, t, lens = ref.to(), _i32(tables), _i32([9600])
+    qs = [_bf(q), _bf(_round(rng.standard_normal(q.shape)))]
+    want = [h.kv_attention(x, c, t, lens) for x in qs]
+    graphs, outs = [], []
+    for x in qs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(h.kv_attention(x, c, t, lens))
+        graphs.append(g)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(10):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+def test_same_bits_every_time():
+    h = _h()
+    rng = np.random.default_rng(61)
+    for rows, blocks in ((1, 120), (40, 60), (300, 20)):
+        ref, tables, q = _case(rng, 10, 2, 128, 2, rows, blocks, seed=61)
+        c, t, lens, x = ref.to(), _i32(tables), _i32([blocks * 64 - 3, blocks * 32]), _bf(q)
+        a = h.kv_attention(x, c, t, lens)
+        for _ in range(5):
+            assert torch.equal(a, h.kv_attention(x, c, t, lens))
+
+
+# ------------------------------------------------------------------ refusals
+
+
+def test_refusals_of_the_python_functions():
+    h = _h()
+    c = h.kv_cache(4, 2, 64)
+    t, lens = _i32([[0, 1]]), _i32([100])
+    x = torch.zeros(1, 10, 2, 64, dtype=torch.bfloat16, device=DEV)
+    q = torch.zeros(1, 10, 4, 64, dtype=torch.bfloat16, device=DEV)
+    bad = [
+        lambda: h.kv_write_(c, x.float(), x, t, lens), lambda: h.kv_write_(c, x, x[:, :5], t, lens),
+        lambda: h.kv_write_(c, q, q, t, lens), lambda: h.kv_write_(c, x[0], x[0], t, lens),
+        lambda: h.kv_write_(c, x.transpose(1, 2), x.transpose(1, 2), t, lens), lambda: h.kv_write_(c, x.cpu(), x, t, lens),
+        lambda: h.kv_write_(c, x, x, t.long(), lens), lambda: h.kv_write_(c, x, x, t, lens.cpu()),
+        lambda: h.kv_write_(c, x, x, t[0], lens), lambda: h.kv_write_(c, x, x, t, _i32([1, 2])),
+        lambda: h.kv_write_(c, x, x, t, lens, counts=_i32([1, 2])), lambda: h.kv_write_(c._replace(k=c.k.float()), x, x, t, lens),
+        lambda: h.kv_write_(c._replace(v=c.k), x, x, t, lens), lambda: h.kv_write_(c._replace(k_sum=c.k_sum.cpu()), x, x, t, lens),
+        lambda: h.kv_write_(c._replace(k_scale=c.k_scale.t().contiguous().t()), x, x, t, lens),
+        lambda: h.kv_read(c, t, lens, -1), lambda: h.kv_read(c, t, lens, 4, starts=_i32([1, 2])),
+        lambda: h.kv_attention(q[..., :32], c, t, lens), lambda: h.kv_attention(q[:, :, :3], c, t, lens),
+        lambda: h.kv_attention(q, c, t, lens, blocks=_i32([[[[0]]]])), lambda: h.kv_attention(q, c, t, lens, scale=float("nan")),
+        lambda: h.kv_attention(q, c, t, lens, scale=float("inf")), lambda: h.kv_attention(q.expand(2, -1, -1, -1), c, t, lens),
+        lambda: h.kv_select(q, c, t, lens, 0), lambda: h.kv_select(q, c, t, lens, 40000), lambda: h.kv_select(q[:, :, :3], c, t, lens, 1),
+        lambda: h.kv_select(q, c, _i32(np.zeros((1, 32769))), lens, 1),
+        lambda: h.kv_attention(torch.zeros(1, 10, 4 * 64 + 4, dtype=torch.bfloat16, device=DEV)[..., 4:].view(1, 10, 4, 64), c, t, lens),
+        lambda: h.kv_cache(1, 1, 96),
+    ]
+    for n, f in enumerate(bad):
+        with pytest.raises((ValueError, RuntimeError)):
+            f()
+            pytest.fail(f"call {n} was taken")
+    with pytest.raises(RuntimeError, match="gradient"):
+        h.kv_attention(q.clone().requires_grad_(), c, t, lens)
+    with torch.no_grad():
+        h.kv_attention(q.clone().requires_grad_(), c, t, lens)
+    # a call with nothing to do
+    assert h.kv_attention(q[:, :0], c, t, lens).shape == (1, 0, 4, 64)
+    assert h.kv_select(q[:, :0], c, t, lens, 3).shape == (1, 0, 2, 3)
+    assert h.kv_attention(q, c, t[:, :0].contiguous(), lens).abs().max() == 0
+    assert (h.kv_select(q, c, t[:, :0].contiguous(), lens, 3) == -1).all()
+    assert h.kv_read(c, t, lens, 0)[0].shape == (1, 0, 2, 64)

@@ -1,0 +1,92 @@
+"""The C entry points of the 8-bit cache refuse bad arguments before touching a device: every pointer here is made up."""
+import ctypes
+
+import pytest
+
+P = ctypes.c_void_p
+BASE = dict(k=4096, v=1 << 19, k_scale=12288, v_scale=16384, k_sum=20480, pages=10, heads=2, dim=128)
+SEQS = dict(tables=24576, lens=28672, counts=None, n=2, blocks=5)
+
+
+def _call(fn, cache=None, seqs=None, **kw):
+    from h3mi import _lib
+    c, s = _lib.KvCacheC(**{**BASE, **(cache or {})}), _lib.KvSeqsC(**{**SEQS, **(seqs or {})})
+    c, s = ctypes.byref(c), ctypes.byref(s)
+    a = dict(p=1 << 20, p2=1 << 21, rows=4, heads=4, ld=512, bs=2048, top=3, length=9, out=1 << 22, scale=1.0, starts=None, blocks=None,
+             work=None, size=0)
+    a.update(kw)
+    L = _lib.lib
+    if fn == "write":
+        rc = L.h3mi_kv_write_i8(P(a["p"]), P(a["p2"]), a["rows"], a["ld"], a["bs"], a["ld"], a["bs"], c, s, None)
+    elif fn == "read":
+        rc = L.h3mi_kv_read_bf16(P(a["p"]), P(a["p2"]), P(a["starts"]), a["length"], c, s, None)
+    elif fn == "select":
+        rc = L.h3mi_kv_select(P(a["p"]), a["rows"], a["heads"], a["ld"], a["bs"], c, s, a["top"], 0, P(a["out"]), None)
+    else:
+        rc = L.h3mi_kv_attention_bf16(P(a["p"]), a["rows"], a["heads"], a["ld"], a["bs"], c, s, ctypes.c_float(a["scale"]), 0,
+                                      P(a["blocks"]), a["top"], P(a["out"]), P(a["work"]), a["size"], None)
+    return rc, L.h3mi_last_error().decode()
+
+
+EVERY = ["write", "read", "select", "attention"]
+
+
+@pytest.mark.parametrize("fn", EVERY)
+@pytest.mark.parametrize("cache,seqs,code,msg", [
+    (dict(dim=96), None, 1, "dim=96"), (dict(dim=0), None, 1, "dim=0"), (dict(heads=0), None, 1, "heads=0"), (dict(pages=-1), None, 1, "pages=-1"),
+    (dict(pages=1 << 31), None, 1, "pages"), (None, dict(n=-1), 1, "n=-1"), (None, dict(blocks=-1), 1, "blocks=-1"),
+    (None, dict(blocks=1 << 25), 1, "blocks"), (dict(k=None), None, 1, "null cache"), (dict(k_sum=None), None, 1, "null cache"),
+    (None, dict(lens=None), 1, "null tables or lens"), (None, dict(tables=None), 1, "null tables or lens"), (dict(v=(1 << 19) + 8), None, 2, "aligned"), (dict(v=8192), None, 3, "k and v overlap"),
+    (dict(k_scale=2), None, 2, "aligned"), (None, dict(lens=6), 2, "4-byte"),
+])
+def test_cache_and_sequences(fn, cache, seqs, code, msg):
+    rc, m = _call(fn, cache, seqs)
+    assert rc == code and msg in m, (rc, m)
+
+
+@pytest.mark.parametrize("fn", ["write", "select", "attention"])
+@pytest.mark.parametrize("kw,code,msg", [
+    (dict(rows=-1), 1, "rows=-1"), (dict(p=None), 1, "null"), (dict(p=(1 << 20) + 8), 2, "aligned"), (dict(ld=8), 1, "shorter"),
+    (dict(bs=8), 1, "shorter"), (dict(ld=516), 2, "multiples of 8"), (dict(bs=2052), 2, "multiples of 8"), (dict(bs=-2048), 1, "shorter"),
+])
+def test_rows(fn, kw, code, msg):
+    rc, m = _call(fn, **kw)
+    assert rc == code and msg in m, (rc, m)
+
+
+@pytest.mark.parametrize("fn,kw,code,msg", [
+    ("read", dict(length=-1), 1, "length=-1"), ("read", dict(p=None), 1, "null k or v"), ("read", dict(p2=8), 2, "aligned"),
+    ("read", dict(starts=2), 2, "aligned"), ("select", dict(heads=3), 1, "multiple of the cache's"), ("select", dict(heads=0), 1, "multiple"),
+    ("attention", dict(heads=5), 1, "multiple of the cache's"), ("select", dict(top=0), 1, "top=0"), ("select", dict(top=32769), 1, "top=32769"),
+    ("select", dict(out=None), 1, "null blocks"), ("select", dict(out=2), 2, "aligned"), ("attention", dict(out=None), 1, "null out"),
+    ("attention", dict(out=8), 2, "aligned"), ("attention", dict(scale=float("nan")), 1, "scale"), ("attention", dict(scale=float("inf")), 1, "scale"),
+    ("attention", dict(blocks=4096, top=0), 1, "top=0"), ("attention", dict(blocks=4098), 2, "aligned"),
+])
+def test_each(fn, kw, code, msg):
+    rc, m = _call(fn, **kw)
+    assert rc == code and msg in m, (rc, m)
+
+
+def test_sizes_past_a_launch():
+    assert _call("write", dict(heads=65536, dim=256, v=1 << 50), dict(blocks=(1 << 25) - 1), rows=1 << 30, ld=65536 * 256, bs=1 << 60)[0] == 1
+    assert _call("read", dict(heads=65536, v=1 << 50), dict(n=1 << 30), length=1 << 30)[0] == 1
+    assert _call("select", dict(heads=65536, v=1 << 50), dict(n=1 << 20), rows=1 << 20, heads=65536, ld=65536 * 128, bs=1 << 60)[0] == 1
+    assert _call("select", None, dict(blocks=32769))[0] == 1
+    assert _call("attention", dict(heads=65536, v=1 << 50), dict(n=1 << 20), rows=1 << 20, heads=65536, ld=65536 * 128, bs=1 << 60)[0] == 1
+
+
+@pytest.mark.parametrize("fn", EVERY)
+def test_nothing_to_do(fn):
+    assert _call(fn, None, dict(n=0, lens=None, tables=None))[0] == 0
+    assert _call(fn, rows=0, length=0, p=None, p2=None, out=None)[0] == 0
+
+
+@pytest.mark.parametrize("fn", EVERY)
+def test_null_structures(fn):
+    from h3mi import _lib
+    L = _lib.lib
+    rc = {"write": lambda: L.h3mi_kv_write_i8(P(4096), P(8192), 1, 256, 256, 256, 256, None, None, None),
+          "read": lambda: L.h3mi_kv_read_bf16(P(4096), P(8192), None, 1, None, None, None),
+          "select": lambda: L.h3mi_kv_select(P(4096), 1, 2, 256, 256, None, None, 1, 0, P(8192), None),
+          "attention": lambda: L.h3mi_kv_attention_bf16(P(4096), 1, 2, 256, 256, None, None, ctypes.c_float(1), 0, None, 0, P(8192), None, 0, None)}[fn]()
+    assert rc == 1 and "null cache or sequences" in L.h3mi_last_error().decode()
