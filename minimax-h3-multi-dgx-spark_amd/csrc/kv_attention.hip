@@ -1,74 +1,591 @@
 // Attention over the 8-bit key/value cache.
+//
+// One pass over a sequence's blocks of 64 tokens with the running maximum m and sum l of
+// the softmax, in base 2:  x = (q . k) c_b, c_b = k_scale scale log2(e);  p = 2^(x - m);
+// l += sum p;  o += sum p v.  Keys and values are 8-bit integers, which bf16 holds
+// exactly, so the products run on bf16 MFMAs with the integers themselves: a block's key
+// scale is a factor of its scores (one fma with the subtraction of m), and its value scale
+// a term of the exponent, p v_scale = 2^(x - m + log2 v_scale), which costs nothing per
+// score; l takes the sum times 1 / v_scale.  Scores and sums are fp32; a probability is
+// rounded once, to the bf16 that the second product multiplies.
+//
+// Both products are formed transposed, S^T = K Q^T and O^T = V^T P^T: a query is then a
+// column, whose scores lie in the registers of two (four) lanes, so that the maximum needs
+// one (two) lane exchanges a block, and the lanes that hold a query's probabilities are
+// those that the second product wants them in.  Rows of K are taken in the order that
+// makes the probabilities' registers whole runs of tokens; V is stored transposed, so that
+// its rows are runs of tokens too.  P never leaves the registers.
+//
+// Two kernels: tiles of 128 or 256 query rows of a head, bound by the MFMAs and the
+// softmax, and up to 16 queries of a kv head's group, bound by the cache's bytes.
 #include "kv.h"
 
 namespace h3mi {
 namespace {
 
-// One wave: one query row of one head; a lane scores a token of each block.
-template <int D>
-__global__ __launch_bounds__(64) void kv_attention_kernel(const uint16_t* __restrict__ q, int64_t ld, int64_t bs, KvCache c,
-                                                          KvSeqs s, int rows, int heads, float scale, int causal,
-                                                          const int32_t* __restrict__ list, int top, uint16_t* __restrict__ out) {
-    __shared__ float qs[D];
-    __shared__ float ps[kKvBlock];
-    const int lane = threadIdx.x;
-    const int hq = blockIdx.x % heads;
-    const int64_t item = blockIdx.x / heads;
-    const int i = static_cast<int>(item / rows), r = static_cast<int>(item % rows);
-    const int h = hq / (heads / c.heads);
-    const int len = s.len(i), count = s.count(i, rows);
-    const int at = s.end(i) - count + r;
-    int last = len - 1;  // the last token seen
-    if (causal && at < last) last = at;
-    if (r >= count) last = -1;
-    const int64_t row = i * bs + static_cast<int64_t>(r) * ld + static_cast<int64_t>(hq) * D;
-    for (int d = lane; d < D; d += 64) qs[d] = bf16_f32(q[row + d]) * scale;
-    __syncthreads();
-    const int tiles = (rows + kKvTile - 1) / kKvTile;
-    const int32_t* const mine = list ? list + ((static_cast<int64_t>(i) * tiles + r / kKvTile) * c.heads + h) * top : nullptr;
-    const int nb = last < 0 ? 0 : block_of(last) + 1;
-    const int steps = mine ? (nb ? top : 0) : nb;
-    float m = -__builtin_inff(), l = 0.0f, o[D / 64] = {};
-    for (int x = 0; x < steps; ++x) {
-        const int b = mine ? mine[x] : x;
-        if (b < 0 || b >= nb) continue;
-        const int page = s.page(i, b, c.pages);
-        if (page < 0) continue;
-        const int64_t tile = static_cast<int64_t>(page) * c.heads + h;
-        const int8_t* const k = c.k + tile * (kKvBlock * D) + lane * D;
-        float dot = 0.0f;
-        for (int d = 0; d < D; d += 16) {
-            const uint4 w = *reinterpret_cast<const uint4*>(k + d);
-            const uint32_t a[4] = {w.x, w.y, w.z, w.w};
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr float kLog2e = 1.44269504088896341f;
+// The running maximum's start: finite, so that a row that has seen nothing has differences
+// that are numbers, and below every finite score that counts.
+constexpr float kLowest = -3.4028234663852886e38f;
+// A row keeps its reference until a score passes it by 2^kSlack (then p <= 2^kSlack, which
+// fp32 sums and bf16 probabilities hold as well as p <= 1): the accumulators are rescaled a
+// few times a sequence, not once a block.
+constexpr float kSlack = 8.0f;
+// Value scales whose log2 goes into the exponent: 2^(+-60) keeps p v_scale a normal number
+// for every p above 2^-66.  Others (zero, not finite) multiply p afterwards.
+constexpr float kFoldLow = 0x1p-60f, kFoldHigh = 0x1p+60f;
+
+// 8 signed bytes as 8 bf16.
+__device__ __forceinline__ uint4 ints_bf16(uint2 q) {
+    float f[8];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) dot += qs[d + j] * static_cast<float>(static_cast<int8_t>(a[j >> 2] >> (8 * (j & 3))));
+    for (int j = 0; j < 8; ++j) f[j] = static_cast<float>(static_cast<int8_t>((j < 4 ? q.x : q.y) >> (8 * (j & 3))));
+    return make_uint4(bf16x2_bits(f[0], f[1]), bf16x2_bits(f[2], f[3]), bf16x2_bits(f[4], f[5]), bf16x2_bits(f[6], f[7]));
+}
+
+__device__ __forceinline__ bf16x8 frag(uint4 w) { return __builtin_bit_cast(bf16x8, w); }
+
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// What a block's scores and probabilities are multiplied by.
+struct Factors {
+    float c;         // scores: k_scale scale log2(e)
+    float lv, iv;    // the exponent's term, and what a sum of probabilities is multiplied by
+    float vs;        // probabilities are multiplied by it where iv is 0
+};
+
+__device__ __forceinline__ Factors factors(float ks, float vs, float scale) {
+    const bool fold = vs >= kFoldLow && vs <= kFoldHigh;
+    return {ks * scale, fold ? log2f(vs) : 0.0f, fold ? 1.0f / vs : 0.0f, vs};
+}
+
+struct Queries {
+    const uint16_t* p;
+    int64_t ld, bs;
+    int rows, heads;
+};
+
+struct Lists {
+    const int32_t* p;  // [n, tiles, kv heads, top], or null
+    int top, tiles;
+};
+
+// Partial results of a split: per (split, query) dim sums, and (m, l).
+struct Partial {
+    float* o;
+    float2* ml;
+    int64_t queries;  // n rows heads
+    int splits;
+};
+
+// ------------------------------------------------------------------ tiles of queries
+
+// W waves of 32 query rows of one head.  The block's keys and values go through LDS as
+// bf16, converted once a workgroup, in two buffers: the next block's bytes are loaded
+// before this block's products and converted after them, one barrier a block.  Rows are
+// 16-byte chunks whose index is XORed with the row's low bits, which puts the 8 lanes of an
+// access on different banks, both for the writes and for the MFMA operands' reads.
+template <int D, int W>
+struct TileShape {
+    static constexpr int kThreads = 64 * W;
+    static constexpr int kRows = 32 * W;
+    static constexpr int kKeyBytes = kKvBlock * D * 2;
+    static constexpr int kBuf = 2 * kKeyBytes;
+    static constexpr int kLds = 2 * kBuf;
+    static constexpr int kLoads = kKvBlock * D / 8 / kThreads;  // 8-byte pieces of K (and of V) a thread
+};
+
+template <int D, int W>
+__global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv_tile_kernel(Queries q, KvCache c, KvSeqs s, float scale, int causal,
+                                                                          Lists list, uint16_t* __restrict__ out, Partial part,
+                                                                          int tiles, int items, int chunk) {
+    using T = TileShape<D, W>;
+    constexpr int NT = D / 32;            // tiles of 32 elements of the output
+    constexpr int KC = D / 8, VC = 8;     // 16-byte chunks of a row of K, of V
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+    __shared__ int2 entry[T::kThreads];   // (page, block) of the blocks at hand
+    __shared__ float4 fact[T::kThreads];
+    __shared__ int wcount[W];
+
+    // Consecutive items (tiles and splits of a head) on one XCD, whose L2 then holds the head's blocks.
+    const int item = (blockIdx.x & 7) * chunk + (blockIdx.x >> 3);
+    if (item >= items) return;
+    const int split = item % part.splits, tile_rev = item / part.splits % tiles;
+    const int nh = item / part.splits / tiles;
+    const int hq = nh % q.heads, i = nh / q.heads, h = hq / (q.heads / c.heads);
+    const int tile = causal ? tiles - 1 - tile_rev : tile_rev;  // the longest first
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, col = lane & 31, half = lane >> 5;
+
+    const int len = s.len(i), count = s.count(i, q.rows), start = s.end(i) - count;
+    const int r0 = tile * T::kRows, row = r0 + wave * 32 + col;
+    // the last token that this lane's query, the wave's last and the workgroup's last see
+    auto last_of = [&](int r) {
+        int x = len - 1;
+        if (causal && start + r < x) x = start + r;
+        return r < count ? x : -1;
+    };
+    const int last = last_of(row);
+    const int wave_row = r0 + wave * 32 + 31 < count ? r0 + wave * 32 + 31 : count - 1;
+    const int wave_last = wave_row >= r0 + wave * 32 ? last_of(wave_row) : -1;
+    const int tile_row = r0 + T::kRows - 1 < count ? r0 + T::kRows - 1 : count - 1;
+    const int tile_last = tile_row >= r0 ? last_of(tile_row) : -1;
+    // below this every query of the wave that is one sees a whole block
+    const int wave_full = wave_last >= 0 ? last_of(r0 + wave * 32) + 1 : 0;
+    const int blocks = tile_last < 0 ? 0 : block_of(tile_last) + 1;
+
+    bf16x8 qf[D / 16];
+    {
+        const int64_t at = i * q.bs + static_cast<int64_t>(row) * q.ld + static_cast<int64_t>(hq) * D + half * 8;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+            qf[k] = frag(last >= 0 ? *reinterpret_cast<const uint4*>(q.p + at + k * 16) : make_uint4(0, 0, 0, 0));
+    }
+    f32x16 o[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[n][r] = 0.0f;
+    float m = kLowest, l = 0.0f;
+
+    const int32_t* const mine =
+        list.p ? list.p + ((static_cast<int64_t>(i) * list.tiles + r0 / kKvTile) * c.heads + h) * list.top : nullptr;
+    const int total = blocks == 0 ? 0 : mine ? list.top : blocks;
+    const int from = static_cast<int>(static_cast<int64_t>(total) * split / part.splits);
+    const int to = static_cast<int>(static_cast<int64_t>(total) * (split + 1) / part.splits);
+
+    uint2 kr[T::kLoads], vr[T::kLoads];
+    auto load = [&](int page) {
+        const int64_t base = (static_cast<int64_t>(page) * c.heads + h) * (kKvBlock * D);
+#pragma unroll
+        for (int j = 0; j < T::kLoads; ++j) {
+            kr[j] = *reinterpret_cast<const uint2*>(c.k + base + (t + j * T::kThreads) * 8);
+            vr[j] = *reinterpret_cast<const uint2*>(c.v + base + (t + j * T::kThreads) * 8);
         }
-        const bool there = b * kKvBlock + lane <= last;
-        const float x0 = there ? dot * c.ks[tile] : -__builtin_inff();
-        float bm = x0;
+    };
+    auto stage = [&](uint8_t* buf) {
 #pragma unroll
-        for (int y = 32; y; y >>= 1) bm = fmaxf(bm, __shfl_xor(bm, y));
-        const float mn = fmaxf(m, bm), fix = __expf(m - mn);
-        const float p = there ? __expf(x0 - mn) : 0.0f;
-        float sum = p;
-#pragma unroll
-        for (int y = 32; y; y >>= 1) sum += __shfl_xor(sum, y);
-        l = l * fix + sum;
-        m = mn;
-        ps[lane] = p * c.vs[tile];
+        for (int j = 0; j < T::kLoads; ++j) {
+            const int piece = t + j * T::kThreads;
+            // token bits 2 and 3 change places: an MFMA row's registers are then runs of 8 tokens
+            const int tok = piece / KC, kc = piece % KC;
+            const int kr_row = (tok & ~12) | ((tok & 4) << 1) | ((tok & 8) >> 1);
+            *reinterpret_cast<uint4*>(buf + kr_row * (D * 2) + ((kc ^ (kr_row & 7)) * 16)) = ints_bf16(kr[j]);
+            const int vrow = piece / VC, vc = piece % VC;
+            *reinterpret_cast<uint4*>(buf + T::kKeyBytes + vrow * (kKvBlock * 2) + ((vc ^ (vrow & 7)) * 16)) = ints_bf16(vr[j]);
+        }
+    };
+
+    for (int x0 = from; x0 < to; x0 += T::kThreads) {
+        // the pages and factors of the next kThreads blocks, those that are not there left out
         __syncthreads();
-#pragma unroll
-        for (int e = 0; e < D / 64; ++e) {
-            const int8_t* const v = c.v + tile * (kKvBlock * D) + (e * 64 + lane) * kKvBlock;
-            float acc = 0.0f;
-            for (int y = 0; y < kKvBlock; ++y) acc += ps[y] * static_cast<float>(v[y]);
-            o[e] = o[e] * fix + acc;
+        {
+            const int x = x0 + t;
+            const int b = x < to ? (mine ? mine[x] : x) : -1;
+            const int page = b >= 0 && b < blocks ? s.page(i, b, c.pages) : -1;
+            const uint64_t got = __ballot(page >= 0);
+            if (lane == 0) wcount[wave] = __popcll(got);
+            __syncthreads();
+            int at = __popcll(got & ((uint64_t{1} << lane) - 1));
+            for (int w = 0; w < wave; ++w) at += wcount[w];
+            if (page >= 0) {
+                const int64_t p = static_cast<int64_t>(page) * c.heads + h;
+                const Factors f = factors(c.ks[p], c.vs[p], scale * kLog2e);
+                entry[at] = make_int2(page, b);
+                fact[at] = make_float4(f.c, f.lv, f.iv, f.vs);
+            }
         }
         __syncthreads();
+        int n = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) n += wcount[w];
+        if (n == 0) continue;
+        load(entry[0].x);
+        stage(smem);
+        __syncthreads();
+        for (int y = 0; y < n; ++y) {
+            if (y + 1 < n) load(entry[y + 1].x);
+            const uint8_t* const kb = smem + (y & 1) * T::kBuf;
+            const uint8_t* const vb = kb + T::kKeyBytes;
+            const int base = __builtin_amdgcn_readfirstlane(entry[y].y) * kKvBlock;
+            if (base <= wave_last) {
+                const float4 f = fact[y];
+                f32x16 sc[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) sc[u][r] = 0.0f;
+                    const int kr_row = u * 32 + col;
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k) {
+                        const bf16x8 a = frag(*reinterpret_cast<const uint4*>(kb + kr_row * (D * 2) + (((2 * k + half) ^ (kr_row & 7)) * 16)));
+                        sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, qf[k], sc[u], 0, 0, 0);
+                    }
+                }
+                // register r of sc[u]: token base + 32 u + 16 (r / 8) + 8 half + r % 8, times f.c
+                float best = -__builtin_inff();
+                if (base + kKvBlock > wave_full) {
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const int tok = base + 32 * u + 16 * (r / 8) + 8 * half + r % 8;
+                            sc[u][r] = tok <= last ? sc[u][r] * f.x : -__builtin_inff();
+                            best = fmaxf(best, sc[u][r]);
+                        }
+                } else {
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            sc[u][r] *= f.x;
+                            best = fmaxf(best, sc[u][r]);
+                        }
+                }
+                best = fmaxf(best, __shfl_xor(best, 32));
+                if (__any(best > m + kSlack)) {
+                    const float mn = fmaxf(m, best), fix = exp2_hw(m - mn);
+                    m = mn;
+                    l *= fix;
+#pragma unroll
+                    for (int d = 0; d < NT; ++d)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) o[d][r] *= fix;
+                }
+                const float off = f.y - m;
+                float sum = 0.0f;
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        sc[u][r] = exp2_hw(sc[u][r] + off);
+                        sum += sc[u][r];
+                    }
+                if (f.z != 0.0f) {
+                    l = __builtin_fmaf(sum, f.z, l);
+                } else {
+                    l += sum;
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) sc[u][r] = sc[u][r] == 0.0f ? 0.0f : sc[u][r] * f.w;
+                }
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int w = 0; w < 2; ++w) {
+                        const bf16x8 p = frag(make_uint4(bf16x2_bits(sc[u][8 * w], sc[u][8 * w + 1]), bf16x2_bits(sc[u][8 * w + 2], sc[u][8 * w + 3]),
+                                                         bf16x2_bits(sc[u][8 * w + 4], sc[u][8 * w + 5]), bf16x2_bits(sc[u][8 * w + 6], sc[u][8 * w + 7])));
+#pragma unroll
+                        for (int d = 0; d < NT; ++d) {
+                            const int vrow = d * 32 + col, vc = 4 * u + 2 * w + half;
+                            const bf16x8 a = frag(*reinterpret_cast<const uint4*>(vb + vrow * (kKvBlock * 2) + ((vc ^ (vrow & 7)) * 16)));
+                            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, p, o[d], 0, 0, 0);
+                        }
+                    }
+            }
+            if (y + 1 < n) stage(smem + ((y + 1) & 1) * T::kBuf);
+            __syncthreads();
+        }
+    }
+
+    l += __shfl_xor(l, 32);
+    if (row >= q.rows) return;
+    if (last < 0) {  // padding, or a row that sees nothing: what the registers hold is no result
+        l = 0.0f;
+#pragma unroll
+        for (int d = 0; d < NT; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
+    }
+    const int64_t query = (static_cast<int64_t>(i) * q.rows + row) * q.heads + hq;
+    // register r of o[d]: element 32 d + 8 (r / 4) + 4 half + r % 4 of the query's output
+    if (part.splits > 1) {
+        const int64_t at = split * part.queries + query;
+        if (half == 0) part.ml[at] = make_float2(m, l);
+#pragma unroll
+        for (int d = 0; d < NT; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<float4*>(part.o + at * D + 32 * d + 8 * g + 4 * half) =
+                    make_float4(o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]);
+        return;
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-    for (int e = 0; e < D / 64; ++e) out[(item * heads + hq) * D + e * 64 + lane] = bf16_bits(o[e] * inv);
+    for (int d = 0; d < NT; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<uint2*>(out + query * D + 32 * d + 8 * g + 4 * half) =
+                make_uint2(bf16x2_bits(o[d][4 * g] * inv, o[d][4 * g + 1] * inv), bf16x2_bits(o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv));
+}
+
+// ------------------------------------------------------------------ few queries
+
+constexpr int kFew = 16;      // queries of a kv head's group: the columns of a 16x16 MFMA
+constexpr int kFewWaves = 4;
+
+// A workgroup: one kv head of one sequence, one split of its blocks.  Its waves take whole
+// blocks in turn, straight from memory into the operands' registers (no LDS, no barrier),
+// and are joined once at the end.
+template <int D>
+__global__ __launch_bounds__(64 * kFewWaves) void kv_few_kernel(Queries q, KvCache c, KvSeqs s, float scale, int causal, Lists list,
+                                                                uint16_t* __restrict__ out, Partial part) {
+    constexpr int KL = D / 64;   // 16-byte pieces of a key row a lane
+    constexpr int NT = D / 16;   // tiles of 16 elements of the output
+    __shared__ float jo[kFewWaves][kFew][D + 4];
+    __shared__ float2 jml[kFewWaves][kFew];
+
+    const int split = blockIdx.x % part.splits;
+    const int nh = blockIdx.x / part.splits;
+    const int h = nh % c.heads, i = nh / c.heads;
+    const int group = q.heads / c.heads, queries = q.rows * group;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, col = lane & 15, quad = lane >> 4;
+
+    const int len = s.len(i), count = s.count(i, q.rows), start = s.end(i) - count;
+    const int row = col / group, hq = h * group + col % group;
+    auto last_of = [&](int r) {
+        int x = len - 1;
+        if (causal && start + r < x) x = start + r;
+        return r < count ? x : -1;
+    };
+    const int last = col < queries ? last_of(row) : -1;
+    const int most = count > 0 ? last_of(count - 1) : -1;
+    // below this every query that is one sees a whole block
+    const int full = count > 0 ? last_of(0) + 1 : 0;
+    const int blocks = most < 0 ? 0 : block_of(most) + 1;
+
+    bf16x8 qf[2 * KL];
+    {
+        const int64_t at = i * q.bs + static_cast<int64_t>(row) * q.ld + static_cast<int64_t>(hq) * D + quad * 16;
+#pragma unroll
+        for (int k = 0; k < 2 * KL; ++k)
+            qf[k] = frag(last >= 0 ? *reinterpret_cast<const uint4*>(q.p + at + (k >> 1) * 64 + (k & 1) * 8) : make_uint4(0, 0, 0, 0));
+    }
+    f32x4 o[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) o[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    float m = kLowest, l = 0.0f;
+
+    const int32_t* const mine = list.p ? list.p + (static_cast<int64_t>(i) * list.tiles * c.heads + h) * list.top : nullptr;
+    const int total = blocks == 0 ? 0 : mine ? list.top : blocks;
+    const int from = static_cast<int>(static_cast<int64_t>(total) * split / part.splits);
+    const int to = static_cast<int>(static_cast<int64_t>(total) * (split + 1) / part.splits);
+
+    uint4 kr[4][KL], vr[NT];
+    auto load_k = [&](int page) {
+        const int8_t* const p = c.k + (static_cast<int64_t>(page) * c.heads + h) * (kKvBlock * D);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int tok = 16 * (col >> 2) + 4 * u + (col & 3);
+#pragma unroll
+            for (int k = 0; k < KL; ++k) kr[u][k] = *reinterpret_cast<const uint4*>(p + tok * D + 64 * k + 16 * quad);
+        }
+    };
+    auto load_v = [&](int page) {
+        const int8_t* const p = c.v + (static_cast<int64_t>(page) * c.heads + h) * (kKvBlock * D);
+#pragma unroll
+        for (int d = 0; d < NT; ++d) vr[d] = *reinterpret_cast<const uint4*>(p + (16 * d + col) * kKvBlock + 16 * quad);
+    };
+
+    // a lane holds the page and the factors of one of the wave's next 64 blocks
+    for (int x0 = from; x0 < to; x0 += 64 * kFewWaves) {
+        const int x = x0 + lane * kFewWaves + wave;
+        const int b = x < to ? (mine ? mine[x] : x) : -1;
+        const int page = b >= 0 && b < blocks ? s.page(i, b, c.pages) : -1;
+        uint64_t left = __ballot(page >= 0);
+        if (!left) continue;
+        Factors f = {};
+        if (page >= 0) {
+            const int64_t p = static_cast<int64_t>(page) * c.heads + h;
+            f = factors(c.ks[p], c.vs[p], scale * kLog2e);
+        }
+        int y = __builtin_ctzll(left);
+        int now = __builtin_amdgcn_readlane(page, y);
+        load_k(now);
+        load_v(now);
+        while (left) {
+            left &= left - 1;
+            const int z = left ? __builtin_ctzll(left) : y;
+            const int next = __builtin_amdgcn_readlane(page, z);
+            const int base = __builtin_amdgcn_readlane(b, y) * kKvBlock;
+            const float fc = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f.c), y));
+            const float flv = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f.lv), y));
+            const float fiv = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f.iv), y));
+            const float fvs = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f.vs), y));
+            f32x4 sc[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                sc[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int k = 0; k < KL; ++k) {
+                    const uint4 w = kr[u][k];
+                    sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(frag(ints_bf16(make_uint2(w.x, w.y))), qf[2 * k], sc[u], 0, 0, 0);
+                    sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(frag(ints_bf16(make_uint2(w.z, w.w))), qf[2 * k + 1], sc[u], 0, 0, 0);
+                }
+            }
+            if (left) load_k(next);
+            // register r of sc[u]: token base + 16 quad + 4 u + r
+            float best = -__builtin_inff();
+            const bool mask = base + kKvBlock > full;
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    sc[u][r] *= fc;
+                    if (mask && base + 16 * quad + 4 * u + r > last) sc[u][r] = -__builtin_inff();
+                    best = fmaxf(best, sc[u][r]);
+                }
+            best = fmaxf(best, __shfl_xor(best, 16));
+            best = fmaxf(best, __shfl_xor(best, 32));
+            if (__any(best > m + kSlack)) {
+                const float mn = fmaxf(m, best), fix = exp2_hw(m - mn);
+                m = mn;
+                l *= fix;
+#pragma unroll
+                for (int d = 0; d < NT; ++d) o[d] *= fix;
+            }
+            const float off = flv - m;
+            float sum = 0.0f;
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    sc[u][r] = exp2_hw(sc[u][r] + off);
+                    sum += sc[u][r];
+                }
+            if (fiv != 0.0f) {
+                l = __builtin_fmaf(sum, fiv, l);
+            } else {
+                l += sum;
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) sc[u][r] = sc[u][r] == 0.0f ? 0.0f : sc[u][r] * fvs;
+            }
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                const f32x4 a = sc[2 * w], e = sc[2 * w + 1];
+                const bf16x8 p = frag(make_uint4(bf16x2_bits(a[0], a[1]), bf16x2_bits(a[2], a[3]), bf16x2_bits(e[0], e[1]), bf16x2_bits(e[2], e[3])));
+#pragma unroll
+                for (int d = 0; d < NT; ++d) {
+                    const uint2 v8 = w ? make_uint2(vr[d].z, vr[d].w) : make_uint2(vr[d].x, vr[d].y);
+                    o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(frag(ints_bf16(v8)), p, o[d], 0, 0, 0);
+                }
+            }
+            if (left) load_v(next);
+            y = z;
+        }
+    }
+
+    // register r of o[d]: element 16 d + 4 quad + r of query col
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (last < 0) {  // padding, or a row that sees nothing: what the registers hold is no result
+        l = 0.0f;
+#pragma unroll
+        for (int d = 0; d < NT; ++d) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    if (quad == 0) jml[wave][col] = make_float2(m, l);
+#pragma unroll
+    for (int d = 0; d < NT; ++d)
+        *reinterpret_cast<float4*>(&jo[wave][col][16 * d + 4 * quad]) = make_float4(o[d][0], o[d][1], o[d][2], o[d][3]);
+    __syncthreads();
+    for (int e = t; e < queries * (D / 4); e += 64 * kFewWaves) {
+        const int qn = e / (D / 4), d = e % (D / 4) * 4;
+        float top = kLowest;
+#pragma unroll
+        for (int w = 0; w < kFewWaves; ++w) top = fmaxf(top, jml[w][qn].x);
+        float sum = 0.0f, a[4] = {};
+#pragma unroll
+        for (int w = 0; w < kFewWaves; ++w) {
+            const float2 ml = jml[w][qn];
+            const float fix = exp2_hw(ml.x - top);
+            sum += ml.y * fix;
+            const float4 x = *reinterpret_cast<const float4*>(&jo[w][qn][d]);
+            a[0] += x.x * fix, a[1] += x.y * fix, a[2] += x.z * fix, a[3] += x.w * fix;
+        }
+        const int64_t query = (static_cast<int64_t>(i) * q.rows + qn / group) * q.heads + h * group + qn % group;
+        if (part.splits > 1) {
+            const int64_t at = split * part.queries + query;
+            if (d == 0) part.ml[at] = make_float2(top, sum);
+            *reinterpret_cast<float4*>(part.o + at * D + d) = make_float4(a[0], a[1], a[2], a[3]);
+        } else {
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            *reinterpret_cast<uint2*>(out + query * D + d) = make_uint2(bf16x2_bits(a[0] * inv, a[1] * inv), bf16x2_bits(a[2] * inv, a[3] * inv));
+        }
+    }
+}
+
+// ------------------------------------------------------------------ joining splits
+
+// D / 4 lanes a query.
+template <int D>
+__global__ __launch_bounds__(256) void kv_join_kernel(Partial part, uint16_t* __restrict__ out) {
+    constexpr int L = D / 4;
+    const int64_t query = static_cast<int64_t>(blockIdx.x) * (256 / L) + threadIdx.x / L;
+    const int d = threadIdx.x % L * 4;
+    if (query >= part.queries) return;
+    float top = kLowest;
+    for (int x = 0; x < part.splits; ++x) top = fmaxf(top, part.ml[x * part.queries + query].x);
+    float sum = 0.0f, a[4] = {};
+    for (int x = 0; x < part.splits; ++x) {
+        const int64_t at = x * part.queries + query;
+        const float2 ml = part.ml[at];
+        const float fix = exp2_hw(ml.x - top);
+        sum += ml.y * fix;
+        const float4 v = *reinterpret_cast<const float4*>(part.o + at * D + d);
+        a[0] += v.x * fix, a[1] += v.y * fix, a[2] += v.z * fix, a[3] += v.w * fix;
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    *reinterpret_cast<uint2*>(out + query * D + d) = make_uint2(bf16x2_bits(a[0] * inv, a[1] * inv), bf16x2_bits(a[2] * inv, a[3] * inv));
+}
+
+// ------------------------------------------------------------------ what a call runs
+
+struct Plan {
+    bool few;
+    int waves;       // of a tile's workgroup
+    int splits;
+    int64_t tiles, groups;
+};
+
+// Sizes checked by the caller.  blocks: the longest that a query's list or table is.
+Plan plan_of(int64_t n, int64_t rows, int64_t heads, int64_t kv, int64_t dim, int64_t blocks, int64_t top) {
+    Plan p = {};
+    const int64_t cus = cu_count(), longest = top > 0 ? top : blocks;
+    p.few = rows * (heads / kv) <= kFew;
+    int64_t want;  // workgroups that fill the card
+    int64_t least; // blocks of a split
+    if (p.few) {
+        p.groups = n * kv;
+        want = 4 * cus;
+        least = 2 * kFewWaves;
+    } else {
+        p.waves = dim == 256 || top > 0 || rows <= kKvTile ? 4 : 8;
+        p.tiles = (rows + 32 * p.waves - 1) / (32 * p.waves);
+        p.groups = n * heads * p.tiles;
+        want = (p.waves == 8 || dim == 256 ? 1 : 2) * cus;
+        least = 8;
+    }
+    int64_t splits = p.groups > 0 ? want / p.groups : 1;
+    if (splits > longest / least) splits = longest / least;
+    if (splits > 64) splits = 64;
+    p.splits = splits < 1 ? 1 : static_cast<int>(splits);
+    return p;
+}
+
+int64_t partial_bytes(const Plan& p, int64_t queries, int64_t dim) {
+    return p.splits > 1 ? p.splits * queries * (dim * 4 + 8) : 0;
+}
+
+bool sizes_ok(int64_t n, int64_t rows, int64_t heads, int64_t kv, int64_t dim, int64_t blocks, int64_t top) {
+    int64_t q;
+    return n >= 0 && rows >= 0 && heads > 0 && kv > 0 && heads % kv == 0 && heads <= 65536 && (dim == 64 || dim == 128 || dim == 256) &&
+           blocks >= 0 && top >= 0 && rows <= (1 << 30) && n <= 0x7FFFFFFF && !__builtin_mul_overflow(n, rows * heads, &q) && q < (int64_t{1} << 40);
 }
 
 }  // namespace
@@ -76,7 +593,29 @@ __global__ __launch_bounds__(64) void kv_attention_kernel(const uint16_t* __rest
 
 using namespace h3mi;
 
-extern "C" int64_t h3mi_kv_attention_workspace(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t) { return 0; }
+extern "C" int64_t h3mi_kv_attention_workspace(int64_t n, int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim, int64_t blocks,
+                                               int64_t top) {
+    if (!sizes_ok(n, rows, heads, kv_heads, dim, blocks, top) || n == 0 || rows == 0) return 0;
+    return partial_bytes(plan_of(n, rows, heads, kv_heads, dim, blocks, top), n * rows * heads, dim);
+}
+
+namespace {
+
+template <int D, int W>
+int launch_tiles(const Plan& p, const Queries& q, const KvCache& c, const KvSeqs& s, float scale, int causal, const Lists& list, uint16_t* out,
+                 const Partial& part, hipStream_t stream) {
+    int64_t items;
+    if (!launchable(p.groups + 8, p.splits, 1, 64 * W, &items)) return fail(H3MI_EINVAL, "kv_attention: too many rows for one call");
+    items = p.groups * p.splits;
+    const int64_t chunk = (items + 7) / 8;
+    const auto fn = kv_tile_kernel<D, W>;
+    constexpr int lds = TileShape<D, W>::kLds;
+    hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(chunk * 8)), dim3(64 * W), lds, stream, q, c, s, scale, causal, list, out, part,
+                       static_cast<int>(p.tiles), static_cast<int>(items), static_cast<int>(chunk));
+    return check_launch("kv_attention");
+}
+
+}  // namespace
 
 extern "C" int h3mi_kv_attention_bf16(const uint16_t* q, int64_t rows, int64_t heads, int64_t ld_q, int64_t bs_q,
                                       const h3mi_kv_cache* cache, const h3mi_kv_seqs* seqs, float scale, int causal,
@@ -87,16 +626,46 @@ extern "C" int h3mi_kv_attention_bf16(const uint16_t* q, int64_t rows, int64_t h
         return fail(H3MI_EINVAL, "kv_attention: heads=%lld must be a multiple of the cache's %lld", (long long)heads, (long long)cache->heads);
     if (int e = kv_check_rows("kv_attention", "q", q, rows, heads, cache->dim, seqs->n, ld_q, bs_q)) return e;
     if (!(scale == scale) || scale - scale != 0.0f) return fail(H3MI_EINVAL, "kv_attention: scale is not finite");
+    if (!blocks) top = 0;
     if (blocks && (top < 1 || top > 0x7FFFFFFF)) return fail(H3MI_EINVAL, "kv_attention: top=%lld", (long long)top);
     if (seqs->n == 0 || rows == 0) return ok();
     if (!out) return fail(H3MI_EINVAL, "kv_attention: null out");
     if (!aligned(out, 16) || !aligned(blocks, 4)) return fail(H3MI_EALIGN, "kv_attention: out must be 16-byte aligned, blocks 4-byte");
-    const int D = static_cast<int>(cache->dim);
+    const int64_t n = seqs->n, dim = cache->dim;
+    if (!sizes_ok(n, rows, heads, cache->heads, dim, seqs->blocks, top)) return fail(H3MI_EINVAL, "kv_attention: too many rows for one call");
+    const Plan p = plan_of(n, rows, heads, cache->heads, dim, seqs->blocks, top);
+    const int64_t queries = n * rows * heads, need = partial_bytes(p, queries, dim);
+    if (need > 0 && (!workspace || workspace_bytes < need))
+        return fail(H3MI_EINVAL, "kv_attention: workspace of %lld bytes, %lld needed", (long long)(workspace ? workspace_bytes : 0), (long long)need);
+    if (!aligned(workspace, 16)) return fail(H3MI_EALIGN, "kv_attention: workspace must be 16-byte aligned");
+    const Queries qs = {q, ld_q, bs_q, static_cast<int>(rows), static_cast<int>(heads)};
+    const Lists list = {blocks, static_cast<int>(top), static_cast<int>((rows + kKvTile - 1) / kKvTile)};
+    Partial part = {static_cast<float*>(workspace), nullptr, queries, p.splits};
+    if (need > 0) part.ml = reinterpret_cast<float2*>(part.o + p.splits * queries * dim);
+    const KvCache c = kv_cache(*cache);
+    const KvSeqs s = kv_seqs(*seqs);
+    const hipStream_t st = as_stream(stream);
+    int rc;
+    if (p.few) {
+        int64_t groups;
+        if (!launchable(p.groups, p.splits, 1, 64 * kFewWaves, &groups)) return fail(H3MI_EINVAL, "kv_attention: too many rows for one call");
+        const auto fn = dim == 64 ? kv_few_kernel<64> : dim == 128 ? kv_few_kernel<128> : kv_few_kernel<256>;
+        hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(groups)), dim3(64 * kFewWaves), 0, st, qs, c, s, scale, causal, list, out, part);
+        rc = check_launch("kv_attention");
+    } else if (dim == 64) {
+        rc = p.waves == 8 ? launch_tiles<64, 8>(p, qs, c, s, scale, causal, list, out, part, st)
+                          : launch_tiles<64, 4>(p, qs, c, s, scale, causal, list, out, part, st);
+    } else if (dim == 128) {
+        rc = p.waves == 8 ? launch_tiles<128, 8>(p, qs, c, s, scale, causal, list, out, part, st)
+                          : launch_tiles<128, 4>(p, qs, c, s, scale, causal, list, out, part, st);
+    } else {
+        rc = launch_tiles<256, 4>(p, qs, c, s, scale, causal, list, out, part, st);
+    }
+    if (rc || p.splits == 1) return rc;
+    const int per = static_cast<int>(256 / (dim / 4));
     int64_t groups;
-    if (!launchable(seqs->n, rows, heads, 64, &groups)) return fail(H3MI_EINVAL, "kv_attention: too many rows for one call");
-    const auto fn = D == 64 ? kv_attention_kernel<64> : D == 128 ? kv_attention_kernel<128> : kv_attention_kernel<256>;
-    hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(groups)), dim3(64), 0, as_stream(stream), q, ld_q, bs_q, kv_cache(*cache),
-                       kv_seqs(*seqs), static_cast<int>(rows), static_cast<int>(heads), scale, causal, blocks,
-                       static_cast<int>(top), out);
+    if (!launchable((queries + per - 1) / per, 1, 1, 256, &groups)) return fail(H3MI_EINVAL, "kv_attention: too many rows for one call");
+    const auto join = dim == 64 ? kv_join_kernel<64> : dim == 128 ? kv_join_kernel<128> : kv_join_kernel<256>;
+    hipLaunchKernelGGL(join, dim3(static_cast<unsigned>(groups)), dim3(256), 0, st, part, out);
     return check_launch("kv_attention");
 }
