@@ -18,7 +18,10 @@
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/GradMode.h>
+#include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
+#include <math.h>
 #include <stdlib.h>
 #include <string.h>
 #include <torch/csrc/Exceptions.h>
@@ -368,6 +371,182 @@ PyObject* rms_rope_(PyObject*, PyObject* const* v, Py_ssize_t n) {
     H3MI_END
 }
 
+// A KVCache and the sequences of a call.
+struct Kv {
+    h3mi_kv_cache c = {};
+    h3mi_kv_seqs s = {};
+    Kv(Args& a, PyObject* cache, PyObject* tables, PyObject* lens, PyObject* counts) {
+        if (!a.ok) return;
+        a.ok = false;
+        if (!PyTuple_Check(cache) || PyTuple_GET_SIZE(cache) != 5) return;
+        a.ok = true;
+        const at::Tensor* k = a.typed(PyTuple_GET_ITEM(cache, 0), c10::kChar);
+        if (!a.ok || k->dim() != 4 || k->size(2) != H3MI_KV_BLOCK || !k->is_contiguous()) {
+            a.ok = false;
+            return;
+        }
+        const int64_t P = k->size(0), H = k->size(1), D = k->size(3);
+        const at::Tensor* v = shaped(a, PyTuple_GET_ITEM(cache, 1), c10::kChar, {P, H, D, H3MI_KV_BLOCK});
+        const at::Tensor* ks = shaped(a, PyTuple_GET_ITEM(cache, 2), c10::kFloat, {P, H});
+        const at::Tensor* vs = shaped(a, PyTuple_GET_ITEM(cache, 3), c10::kFloat, {P, H});
+        const at::Tensor* sum = shaped(a, PyTuple_GET_ITEM(cache, 4), c10::kShort, {P, H, D});
+        const at::Tensor* tab = a.typed(tables, c10::kInt);
+        if (!a.ok || tab->dim() != 2 || !tab->is_contiguous() || a.dev.index() != c10::hip::current_device()) {
+            a.ok = false;
+            return;
+        }
+        const at::Tensor* l = shaped(a, lens, c10::kInt, {tab->size(0)});
+        const at::Tensor* n = counts == Py_None ? nullptr : shaped(a, counts, c10::kInt, {tab->size(0)});
+        if (!a.ok) return;
+        c = {i8(k), i8(v), mf32(ks), mf32(vs), static_cast<int16_t*>(sum->data_ptr()), P, H, D};
+        s = {i32(tab), i32(l), n ? i32(n) : nullptr, tab->size(0), tab->size(1)};
+    }
+    static const at::Tensor* shaped(Args& a, PyObject* o, c10::ScalarType type, std::initializer_list<int64_t> size) {
+        const at::Tensor* t = a.typed(o, type);
+        if (t && (t->sizes() != at::IntArrayRef(size) || !t->is_contiguous())) a.ok = false;
+        return t;
+    }
+    static int8_t* i8(const at::Tensor* t) { return static_cast<int8_t*>(t->data_ptr()); }
+    static float* mf32(const at::Tensor* t) { return static_cast<float*>(t->data_ptr()); }
+    static const int32_t* i32(const at::Tensor* t) { return static_cast<const int32_t*>(t->data_ptr()); }
+};
+
+// [n, rows, heads, dim] with contiguous heads, that no gradient is wanted of
+struct KvRows {
+    const at::Tensor* t;
+    int64_t rows = 0, heads = 0, ld = 0, bs = 0;
+    KvRows(Args& a, PyObject* o, const Kv& kv) {
+        t = a.typed(o, c10::kBFloat16);
+        if (!a.ok) return;
+        const int64_t D = kv.c.dim;
+        if (t->dim() != 4 || t->size(0) != kv.s.n || t->size(3) != D || t->stride(3) != 1 || (t->size(2) > 1 && t->stride(2) != D) ||
+            (t->requires_grad() && c10::GradMode::is_enabled())) {
+            a.ok = false;
+            return;
+        }
+        rows = t->size(1), heads = t->size(2);
+        ld = rows > 1 ? t->stride(1) : heads * D;
+        bs = kv.s.n > 1 ? t->stride(0) : rows * heads * D;
+    }
+};
+
+bool truth(PyObject* o, int* v) {
+    *v = o == Py_True;
+    return o == Py_True || o == Py_False;
+}
+
+bool whole(PyObject* o, int64_t* v) {
+    if (!PyLong_CheckExact(o)) return false;
+    *v = PyLong_AsLongLong(o);
+    if (*v != -1 || !PyErr_Occurred()) return true;
+    PyErr_Clear();
+    return false;
+}
+
+// (cache, k, v, tables, lens, counts) -> cache
+PyObject* kv_write_(PyObject*, PyObject* const* v, Py_ssize_t n) {
+    H3MI_BEGIN
+    H3MI_ARGS(6)
+    Args a;
+    const Kv kv(a, v[0], v[3], v[4], v[5]);
+    if (!a.ok) Py_RETURN_NONE;
+    const KvRows k(a, v[1], kv);
+    const KvRows x(a, v[2], kv);
+    if (!a.ok || k.heads != kv.c.heads || x.heads != kv.c.heads || k.rows != x.rows) Py_RETURN_NONE;
+    int rc;
+    {
+        pybind11::gil_scoped_release nogil;
+        rc = h3mi_kv_write_i8(u16(k.t), u16(x.t), k.rows, k.ld, k.bs, x.ld, x.bs, &kv.c, &kv.s, a.stream());
+    }
+    if (rc) return raise_status(rc);
+    Py_INCREF(v[0]);
+    return v[0];
+    H3MI_END
+}
+
+// (cache, tables, lens, length, starts) -> (k, v)
+PyObject* kv_read(PyObject*, PyObject* const* v, Py_ssize_t n) {
+    H3MI_BEGIN
+    H3MI_ARGS(5)
+    Args a;
+    const Kv kv(a, v[0], v[1], v[2], Py_None);
+    int64_t length = 0;
+    if (!a.ok || !whole(v[3], &length) || length < 0) Py_RETURN_NONE;
+    const at::Tensor* starts = v[4] == Py_None ? nullptr : Kv::shaped(a, v[4], c10::kInt, {kv.s.n});
+    if (!a.ok) Py_RETURN_NONE;
+    at::Tensor k, x;
+    int rc;
+    {
+        pybind11::gil_scoped_release nogil;
+        k = a.empty({kv.s.n, length, kv.c.heads, kv.c.dim}, c10::kBFloat16);
+        x = a.empty({kv.s.n, length, kv.c.heads, kv.c.dim}, c10::kBFloat16);
+        rc = h3mi_kv_read_bf16(mu16(k), mu16(x), starts ? Kv::i32(starts) : nullptr, length, &kv.c, &kv.s, a.stream());
+    }
+    return rc ? raise_status(rc) : pair(k, x);
+    H3MI_END
+}
+
+// (q, cache, tables, lens, top, causal, counts) -> blocks
+PyObject* kv_select(PyObject*, PyObject* const* v, Py_ssize_t n) {
+    H3MI_BEGIN
+    H3MI_ARGS(7)
+    Args a;
+    const Kv kv(a, v[1], v[2], v[3], v[6]);
+    if (!a.ok) Py_RETURN_NONE;
+    const KvRows q(a, v[0], kv);
+    int64_t top = 0;
+    int causal = 0;
+    if (!a.ok || !whole(v[4], &top) || top < 1 || !truth(v[5], &causal)) Py_RETURN_NONE;
+    at::Tensor out;
+    int rc;
+    {
+        pybind11::gil_scoped_release nogil;
+        out = a.empty({kv.s.n, (q.rows + H3MI_KV_TILE - 1) / H3MI_KV_TILE, kv.c.heads, top}, c10::kInt);
+        rc = h3mi_kv_select(u16(q.t), q.rows, q.heads, q.ld, q.bs, &kv.c, &kv.s, top, causal, static_cast<int32_t*>(out.data_ptr()),
+                            a.stream());
+    }
+    return rc ? raise_status(rc) : THPVariable_Wrap(out);
+    H3MI_END
+}
+
+// (q, cache, tables, lens, causal, counts, scale, blocks) -> out
+PyObject* kv_attention(PyObject*, PyObject* const* v, Py_ssize_t n) {
+    H3MI_BEGIN
+    H3MI_ARGS(8)
+    Args a;
+    const Kv kv(a, v[1], v[2], v[3], v[5]);
+    if (!a.ok) Py_RETURN_NONE;
+    const KvRows q(a, v[0], kv);
+    int causal = 0;
+    double scale = 0.0;
+    if (!a.ok || !truth(v[4], &causal)) Py_RETURN_NONE;
+    if (v[6] == Py_None)
+        scale = 1.0 / sqrt(static_cast<double>(kv.c.dim));
+    else if (!number(v[6], &scale))
+        Py_RETURN_NONE;
+    const at::Tensor* list = nullptr;
+    int64_t top = 0;
+    if (v[7] != Py_None) {
+        list = a.typed(v[7], c10::kInt);
+        if (!a.ok || list->dim() != 4 || !list->is_contiguous() || list->size(0) != kv.s.n ||
+            list->size(1) != (q.rows + H3MI_KV_TILE - 1) / H3MI_KV_TILE || list->size(2) != kv.c.heads)
+            Py_RETURN_NONE;
+        top = list->size(3);
+    }
+    at::Tensor out, work;
+    int rc;
+    {
+        pybind11::gil_scoped_release nogil;
+        out = a.empty(q.t->sizes(), c10::kBFloat16);
+        const int64_t need = h3mi_kv_attention_workspace(kv.s.n, q.rows, q.heads, kv.c.heads, kv.c.dim, kv.s.blocks, top);
+        if (need > 0) work = a.empty({need}, c10::kByte);
+        rc = h3mi_kv_attention_bf16(u16(q.t), q.rows, q.heads, q.ld, q.bs, &kv.c, &kv.s, static_cast<float>(scale), causal,
+                                    list ? Kv::i32(list) : nullptr, top, mu16(out), need > 0 ? work.data_ptr() : nullptr, need, a.stream());
+    }
+    return rc ? raise_status(rc) : THPVariable_Wrap(out);
+    H3MI_END
+}
+
 // (set,): set False forgets the last GEMM's shape; returns it, or None
 PyObject* last_shape(PyObject*, PyObject* const* v, Py_ssize_t n) {
     H3MI_ARGS(1)
@@ -388,7 +567,8 @@ PyObject* set_error(PyObject*, PyObject* cls) {
 PyMethodDef kMethods[] = {
     H3MI_FN("w8a8_linear", &w8a8_linear), H3MI_FN("int8_mm_scaled", &int8_mm_scaled), H3MI_FN("quantize", &quantize),
     H3MI_FN("norm_mod", &norm_any<false>), H3MI_FN("gate_norm_mod_", &norm_any<true>), H3MI_FN("gate_", &gate_),
-    H3MI_FN("rms_rope_", &rms_rope_), H3MI_FN("last_shape", &last_shape),
+    H3MI_FN("rms_rope_", &rms_rope_), H3MI_FN("last_shape", &last_shape), H3MI_FN("kv_write_", &kv_write_),
+    H3MI_FN("kv_read", &kv_read), H3MI_FN("kv_select", &kv_select), H3MI_FN("kv_attention", &kv_attention),
     {"set_error", set_error, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_fast", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

@@ -26,7 +26,7 @@ import typing
 
 import torch
 
-from ._lib import KvCacheC, KvSeqsC, check, lib, ptr, same_gpu, stream_of
+from ._lib import KvCacheC, KvSeqsC, _fast, check, lib, ptr, same_gpu, stream_of
 
 KV_BLOCK = 64   # tokens of a block, one scale per block and head, and of a page
 KV_TILE = 128   # query rows that share a selection
@@ -48,6 +48,11 @@ def kv_cache(pages, heads, dim, device="cuda"):
     z = lambda *s, t: torch.zeros(*s, dtype=t, device=device)  # noqa: E731
     return KVCache(z(pages, heads, KV_BLOCK, dim, t=torch.int8), z(pages, heads, dim, KV_BLOCK, t=torch.int8),
                    z(pages, heads, t=torch.float32), z(pages, heads, t=torch.float32), z(pages, heads, dim, t=torch.int16))
+
+
+# The functions below first offer the call to native code, which takes it in the
+# plain form (csrc/fastcall.cpp) or returns None; the checks here then decide every
+# other form.
 
 
 def _cache(c):
@@ -106,6 +111,9 @@ def kv_write_(cache, k, v, tables, lens, counts=None):
     A block's scale is max|x| / 127 of its first write.  A later write of tokens that do not fit doubles it as often
     as they need and halves the block's older 8-bit values as often, so that an error stays within one step.  A NaN or
     an infinity makes its block read back as NaN.  The pages that a call writes have to be distinct."""
+    done = _fast.kv_write_(cache, k, v, tables, lens, counts)
+    if done is not None:
+        return done
     _no_grad(k, v)
     c = _cache(cache)
     s = _seqs(cache, tables, lens, counts)
@@ -120,6 +128,9 @@ def kv_write_(cache, k, v, tables, lens, counts=None):
 
 def kv_read(cache, tables, lens, length, starts=None):
     """(k, v) bf16 [n, length, heads, dim]: tokens starts[i] (default 0) on of each sequence, zeros where it has none."""
+    got = _fast.kv_read(cache, tables, lens, length, starts)
+    if got is not None:
+        return got
     c = _cache(cache)
     s = _seqs(cache, tables, lens, None)
     _ints(starts, (s.n,), "starts")
@@ -141,6 +152,9 @@ def kv_select(q, cache, tables, lens, top, causal=False, counts=None):
     A block's score is the product of its mean key with the mean of the tile's queries (of all heads that share the kv
     head), formed from 8-bit keys and 11-bit queries in whole numbers.  With causal, the blocks of the tile's own tokens
     are taken first and later ones never.  Equal scores go to the lowest block."""
+    out = _fast.kv_select(q, cache, tables, lens, top, causal, counts)
+    if out is not None:
+        return out
     _no_grad(q)
     c = _cache(cache)
     s = _seqs(cache, tables, lens, counts)
@@ -159,6 +173,9 @@ def kv_attention(q, cache, tables, lens, causal=False, counts=None, scale=None, 
     q bf16 [n, rows, heads, dim]; query head h reads kv head h / (heads / kv heads); scale defaults to dim ** -0.5.
     causal: a row sees tokens up to its own.  blocks (from kv_select, or any distinct ones in its shape): a row sees the
     tokens of its tile's blocks alone.  Rows that see no token, and padding rows, are 0."""
+    out = _fast.kv_attention(q, cache, tables, lens, causal, counts, scale, blocks)
+    if out is not None:
+        return out
     _no_grad(q)
     c = _cache(cache)
     s = _seqs(cache, tables, lens, counts)
