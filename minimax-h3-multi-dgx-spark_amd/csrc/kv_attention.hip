@@ -74,12 +74,13 @@ struct Lists {
     int top, tiles;
 };
 
-// Partial results of a split: per (split, query) dim sums, and (m, l).
+// Partial results of the items whose blocks are split: for each (item, split, row of the
+// item) dim sums, and (m, l).  A split without a token writes l = 0 and no sums.
 struct Partial {
     float* o;
     float2* ml;
-    int64_t queries;  // n rows heads
-    int splits;
+    int splits, rows;  // of an item
+    __device__ __forceinline__ int64_t at(int64_t item, int split, int row) const { return (item * splits + split) * rows + row; }
 };
 
 // ------------------------------------------------------------------ tiles of queries
@@ -99,10 +100,28 @@ struct TileShape {
     static constexpr int kLoads = kKvBlock * D / 8 / kThreads;  // 8-byte pieces of K (and of V) a thread
 };
 
+// The items (tiles of a head, heads of a sequence) of a launch: the first `whole` take one
+// workgroup each, a multiple of what the card holds at once; the rest, which would leave a
+// last round part empty, are split over their blocks to fill it.
+struct Grid {
+    int tiles, items, whole, chunk, rest_chunk;
+    // Consecutive items on one XCD, whose L2 then holds their head's blocks.
+    __device__ __forceinline__ int item(int block, int tail_splits, int& split, int& splits) const {
+        if (block < whole) {
+            split = 0, splits = 1;
+            return (block & 7) * chunk + (block >> 3);
+        }
+        const int x = ((block - whole) & 7) * rest_chunk + ((block - whole) >> 3);
+        splits = tail_splits;
+        split = x % splits;
+        return whole + x / splits;
+    }
+};
+
 template <int D, int W>
 __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv_tile_kernel(Queries q, KvCache c, KvSeqs s, float scale, int causal,
                                                                           Lists list, uint16_t* __restrict__ out, Partial part,
-                                                                          int tiles, int items, int chunk) {
+                                                                          Grid grid) {
     using T = TileShape<D, W>;
     constexpr int NT = D / 32;            // tiles of 32 elements of the output
     constexpr int KC = D / 8, VC = 8;     // 16-byte chunks of a row of K, of V
@@ -111,13 +130,12 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv_tile_kernel(Queri
     __shared__ float4 fact[T::kThreads];
     __shared__ int wcount[W];
 
-    // Consecutive items (tiles and splits of a head) on one XCD, whose L2 then holds the head's blocks.
-    const int item = (blockIdx.x & 7) * chunk + (blockIdx.x >> 3);
-    if (item >= items) return;
-    const int split = item % part.splits, tile_rev = item / part.splits % tiles;
-    const int nh = item / part.splits / tiles;
+    int split, splits;
+    const int item = grid.item(blockIdx.x, part.splits, split, splits);
+    if (item >= grid.items) return;
+    const int nh = item / grid.tiles;
     const int hq = nh % q.heads, i = nh / q.heads, h = hq / (q.heads / c.heads);
-    const int tile = causal ? tiles - 1 - tile_rev : tile_rev;  // the longest first
+    const int tile = causal ? grid.tiles - 1 - item % grid.tiles : item % grid.tiles;  // the longest first
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, col = lane & 31, half = lane >> 5;
 
     const int len = s.len(i), count = s.count(i, q.rows), start = s.end(i) - count;
@@ -154,8 +172,8 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv_tile_kernel(Queri
     const int32_t* const mine =
         list.p ? list.p + ((static_cast<int64_t>(i) * list.tiles + r0 / kKvTile) * c.heads + h) * list.top : nullptr;
     const int total = blocks == 0 ? 0 : mine ? list.top : blocks;
-    const int from = static_cast<int>(static_cast<int64_t>(total) * split / part.splits);
-    const int to = static_cast<int>(static_cast<int64_t>(total) * (split + 1) / part.splits);
+    const int from = static_cast<int>(static_cast<int64_t>(total) * split / splits);
+    const int to = static_cast<int>(static_cast<int64_t>(total) * (split + 1) / splits);
 
     uint2 kr[T::kLoads], vr[T::kLoads];
     auto load = [&](int page) {
@@ -303,9 +321,10 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv_tile_kernel(Queri
     }
     const int64_t query = (static_cast<int64_t>(i) * q.rows + row) * q.heads + hq;
     // register r of o[d]: element 32 d + 8 (r / 4) + 4 half + r % 4 of the query's output
-    if (part.splits > 1) {
-        const int64_t at = split * part.queries + query;
+    if (splits > 1) {
+        const int64_t at = part.at(item - grid.whole, split, row - r0);
         if (half == 0) part.ml[at] = make_float2(m, l);
+        if (from >= to) return;
 #pragma unroll
         for (int d = 0; d < NT; ++d)
 #pragma unroll
@@ -333,7 +352,7 @@ constexpr int kFewWaves = 4;
 // and are joined once at the end.
 template <int D>
 __global__ __launch_bounds__(64 * kFewWaves) void kv_few_kernel(Queries q, KvCache c, KvSeqs s, float scale, int causal, Lists list,
-                                                                uint16_t* __restrict__ out, Partial part) {
+                                                                uint16_t* __restrict__ out, Partial part, int per) {
     constexpr int KL = D / 64;   // 16-byte pieces of a key row a lane
     constexpr int NT = D / 16;   // tiles of 16 elements of the output
     __shared__ float jo[kFewWaves][kFew][D + 4];
@@ -372,8 +391,13 @@ __global__ __launch_bounds__(64 * kFewWaves) void kv_few_kernel(Queries q, KvCac
 
     const int32_t* const mine = list.p ? list.p + (static_cast<int64_t>(i) * list.tiles * c.heads + h) * list.top : nullptr;
     const int total = blocks == 0 ? 0 : mine ? list.top : blocks;
-    const int from = static_cast<int>(static_cast<int64_t>(total) * split / part.splits);
-    const int to = static_cast<int>(static_cast<int64_t>(total) * (split + 1) / part.splits);
+    // splits of a fixed length, so that those of uneven sequences are even
+    const int from = split * per < total ? split * per : total;
+    const int to = from + per < total ? from + per : total;
+    if (part.splits > 1 && from >= to) {
+        if (t < queries) part.ml[part.at(nh, split, t)] = make_float2(kLowest, 0.0f);
+        return;
+    }
 
     uint4 kr[4][KL], vr[NT];
     auto load_k = [&](int page) {
@@ -510,7 +534,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void kv_few_kernel(Queries q, KvCac
         }
         const int64_t query = (static_cast<int64_t>(i) * q.rows + qn / group) * q.heads + h * group + qn % group;
         if (part.splits > 1) {
-            const int64_t at = split * part.queries + query;
+            const int64_t at = part.at(nh, split, qn);
             if (d == 0) part.ml[at] = make_float2(top, sum);
             *reinterpret_cast<float4*>(part.o + at * D + d) = make_float4(a[0], a[1], a[2], a[3]);
         } else {
@@ -522,35 +546,69 @@ __global__ __launch_bounds__(64 * kFewWaves) void kv_few_kernel(Queries q, KvCac
 
 // ------------------------------------------------------------------ joining splits
 
-// D / 4 lanes a query.
+constexpr int kMaxSplits = 64;  // a lane of the join's wave each
+
+// A wave a row of an item: D / 4 lanes a row of sums, 256 / D splits at once.
 template <int D>
-__global__ __launch_bounds__(256) void kv_join_kernel(Partial part, uint16_t* __restrict__ out) {
-    constexpr int L = D / 4;
-    const int64_t query = static_cast<int64_t>(blockIdx.x) * (256 / L) + threadIdx.x / L;
-    const int d = threadIdx.x % L * 4;
-    if (query >= part.queries) return;
-    float top = kLowest;
-    for (int x = 0; x < part.splits; ++x) top = fmaxf(top, part.ml[x * part.queries + query].x);
-    float sum = 0.0f, a[4] = {};
-    for (int x = 0; x < part.splits; ++x) {
-        const int64_t at = x * part.queries + query;
-        const float2 ml = part.ml[at];
-        const float fix = exp2_hw(ml.x - top);
-        sum += ml.y * fix;
-        const float4 v = *reinterpret_cast<const float4*>(part.o + at * D + d);
-        a[0] += v.x * fix, a[1] += v.y * fix, a[2] += v.z * fix, a[3] += v.w * fix;
+__global__ __launch_bounds__(256) void kv_join_kernel(Partial part, Queries q, int kv_heads, int tiles, int whole, int causal, int64_t all,
+                                                      uint16_t* __restrict__ out) {
+    constexpr int L = D / 4, SG = 64 / L;
+    const int64_t x = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    if (x >= all) return;
+    const int lane = threadIdx.x & 63, d = lane % L * 4, sg = lane / L;
+    const int64_t item = x / part.rows;
+    const int r = static_cast<int>(x % part.rows);
+    int64_t query;
+    if (tiles == 0) {  // a kv head's group: its queries in the order of rows, then heads
+        const int group = q.heads / kv_heads;
+        query = (item / kv_heads * q.rows + r / group) * q.heads + item % kv_heads * group + r % group;
+    } else {
+        const int64_t nh = (whole + item) / tiles;
+        const int tile = static_cast<int>((whole + item) % tiles);
+        const int row = (causal ? tiles - 1 - tile : tile) * part.rows + r;
+        if (row >= q.rows) return;
+        query = (nh / q.heads * q.rows + row) * q.heads + nh % q.heads;
     }
+    const float2 ml = lane < part.splits ? part.ml[part.at(item, lane, r)] : make_float2(kLowest, 0.0f);
+    float top = ml.x;
+#pragma unroll
+    for (int y = 32; y; y >>= 1) top = fmaxf(top, __shfl_xor(top, y));
+    const float fix = ml.y == 0.0f ? 0.0f : exp2_hw(ml.x - top);
+    float sum = ml.y * fix;
+#pragma unroll
+    for (int y = 32; y; y >>= 1) sum += __shfl_xor(sum, y);
+    float a[4] = {};
+    for (int y = 0; y < part.splits; y += 4 * SG) {
+        float f[4];
+        float4 v[4];
+#pragma unroll
+        for (int z = 0; z < 4; ++z) {
+            const int sp = y + z * SG + sg;
+            f[z] = __shfl(fix, sp & 63);
+            if (sp >= part.splits) f[z] = 0.0f;
+            v[z] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (f[z] != 0.0f) v[z] = *reinterpret_cast<const float4*>(part.o + part.at(item, sp, r) * D + d);
+        }
+#pragma unroll
+        for (int z = 0; z < 4; ++z) a[0] += v[z].x * f[z], a[1] += v[z].y * f[z], a[2] += v[z].z * f[z], a[3] += v[z].w * f[z];
+    }
+#pragma unroll
+    for (int y = 32; y >= L; y >>= 1)
+#pragma unroll
+        for (int z = 0; z < 4; ++z) a[z] += __shfl_xor(a[z], y);
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    *reinterpret_cast<uint2*>(out + query * D + d) = make_uint2(bf16x2_bits(a[0] * inv, a[1] * inv), bf16x2_bits(a[2] * inv, a[3] * inv));
+    if (sg == 0)
+        *reinterpret_cast<uint2*>(out + query * D + d) = make_uint2(bf16x2_bits(a[0] * inv, a[1] * inv), bf16x2_bits(a[2] * inv, a[3] * inv));
 }
 
 // ------------------------------------------------------------------ what a call runs
 
 struct Plan {
     bool few;
-    int waves;       // of a tile's workgroup
-    int splits;
-    int64_t tiles, groups;
+    int waves;          // of a tile's workgroup
+    int splits, per;    // of a split item; blocks of a split (few)
+    int64_t tiles, items, whole;  // items of one workgroup each come first
+    int64_t part_items() const { return splits > 1 ? items - whole : 0; }
 };
 
 // Sizes checked by the caller.  blocks: the longest that a query's list or table is.
@@ -558,29 +616,35 @@ Plan plan_of(int64_t n, int64_t rows, int64_t heads, int64_t kv, int64_t dim, in
     Plan p = {};
     const int64_t cus = cu_count(), longest = top > 0 ? top : blocks;
     p.few = rows * (heads / kv) <= kFew;
-    int64_t want;  // workgroups that fill the card
-    int64_t least; // blocks of a split
     if (p.few) {
-        p.groups = n * kv;
-        want = 4 * cus;
-        least = 2 * kFewWaves;
-    } else {
-        p.waves = dim == 256 || top > 0 || rows <= kKvTile ? 4 : 8;
-        p.tiles = (rows + 32 * p.waves - 1) / (32 * p.waves);
-        p.groups = n * heads * p.tiles;
-        want = (p.waves == 8 || dim == 256 ? 1 : 2) * cus;
-        least = 8;
+        p.items = n * kv;
+        int64_t splits = 4 * cus / p.items;
+        if (splits > longest / (2 * kFewWaves)) splits = longest / (2 * kFewWaves);
+        if (splits > kMaxSplits) splits = kMaxSplits;
+        if (splits < 1) splits = 1;
+        p.per = static_cast<int>((longest + splits - 1) / splits);
+        p.splits = p.per > 0 ? static_cast<int>((longest + p.per - 1) / p.per) : 1;
+        if (p.splits < 1) p.splits = 1;
+        return p;
     }
-    int64_t splits = p.groups > 0 ? want / p.groups : 1;
-    if (splits > longest / least) splits = longest / least;
-    if (splits > 64) splits = 64;
-    p.splits = splits < 1 ? 1 : static_cast<int>(splits);
+    const int64_t tiles8 = (rows + 255) / 256;
+    p.waves = dim == 256 || top > 0 || n * heads * tiles8 < cus ? 4 : 8;
+    p.tiles = p.waves == 8 ? tiles8 : (rows + 127) / 128;
+    p.items = n * heads * p.tiles;
+    const int64_t slots = (p.waves == 8 || dim == 256 ? 1 : 2) * cus;
+    p.whole = p.items / slots * slots;
+    const int64_t rest = p.items - p.whole;
+    int64_t splits = rest > 0 ? slots / rest : 1;
+    if (splits > longest / 8) splits = longest / 8;
+    if (splits > kMaxSplits) splits = kMaxSplits;
+    if (splits <= 1) p.whole = p.items / 8 * 8, splits = 1;
+    p.splits = static_cast<int>(splits);
     return p;
 }
 
-int64_t partial_bytes(const Plan& p, int64_t queries, int64_t dim) {
-    return p.splits > 1 ? p.splits * queries * (dim * 4 + 8) : 0;
-}
+int64_t item_rows(const Plan& p, int64_t rows, int64_t group) { return p.few ? rows * group : 32 * p.waves; }
+
+int64_t partial_rows(const Plan& p, int64_t rows, int64_t group) { return p.part_items() * p.splits * item_rows(p, rows, group); }
 
 bool sizes_ok(int64_t n, int64_t rows, int64_t heads, int64_t kv, int64_t dim, int64_t blocks, int64_t top) {
     int64_t q;
@@ -596,7 +660,7 @@ using namespace h3mi;
 extern "C" int64_t h3mi_kv_attention_workspace(int64_t n, int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim, int64_t blocks,
                                                int64_t top) {
     if (!sizes_ok(n, rows, heads, kv_heads, dim, blocks, top) || n == 0 || rows == 0) return 0;
-    return partial_bytes(plan_of(n, rows, heads, kv_heads, dim, blocks, top), n * rows * heads, dim);
+    return partial_rows(plan_of(n, rows, heads, kv_heads, dim, blocks, top), rows, heads / kv_heads) * (dim * 4 + 8);
 }
 
 namespace {
@@ -604,14 +668,14 @@ namespace {
 template <int D, int W>
 int launch_tiles(const Plan& p, const Queries& q, const KvCache& c, const KvSeqs& s, float scale, int causal, const Lists& list, uint16_t* out,
                  const Partial& part, hipStream_t stream) {
-    int64_t items;
-    if (!launchable(p.groups + 8, p.splits, 1, 64 * W, &items)) return fail(H3MI_EINVAL, "kv_attention: too many rows for one call");
-    items = p.groups * p.splits;
-    const int64_t chunk = (items + 7) / 8;
+    const int64_t rest = (p.items - p.whole) * p.splits, rest_chunk = (rest + 7) / 8;
+    int64_t groups;
+    if (!launchable(p.whole + rest_chunk * 8, 1, 1, 64 * W, &groups)) return fail(H3MI_EINVAL, "kv_attention: too many rows for one call");
+    const Grid grid = {static_cast<int>(p.tiles), static_cast<int>(p.items), static_cast<int>(p.whole), static_cast<int>(p.whole / 8),
+                       static_cast<int>(rest_chunk)};
     const auto fn = kv_tile_kernel<D, W>;
     constexpr int lds = TileShape<D, W>::kLds;
-    hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(chunk * 8)), dim3(64 * W), lds, stream, q, c, s, scale, causal, list, out, part,
-                       static_cast<int>(p.tiles), static_cast<int>(items), static_cast<int>(chunk));
+    hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(groups)), dim3(64 * W), lds, stream, q, c, s, scale, causal, list, out, part, grid);
     return check_launch("kv_attention");
 }
 
@@ -634,23 +698,24 @@ extern "C" int h3mi_kv_attention_bf16(const uint16_t* q, int64_t rows, int64_t h
     const int64_t n = seqs->n, dim = cache->dim;
     if (!sizes_ok(n, rows, heads, cache->heads, dim, seqs->blocks, top)) return fail(H3MI_EINVAL, "kv_attention: too many rows for one call");
     const Plan p = plan_of(n, rows, heads, cache->heads, dim, seqs->blocks, top);
-    const int64_t queries = n * rows * heads, need = partial_bytes(p, queries, dim);
+    const int64_t group = heads / cache->heads, part_rows = partial_rows(p, rows, group), need = part_rows * (dim * 4 + 8);
     if (need > 0 && (!workspace || workspace_bytes < need))
         return fail(H3MI_EINVAL, "kv_attention: workspace of %lld bytes, %lld needed", (long long)(workspace ? workspace_bytes : 0), (long long)need);
     if (!aligned(workspace, 16)) return fail(H3MI_EALIGN, "kv_attention: workspace must be 16-byte aligned");
     const Queries qs = {q, ld_q, bs_q, static_cast<int>(rows), static_cast<int>(heads)};
     const Lists list = {blocks, static_cast<int>(top), static_cast<int>((rows + kKvTile - 1) / kKvTile)};
-    Partial part = {static_cast<float*>(workspace), nullptr, queries, p.splits};
-    if (need > 0) part.ml = reinterpret_cast<float2*>(part.o + p.splits * queries * dim);
+    Partial part = {static_cast<float*>(workspace), nullptr, p.splits, static_cast<int>(item_rows(p, rows, group))};
+    if (need > 0) part.ml = reinterpret_cast<float2*>(part.o + part_rows * dim);
     const KvCache c = kv_cache(*cache);
     const KvSeqs s = kv_seqs(*seqs);
     const hipStream_t st = as_stream(stream);
     int rc;
     if (p.few) {
         int64_t groups;
-        if (!launchable(p.groups, p.splits, 1, 64 * kFewWaves, &groups)) return fail(H3MI_EINVAL, "kv_attention: too many rows for one call");
+        if (!launchable(p.items, p.splits, 1, 64 * kFewWaves, &groups)) return fail(H3MI_EINVAL, "kv_attention: too many rows for one call");
         const auto fn = dim == 64 ? kv_few_kernel<64> : dim == 128 ? kv_few_kernel<128> : kv_few_kernel<256>;
-        hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(groups)), dim3(64 * kFewWaves), 0, st, qs, c, s, scale, causal, list, out, part);
+        hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(groups)), dim3(64 * kFewWaves), 0, st, qs, c, s, scale, causal, list, out, part,
+                           p.per);
         rc = check_launch("kv_attention");
     } else if (dim == 64) {
         rc = p.waves == 8 ? launch_tiles<64, 8>(p, qs, c, s, scale, causal, list, out, part, st)
@@ -662,10 +727,11 @@ extern "C" int h3mi_kv_attention_bf16(const uint16_t* q, int64_t rows, int64_t h
         rc = launch_tiles<256, 4>(p, qs, c, s, scale, causal, list, out, part, st);
     }
     if (rc || p.splits == 1) return rc;
-    const int per = static_cast<int>(256 / (dim / 4));
+    const int64_t all = p.part_items() * part.rows;
     int64_t groups;
-    if (!launchable((queries + per - 1) / per, 1, 1, 256, &groups)) return fail(H3MI_EINVAL, "kv_attention: too many rows for one call");
+    if (!launchable((all + 3) / 4, 1, 1, 256, &groups)) return fail(H3MI_EINVAL, "kv_attention: too many rows for one call");
     const auto join = dim == 64 ? kv_join_kernel<64> : dim == 128 ? kv_join_kernel<128> : kv_join_kernel<256>;
-    hipLaunchKernelGGL(join, dim3(static_cast<unsigned>(groups)), dim3(256), 0, st, part, out);
+    hipLaunchKernelGGL(join, dim3(static_cast<unsigned>(groups)), dim3(256), 0, st, part, qs, c.heads, static_cast<int>(p.tiles),
+                       static_cast<int>(p.whole), causal, all, out);
     return check_launch("kv_attention");
 }

@@ -18,6 +18,7 @@ namespace {
 constexpr int kMaxSelect = 32768;  // blocks: their keys fill 128 KiB of LDS
 constexpr int kSelThreads = 512;
 constexpr int kSelWaves = kSelThreads / 64;
+constexpr int kBatch = 8;  // blocks whose sums a lane has in flight
 
 typedef short s16x2 __attribute__((ext_vector_type(2)));
 
@@ -107,27 +108,47 @@ __global__ __launch_bounds__(kSelThreads) void kv_select_kernel(const uint16_t* 
 
     const uint4 qw = *reinterpret_cast<const uint4*>(qi + ch * 8);
     const int own = first < 0 ? 0 : block_of(first);
-    const int blocks_up = (seen + GROUPS - 1) / GROUPS * GROUPS;  // whole groups, so that every lane takes part
-    for (int b = grp; b < blocks_up; b += GROUPS) {
-        const int page = b < seen ? s.page(i, b, c.pages) : -1;
-        int dot = 0;
-        const int64_t at = static_cast<int64_t>(page < 0 ? 0 : page) * c.heads + h;
-        if (page >= 0) {
-            const uint4 k = *reinterpret_cast<const uint4*>(c.ksum + at * D + ch * 8);
-            dot = __builtin_amdgcn_sdot2(__builtin_bit_cast(s16x2, qw.x), __builtin_bit_cast(s16x2, k.x), dot, false);
-            dot = __builtin_amdgcn_sdot2(__builtin_bit_cast(s16x2, qw.y), __builtin_bit_cast(s16x2, k.y), dot, false);
-            dot = __builtin_amdgcn_sdot2(__builtin_bit_cast(s16x2, qw.z), __builtin_bit_cast(s16x2, k.z), dot, false);
-            dot = __builtin_amdgcn_sdot2(__builtin_bit_cast(s16x2, qw.w), __builtin_bit_cast(s16x2, k.w), dot, false);
+    // The blocks' pages first, so that nothing but the sums' own latency stands in the way of kBatch of them at once.
+    for (int b = t; b < seen; b += kSelThreads) keys[b] = static_cast<uint32_t>(s.page(i, b, c.pages));
+    __syncthreads();
+    const int waves_up = (seen + GROUPS - 1) / GROUPS * GROUPS;  // whole groups, so that every lane takes part
+    for (int b0 = grp; b0 < waves_up; b0 += GROUPS * kBatch) {
+        int page[kBatch], dot[kBatch];
+        uint4 k[kBatch];
+        float ks[kBatch];
+#pragma unroll
+        for (int x = 0; x < kBatch; ++x) {
+            const int b = b0 + x * GROUPS;
+            page[x] = b < seen ? static_cast<int>(keys[b]) : -1;
+            k[x] = make_uint4(0, 0, 0, 0);
+            ks[x] = 0.0f;
+            if (page[x] >= 0) {
+                const int64_t at = static_cast<int64_t>(page[x]) * c.heads + h;
+                k[x] = *reinterpret_cast<const uint4*>(c.ksum + at * D + ch * 8);
+                if (ch == 0) ks[x] = c.ks[at];
+            }
         }
 #pragma unroll
-        for (int x = CH / 2; x; x >>= 1) dot += __shfl_xor(dot, x);
-        if (ch == 0 && b < seen) {
-            uint32_t key = 0;
-            if (page >= 0) {
-                const int held = len - b * kKvBlock < kKvBlock ? len - b * kKvBlock : kKvBlock;
-                key = causal && b >= own ? 0xFFFFFFFFu : key_of(static_cast<float>(dot) * (c.ks[at] / static_cast<float>(held)));
+        for (int x = 0; x < kBatch; ++x) {
+            dot[x] = __builtin_amdgcn_sdot2(__builtin_bit_cast(s16x2, qw.x), __builtin_bit_cast(s16x2, k[x].x), 0, false);
+            dot[x] = __builtin_amdgcn_sdot2(__builtin_bit_cast(s16x2, qw.y), __builtin_bit_cast(s16x2, k[x].y), dot[x], false);
+            dot[x] = __builtin_amdgcn_sdot2(__builtin_bit_cast(s16x2, qw.z), __builtin_bit_cast(s16x2, k[x].z), dot[x], false);
+            dot[x] = __builtin_amdgcn_sdot2(__builtin_bit_cast(s16x2, qw.w), __builtin_bit_cast(s16x2, k[x].w), dot[x], false);
+#pragma unroll
+            for (int y = CH / 2; y; y >>= 1) dot[x] += __shfl_xor(dot[x], y);
+        }
+        if (ch == 0) {
+#pragma unroll
+            for (int x = 0; x < kBatch; ++x) {
+                const int b = b0 + x * GROUPS;
+                if (b >= seen) continue;
+                uint32_t key = 0;
+                if (page[x] >= 0) {
+                    const int held = len - b * kKvBlock < kKvBlock ? len - b * kKvBlock : kKvBlock;
+                    key = causal && b >= own ? 0xFFFFFFFFu : key_of(static_cast<float>(dot[x]) * (ks[x] / static_cast<float>(held)));
+                }
+                keys[b] = key;
             }
-            keys[b] = key;
         }
     }
     __syncthreads();
