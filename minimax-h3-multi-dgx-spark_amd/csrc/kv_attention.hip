@@ -36,7 +36,8 @@ constexpr float kLowest = -3.4028234663852886e38f;
 // few times a sequence, not once a block.
 constexpr float kSlack = 8.0f;
 // Value scales whose log2 goes into the exponent: 2^(+-60) keeps p v_scale a normal number
-// for every p above 2^-66.  Others (zero, not finite) multiply p afterwards.
+// for every p above 2^-66.  Others (zero, not finite) multiply p afterwards, as in a block
+// whose key scale is not finite.
 constexpr float kFoldLow = 0x1p-60f, kFoldHigh = 0x1p+60f;
 
 // 8 signed bytes as 8 bf16.
@@ -49,18 +50,28 @@ __device__ __forceinline__ uint4 ints_bf16(uint2 q) {
 
 __device__ __forceinline__ bf16x8 frag(uint4 w) { return __builtin_bit_cast(bf16x8, w); }
 
+// 8 query elements, with the sign of the scale.
+__device__ __forceinline__ bf16x8 query_frag(const uint16_t* p, float scale) {
+    uint4 w = *reinterpret_cast<const uint4*>(p);
+    const uint32_t flip = scale < 0.0f ? 0x80008000u : 0u;
+    w.x ^= flip, w.y ^= flip, w.z ^= flip, w.w ^= flip;
+    return frag(w);
+}
+
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // What a block's scores and probabilities are multiplied by.
 struct Factors {
-    float c;         // scores: k_scale scale log2(e)
+    float c;         // scores: k_scale |scale| log2(e), the sign being the queries'; never 0, so that a masked score's
+                     // -inf stays one: 2^-126 makes as much of a score as 0 does
     float lv, iv;    // the exponent's term, and what a sum of probabilities is multiplied by
     float vs;        // probabilities are multiplied by it where iv is 0
 };
 
 __device__ __forceinline__ Factors factors(float ks, float vs, float scale) {
-    const bool fold = vs >= kFoldLow && vs <= kFoldHigh;
-    return {ks * scale, fold ? log2f(vs) : 0.0f, fold ? 1.0f / vs : 0.0f, vs};
+    const float c = ks * fabsf(scale);
+    const bool fold = vs >= kFoldLow && vs <= kFoldHigh && __builtin_isfinite(c);
+    return {c < 0x1p-126f ? 0x1p-126f : c, fold ? log2f(vs) : 0.0f, fold ? 1.0f / vs : 0.0f, vs};
 }
 
 struct Queries {
@@ -88,8 +99,15 @@ struct Partial {
 // W waves of 32 query rows of one head.  The block's keys and values go through LDS as
 // bf16, converted once a workgroup, in two buffers: the next block's bytes are loaded
 // before this block's products and converted after them, one barrier a block.  Rows are
-// 16-byte chunks whose index is XORed with the row's low bits, which puts the 8 lanes of an
-// access on different banks, both for the writes and for the MFMA operands' reads.
+// 16-byte chunks whose index is XORed with row bits, so that 16 lanes of an access lie on
+// the 16 different 16-byte groups of LDS's 256 bytes of banks, both for the writes (rows)
+// and for the MFMA operands' reads (columns).
+// The place of chunk ch of a row of CH chunks (8: two rows share the banks).
+template <int CH>
+__device__ __forceinline__ int chunk_at(int row, int ch) {
+    return CH == 8 ? ch ^ ((row >> 1) & 7) : ch ^ (row & 15);
+}
+
 template <int D, int W>
 struct TileShape {
     static constexpr int kThreads = 64 * W;
@@ -160,7 +178,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv_tile_kernel(Queri
         const int64_t at = i * q.bs + static_cast<int64_t>(row) * q.ld + static_cast<int64_t>(hq) * D + half * 8;
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
-            qf[k] = frag(last >= 0 ? *reinterpret_cast<const uint4*>(q.p + at + k * 16) : make_uint4(0, 0, 0, 0));
+            qf[k] = last >= 0 ? query_frag(q.p + at + k * 16, scale) : frag(make_uint4(0, 0, 0, 0));
     }
     f32x16 o[NT];
 #pragma unroll
@@ -191,9 +209,9 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv_tile_kernel(Queri
             // token bits 2 and 3 change places: an MFMA row's registers are then runs of 8 tokens
             const int tok = piece / KC, kc = piece % KC;
             const int kr_row = (tok & ~12) | ((tok & 4) << 1) | ((tok & 8) >> 1);
-            *reinterpret_cast<uint4*>(buf + kr_row * (D * 2) + ((kc ^ (kr_row & 7)) * 16)) = ints_bf16(kr[j]);
+            *reinterpret_cast<uint4*>(buf + kr_row * (D * 2) + (chunk_at<KC>(kr_row, kc) * 16)) = ints_bf16(kr[j]);
             const int vrow = piece / VC, vc = piece % VC;
-            *reinterpret_cast<uint4*>(buf + T::kKeyBytes + vrow * (kKvBlock * 2) + ((vc ^ (vrow & 7)) * 16)) = ints_bf16(vr[j]);
+            *reinterpret_cast<uint4*>(buf + T::kKeyBytes + vrow * (kKvBlock * 2) + (chunk_at<VC>(vrow, vc) * 16)) = ints_bf16(vr[j]);
         }
     };
 
@@ -239,31 +257,24 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv_tile_kernel(Queri
                     const int kr_row = u * 32 + col;
 #pragma unroll
                     for (int k = 0; k < D / 16; ++k) {
-                        const bf16x8 a = frag(*reinterpret_cast<const uint4*>(kb + kr_row * (D * 2) + (((2 * k + half) ^ (kr_row & 7)) * 16)));
+                        const bf16x8 a = frag(*reinterpret_cast<const uint4*>(kb + kr_row * (D * 2) + (chunk_at<KC>(kr_row, 2 * k + half) * 16)));
                         sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, qf[k], sc[u], 0, 0, 0);
                     }
                 }
-                // register r of sc[u]: token base + 32 u + 16 (r / 8) + 8 half + r % 8, times f.c
-                float best = -__builtin_inff();
+                // register r of sc[u]: token base + 32 u + 16 (r / 8) + 8 half + r % 8
                 if (base + kKvBlock > wave_full) {
 #pragma unroll
                     for (int u = 0; u < 2; ++u)
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const int tok = base + 32 * u + 16 * (r / 8) + 8 * half + r % 8;
-                            sc[u][r] = tok <= last ? sc[u][r] * f.x : -__builtin_inff();
-                            best = fmaxf(best, sc[u][r]);
-                        }
-                } else {
-#pragma unroll
-                    for (int u = 0; u < 2; ++u)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            sc[u][r] *= f.x;
-                            best = fmaxf(best, sc[u][r]);
-                        }
+                        for (int r = 0; r < 16; ++r)
+                            if (base + 32 * u + 16 * (r / 8) + 8 * half + r % 8 > last) sc[u][r] = -__builtin_inff();
                 }
-                best = fmaxf(best, __shfl_xor(best, 32));
+                float best = -__builtin_inff();
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) best = fmaxf(best, sc[u][r]);
+                best = fmaxf(best, __shfl_xor(best, 32)) * f.x;
                 if (__any(best > m + kSlack)) {
                     const float mn = fmaxf(m, best), fix = exp2_hw(m - mn);
                     m = mn;
@@ -279,17 +290,21 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv_tile_kernel(Queri
                 for (int u = 0; u < 2; ++u)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
-                        sc[u][r] = exp2_hw(sc[u][r] + off);
+                        sc[u][r] = exp2_hw(__builtin_fmaf(sc[u][r], f.x, off));
                         sum += sc[u][r];
                     }
                 if (f.z != 0.0f) {
                     l = __builtin_fmaf(sum, f.z, l);
                 } else {
-                    l += sum;
+                    // a scale that is no ordinary number: what a row does not see must not reach it
 #pragma unroll
                     for (int u = 0; u < 2; ++u)
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) sc[u][r] = sc[u][r] == 0.0f ? 0.0f : sc[u][r] * f.w;
+                        for (int r = 0; r < 16; ++r) {
+                            const float p = base + 32 * u + 16 * (r / 8) + 8 * half + r % 8 > last ? 0.0f : sc[u][r];
+                            l += p;
+                            sc[u][r] = p == 0.0f ? 0.0f : p * f.w;
+                        }
                 }
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
@@ -300,7 +315,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv_tile_kernel(Queri
 #pragma unroll
                         for (int d = 0; d < NT; ++d) {
                             const int vrow = d * 32 + col, vc = 4 * u + 2 * w + half;
-                            const bf16x8 a = frag(*reinterpret_cast<const uint4*>(vb + vrow * (kKvBlock * 2) + ((vc ^ (vrow & 7)) * 16)));
+                            const bf16x8 a = frag(*reinterpret_cast<const uint4*>(vb + vrow * (kKvBlock * 2) + (chunk_at<VC>(vrow, vc) * 16)));
                             o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, p, o[d], 0, 0, 0);
                         }
                     }
@@ -382,7 +397,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void kv_few_kernel(Queries q, KvCac
         const int64_t at = i * q.bs + static_cast<int64_t>(row) * q.ld + static_cast<int64_t>(hq) * D + quad * 16;
 #pragma unroll
         for (int k = 0; k < 2 * KL; ++k)
-            qf[k] = frag(last >= 0 ? *reinterpret_cast<const uint4*>(q.p + at + (k >> 1) * 64 + (k & 1) * 8) : make_uint4(0, 0, 0, 0));
+            qf[k] = last >= 0 ? query_frag(q.p + at + (k >> 1) * 64 + (k & 1) * 8, scale) : frag(make_uint4(0, 0, 0, 0));
     }
     f32x4 o[NT];
 #pragma unroll
@@ -459,12 +474,11 @@ __global__ __launch_bounds__(64 * kFewWaves) void kv_few_kernel(Queries q, KvCac
             for (int u = 0; u < 4; ++u)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    sc[u][r] *= fc;
                     if (mask && base + 16 * quad + 4 * u + r > last) sc[u][r] = -__builtin_inff();
                     best = fmaxf(best, sc[u][r]);
                 }
             best = fmaxf(best, __shfl_xor(best, 16));
-            best = fmaxf(best, __shfl_xor(best, 32));
+            best = fmaxf(best, __shfl_xor(best, 32)) * fc;
             if (__any(best > m + kSlack)) {
                 const float mn = fmaxf(m, best), fix = exp2_hw(m - mn);
                 m = mn;
@@ -478,17 +492,21 @@ __global__ __launch_bounds__(64 * kFewWaves) void kv_few_kernel(Queries q, KvCac
             for (int u = 0; u < 4; ++u)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    sc[u][r] = exp2_hw(sc[u][r] + off);
+                    sc[u][r] = exp2_hw(__builtin_fmaf(sc[u][r], fc, off));
                     sum += sc[u][r];
                 }
             if (fiv != 0.0f) {
                 l = __builtin_fmaf(sum, fiv, l);
             } else {
-                l += sum;
+                // a scale that is no ordinary number: what a row does not see must not reach it
 #pragma unroll
                 for (int u = 0; u < 4; ++u)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) sc[u][r] = sc[u][r] == 0.0f ? 0.0f : sc[u][r] * fvs;
+                    for (int r = 0; r < 4; ++r) {
+                        const float p = base + 16 * quad + 4 * u + r > last ? 0.0f : sc[u][r];
+                        l += p;
+                        sc[u][r] = p == 0.0f ? 0.0f : p * fvs;
+                    }
             }
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
@@ -550,24 +568,23 @@ constexpr int kMaxSplits = 64;  // a lane of the join's wave each
 
 // A wave a row of an item: D / 4 lanes a row of sums, 256 / D splits at once.
 template <int D>
-__global__ __launch_bounds__(256) void kv_join_kernel(Partial part, Queries q, int kv_heads, int tiles, int whole, int causal, int64_t all,
+__global__ __launch_bounds__(256) void kv_join_kernel(Partial part, Queries q, int kv_heads, int tiles, int whole, int causal, uint32_t all,
                                                       uint16_t* __restrict__ out) {
     constexpr int L = D / 4, SG = 64 / L;
-    const int64_t x = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    const uint32_t x = blockIdx.x * 4 + (threadIdx.x >> 6);
     if (x >= all) return;
     const int lane = threadIdx.x & 63, d = lane % L * 4, sg = lane / L;
-    const int64_t item = x / part.rows;
-    const int r = static_cast<int>(x % part.rows);
+    const uint32_t per = part.rows;
+    const int item = static_cast<int>(x / per), r = static_cast<int>(x % per);
     int64_t query;
     if (tiles == 0) {  // a kv head's group: its queries in the order of rows, then heads
         const int group = q.heads / kv_heads;
-        query = (item / kv_heads * q.rows + r / group) * q.heads + item % kv_heads * group + r % group;
+        query = (static_cast<int64_t>(item / kv_heads) * q.rows + r / group) * q.heads + item % kv_heads * group + r % group;
     } else {
-        const int64_t nh = (whole + item) / tiles;
-        const int tile = static_cast<int>((whole + item) % tiles);
+        const int nh = (whole + item) / tiles, tile = (whole + item) % tiles;
         const int row = (causal ? tiles - 1 - tile : tile) * part.rows + r;
         if (row >= q.rows) return;
-        query = (nh / q.heads * q.rows + row) * q.heads + nh % q.heads;
+        query = (static_cast<int64_t>(nh / q.heads) * q.rows + row) * q.heads + nh % q.heads;
     }
     const float2 ml = lane < part.splits ? part.ml[part.at(item, lane, r)] : make_float2(kLowest, 0.0f);
     float top = ml.x;
@@ -732,6 +749,6 @@ extern "C" int h3mi_kv_attention_bf16(const uint16_t* q, int64_t rows, int64_t h
     if (!launchable((all + 3) / 4, 1, 1, 256, &groups)) return fail(H3MI_EINVAL, "kv_attention: too many rows for one call");
     const auto join = dim == 64 ? kv_join_kernel<64> : dim == 128 ? kv_join_kernel<128> : kv_join_kernel<256>;
     hipLaunchKernelGGL(join, dim3(static_cast<unsigned>(groups)), dim3(256), 0, st, part, qs, c.heads, static_cast<int>(p.tiles),
-                       static_cast<int>(p.whole), causal, all, out);
+                       static_cast<int>(p.whole), causal, static_cast<uint32_t>(all), out);
     return check_launch("kv_attention");
 }
