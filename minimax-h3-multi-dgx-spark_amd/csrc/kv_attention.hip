@@ -18,6 +18,8 @@
 //
 // Two kernels: tiles of 128 or 256 query rows of a head, bound by the MFMAs and the
 // softmax, and up to 16 queries of a kv head's group, bound by the cache's bytes.
+#include <type_traits>
+
 #include "kv.h"
 
 namespace h3mi {
@@ -56,6 +58,17 @@ __device__ __forceinline__ bf16x8 query_frag(const uint16_t* p, float scale) {
     const uint32_t flip = scale < 0.0f ? 0x80008000u : 0u;
     w.x ^= flip, w.y ^= flip, w.z ^= flip, w.w ^= flip;
     return frag(w);
+}
+
+// 8 probabilities, rounded to nearest even.
+__device__ __forceinline__ bf16x8 pack(const float (&x)[8]) {
+    return frag(make_uint4(bf16x2_bits(x[0], x[1]), bf16x2_bits(x[2], x[3]), bf16x2_bits(x[4], x[5]), bf16x2_bits(x[6], x[7])));
+}
+
+// The larger of lanes l and l ^ 32.
+__device__ __forceinline__ float max_halves(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -97,8 +110,13 @@ struct Partial {
 // ------------------------------------------------------------------ tiles of queries
 
 // W waves of 32 query rows of one head.  The block's keys and values go through LDS as
-// bf16, converted once a workgroup, in two buffers: the next block's bytes are loaded
-// before this block's products and converted after them, one barrier a block.  Rows are
+// bf16, converted once a workgroup, in two buffers each.  A wave's step y has two halves:
+// the products of block y's keys and of block y - 1's values (MFMA, while a later block's
+// bytes are loaded), then block y's softmax and that later block's conversion (VALU).  Of 8
+// waves the second four run half a step behind the first, with a barrier after each half:
+// of the two waves on a SIMD one is in its products while the other is in its softmax.  They
+// convert their share of a block one step earlier in turn, so that it is there in time.
+// (With 4 waves a barrier a step; two workgroups share a CU.)  Rows are
 // 16-byte chunks whose index is XORed with row bits, so that 16 lanes of an access lie on
 // the 16 different 16-byte groups of LDS's 256 bytes of banks, both for the writes (rows)
 // and for the MFMA operands' reads (columns).
@@ -108,13 +126,16 @@ __device__ __forceinline__ int chunk_at(int row, int ch) {
     return CH == 8 ? ch ^ ((row >> 1) & 7) : ch ^ (row & 15);
 }
 
+constexpr int kAhead = 8;
+constexpr int kSchedMfma = 0x8, kSchedLdsRead = 0x100;  // instruction classes of sched_group_barrier
+
 template <int D, int W>
 struct TileShape {
     static constexpr int kThreads = 64 * W;
     static constexpr int kRows = 32 * W;
     static constexpr int kKeyBytes = kKvBlock * D * 2;
-    static constexpr int kBuf = 2 * kKeyBytes;
-    static constexpr int kLds = 2 * kBuf;
+    static constexpr int kLds = 4 * kKeyBytes;
+    static constexpr int kGroups = W == 8 ? 2 : 1;
     static constexpr int kLoads = kKvBlock * D / 8 / kThreads;  // 8-byte pieces of K (and of V) a thread
 };
 
@@ -193,27 +214,36 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv_tile_kernel(Queri
     const int from = static_cast<int>(static_cast<int64_t>(total) * split / splits);
     const int to = static_cast<int>(static_cast<int64_t>(total) * (split + 1) / splits);
 
+    // Bytes of a block into registers, and as bf16 into LDS.
     uint2 kr[T::kLoads], vr[T::kLoads];
-    auto load = [&](int page) {
-        const int64_t base = (static_cast<int64_t>(page) * c.heads + h) * (kKvBlock * D);
+    auto load = [&](const int8_t* from_pages, int page, uint2 (&to_regs)[T::kLoads]) __attribute__((always_inline)) {
+        const int8_t* const at = from_pages + (static_cast<int64_t>(page) * c.heads + h) * (kKvBlock * D) + t * 8;
 #pragma unroll
-        for (int j = 0; j < T::kLoads; ++j) {
-            kr[j] = *reinterpret_cast<const uint2*>(c.k + base + (t + j * T::kThreads) * 8);
-            vr[j] = *reinterpret_cast<const uint2*>(c.v + base + (t + j * T::kThreads) * 8);
-        }
+        for (int j = 0; j < T::kLoads; ++j) to_regs[j] = *reinterpret_cast<const uint2*>(at + j * T::kThreads * 8);
     };
-    auto stage = [&](uint8_t* buf) {
+    auto stage_k = [&](int which) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < T::kLoads; ++j) {
-            const int piece = t + j * T::kThreads;
+            const int piece = t + j * T::kThreads, tok = piece / KC, kc = piece % KC;
             // token bits 2 and 3 change places: an MFMA row's registers are then runs of 8 tokens
-            const int tok = piece / KC, kc = piece % KC;
-            const int kr_row = (tok & ~12) | ((tok & 4) << 1) | ((tok & 8) >> 1);
-            *reinterpret_cast<uint4*>(buf + kr_row * (D * 2) + (chunk_at<KC>(kr_row, kc) * 16)) = ints_bf16(kr[j]);
-            const int vrow = piece / VC, vc = piece % VC;
-            *reinterpret_cast<uint4*>(buf + T::kKeyBytes + vrow * (kKvBlock * 2) + (chunk_at<VC>(vrow, vc) * 16)) = ints_bf16(vr[j]);
+            const int row = (tok & ~12) | ((tok & 4) << 1) | ((tok & 8) >> 1);
+            *reinterpret_cast<uint4*>(smem + (which & 1) * T::kKeyBytes + row * (D * 2) + chunk_at<KC>(row, kc) * 16) = ints_bf16(kr[j]);
         }
     };
+    auto stage_v = [&](int which) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < T::kLoads; ++j) {
+            const int piece = t + j * T::kThreads, row = piece / VC, vc = piece % VC;
+            *reinterpret_cast<uint4*>(smem + (2 + (which & 1)) * T::kKeyBytes + row * (kKvBlock * 2) + chunk_at<VC>(row, vc) * 16) = ints_bf16(vr[j]);
+        }
+    };
+    auto arrive = [&]() __attribute__((always_inline)) {
+        wait_lgkm0();
+        __builtin_amdgcn_sched_barrier(0);
+        wg_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    const int behind = T::kGroups == 2 && __builtin_amdgcn_readfirstlane(wave) >= W / 2;
 
     for (int x0 = from; x0 < to; x0 += T::kThreads) {
         // the pages and factors of the next kThreads blocks, those that are not there left out
@@ -239,90 +269,128 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv_tile_kernel(Queri
 #pragma unroll
         for (int w = 0; w < W; ++w) n += wcount[w];
         if (n == 0) continue;
-        load(entry[0].x);
-        stage(smem);
-        __syncthreads();
-        for (int y = 0; y < n; ++y) {
-            if (y + 1 < n) load(entry[y + 1].x);
-            const uint8_t* const kb = smem + (y & 1) * T::kBuf;
-            const uint8_t* const vb = kb + T::kKeyBytes;
+        load(c.k, entry[0].x, kr);
+        stage_k(0);
+        arrive();
+        if (behind) {
+            load(c.v, entry[0].x, vr);
+            if (n > 1) {
+                load(c.k, entry[1].x, kr);
+                stage_k(1);
+            }
+            stage_v(0);
+            arrive();
+        }
+        // Step y's halves.  The products take their operands from LDS kAhead MFMAs ahead.
+        bf16x8 p[4];
+        f32x16 sc[2];
+        auto products = [&](int y, auto keys, auto values) __attribute__((always_inline)) {
+            constexpr int NK = keys ? D / 8 : 0, N = NK + (values ? 4 * NT : 0);
+            const uint8_t* const kb = smem + (y & 1) * T::kKeyBytes;
+            const uint8_t* const vb = smem + (3 - (y & 1)) * T::kKeyBytes;
+            auto fetch = [&](int x) __attribute__((always_inline)) {
+                if (x < NK) {
+                    const int row = x % 2 * 32 + col;
+                    return frag(*reinterpret_cast<const uint4*>(kb + row * (D * 2) + chunk_at<KC>(row, x / 2 * 2 + half) * 16));
+                }
+                const int row = (x - NK) % NT * 32 + col, w = (x - NK) / NT;
+                return frag(*reinterpret_cast<const uint4*>(vb + row * (kKvBlock * 2) + chunk_at<VC>(row, 2 * w + half) * 16));
+            };
+            bf16x8 a[kAhead];
+#pragma unroll
+            for (int x = 0; x < kAhead; ++x) a[x] = fetch(x);
+            if constexpr (NK > 0) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sc[0][r] = sc[1][r] = 0.0f;
+            }
+#pragma unroll
+            for (int x = 0; x < N; ++x) {
+                if (x < NK)
+                    sc[x % 2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[x % kAhead], qf[x / 2], sc[x % 2], 0, 0, 0);
+                else
+                    o[(x - NK) % NT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[x % kAhead], p[(x - NK) / NT], o[(x - NK) % NT], 0, 0, 0);
+                if (x + kAhead < N) a[x % kAhead] = fetch(x + kAhead);
+            }
+            __builtin_amdgcn_sched_group_barrier(kSchedLdsRead, kAhead, 0);
+#pragma unroll
+            for (int x = 0; x < N; ++x) {
+                __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
+                if (x + kAhead < N) __builtin_amdgcn_sched_group_barrier(kSchedLdsRead, 1, 0);
+            }
+        };
+        auto softmax = [&](int y) __attribute__((always_inline)) {
             const int base = __builtin_amdgcn_readfirstlane(entry[y].y) * kKvBlock;
-            if (base <= wave_last) {
-                const float4 f = fact[y];
-                f32x16 sc[2];
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) sc[u][r] = 0.0f;
-                    const int kr_row = u * 32 + col;
-#pragma unroll
-                    for (int k = 0; k < D / 16; ++k) {
-                        const bf16x8 a = frag(*reinterpret_cast<const uint4*>(kb + kr_row * (D * 2) + (chunk_at<KC>(kr_row, 2 * k + half) * 16)));
-                        sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, qf[k], sc[u], 0, 0, 0);
-                    }
-                }
-                // register r of sc[u]: token base + 32 u + 16 (r / 8) + 8 half + r % 8
-                if (base + kKvBlock > wave_full) {
-#pragma unroll
-                    for (int u = 0; u < 2; ++u)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r)
-                            if (base + 32 * u + 16 * (r / 8) + 8 * half + r % 8 > last) sc[u][r] = -__builtin_inff();
-                }
-                float best = -__builtin_inff();
+            const float4 f = fact[y];
+            // register r of sc[u]: token base + 32 u + 16 (r / 8) + 8 half + r % 8
+            if (base + kKvBlock > wave_full) {
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) best = fmaxf(best, sc[u][r]);
-                best = fmaxf(best, __shfl_xor(best, 32)) * f.x;
-                if (__any(best > m + kSlack)) {
-                    const float mn = fmaxf(m, best), fix = exp2_hw(m - mn);
-                    m = mn;
-                    l *= fix;
+                    for (int r = 0; r < 16; ++r)
+                        if (base + 32 * u + 16 * (r / 8) + 8 * half + r % 8 > last) sc[u][r] = -__builtin_inff();
+            }
+            float best = -__builtin_inff();
 #pragma unroll
-                    for (int d = 0; d < NT; ++d)
+            for (int u = 0; u < 2; ++u)
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) o[d][r] *= fix;
-                }
-                const float off = f.y - m;
+                for (int r = 0; r < 16; ++r) best = fmaxf(best, sc[u][r]);
+            best = max_halves(best) * f.x;
+            if (__any(best > m + kSlack)) {
+                const float mn = fmaxf(m, best), fix = exp2_hw(m - mn);
+                m = mn;
+                l *= fix;
+#pragma unroll
+                for (int d = 0; d < NT; ++d)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[d][r] *= fix;
+            }
+            const float off = f.y - m;
+            if (f.z != 0.0f) {
                 float sum = 0.0f;
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
+                for (int w = 0; w < 4; ++w) {
+                    float x[8];
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        sc[u][r] = exp2_hw(__builtin_fmaf(sc[u][r], f.x, off));
-                        sum += sc[u][r];
+                    for (int r = 0; r < 8; ++r) {
+                        x[r] = exp2_hw(__builtin_fmaf(sc[w / 2][w % 2 * 8 + r], f.x, off));
+                        sum += x[r];
                     }
-                if (f.z != 0.0f) {
-                    l = __builtin_fmaf(sum, f.z, l);
-                } else {
-                    // a scale that is no ordinary number: what a row does not see must not reach it
-#pragma unroll
-                    for (int u = 0; u < 2; ++u)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const float p = base + 32 * u + 16 * (r / 8) + 8 * half + r % 8 > last ? 0.0f : sc[u][r];
-                            l += p;
-                            sc[u][r] = p == 0.0f ? 0.0f : p * f.w;
-                        }
+                    p[w] = pack(x);
                 }
+                l = __builtin_fmaf(sum, f.z, l);
+            } else {
+                // a scale that is no ordinary number: what a row does not see must not reach it
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
+                for (int w = 0; w < 4; ++w) {
+                    float x[8];
 #pragma unroll
-                    for (int w = 0; w < 2; ++w) {
-                        const bf16x8 p = frag(make_uint4(bf16x2_bits(sc[u][8 * w], sc[u][8 * w + 1]), bf16x2_bits(sc[u][8 * w + 2], sc[u][8 * w + 3]),
-                                                         bf16x2_bits(sc[u][8 * w + 4], sc[u][8 * w + 5]), bf16x2_bits(sc[u][8 * w + 6], sc[u][8 * w + 7])));
-#pragma unroll
-                        for (int d = 0; d < NT; ++d) {
-                            const int vrow = d * 32 + col, vc = 4 * u + 2 * w + half;
-                            const bf16x8 a = frag(*reinterpret_cast<const uint4*>(vb + vrow * (kKvBlock * 2) + (chunk_at<VC>(vrow, vc) * 16)));
-                            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, p, o[d], 0, 0, 0);
-                        }
+                    for (int r = 0; r < 8; ++r) {
+                        x[r] = exp2_hw(__builtin_fmaf(sc[w / 2][w % 2 * 8 + r], f.x, off));
+                        if (base + 16 * w + 8 * half + r > last) x[r] = 0.0f;
+                        l += x[r];
+                        x[r] = x[r] == 0.0f ? 0.0f : x[r] * f.w;
                     }
+                    p[w] = pack(x);
+                }
             }
-            if (y + 1 < n) stage(smem + ((y + 1) & 1) * T::kBuf);
-            __syncthreads();
-        }
+        };
+        auto step = [&](int y, auto values) __attribute__((always_inline)) {
+            const int next_k = y + 1 + behind, next_v = y + behind;
+            if (next_k < n) load(c.k, entry[next_k].x, kr);
+            if (next_v < n) load(c.v, entry[next_v].x, vr);
+            __builtin_amdgcn_s_setprio(1);
+            products(y, std::true_type{}, values);
+            __builtin_amdgcn_s_setprio(0);
+            if constexpr (T::kGroups == 2) arrive();
+            softmax(y);
+            if (next_k < n) stage_k(next_k);
+            if (next_v < n) stage_v(next_v);
+            arrive();
+        };
+        step(0, std::false_type{});
+        for (int y = 1; y < n; ++y) step(y, std::true_type{});
+        products(n, std::false_type{}, std::true_type{});
+        if (T::kGroups == 2 && !behind) arrive();
     }
 
     l += __shfl_xor(l, 32);
