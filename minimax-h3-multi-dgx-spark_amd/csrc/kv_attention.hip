@@ -65,6 +65,9 @@ __device__ __forceinline__ bf16x8 pack(const float (&x)[8]) {
     return frag(make_uint4(bf16x2_bits(x[0], x[1]), bf16x2_bits(x[2], x[3]), bf16x2_bits(x[4], x[5]), bf16x2_bits(x[6], x[7])));
 }
 
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ float uniform(float v) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v))); }
+
 // The larger of lanes l and l ^ 32.
 __device__ __forceinline__ float max_halves(float v) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -165,8 +168,8 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv_tile_kernel(Queri
     constexpr int NT = D / 32;            // tiles of 32 elements of the output
     constexpr int KC = D / 8, VC = 8;     // 16-byte chunks of a row of K, of V
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-    __shared__ int2 entry[T::kThreads];   // (page, block) of the blocks at hand
-    __shared__ float4 fact[T::kThreads];
+    __shared__ int2 entry[T::kThreads + 3];  // (page, block) of the blocks at hand
+    __shared__ Factors fact[T::kThreads + 1];
     __shared__ int wcount[W];
 
     int split, splits;
@@ -217,9 +220,9 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv_tile_kernel(Queri
     // Bytes of a block into registers, and as bf16 into LDS.
     uint2 kr[T::kLoads], vr[T::kLoads];
     auto load = [&](const int8_t* from_pages, int page, uint2 (&to_regs)[T::kLoads]) __attribute__((always_inline)) {
-        const int8_t* const at = from_pages + (static_cast<int64_t>(page) * c.heads + h) * (kKvBlock * D) + t * 8;
+        const int8_t* const at = from_pages + (static_cast<int64_t>(page) * c.heads + h) * (kKvBlock * D);  // uniform
 #pragma unroll
-        for (int j = 0; j < T::kLoads; ++j) to_regs[j] = *reinterpret_cast<const uint2*>(at + j * T::kThreads * 8);
+        for (int j = 0; j < T::kLoads; ++j) to_regs[j] = *reinterpret_cast<const uint2*>(at + static_cast<uint32_t>(t + j * T::kThreads) * 8);
     };
     auto stage_k = [&](int which) __attribute__((always_inline)) {
 #pragma unroll
@@ -261,7 +264,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv_tile_kernel(Queri
                 const int64_t p = static_cast<int64_t>(page) * c.heads + h;
                 const Factors f = factors(c.ks[p], c.vs[p], scale * kLog2e);
                 entry[at] = make_int2(page, b);
-                fact[at] = make_float4(f.c, f.lv, f.iv, f.vs);
+                fact[at] = f;
             }
         }
         __syncthreads();
@@ -269,18 +272,22 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv_tile_kernel(Queri
 #pragma unroll
         for (int w = 0; w < W; ++w) n += wcount[w];
         if (n == 0) continue;
-        load(c.k, entry[0].x, kr);
+        load(c.k, uniform(entry[0].x), kr);
         stage_k(0);
         arrive();
         if (behind) {
-            load(c.v, entry[0].x, vr);
+            load(c.v, uniform(entry[0].x), vr);
             if (n > 1) {
-                load(c.k, entry[1].x, kr);
+                load(c.k, uniform(entry[1].x), kr);
                 stage_k(1);
             }
             stage_v(0);
             arrive();
         }
+        // What a step needs to know of its blocks is read a step ahead: the pages that it loads, and its own block and factors.
+        int page_k = uniform(entry[1 + behind].x), page_v = uniform(entry[behind].x), base = uniform(entry[0].y) * kKvBlock;
+        Factors f = fact[0];
+        f = {uniform(f.c), uniform(f.lv), uniform(f.iv), uniform(f.vs)};
         // Step y's halves.  The products take their operands from LDS kAhead MFMAs ahead.
         bf16x8 p[4];
         f32x16 sc[2];
@@ -318,9 +325,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv_tile_kernel(Queri
                 if (x + kAhead < N) __builtin_amdgcn_sched_group_barrier(kSchedLdsRead, 1, 0);
             }
         };
-        auto softmax = [&](int y) __attribute__((always_inline)) {
-            const int base = __builtin_amdgcn_readfirstlane(entry[y].y) * kKvBlock;
-            const float4 f = fact[y];
+        auto softmax = [&]() __attribute__((always_inline)) {
             // register r of sc[u]: token base + 32 u + 16 (r / 8) + 8 half + r % 8
             if (base + kKvBlock > wave_full) {
 #pragma unroll
@@ -334,7 +339,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv_tile_kernel(Queri
             for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) best = fmaxf(best, sc[u][r]);
-            best = max_halves(best) * f.x;
+            best = max_halves(best) * f.c;
             if (__any(best > m + kSlack)) {
                 const float mn = fmaxf(m, best), fix = exp2_hw(m - mn);
                 m = mn;
@@ -344,20 +349,20 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv_tile_kernel(Queri
 #pragma unroll
                     for (int r = 0; r < 16; ++r) o[d][r] *= fix;
             }
-            const float off = f.y - m;
-            if (f.z != 0.0f) {
+            const float off = f.lv - m;
+            if (f.iv != 0.0f) {
                 float sum = 0.0f;
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
                     float x[8];
 #pragma unroll
                     for (int r = 0; r < 8; ++r) {
-                        x[r] = exp2_hw(__builtin_fmaf(sc[w / 2][w % 2 * 8 + r], f.x, off));
+                        x[r] = exp2_hw(__builtin_fmaf(sc[w / 2][w % 2 * 8 + r], f.c, off));
                         sum += x[r];
                     }
                     p[w] = pack(x);
                 }
-                l = __builtin_fmaf(sum, f.z, l);
+                l = __builtin_fmaf(sum, f.iv, l);
             } else {
                 // a scale that is no ordinary number: what a row does not see must not reach it
 #pragma unroll
@@ -365,10 +370,10 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv_tile_kernel(Queri
                     float x[8];
 #pragma unroll
                     for (int r = 0; r < 8; ++r) {
-                        x[r] = exp2_hw(__builtin_fmaf(sc[w / 2][w % 2 * 8 + r], f.x, off));
+                        x[r] = exp2_hw(__builtin_fmaf(sc[w / 2][w % 2 * 8 + r], f.c, off));
                         if (base + 16 * w + 8 * half + r > last) x[r] = 0.0f;
                         l += x[r];
-                        x[r] = x[r] == 0.0f ? 0.0f : x[r] * f.w;
+                        x[r] = x[r] == 0.0f ? 0.0f : x[r] * f.vs;
                     }
                     p[w] = pack(x);
                 }
@@ -376,15 +381,23 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv_tile_kernel(Queri
         };
         auto step = [&](int y, auto values) __attribute__((always_inline)) {
             const int next_k = y + 1 + behind, next_v = y + behind;
-            if (next_k < n) load(c.k, entry[next_k].x, kr);
-            if (next_v < n) load(c.v, entry[next_v].x, vr);
+            if (next_k < n) load(c.k, page_k, kr);
+            if (next_v < n) load(c.v, page_v, vr);
+            // (past the last block: whatever the arrays hold, which is then not used)
+            const int2 after = entry[next_k + 1];
+            const int block = entry[y + 1].y;
+            const Factors next = fact[y + 1];
             __builtin_amdgcn_s_setprio(1);
             products(y, std::true_type{}, values);
             __builtin_amdgcn_s_setprio(0);
             if constexpr (T::kGroups == 2) arrive();
-            softmax(y);
+            softmax();
             if (next_k < n) stage_k(next_k);
             if (next_v < n) stage_v(next_v);
+            page_v = page_k;
+            page_k = uniform(after.x);
+            base = uniform(block) * kKvBlock;
+            f = {uniform(next.c), uniform(next.lv), uniform(next.iv), uniform(next.vs)};
             arrive();
         };
         step(0, std::false_type{});
