@@ -52,6 +52,12 @@ struct KvSeqs {
     }
 };
 
+// The item of a workgroup such that an XCD's workgroups, every eighth of the launch, take consecutive items.
+__device__ __forceinline__ int xcd_item() {
+    const int all = gridDim.x, per = all >> 3, more = all & 7, xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
+    return xcd * per + (xcd < more ? xcd : more) + at;
+}
+
 inline KvCache kv_cache(const h3mi_kv_cache& c) {
     return {c.k, c.v, c.k_scale, c.v_scale, c.k_sum, c.pages, static_cast<int>(c.heads)};
 }

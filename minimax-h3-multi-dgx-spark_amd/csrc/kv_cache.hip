@@ -6,6 +6,10 @@
 // of bf16 rows are whole 128- to 512-byte rows of the head, the block's maximum
 // needs one barrier, and four tokens of an element are one word of the transposed
 // values, which pass through LDS so that their global rows are written (read) whole.
+// Consecutive blocks and heads run on one XCD (a clip of 19200 tokens of 56 x 128 written
+// in 155 us against 161 with heads dealt over the XCDs, read back in 154 against 160), and
+// what is written goes past the L2 (161 against 167, 160 against 168; 2401 tokens 19.0
+// against 25.0 and 17.3 against 20.4).
 #include "kv.h"
 
 namespace h3mi {
@@ -45,9 +49,27 @@ int kv_check_rows(const char* what, const char* name, const uint16_t* p, int64_t
 
 namespace {
 
+constexpr int64_t kMemoryCache = int64_t{256} << 20;  // bytes that the memory-side cache holds
+
 // Words of a head's transposed block in LDS: 16 words of 4 tokens a row, one row's
 // words off the next's banks.
 constexpr int kVtStride = 17;
+
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ void store_past(void* p, uint4 v) {
+    __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v), static_cast<u32x4*>(p));
+}
+__device__ __forceinline__ void store_past(void* p, uint2 v) {
+    __builtin_nontemporal_store(__builtin_bit_cast(u32x2, v), static_cast<u32x2*>(p));
+}
+
+template <bool STREAM>
+__device__ __forceinline__ uint4 load_row(const uint16_t* p) {
+    if constexpr (STREAM) return __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p)));
+    return *reinterpret_cast<const uint4*>(p);
+}
 
 // The larger of packed 16-bit magnitudes (bit patterns of |bf16|, so a NaN wins).
 __device__ __forceinline__ uint32_t max_mag(uint32_t a, uint32_t b) {
@@ -108,8 +130,11 @@ struct Rows {
     int64_t ld, bs;
 };
 
-// One workgroup: block blockIdx of the blocks that a sequence's new tokens touch, one head.  2 D threads.
-template <int D>
+// One workgroup: one of the blocks that a sequence's new tokens touch, one head.  2 D threads.
+// STREAM: the rows are loaded past the caches as well (a clip of 19200 tokens 150 us against
+// 155), unless they fit the memory-side cache and may still be there (2401 tokens 22.6 us so,
+// 19.0 cached).
+template <int D, bool STREAM>
 __global__ __launch_bounds__(2 * D) void kv_write_kernel(Rows kin, Rows vin, KvCache c, KvSeqs s, int rows, int touched) {
     constexpr int CH = D / 8;  // 16-byte chunks of a row
     constexpr int WAVES = 2 * D / 64;
@@ -117,8 +142,7 @@ __global__ __launch_bounds__(2 * D) void kv_write_kernel(Rows kin, Rows vin, KvC
     __shared__ uint32_t part[2][WAVES];
     __shared__ int sums[D];
 
-    const int h = blockIdx.x % c.heads;
-    const int item = blockIdx.x / c.heads;
+    const int at_all = xcd_item(), h = at_all % c.heads, item = at_all / c.heads;
     const int i = item / touched;
     const int len = s.len(i), count = s.count(i, rows), start = s.end(i) - count;
     // a negative start: tokens before the sequence's first are dropped
@@ -141,8 +165,8 @@ __global__ __launch_bounds__(2 * D) void kv_write_kernel(Rows kin, Rows vin, KvC
         kx[j] = vx[j] = make_uint4(0, 0, 0, 0);
         if (fresh[j]) {
             const int64_t row = at - start;
-            kx[j] = *reinterpret_cast<const uint4*>(kin.p + i * kin.bs + row * kin.ld + h * D + col);
-            vx[j] = *reinterpret_cast<const uint4*>(vin.p + i * vin.bs + row * vin.ld + h * D + col);
+            kx[j] = load_row<STREAM>(kin.p + i * kin.bs + row * kin.ld + h * D + col);
+            vx[j] = load_row<STREAM>(vin.p + i * vin.bs + row * vin.ld + h * D + col);
         }
     }
     const bool first = start <= base;  // no token of the block is older
@@ -200,7 +224,7 @@ __global__ __launch_bounds__(2 * D) void kv_write_kernel(Rows kin, Rows vin, KvC
             q = *at;
             q = make_uint2(refit(q.x, sk.mul), refit(q.y, sk.mul));
         }
-        *at = q;
+        store_past(at, q);
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
             acc[p] += static_cast<int8_t>(q.x >> (8 * p));
@@ -228,7 +252,7 @@ __global__ __launch_bounds__(2 * D) void kv_write_kernel(Rows kin, Rows vin, KvC
     for (int p = 0; p < 2; ++p) {
         const int piece = t + p * 2 * D, row = piece >> 2, at = (piece & 3) * 4;
         const uint32_t* const src = vt + row * kVtStride + at;
-        *reinterpret_cast<uint4*>(vout + piece * 16) = make_uint4(src[0], src[1], src[2], src[3]);
+        store_past(vout + piece * 16, make_uint4(src[0], src[1], src[2], src[3]));
     }
     if (t < D) c.ksum[tile * D + t] = static_cast<int16_t>(sums[t]);
 }
@@ -248,8 +272,7 @@ __global__ __launch_bounds__(2 * D) void kv_read_kernel(uint16_t* __restrict__ k
                                                         int touched) {
     constexpr int CH = D / 8;
     __shared__ uint32_t vt[D * kVtStride];
-    const int h = blockIdx.x % c.heads;
-    const int item = blockIdx.x / c.heads;
+    const int at_all = xcd_item(), h = at_all % c.heads, item = at_all / c.heads;
     const int i = item / touched;
     const int start = starts ? starts[i] : 0;
     const int64_t b = static_cast<int64_t>(block_of(start)) + item % touched;
@@ -289,8 +312,8 @@ __global__ __launch_bounds__(2 * D) void kv_read_kernel(uint16_t* __restrict__ k
         const int64_t o = ((i * static_cast<int64_t>(length) + r) * c.heads + h) * D + col;
         const bool there = page >= 0 && at < len;
         const uint4 none = make_uint4(0, 0, 0, 0);
-        *reinterpret_cast<uint4*>(kout + o) = there ? widen(kq[j], ks) : none;
-        *reinterpret_cast<uint4*>(vout + o) = there ? widen(make_uint2(x[j], x[4 + j]), vs) : none;
+        store_past(kout + o, there ? widen(kq[j], ks) : none);
+        store_past(vout + o, there ? widen(make_uint2(x[j], x[4 + j]), vs) : none);
     }
 }
 
@@ -310,7 +333,9 @@ extern "C" int h3mi_kv_write_i8(const uint16_t* k, const uint16_t* v, int64_t ro
     const int D = static_cast<int>(cache->dim);
     int64_t groups;
     if (!launchable(seqs->n, touched, cache->heads, 2 * D, &groups)) return fail(H3MI_EINVAL, "kv_write: too many tokens for one call");
-    const auto fn = D == 64 ? kv_write_kernel<64> : D == 128 ? kv_write_kernel<128> : kv_write_kernel<256>;
+    const bool stream_in = seqs->n * rows * cache->heads * D * 4 > kMemoryCache;
+    const auto fn = stream_in ? (D == 64 ? kv_write_kernel<64, true> : D == 128 ? kv_write_kernel<128, true> : kv_write_kernel<256, true>)
+                              : (D == 64 ? kv_write_kernel<64, false> : D == 128 ? kv_write_kernel<128, false> : kv_write_kernel<256, false>);
     hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(groups)), dim3(2 * D), 0, as_stream(stream), Rows{k, ld_k, bs_k},
                        Rows{v, ld_v, bs_v}, kv_cache(*cache), kv_seqs(*seqs), static_cast<int>(rows), static_cast<int>(touched));
     return check_launch("kv_write");
