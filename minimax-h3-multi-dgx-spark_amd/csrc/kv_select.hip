@@ -16,9 +16,18 @@ namespace h3mi {
 namespace {
 
 constexpr int kMaxSelect = 32768;  // blocks: their keys fill 128 KiB of LDS
-constexpr int kSelThreads = 512;
-constexpr int kSelWaves = kSelThreads / 64;
-constexpr int kBatch = 8;  // blocks whose sums a lane has in flight
+constexpr int kBatch = 8;  // blocks whose sums a lane has in flight; at most the lanes of a block
+
+// Sum over groups of CH lanes, by DPP moves within 16: a neighbour, the other pair, the mirrored other four, the other eight.
+template <int CH>
+__device__ __forceinline__ int lane_sum(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x141, 0xF, 0xF, false);
+    if constexpr (CH >= 16) v += __builtin_amdgcn_update_dpp(0, v, 0x128, 0xF, 0xF, false);
+    if constexpr (CH >= 32) v += __shfl_xor(v, 16);
+    return v;
+}
 
 typedef short s16x2 __attribute__((ext_vector_type(2)));
 
@@ -31,12 +40,12 @@ __device__ __forceinline__ uint32_t key_of(float s) {
     return k < 2u ? 2u : k;
 }
 
-template <int D>
-__global__ __launch_bounds__(kSelThreads) void kv_select_kernel(const uint16_t* __restrict__ q, int64_t ld, int64_t bs, KvCache c,
+template <int D, int THREADS>
+__global__ __launch_bounds__(THREADS) void kv_select_kernel(const uint16_t* __restrict__ q, int64_t ld, int64_t bs, KvCache c,
                                                                 KvSeqs s, int rows, int heads, int top, int causal, int tiles,
                                                                 int32_t* __restrict__ out) {
-    constexpr int CH = D / 8;
-    constexpr int GROUPS = kSelThreads / CH;  // row groups while pooling, blocks at once while scoring
+    constexpr int CH = D / 8, kSelWaves = THREADS / 64;
+    constexpr int GROUPS = THREADS / CH;  // row groups while pooling, blocks at once while scoring
     extern __shared__ uint32_t keys[];
     __shared__ double part[kSelWaves][D];
     __shared__ double pool[D];
@@ -47,19 +56,18 @@ __global__ __launch_bounds__(kSelThreads) void kv_select_kernel(const uint16_t* 
     __shared__ double wmax[kSelWaves];
 
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    const int h = blockIdx.x % c.heads;
-    const int item = blockIdx.x / c.heads;
-    const int i = item / tiles, tile = item % tiles;
-    int32_t* const to = out + (static_cast<int64_t>(item) * c.heads + h) * top;
+    // an XCD takes whole heads, whose sums its L2 then holds for every tile
+    const int at_all = xcd_item(), tile = at_all % tiles, h = at_all / tiles % c.heads, i = at_all / tiles / c.heads;
+    int32_t* const to = out + ((static_cast<int64_t>(i) * tiles + tile) * c.heads + h) * top;
     const int len = s.len(i), count = s.count(i, rows), group = heads / c.heads;
     const int r0 = tile * kKvTile, live = count - r0 < kKvTile ? count - r0 : kKvTile;
     // the tile's own tokens, and the blocks it sees
     const int first = s.end(i) - count + r0, last = first + live - 1;
     int seen = (len + kKvBlock - 1) / kKvBlock;
     if (causal && last < len) seen = last < 0 ? 0 : block_of(last) + 1;
-    if (live <= 0) seen = 0;
+    if (live <= 0 || c.pages == 0) seen = 0;
     if (seen == 0) {
-        for (int j = t; j < top; j += kSelThreads) to[j] = -1;
+        for (int j = t; j < top; j += THREADS) to[j] = -1;
         return;
     }
 
@@ -109,46 +117,34 @@ __global__ __launch_bounds__(kSelThreads) void kv_select_kernel(const uint16_t* 
     const uint4 qw = *reinterpret_cast<const uint4*>(qi + ch * 8);
     const int own = first < 0 ? 0 : block_of(first);
     // The blocks' pages first, so that nothing but the sums' own latency stands in the way of kBatch of them at once.
-    for (int b = t; b < seen; b += kSelThreads) keys[b] = static_cast<uint32_t>(s.page(i, b, c.pages));
+    for (int b = t; b < seen; b += THREADS) keys[b] = static_cast<uint32_t>(s.page(i, b, c.pages));
     __syncthreads();
     const int waves_up = (seen + GROUPS - 1) / GROUPS * GROUPS;  // whole groups, so that every lane takes part
     for (int b0 = grp; b0 < waves_up; b0 += GROUPS * kBatch) {
-        int page[kBatch], dot[kBatch];
         uint4 k[kBatch];
-        float ks[kBatch];
 #pragma unroll
         for (int x = 0; x < kBatch; ++x) {
-            const int b = b0 + x * GROUPS;
-            page[x] = b < seen ? static_cast<int>(keys[b]) : -1;
-            k[x] = make_uint4(0, 0, 0, 0);
-            ks[x] = 0.0f;
-            if (page[x] >= 0) {
-                const int64_t at = static_cast<int64_t>(page[x]) * c.heads + h;
-                k[x] = *reinterpret_cast<const uint4*>(c.ksum + at * D + ch * 8);
-                if (ch == 0) ks[x] = c.ks[at];
-            }
+            const int b = b0 + x * GROUPS, page = b < seen ? static_cast<int>(keys[b]) : -1;
+            // (a page that is not there: page 0's, not used)
+            k[x] = *reinterpret_cast<const uint4*>(c.ksum + (static_cast<int64_t>(page < 0 ? 0 : page) * c.heads + h) * D + ch * 8);
         }
+        // every lane of a group has the sums; lane x makes the key of the group's block x
+        const int b = b0 + ch * GROUPS, page = ch < kBatch && b < seen ? static_cast<int>(keys[b]) : -1;
+        const float ks = page < 0 ? 0.0f : c.ks[static_cast<int64_t>(page) * c.heads + h];
+        int mine = 0;
 #pragma unroll
         for (int x = 0; x < kBatch; ++x) {
-            dot[x] = __builtin_amdgcn_sdot2(__builtin_bit_cast(s16x2, qw.x), __builtin_bit_cast(s16x2, k[x].x), 0, false);
-            dot[x] = __builtin_amdgcn_sdot2(__builtin_bit_cast(s16x2, qw.y), __builtin_bit_cast(s16x2, k[x].y), dot[x], false);
-            dot[x] = __builtin_amdgcn_sdot2(__builtin_bit_cast(s16x2, qw.z), __builtin_bit_cast(s16x2, k[x].z), dot[x], false);
-            dot[x] = __builtin_amdgcn_sdot2(__builtin_bit_cast(s16x2, qw.w), __builtin_bit_cast(s16x2, k[x].w), dot[x], false);
-#pragma unroll
-            for (int y = CH / 2; y; y >>= 1) dot[x] += __shfl_xor(dot[x], y);
+            int dot = __builtin_amdgcn_sdot2(__builtin_bit_cast(s16x2, qw.x), __builtin_bit_cast(s16x2, k[x].x), 0, false);
+            dot = __builtin_amdgcn_sdot2(__builtin_bit_cast(s16x2, qw.y), __builtin_bit_cast(s16x2, k[x].y), dot, false);
+            dot = __builtin_amdgcn_sdot2(__builtin_bit_cast(s16x2, qw.z), __builtin_bit_cast(s16x2, k[x].z), dot, false);
+            dot = __builtin_amdgcn_sdot2(__builtin_bit_cast(s16x2, qw.w), __builtin_bit_cast(s16x2, k[x].w), dot, false);
+            dot = lane_sum<CH>(dot);
+            mine = ch == x ? dot : mine;
         }
-        if (ch == 0) {
-#pragma unroll
-            for (int x = 0; x < kBatch; ++x) {
-                const int b = b0 + x * GROUPS;
-                if (b >= seen) continue;
-                uint32_t key = 0;
-                if (page[x] >= 0) {
-                    const int held = len - b * kKvBlock < kKvBlock ? len - b * kKvBlock : kKvBlock;
-                    key = causal && b >= own ? 0xFFFFFFFFu : key_of(static_cast<float>(dot[x]) * (ks[x] / static_cast<float>(held)));
-                }
-                keys[b] = key;
-            }
+        if (ch < kBatch && b < seen) {
+            const int held = len - b * kKvBlock < kKvBlock ? len - b * kKvBlock : kKvBlock;
+            const float score = static_cast<float>(mine) * (ks / static_cast<float>(held));
+            keys[b] = page < 0 ? 0u : causal && b >= own ? 0xFFFFFFFFu : key_of(score);
         }
     }
     __syncthreads();
@@ -160,9 +156,9 @@ __global__ __launch_bounds__(kSelThreads) void kv_select_kernel(const uint16_t* 
         uint32_t prefix = 0, have = 0;
         int want = top;
         for (int shift = 24; shift >= 0; shift -= 8) {
-            for (int x = t; x < 256; x += kSelThreads) hist[x] = 0;
+            for (int x = t; x < 256; x += THREADS) hist[x] = 0;
             __syncthreads();
-            for (int b = t; b < seen; b += kSelThreads)
+            for (int b = t; b < seen; b += THREADS)
                 if (shift == 24 || (keys[b] >> (shift + 8)) == prefix) atomicAdd(&hist[(keys[b] >> shift) & 255u], 1u);
             __syncthreads();
             if (wave == 0) {
@@ -205,7 +201,7 @@ __global__ __launch_bounds__(kSelThreads) void kv_select_kernel(const uint16_t* 
 
     // In order: blocks above thr, and the first `need` at it.
     int done = 0, ties = 0;
-    for (int b0 = 0; b0 < seen; b0 += kSelThreads) {
+    for (int b0 = 0; b0 < seen; b0 += THREADS) {
         const int b = b0 + t;
         const uint32_t key = b < seen ? keys[b] : 0u;
         const bool over = key > thr, tie = key == thr;
@@ -227,7 +223,7 @@ __global__ __launch_bounds__(kSelThreads) void kv_select_kernel(const uint16_t* 
         ties += all_e;
         __syncthreads();
     }
-    for (int j = done + t; j < top; j += kSelThreads) to[j] = -1;
+    for (int j = done + t; j < top; j += THREADS) to[j] = -1;
 }
 
 }  // namespace
@@ -249,11 +245,15 @@ extern "C" int h3mi_kv_select(const uint16_t* q, int64_t rows, int64_t heads, in
     if (!blocks) return fail(H3MI_EINVAL, "kv_select: null blocks");
     if (!aligned(blocks, 4)) return fail(H3MI_EALIGN, "kv_select: blocks must be 4-byte aligned");
     const int64_t tiles = (rows + kKvTile - 1) / kKvTile;
-    int64_t groups;
-    if (!launchable(seqs->n, tiles, cache->heads, kSelThreads, &groups)) return fail(H3MI_EINVAL, "kv_select: too many rows for one call");
     const int D = static_cast<int>(cache->dim);
-    const auto fn = D == 64 ? kv_select_kernel<64> : D == 128 ? kv_select_kernel<128> : kv_select_kernel<256>;
-    hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(groups)), dim3(kSelThreads), static_cast<unsigned>(seqs->blocks * 4),
+    int64_t groups;
+    if (!launchable(seqs->n, tiles, cache->heads, 1024, &groups)) return fail(H3MI_EINVAL, "kv_select: too many rows for one call");
+    // one workgroup a CU or less: more of its own waves (2048 blocks, 32 groups: 21.0 us against 26; 150 blocks, 240 groups
+    // 11.2 against 8.3, 609 blocks, 1064 groups 25.3 against 29.3 with 512)
+    const int threads = 2 * groups <= cu_count() ? 1024 : 256;
+    const auto fn = threads == 1024 ? (D == 64 ? kv_select_kernel<64, 1024> : D == 128 ? kv_select_kernel<128, 1024> : kv_select_kernel<256, 1024>)
+                                    : (D == 64 ? kv_select_kernel<64, 256> : D == 128 ? kv_select_kernel<128, 256> : kv_select_kernel<256, 256>);
+    hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(groups)), dim3(threads), static_cast<unsigned>(seqs->blocks * 4),
                        as_stream(stream), q, ld_q, bs_q, kv_cache(*cache), kv_seqs(*seqs), static_cast<int>(rows),
                        static_cast<int>(heads), static_cast<int>(top), causal, static_cast<int>(tiles), blocks);
     return check_launch("kv_select");
