@@ -440,6 +440,13 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv_tile_kernel(Queri
 
 // ------------------------------------------------------------------ few queries
 
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+
+// A load of what no other workgroup reads, past the caches: 537 MB of cache in 87 us against 99.
+__device__ __forceinline__ uint4 load_once(const int8_t* p) {
+    return __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p)));
+}
+
 constexpr int kFew = 16;      // queries of a kv head's group: the columns of a 16x16 MFMA
 constexpr int kFewWaves = 4;
 
