@@ -142,28 +142,41 @@ struct TileShape {
     static constexpr int kLoads = kKvBlock * D / 8 / kThreads;  // 8-byte pieces of K (and of V) a thread
 };
 
-// The items (tiles of a head, heads of a sequence) of a launch: the first `whole` take one
+// The items of a launch: tiles of the queries of a head, or (pack > 1) of the queries of all
+// heads that share a kv head, in the order of rows, then heads.  The first `whole` take one
 // workgroup each, a multiple of what the card holds at once; the rest, which would leave a
 // last round part empty, are split over their blocks to fill it.
-struct Grid {
-    int tiles, items, whole, chunk, rest_chunk;
-    // Consecutive items on one XCD, whose L2 then holds their head's blocks.
-    __device__ __forceinline__ int item(int block, int tail_splits, int& split, int& splits) const {
+struct Items {
+    int tiles, heads;  // of a head (or a kv head's group); heads (groups) of a sequence
+    int pack, rows;    // query heads and queries of an item
+    int count, whole, chunk, rest_chunk;
+    bool flat, last_first;
+    // Consecutive items on one XCD, whose L2 then holds their head's blocks.  flat (one round, every workgroup at once):
+    // dealt out in order.
+    __device__ __forceinline__ int of(int block, int tail_splits, int& split, int& splits) const {
         if (block < whole) {
             split = 0, splits = 1;
-            return (block & 7) * chunk + (block >> 3);
+            return flat ? block : (block & 7) * chunk + (block >> 3);
         }
-        const int x = ((block - whole) & 7) * rest_chunk + ((block - whole) >> 3);
+        const int x = flat ? block - whole : ((block - whole) & 7) * rest_chunk + ((block - whole) >> 3);
         splits = tail_splits;
         split = x % splits;
         return whole + x / splits;
+    }
+    // Of causal items those of a head's last rows, the longest, come first: first of all in a flat launch.
+    __device__ __forceinline__ void place(int item, int& seq, int& head, int& tile) const {
+        const int all = count / tiles, nh = flat ? item % all : item / tiles;
+        tile = flat ? item / all : item % tiles;
+        if (last_first) tile = tiles - 1 - tile;
+        seq = nh / heads;
+        head = nh % heads;
     }
 };
 
 template <int D, int W>
 __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv_tile_kernel(Queries q, KvCache c, KvSeqs s, float scale, int causal,
                                                                           Lists list, uint16_t* __restrict__ out, Partial part,
-                                                                          Grid grid) {
+                                                                          Items items) {
     using T = TileShape<D, W>;
     constexpr int NT = D / 32;            // tiles of 32 elements of the output
     constexpr int KC = D / 8, VC = 8;     // 16-byte chunks of a row of K, of V
@@ -173,28 +186,29 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv_tile_kernel(Queri
     __shared__ int wcount[W];
 
     int split, splits;
-    const int item = grid.item(blockIdx.x, part.splits, split, splits);
-    if (item >= grid.items) return;
-    const int nh = item / grid.tiles;
-    const int hq = nh % q.heads, i = nh / q.heads, h = hq / (q.heads / c.heads);
-    const int tile = causal ? grid.tiles - 1 - item % grid.tiles : item % grid.tiles;  // the longest first
+    const int item = items.of(blockIdx.x, part.splits, split, splits);
+    if (item >= items.count) return;
+    int i, head, tile;
+    items.place(item, i, head, tile);
+    const int h = head * items.pack / (q.heads / c.heads);
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, col = lane & 31, half = lane >> 5;
 
-    const int len = s.len(i), count = s.count(i, q.rows), start = s.end(i) - count;
-    const int r0 = tile * T::kRows, row = r0 + wave * 32 + col;
+    const int len = s.len(i), count = s.count(i, q.rows), start = s.end(i) - count, queries = count * items.pack;
+    // this lane's query, its row and its head
+    const int r0 = tile * T::kRows, w0 = r0 + wave * 32, query = w0 + col;
+    const int row = query / items.pack, hq = head * items.pack + query % items.pack;
     // the last token that this lane's query, the wave's last and the workgroup's last see
-    auto last_of = [&](int r) {
-        int x = len - 1;
-        if (causal && start + r < x) x = start + r;
-        return r < count ? x : -1;
+    auto last_of = [&](int x) {
+        const int y = start + x / items.pack, most = causal && y < len - 1 ? y : len - 1;
+        return x < queries ? most : -1;
     };
-    const int last = last_of(row);
-    const int wave_row = r0 + wave * 32 + 31 < count ? r0 + wave * 32 + 31 : count - 1;
-    const int wave_last = wave_row >= r0 + wave * 32 ? last_of(wave_row) : -1;
-    const int tile_row = r0 + T::kRows - 1 < count ? r0 + T::kRows - 1 : count - 1;
-    const int tile_last = tile_row >= r0 ? last_of(tile_row) : -1;
+    const int last = last_of(query);
+    const int wave_query = w0 + 31 < queries ? w0 + 31 : queries - 1;
+    const int wave_last = wave_query >= w0 ? last_of(wave_query) : -1;
+    const int tile_query = r0 + T::kRows - 1 < queries ? r0 + T::kRows - 1 : queries - 1;
+    const int tile_last = tile_query >= r0 ? last_of(tile_query) : -1;
     // below this every query of the wave that is one sees a whole block
-    const int wave_full = wave_last >= 0 ? last_of(r0 + wave * 32) + 1 : 0;
+    const int wave_full = wave_last >= 0 ? last_of(w0) + 1 : 0;
     const int blocks = tile_last < 0 ? 0 : block_of(tile_last) + 1;
 
     bf16x8 qf[D / 16];
@@ -212,7 +226,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv_tile_kernel(Queri
     float m = kLowest, l = 0.0f;
 
     const int32_t* const mine =
-        list.p ? list.p + ((static_cast<int64_t>(i) * list.tiles + r0 / kKvTile) * c.heads + h) * list.top : nullptr;
+        list.p ? list.p + ((static_cast<int64_t>(i) * list.tiles + r0 / items.pack / kKvTile) * c.heads + h) * list.top : nullptr;
     const int total = blocks == 0 ? 0 : mine ? list.top : blocks;
     const int from = static_cast<int>(static_cast<int64_t>(total) * split / splits);
     const int to = static_cast<int>(static_cast<int64_t>(total) * (split + 1) / splits);
@@ -415,10 +429,10 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv_tile_kernel(Queri
 #pragma unroll
             for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
     }
-    const int64_t query = (static_cast<int64_t>(i) * q.rows + row) * q.heads + hq;
+    const int64_t to_row = (static_cast<int64_t>(i) * q.rows + row) * q.heads + hq;
     // register r of o[d]: element 32 d + 8 (r / 4) + 4 half + r % 4 of the query's output
     if (splits > 1) {
-        const int64_t at = part.at(item - grid.whole, split, row - r0);
+        const int64_t at = part.at(item - items.whole, split, query - r0);
         if (half == 0) part.ml[at] = make_float2(m, l);
         if (from >= to) return;
 #pragma unroll
@@ -434,7 +448,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv_tile_kernel(Queri
     for (int d = 0; d < NT; ++d)
 #pragma unroll
         for (int g = 0; g < 4; ++g)
-            *reinterpret_cast<uint2*>(out + query * D + 32 * d + 8 * g + 4 * half) =
+            *reinterpret_cast<uint2*>(out + to_row * D + 32 * d + 8 * g + 4 * half) =
                 make_uint2(bf16x2_bits(o[d][4 * g] * inv, o[d][4 * g + 1] * inv), bf16x2_bits(o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv));
 }
 
@@ -656,7 +670,7 @@ constexpr int kMaxSplits = 64;  // a lane of the join's wave each
 
 // A wave a row of an item: D / 4 lanes a row of sums, 256 / D splits at once.
 template <int D>
-__global__ __launch_bounds__(256) void kv_join_kernel(Partial part, Queries q, int kv_heads, int tiles, int whole, int causal, uint32_t all,
+__global__ __launch_bounds__(256) void kv_join_kernel(Partial part, Queries q, Items items, uint32_t all,
                                                       uint16_t* __restrict__ out) {
     constexpr int L = D / 4, SG = 64 / L;
     const uint32_t x = blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -664,16 +678,11 @@ __global__ __launch_bounds__(256) void kv_join_kernel(Partial part, Queries q, i
     const int lane = threadIdx.x & 63, d = lane % L * 4, sg = lane / L;
     const uint32_t per = part.rows;
     const int item = static_cast<int>(x / per), r = static_cast<int>(x % per);
-    int64_t query;
-    if (tiles == 0) {  // a kv head's group: its queries in the order of rows, then heads
-        const int group = q.heads / kv_heads;
-        query = (static_cast<int64_t>(item / kv_heads) * q.rows + r / group) * q.heads + item % kv_heads * group + r % group;
-    } else {
-        const int nh = (whole + item) / tiles, tile = (whole + item) % tiles;
-        const int row = (causal ? tiles - 1 - tile : tile) * part.rows + r;
-        if (row >= q.rows) return;
-        query = (static_cast<int64_t>(nh / q.heads) * q.rows + row) * q.heads + nh % q.heads;
-    }
+    int i, head, tile;
+    items.place(items.whole + item, i, head, tile);
+    const int y = tile * part.rows + r, row = y / items.pack;
+    if (row >= q.rows) return;
+    const int64_t query = (static_cast<int64_t>(i) * q.rows + row) * q.heads + head * items.pack + y % items.pack;
     const float2 ml = lane < part.splits ? part.ml[part.at(item, lane, r)] : make_float2(kLowest, 0.0f);
     float top = ml.x;
 #pragma unroll
@@ -709,19 +718,26 @@ __global__ __launch_bounds__(256) void kv_join_kernel(Partial part, Queries q, i
 // ------------------------------------------------------------------ what a call runs
 
 struct Plan {
-    bool few;
+    bool few, flat;
     int waves;          // of a tile's workgroup
+    int pack;           // query heads of an item
     int splits, per;    // of a split item; blocks of a split (few)
-    int64_t tiles, items, whole;  // items of one workgroup each come first
-    int64_t part_items() const { return splits > 1 ? items - whole : 0; }
+    int64_t rows;       // queries of an item
+    int64_t heads, tiles, items, whole;  // items of one workgroup each come first
+    int64_t part_rows() const { return splits > 1 ? (items - whole) * splits * rows : 0; }
 };
 
-// Sizes checked by the caller.  blocks: the longest that a query's list or table is.
+// Sizes checked by the caller.
 Plan plan_of(int64_t n, int64_t rows, int64_t heads, int64_t kv, int64_t dim, int64_t blocks, int64_t top) {
     Plan p = {};
-    const int64_t cus = cu_count(), longest = top > 0 ? top : blocks;
-    p.few = rows * (heads / kv) <= kFew;
+    const int64_t cus = cu_count(), group = heads / kv;
+    const int64_t longest = top > 0 ? top : blocks;  // blocks that a query may read
+    p.few = rows * group <= kFew;
     if (p.few) {
+        p.pack = static_cast<int>(group);
+        p.rows = rows * group;
+        p.heads = kv;
+        p.tiles = 1;
         p.items = n * kv;
         // two workgroups a CU: 145 us for 16 uneven sequences against 151 with four, a single query's 51 against 54
         int64_t splits = 2 * cus / p.items;
@@ -730,27 +746,29 @@ Plan plan_of(int64_t n, int64_t rows, int64_t heads, int64_t kv, int64_t dim, in
         if (splits < 1) splits = 1;
         p.per = static_cast<int>((longest + splits - 1) / splits);
         p.splits = p.per > 0 ? static_cast<int>((longest + p.per - 1) / p.per) : 1;
-        if (p.splits < 1) p.splits = 1;
         return p;
     }
-    const int64_t tiles8 = (rows + 255) / 256;
-    p.waves = dim == 256 || top > 0 || n * heads * tiles8 < cus ? 4 : 8;
-    p.tiles = p.waves == 8 ? tiles8 : (rows + 127) / 128;
-    p.items = n * heads * p.tiles;
+    // Rows that leave a tile part empty share it with the other heads of their group (a list is a kv head's).
+    p.pack = rows < kKvTile ? static_cast<int>(group) : 1;
+    p.heads = heads / p.pack;
+    const int64_t queries = rows * p.pack, tiles8 = (queries + 255) / 256;
+    p.waves = dim == 256 || top > 0 || n * p.heads * tiles8 < cus ? 4 : 8;
+    p.rows = 32 * p.waves;
+    p.tiles = (queries + p.rows - 1) / p.rows;
+    p.items = n * p.heads * p.tiles;
     const int64_t slots = (p.waves == 8 || dim == 256 ? 1 : 2) * cus;
+    p.flat = p.items <= slots;
     p.whole = p.items / slots * slots;
     const int64_t rest = p.items - p.whole;
-    int64_t splits = rest > 0 ? slots / rest : 1;
-    if (splits > longest / 8) splits = longest / 8;
+    // A split pays for its join (5 us and the sums' bytes) by the blocks that it saves (1.3 us each, alone on a CU): a CU
+    // each, or a slot each where lists are long.
+    int64_t splits = rest > 0 ? (longest >= 64 ? slots : cus) / rest : 1;
+    if (splits > longest / 4) splits = longest / 4;
     if (splits > kMaxSplits) splits = kMaxSplits;
     if (splits <= 1) p.whole = p.items / 8 * 8, splits = 1;
     p.splits = static_cast<int>(splits);
     return p;
 }
-
-int64_t item_rows(const Plan& p, int64_t rows, int64_t group) { return p.few ? rows * group : 32 * p.waves; }
-
-int64_t partial_rows(const Plan& p, int64_t rows, int64_t group) { return p.part_items() * p.splits * item_rows(p, rows, group); }
 
 bool sizes_ok(int64_t n, int64_t rows, int64_t heads, int64_t kv, int64_t dim, int64_t blocks, int64_t top) {
     int64_t q;
@@ -766,22 +784,20 @@ using namespace h3mi;
 extern "C" int64_t h3mi_kv_attention_workspace(int64_t n, int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim, int64_t blocks,
                                                int64_t top) {
     if (!sizes_ok(n, rows, heads, kv_heads, dim, blocks, top) || n == 0 || rows == 0) return 0;
-    return partial_rows(plan_of(n, rows, heads, kv_heads, dim, blocks, top), rows, heads / kv_heads) * (dim * 4 + 8);
+    return plan_of(n, rows, heads, kv_heads, dim, blocks, top).part_rows() * (dim * 4 + 8);
 }
 
 namespace {
 
 template <int D, int W>
-int launch_tiles(const Plan& p, const Queries& q, const KvCache& c, const KvSeqs& s, float scale, int causal, const Lists& list, uint16_t* out,
-                 const Partial& part, hipStream_t stream) {
-    const int64_t rest = (p.items - p.whole) * p.splits, rest_chunk = (rest + 7) / 8;
+int launch_tiles(const Items& items, const Queries& q, const KvCache& c, const KvSeqs& s, float scale, int causal, const Lists& list,
+                 uint16_t* out, const Partial& part, hipStream_t stream) {
     int64_t groups;
-    if (!launchable(p.whole + rest_chunk * 8, 1, 1, 64 * W, &groups)) return fail(H3MI_EINVAL, "kv_attention: too many rows for one call");
-    const Grid grid = {static_cast<int>(p.tiles), static_cast<int>(p.items), static_cast<int>(p.whole), static_cast<int>(p.whole / 8),
-                       static_cast<int>(rest_chunk)};
+    if (!launchable(items.whole + int64_t{8} * items.rest_chunk, 1, 1, 64 * W, &groups))
+        return fail(H3MI_EINVAL, "kv_attention: too many rows for one call");
     const auto fn = kv_tile_kernel<D, W>;
     constexpr int lds = TileShape<D, W>::kLds;
-    hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(groups)), dim3(64 * W), lds, stream, q, c, s, scale, causal, list, out, part, grid);
+    hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(groups)), dim3(64 * W), lds, stream, q, c, s, scale, causal, list, out, part, items);
     return check_launch("kv_attention");
 }
 
@@ -804,13 +820,17 @@ extern "C" int h3mi_kv_attention_bf16(const uint16_t* q, int64_t rows, int64_t h
     const int64_t n = seqs->n, dim = cache->dim;
     if (!sizes_ok(n, rows, heads, cache->heads, dim, seqs->blocks, top)) return fail(H3MI_EINVAL, "kv_attention: too many rows for one call");
     const Plan p = plan_of(n, rows, heads, cache->heads, dim, seqs->blocks, top);
-    const int64_t group = heads / cache->heads, part_rows = partial_rows(p, rows, group), need = part_rows * (dim * 4 + 8);
+    const int64_t part_rows = p.part_rows(), need = part_rows * (dim * 4 + 8);
+    const int64_t rest = (p.items - p.whole) * p.splits;
+    if (p.items > (1 << 30) || rest > (1 << 30)) return fail(H3MI_EINVAL, "kv_attention: too many rows for one call");
     if (need > 0 && (!workspace || workspace_bytes < need))
         return fail(H3MI_EINVAL, "kv_attention: workspace of %lld bytes, %lld needed", (long long)(workspace ? workspace_bytes : 0), (long long)need);
     if (!aligned(workspace, 16)) return fail(H3MI_EALIGN, "kv_attention: workspace must be 16-byte aligned");
     const Queries qs = {q, ld_q, bs_q, static_cast<int>(rows), static_cast<int>(heads)};
     const Lists list = {blocks, static_cast<int>(top), static_cast<int>((rows + kKvTile - 1) / kKvTile)};
-    Partial part = {static_cast<float*>(workspace), nullptr, p.splits, static_cast<int>(item_rows(p, rows, group))};
+    Partial part = {static_cast<float*>(workspace), nullptr, p.splits, static_cast<int>(p.rows)};
+    const Items items = {static_cast<int>(p.tiles), static_cast<int>(p.heads), p.pack, static_cast<int>(p.rows), static_cast<int>(p.items),
+                         static_cast<int>(p.whole), static_cast<int>(p.whole / 8), static_cast<int>((rest + 7) / 8), p.flat, causal != 0 && !p.few};
     if (need > 0) part.ml = reinterpret_cast<float2*>(part.o + part_rows * dim);
     const KvCache c = kv_cache(*cache);
     const KvSeqs s = kv_seqs(*seqs);
@@ -824,20 +844,20 @@ extern "C" int h3mi_kv_attention_bf16(const uint16_t* q, int64_t rows, int64_t h
                            p.per);
         rc = check_launch("kv_attention");
     } else if (dim == 64) {
-        rc = p.waves == 8 ? launch_tiles<64, 8>(p, qs, c, s, scale, causal, list, out, part, st)
-                          : launch_tiles<64, 4>(p, qs, c, s, scale, causal, list, out, part, st);
+        rc = p.waves == 8 ? launch_tiles<64, 8>(items, qs, c, s, scale, causal, list, out, part, st)
+                          : launch_tiles<64, 4>(items, qs, c, s, scale, causal, list, out, part, st);
     } else if (dim == 128) {
-        rc = p.waves == 8 ? launch_tiles<128, 8>(p, qs, c, s, scale, causal, list, out, part, st)
-                          : launch_tiles<128, 4>(p, qs, c, s, scale, causal, list, out, part, st);
+        rc = p.waves == 8 ? launch_tiles<128, 8>(items, qs, c, s, scale, causal, list, out, part, st)
+                          : launch_tiles<128, 4>(items, qs, c, s, scale, causal, list, out, part, st);
     } else {
-        rc = launch_tiles<256, 4>(p, qs, c, s, scale, causal, list, out, part, st);
+        rc = launch_tiles<256, 4>(items, qs, c, s, scale, causal, list, out, part, st);
     }
     if (rc || p.splits == 1) return rc;
-    const int64_t all = p.part_items() * part.rows;
+    const int64_t all = (p.items - p.whole) * p.rows;
     int64_t groups;
     if (!launchable((all + 3) / 4, 1, 1, 256, &groups)) return fail(H3MI_EINVAL, "kv_attention: too many rows for one call");
     const auto join = dim == 64 ? kv_join_kernel<64> : dim == 128 ? kv_join_kernel<128> : kv_join_kernel<256>;
-    hipLaunchKernelGGL(join, dim3(static_cast<unsigned>(groups)), dim3(256), 0, st, part, qs, c.heads, static_cast<int>(p.tiles),
-                       static_cast<int>(p.whole), causal, static_cast<uint32_t>(all), out);
+    hipLaunchKernelGGL(join, dim3(static_cast<unsigned>(groups)), dim3(256), 0, st, part, qs, items,
+                       static_cast<uint32_t>(all), out);
     return check_launch("kv_attention");
 }
