@@ -291,8 +291,9 @@ int h3mi_kv_select(const uint16_t* q, int64_t rows, int64_t heads, int64_t ld_q,
 /* out (bf16 [n, rows, heads, dim], contiguous) <- softmax(scale q k^T) v over the
  * tokens of each sequence; query head h reads kv head h / (heads / kv heads).
  * causal: row r sees tokens up to its own.  blocks (NULL: all) as h3mi_kv_select
- * gives them: a row sees the tokens of its tile's blocks alone; entries outside the
- * sequence are passed over, and a tile's entries have to be distinct.  Rows that
+ * gives them, top < 2^25: a row sees the tokens of its tile's blocks alone; entries
+ * outside the sequence are passed over, and a tile's entries have to be distinct (one
+ * that comes twice counts twice).  Rows that
  * see no token, and rows behind counts, are 0.  Sums and statistics are fp32, the
  * products' operands bf16 (8-bit keys and values are exact in it, probabilities
  * are rounded to it).

@@ -820,7 +820,7 @@ extern "C" int h3mi_kv_attention_bf16(const uint16_t* q, int64_t rows, int64_t h
     if (int e = kv_check_rows("kv_attention", "q", q, rows, heads, cache->dim, seqs->n, ld_q, bs_q)) return e;
     if (!(scale == scale) || scale - scale != 0.0f) return fail(H3MI_EINVAL, "kv_attention: scale is not finite");
     if (!blocks) top = 0;
-    if (blocks && (top < 1 || top > 0x7FFFFFFF)) return fail(H3MI_EINVAL, "kv_attention: top=%lld", (long long)top);
+    if (blocks && (top < 1 || top >= (1 << 25))) return fail(H3MI_EINVAL, "kv_attention: top=%lld", (long long)top);
     if (seqs->n == 0 || rows == 0) return ok();
     if (!out) return fail(H3MI_EINVAL, "kv_attention: null out");
     if (!aligned(out, 16) || !aligned(blocks, 4)) return fail(H3MI_EALIGN, "kv_attention: out must be 16-byte aligned, blocks 4-byte");

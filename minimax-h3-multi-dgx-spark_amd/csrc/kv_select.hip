@@ -250,7 +250,8 @@ extern "C" int h3mi_kv_select(const uint16_t* q, int64_t rows, int64_t heads, in
     if (!launchable(seqs->n, tiles, cache->heads, 1024, &groups)) return fail(H3MI_EINVAL, "kv_select: too many rows for one call");
     // one workgroup a CU or less: more of its own waves (2048 blocks, 32 groups: 21.0 us against 26; 150 blocks, 240 groups
     // 11.2 against 8.3, 609 blocks, 1064 groups 25.3 against 29.3 with 512)
-    const int threads = 2 * groups <= cu_count() ? 1024 : 256;
+    // (whose partial sums leave LDS for 16384 blocks' keys at every dim)
+    const int threads = 2 * groups <= cu_count() && seqs->blocks <= kMaxSelect / 2 ? 1024 : 256;
     const auto fn = threads == 1024 ? (D == 64 ? kv_select_kernel<64, 1024> : D == 128 ? kv_select_kernel<128, 1024> : kv_select_kernel<256, 1024>)
                                     : (D == 64 ? kv_select_kernel<64, 256> : D == 128 ? kv_select_kernel<128, 256> : kv_select_kernel<256, 256>);
     hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(groups)), dim3(threads), static_cast<unsigned>(seqs->blocks * 4),

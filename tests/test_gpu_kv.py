@@ -344,16 +344,30 @@ def test_select_ties_and_specials():
             assert np.array_equal(got.cpu().numpy(), want), (scale, top)
 
 
-def test_select_long():
-    """The longest table, and one page under many blocks: all scores equal but one."""
-    ref = R.Cache(3, 1, 64, seed=32)
+@pytest.mark.parametrize("dim", [64, 256])
+@pytest.mark.parametrize("blocks", [16384, 16385, 32768])
+def test_select_long(dim, blocks):
+    """The longest tables, and one page under many blocks: all scores equal but one."""
+    ref = R.Cache(3, 1, dim, seed=32)
     ref.ksum[0], ref.ks[:] = 1, 0.01
     ref.ksum[1] = 2
-    tables = np.zeros((1, 32768), np.int32)
-    tables[0, 30001] = 1
-    q = np.ones((1, 1, 1, 64), np.float32)
-    got = _h().kv_select(_bf(q), ref.to(), _i32(tables), _i32([32768 * 64]), 100).cpu().numpy().reshape(-1)
-    assert got.tolist() == list(range(99)) + [30001]
+    tables = np.zeros((1, blocks), np.int32)
+    tables[0, 16001] = 1
+    q = np.ones((1, 1, 1, dim), np.float32)
+    got = _h().kv_select(_bf(q), ref.to(), _i32(tables), _i32([blocks * 64]), 100).cpu().numpy().reshape(-1)
+    assert got.tolist() == list(range(99)) + [16001]
+
+
+def test_select_with_more_than_there_is():
+    """A pool without pages, and top at its largest."""
+    h = _h()
+    q = torch.ones(1, 1, 2, 64, dtype=torch.bfloat16, device=DEV)
+    none = h.kv_cache(0, 2, 64)
+    assert (h.kv_select(q, none, _i32([[0, 0]]), _i32([128]), 5) == -1).all()
+    assert (h.kv_attention(q, none, _i32([[0, 0]]), _i32([128])) == 0).all()
+    assert (h.kv_read(none, _i32([[0, 0]]), _i32([128]), 128)[0] == 0).all()
+    got = h.kv_select(q, h.kv_cache(2, 2, 64), _i32([[0, 1]]), _i32([128]), 32768)
+    assert got.shape == (1, 1, 2, 32768) and got[0, 0, 0, :3].tolist() == [0, 1, -1] and (got[..., 2:] == -1).all()
 
 
 @pytest.mark.parametrize("heads,kv,dim", [(3, 3, 64), (10, 2, 128), (6, 2, 256), (20, 1, 64)])
@@ -448,6 +462,24 @@ def test_steps_captured_and_replayed(S):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want)), r
+
+
+@pytest.mark.parametrize("rows", [1, 40, 300])
+def test_another_stream(rows):
+    """Calls on a side stream, whose results and workspace are freed and reused at once, against the default stream."""
+    h = _h()
+    rng = np.random.default_rng(71)
+    ref, tables, q = _case(rng, 4, 4, 128, 1, rows, 120, seed=71)
+    c, t, lens, x = ref.to(), _i32(tables), _i32([7600]), _bf(q)
+    want = h.kv_attention(x, c, t, lens)
+    blocks = h.kv_select(x, c, t, lens, 9)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            assert torch.equal(h.kv_attention(x, c, t, lens), want)
+            assert torch.equal(h.kv_select(x, c, t, lens, 9), blocks)
+    torch.cuda.current_stream().wait_stream(side)
 
 
 def test_two_graphs_share_no_workspace():

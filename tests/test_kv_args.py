@@ -60,7 +60,7 @@ def test_rows(fn, kw, code, msg):
     ("attention", dict(heads=5), 1, "multiple of the cache's"), ("select", dict(top=0), 1, "top=0"), ("select", dict(top=32769), 1, "top=32769"),
     ("select", dict(out=None), 1, "null blocks"), ("select", dict(out=2), 2, "aligned"), ("attention", dict(out=None), 1, "null out"),
     ("attention", dict(out=8), 2, "aligned"), ("attention", dict(scale=float("nan")), 1, "scale"), ("attention", dict(scale=float("inf")), 1, "scale"),
-    ("attention", dict(blocks=4096, top=0), 1, "top=0"), ("attention", dict(blocks=4098), 2, "aligned"),
+    ("attention", dict(blocks=4096, top=0), 1, "top=0"), ("attention", dict(blocks=4096, top=1 << 25), 1, "top="), ("attention", dict(blocks=4098), 2, "aligned"),
 ])
 def test_each(fn, kw, code, msg):
     rc, m = _call(fn, **kw)
@@ -90,3 +90,43 @@ def test_null_structures(fn):
           "select": lambda: L.h3mi_kv_select(P(4096), 1, 2, 256, 256, None, None, 1, 0, P(8192), None),
           "attention": lambda: L.h3mi_kv_attention_bf16(P(4096), 1, 2, 256, 256, None, None, ctypes.c_float(1), 0, None, 0, P(8192), None, 0, None)}[fn]()
     assert rc == 1 and "null cache or sequences" in L.h3mi_last_error().decode()
+
+
+@pytest.mark.parametrize("rows,heads,kv,dim,blocks,top", [(1, 56, 56, 128, 309, 0), (1, 40, 8, 128, 2048, 64), (40, 40, 8, 128, 141, 0),
+                                                          (4800, 56, 56, 128, 309, 0), (2401, 56, 56, 128, 609, 100)])
+def test_workspace(rows, heads, kv, dim, blocks, top):
+    """A call that splits its work asks for whole partial rows, and refuses less than it asked for."""
+    from h3mi import _lib
+    need = _lib.lib.h3mi_kv_attention_workspace(1, rows, heads, kv, dim, blocks, top)
+    assert need > 0 and need % (dim * 4 + 8) == 0
+    kw = dict(rows=rows, heads=heads, ld=heads * dim, bs=rows * heads * dim, blocks=4096 if top else None, top=top)
+    seqs = dict(n=1, blocks=blocks)
+    cache = dict(heads=kv, dim=dim, v=1 << 40)
+    for work, size in ((None, need), (1 << 30, need - 1), (1 << 30, 0)):
+        rc, m = _call("attention", cache, seqs, work=work, size=size, **kw)
+        assert rc == 1 and "workspace" in m
+    rc, m = _call("attention", cache, seqs, work=(1 << 30) + 8, size=need, **kw)
+    assert rc == 2 and "workspace" in m
+
+
+@pytest.mark.parametrize("a", [(0, 1, 2, 2, 128, 5, 0), (1, 0, 2, 2, 128, 5, 0), (-1, 1, 2, 2, 128, 5, 0), (1, 1, 3, 2, 128, 5, 0),
+                               (1, 1, 2, 0, 128, 5, 0), (1, 1, 2, 2, 96, 5, 0), (1 << 62, 1 << 30, 65536, 1, 256, 5, 0), (1, 1, 2, 2, 128, -5, 0)])
+def test_workspace_of_nothing(a):
+    from h3mi import _lib
+    assert _lib.lib.h3mi_kv_attention_workspace(*a) == 0
+
+
+def test_cpu_tensors_are_refused():
+    """The Python functions refuse host tensors before a kernel could see their addresses."""
+    import torch
+
+    import h3mi
+    c = h3mi.kv_cache(2, 2, 64, device="cpu")
+    t, lens = torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    x = torch.zeros(1, 1, 2, 64, dtype=torch.bfloat16)
+    for f in (lambda: h3mi.kv_write_(c, x, x, t, lens), lambda: h3mi.kv_read(c, t, lens, 1), lambda: h3mi.kv_select(x, c, t, lens, 1),
+              lambda: h3mi.kv_attention(x, c, t, lens)):
+        with pytest.raises(ValueError, match="GPU"):
+            f()
+    with pytest.raises(ValueError, match="dim"):
+        h3mi.kv_cache(2, 2, 100, device="cpu")
