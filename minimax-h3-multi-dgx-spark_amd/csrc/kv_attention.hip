@@ -129,7 +129,6 @@ __device__ __forceinline__ int chunk_at(int row, int ch) {
     return CH == 8 ? ch ^ ((row >> 1) & 7) : ch ^ (row & 15);
 }
 
-constexpr int kAhead = 8;
 constexpr int kSchedMfma = 0x8, kSchedLdsRead = 0x100;  // instruction classes of sched_group_barrier
 
 template <int D, int W>
@@ -139,7 +138,12 @@ struct TileShape {
     static constexpr int kKeyBytes = kKvBlock * D * 2;
     static constexpr int kLds = 4 * kKeyBytes;
     static constexpr int kGroups = W == 8 ? 2 : 1;
-    static constexpr int kLoads = kKvBlock * D / 8 / kThreads;  // 8-byte pieces of K (and of V) a thread
+    // MFMAs that an operand is read ahead; 8 waves step together, and 4 there cost them 0.5%, 8 elsewhere gain nothing
+    static constexpr int kAhead = W == 8 ? 8 : 4;
+    // A thread's pieces of K (and of V): 16 bytes, or 8 where that would leave threads without one.
+    using Piece = std::conditional_t<(kKvBlock * D >= 16 * kThreads), uint4, uint2>;
+    static constexpr int kPiece = sizeof(Piece);
+    static constexpr int kLoads = kKvBlock * D / kPiece / kThreads;
 };
 
 // The items of a launch: tiles of the queries of a head, or (pack > 1) of the queries of all
@@ -231,28 +235,35 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv_tile_kernel(Queri
     const int from = static_cast<int>(static_cast<int64_t>(total) * split / splits);
     const int to = static_cast<int>(static_cast<int64_t>(total) * (split + 1) / splits);
 
-    // Bytes of a block into registers, and as bf16 into LDS.
-    uint2 kr[T::kLoads], vr[T::kLoads];
-    auto load = [&](const int8_t* from_pages, int page, uint2 (&to_regs)[T::kLoads]) __attribute__((always_inline)) {
+    // Bytes of a block into registers, and as bf16 into LDS: 8 of them a chunk.
+    using Piece = typename T::Piece;
+    Piece kr[T::kLoads], vr[T::kLoads];
+    auto load = [&](const int8_t* from_pages, int page, Piece (&to_regs)[T::kLoads]) __attribute__((always_inline)) {
         const int8_t* const at = from_pages + (static_cast<int64_t>(page) * c.heads + h) * (kKvBlock * D);  // uniform
 #pragma unroll
-        for (int j = 0; j < T::kLoads; ++j) to_regs[j] = *reinterpret_cast<const uint2*>(at + static_cast<uint32_t>(t + j * T::kThreads) * 8);
+        for (int j = 0; j < T::kLoads; ++j) to_regs[j] = *reinterpret_cast<const Piece*>(at + static_cast<uint32_t>(t + j * T::kThreads) * T::kPiece);
+    };
+    auto stage = [&](uint8_t* buf, const Piece (&regs)[T::kLoads], auto chunks, auto swap) __attribute__((always_inline)) {
+        constexpr int CH = chunks, PC = T::kPiece / 8;  // chunks of a row, of a piece
+#pragma unroll
+        for (int j = 0; j < T::kLoads; ++j) {
+            const int piece = t + j * T::kThreads, line = piece / (CH / PC), ch = piece % (CH / PC) * PC;
+            // token bits 2 and 3 change places: an MFMA row's registers are then runs of 8 tokens
+            const int row = swap ? (line & ~12) | ((line & 4) << 1) | ((line & 8) >> 1) : line;
+            uint8_t* const to_row = buf + row * (CH * 16);
+            if constexpr (PC == 2) {
+                *reinterpret_cast<uint4*>(to_row + chunk_at<CH>(row, ch) * 16) = ints_bf16(make_uint2(regs[j].x, regs[j].y));
+                *reinterpret_cast<uint4*>(to_row + chunk_at<CH>(row, ch + 1) * 16) = ints_bf16(make_uint2(regs[j].z, regs[j].w));
+            } else {
+                *reinterpret_cast<uint4*>(to_row + chunk_at<CH>(row, ch) * 16) = ints_bf16(regs[j]);
+            }
+        }
     };
     auto stage_k = [&](int which) __attribute__((always_inline)) {
-#pragma unroll
-        for (int j = 0; j < T::kLoads; ++j) {
-            const int piece = t + j * T::kThreads, tok = piece / KC, kc = piece % KC;
-            // token bits 2 and 3 change places: an MFMA row's registers are then runs of 8 tokens
-            const int row = (tok & ~12) | ((tok & 4) << 1) | ((tok & 8) >> 1);
-            *reinterpret_cast<uint4*>(smem + (which & 1) * T::kKeyBytes + row * (D * 2) + chunk_at<KC>(row, kc) * 16) = ints_bf16(kr[j]);
-        }
+        stage(smem + (which & 1) * T::kKeyBytes, kr, std::integral_constant<int, KC>{}, std::true_type{});
     };
     auto stage_v = [&](int which) __attribute__((always_inline)) {
-#pragma unroll
-        for (int j = 0; j < T::kLoads; ++j) {
-            const int piece = t + j * T::kThreads, row = piece / VC, vc = piece % VC;
-            *reinterpret_cast<uint4*>(smem + (2 + (which & 1)) * T::kKeyBytes + row * (kKvBlock * 2) + chunk_at<VC>(row, vc) * 16) = ints_bf16(vr[j]);
-        }
+        stage(smem + (2 + (which & 1)) * T::kKeyBytes, vr, std::integral_constant<int, VC>{}, std::false_type{});
     };
     auto arrive = [&]() __attribute__((always_inline)) {
         wait_lgkm0();
@@ -324,9 +335,9 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv_tile_kernel(Queri
                 const uint32_t at = D == 256 ? (vx ^ (w * 32)) + d * (32 * kKvBlock * 2) : row * (kKvBlock * 2) + chunk_at<VC>(row, 2 * w + half) * 16;
                 return frag(*reinterpret_cast<const uint4*>(vb + at));
             };
-            bf16x8 a[kAhead];
+            bf16x8 a[T::kAhead];
 #pragma unroll
-            for (int x = 0; x < kAhead; ++x) a[x] = fetch(x);
+            for (int x = 0; x < T::kAhead; ++x) a[x] = fetch(x);
             if constexpr (NK > 0) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) sc[0][r] = sc[1][r] = 0.0f;
@@ -334,16 +345,16 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv_tile_kernel(Queri
 #pragma unroll
             for (int x = 0; x < N; ++x) {
                 if (x < NK)
-                    sc[x % 2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[x % kAhead], qf[x / 2], sc[x % 2], 0, 0, 0);
+                    sc[x % 2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[x % T::kAhead], qf[x / 2], sc[x % 2], 0, 0, 0);
                 else
-                    o[(x - NK) % NT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[x % kAhead], p[(x - NK) / NT], o[(x - NK) % NT], 0, 0, 0);
-                if (x + kAhead < N) a[x % kAhead] = fetch(x + kAhead);
+                    o[(x - NK) % NT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[x % T::kAhead], p[(x - NK) / NT], o[(x - NK) % NT], 0, 0, 0);
+                if (x + T::kAhead < N) a[x % T::kAhead] = fetch(x + T::kAhead);
             }
-            __builtin_amdgcn_sched_group_barrier(kSchedLdsRead, kAhead, 0);
+            __builtin_amdgcn_sched_group_barrier(kSchedLdsRead, T::kAhead, 0);
 #pragma unroll
             for (int x = 0; x < N; ++x) {
                 __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
-                if (x + kAhead < N) __builtin_amdgcn_sched_group_barrier(kSchedLdsRead, 1, 0);
+                if (x + T::kAhead < N) __builtin_amdgcn_sched_group_barrier(kSchedLdsRead, 1, 0);
             }
         };
         auto softmax = [&]() __attribute__((always_inline)) {

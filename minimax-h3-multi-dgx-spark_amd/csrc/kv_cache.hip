@@ -170,7 +170,21 @@ __global__ __launch_bounds__(2 * D) void kv_write_kernel(Rows kin, Rows vin, KvC
         }
     }
     const bool first = start <= base;  // no token of the block is older
-    const float old_k = first ? 0.0f : c.ks[tile], old_v = first ? 0.0f : c.vs[tile];
+    int8_t* const kout = c.k + tile * (kKvBlock * D);
+    int8_t* const vout = c.v + tile * (kKvBlock * D);
+    // what an older block held, asked for before the maximum is known
+    float old_k = 0.0f, old_v = 0.0f;
+    uint2 ko[4] = {};
+    uint32_t vo[8] = {};
+    if (!first) {
+        old_k = c.ks[tile], old_v = c.vs[tile];
+        if (base + 4 * quad < start) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) ko[j] = *reinterpret_cast<const uint2*>(kout + (4 * quad + j) * D + col);
+#pragma unroll
+            for (int p = 0; p < 8; ++p) vo[p] = *reinterpret_cast<const uint32_t*>(vout + (col + p) * kKvBlock + 4 * quad);
+        }
+    }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const uint32_t a[4] = {kx[j].x, kx[j].y, kx[j].z, kx[j].w}, e[4] = {vx[j].x, vx[j].y, vx[j].z, vx[j].w};
@@ -206,8 +220,6 @@ __global__ __launch_bounds__(2 * D) void kv_write_kernel(Rows kin, Rows vin, KvC
     const float rk = 1.0f / sk.s, rv = 1.0f / sv.s;
     const bool live_k = sk.s > 0.0f && __builtin_isfinite(sk.s), live_v = sv.s > 0.0f && __builtin_isfinite(sv.s);
     const bool exact_k = quot_exact(sk.s, rk), exact_v = quot_exact(sv.s, rv);
-    int8_t* const kout = c.k + tile * (kKvBlock * D);
-    int8_t* const vout = c.v + tile * (kKvBlock * D);
     int acc[8] = {};
     uint2 vq[4];
 #pragma unroll
@@ -215,16 +227,14 @@ __global__ __launch_bounds__(2 * D) void kv_write_kernel(Rows kin, Rows vin, KvC
         const int tok = 4 * quad + j;
         uint2 q = make_uint2(0, 0);
         vq[j] = q;
-        uint2* const at = reinterpret_cast<uint2*>(kout + tok * D + col);
         if (fresh[j]) {
             const uint32_t a[4] = {kx[j].x, kx[j].y, kx[j].z, kx[j].w}, e[4] = {vx[j].x, vx[j].y, vx[j].z, vx[j].w};
             if (live_k) q = quant8(a, sk.s, rk, exact_k);
             if (live_v) vq[j] = quant8(e, sv.s, rv, exact_v);
         } else if (kept[j] && live_k && sk.mul != 0.0f) {
-            q = *at;
-            q = make_uint2(refit(q.x, sk.mul), refit(q.y, sk.mul));
+            q = make_uint2(refit(ko[j].x, sk.mul), refit(ko[j].y, sk.mul));
         }
-        store_past(at, q);
+        store_past(kout + tok * D + col, q);
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
             acc[p] += static_cast<int8_t>(q.x >> (8 * p));
@@ -233,16 +243,13 @@ __global__ __launch_bounds__(2 * D) void kv_write_kernel(Rows kin, Rows vin, KvC
     }
     uint32_t w[8];
     transpose4(vq, w);
-    const bool olds = base + 4 * quad < start && live_v && sv.mul != 0.0f;
+    const bool olds = live_v && sv.mul != 0.0f;
     uint32_t mask = 0;  // bytes of the tokens kept
 #pragma unroll
     for (int j = 0; j < 4; ++j) mask |= kept[j] ? 0xFFu << (8 * j) : 0u;
 #pragma unroll
     for (int p = 0; p < 8; ++p) {
-        if (olds) {
-            const uint32_t old = *reinterpret_cast<const uint32_t*>(vout + (col + p) * kKvBlock + 4 * quad);
-            w[p] |= refit(old, sv.mul) & mask;
-        }
+        if (olds && mask) w[p] |= refit(vo[p], sv.mul) & mask;
         vt[(col + p) * kVtStride + quad] = w[p];
         atomicAdd(&sums[col + p], acc[p]);
     }
