@@ -197,12 +197,9 @@ __global__ __launch_bounds__(2 * D) void kv_write_kernel(Rows kin, Rows vin, KvC
     uint32_t km1 = km & 0xFFFFu, vm1 = vm & 0xFFFFu;
     km1 = km1 > (km >> 16) ? km1 : km >> 16;
     vm1 = vm1 > (vm >> 16) ? vm1 : vm >> 16;
-#pragma unroll
-    for (int m = 32; m; m >>= 1) {
-        const uint32_t a = __shfl_xor(km1, m), e = __shfl_xor(vm1, m);
-        km1 = km1 > a ? km1 : a;
-        vm1 = vm1 > e ? vm1 : e;
-    }
+    // (16-bit patterns as whole numbers in fp32)
+    km1 = static_cast<uint32_t>(wave_max(static_cast<float>(km1)));
+    vm1 = static_cast<uint32_t>(wave_max(static_cast<float>(vm1)));
     if ((t & 63) == 0) part[0][t >> 6] = km1, part[1][t >> 6] = vm1;
     if (t < D) sums[t] = 0;
     __syncthreads();
