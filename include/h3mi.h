@@ -283,10 +283,13 @@ int h3mi_kv_read_bf16(uint16_t* k, uint16_t* v, const int32_t* starts, int64_t l
  * It is a whole number's rounding, so no order of summing changes a selection.
  * causal: the blocks with the tile's own tokens come first, later ones are not
  * seen.  Equal scores: the lowest block first; NaN scores come last.  A tile with no
- * rows of its own selects nothing.  top in [1, 32768], seqs->blocks <= 32768. */
+ * rows of its own selects nothing.  top in [1, 32768], seqs->blocks <= 32768.
+ * workspace: h3mi_kv_select_workspace bytes of device memory, 4-byte aligned (NULL
+ * where that is 0), for this call alone until it has run. */
+int64_t h3mi_kv_select_workspace(int64_t n, int64_t rows, int64_t kv_heads, int64_t blocks);
 int h3mi_kv_select(const uint16_t* q, int64_t rows, int64_t heads, int64_t ld_q, int64_t bs_q,
                    const h3mi_kv_cache* cache, const h3mi_kv_seqs* seqs, int64_t top, int causal,
-                   int32_t* blocks, void* stream);
+                   int32_t* blocks, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* out (bf16 [n, rows, heads, dim], contiguous) <- softmax(scale q k^T) v over the
  * tokens of each sequence; query head h reads kv head h / (heads / kv heads).

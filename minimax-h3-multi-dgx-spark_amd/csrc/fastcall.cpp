@@ -497,13 +497,15 @@ PyObject* kv_select(PyObject*, PyObject* const* v, Py_ssize_t n) {
     int64_t top = 0;
     int causal = 0;
     if (!a.ok || !whole(v[4], &top) || top < 1 || !truth(v[5], &causal)) Py_RETURN_NONE;
-    at::Tensor out;
+    at::Tensor out, work;
     int rc;
     {
         pybind11::gil_scoped_release nogil;
         out = a.empty({kv.s.n, (q.rows + H3MI_KV_TILE - 1) / H3MI_KV_TILE, kv.c.heads, top}, c10::kInt);
+        const int64_t need = h3mi_kv_select_workspace(kv.s.n, q.rows, kv.c.heads, kv.s.blocks);
+        if (need > 0) work = a.empty({need}, c10::kByte);
         rc = h3mi_kv_select(u16(q.t), q.rows, q.heads, q.ld, q.bs, &kv.c, &kv.s, top, causal, static_cast<int32_t*>(out.data_ptr()),
-                            a.stream());
+                            need > 0 ? work.data_ptr() : nullptr, need, a.stream());
     }
     return rc ? raise_status(rc) : THPVariable_Wrap(out);
     H3MI_END

@@ -9,7 +9,9 @@
 // A workgroup takes one tile of one kv head: it pools the queries, scores every block
 // (dim / 8 lanes a block, 16 bytes of k_sum each, v_dot2_i32_i16), keeps the scores as
 // ordered 32-bit keys in LDS, finds the last selected key by four passes over 8 bits of
-// it, and writes the selected blocks in order.
+// it, and writes the selected blocks in order.  Few tiles over long tables, whose scoring
+// would wait on a few CUs' loads, score in a launch of their own, a workgroup for every
+// kChunk blocks, and the keys pass through memory.
 #include "kv.h"
 
 namespace h3mi {
@@ -40,10 +42,13 @@ __device__ __forceinline__ uint32_t key_of(float s) {
     return k < 2u ? 2u : k;
 }
 
-template <int D, int THREADS>
+enum Part { kWhole, kScores, kSelection };
+constexpr int kChunk = 256;
+
+template <int D, int THREADS, Part PART>
 __global__ __launch_bounds__(THREADS) void kv_select_kernel(const uint16_t* __restrict__ q, int64_t ld, int64_t bs, KvCache c,
-                                                                KvSeqs s, int rows, int heads, int top, int causal, int tiles,
-                                                                int32_t* __restrict__ out) {
+                                                            KvSeqs s, int rows, int heads, int top, int causal, int tiles, int chunks,
+                                                            uint32_t* __restrict__ all_keys, int32_t* __restrict__ out) {
     constexpr int CH = D / 8, kSelWaves = THREADS / 64;
     constexpr int GROUPS = THREADS / CH;  // row groups while pooling, blocks at once while scoring
     extern __shared__ uint32_t keys[];
@@ -57,7 +62,9 @@ __global__ __launch_bounds__(THREADS) void kv_select_kernel(const uint16_t* __re
 
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     // an XCD takes whole heads, whose sums its L2 then holds for every tile
-    const int at_all = xcd_item(), tile = at_all % tiles, h = at_all / tiles % c.heads, i = at_all / tiles / c.heads;
+    const int at_all = xcd_item() / chunks, chunk = xcd_item() % chunks;
+    uint32_t* const my_keys = all_keys + static_cast<int64_t>(at_all) * s.blocks;
+    const int tile = at_all % tiles, h = at_all / tiles % c.heads, i = at_all / tiles / c.heads;
     int32_t* const to = out + ((static_cast<int64_t>(i) * tiles + tile) * c.heads + h) * top;
     const int len = s.len(i), count = s.count(i, rows), group = heads / c.heads;
     const int r0 = tile * kKvTile, live = count - r0 < kKvTile ? count - r0 : kKvTile;
@@ -67,85 +74,95 @@ __global__ __launch_bounds__(THREADS) void kv_select_kernel(const uint16_t* __re
     if (causal && last < len) seen = last < 0 ? 0 : block_of(last) + 1;
     if (live <= 0 || c.pages == 0) seen = 0;
     if (seen == 0) {
-        for (int j = t; j < top; j += THREADS) to[j] = -1;
+        if constexpr (PART != kScores)
+            for (int j = t; j < top; j += THREADS) to[j] = -1;
         return;
     }
-
-    const int ch = t % CH, grp = t / CH;
-    {
-        double p[8] = {};
-        for (int x = grp; x < live * group; x += GROUPS) {
-            const int64_t r = r0 + x / group;
-            const int hq = h * group + x % group;
-            const uint4 w = *reinterpret_cast<const uint4*>(q + i * bs + r * ld + static_cast<int64_t>(hq) * D + ch * 8);
-            const uint32_t a[4] = {w.x, w.y, w.z, w.w};
+    if constexpr (PART == kSelection) {
+        for (int b = t; b < seen; b += THREADS) keys[b] = my_keys[b];
+    } else {
+        // the blocks to score: keys[0] is block low's
+        const int low = chunk * kChunk, high = PART == kScores && low + kChunk < seen ? low + kChunk : seen;
+        if (low >= high) return;
+        const int ch = t % CH, grp = t / CH;
+        {
+            double p[8] = {};
+            for (int x = grp; x < live * group; x += GROUPS) {
+                const int64_t r = r0 + x / group;
+                const int hq = h * group + x % group;
+                const uint4 w = *reinterpret_cast<const uint4*>(q + i * bs + r * ld + static_cast<int64_t>(hq) * D + ch * 8);
+                const uint32_t a[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                p[2 * j] += bf16_lo(a[j]);
-                p[2 * j + 1] += bf16_hi(a[j]);
+                for (int j = 0; j < 4; ++j) {
+                    p[2 * j] += bf16_lo(a[j]);
+                    p[2 * j + 1] += bf16_hi(a[j]);
+                }
+            }
+            // the row groups of a wave, then the waves through LDS
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+#pragma unroll
+                for (int m = 32; m >= CH; m >>= 1) p[j] += __shfl_xor(p[j], m);
+                if (lane < CH) part[wave][ch * 8 + j] = p[j];
             }
         }
-        // the row groups of a wave, then the waves through LDS
+        __syncthreads();
+        if (t < D) {
+            double p = 0.0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-#pragma unroll
-            for (int m = 32; m >= CH; m >>= 1) p[j] += __shfl_xor(p[j], m);
-            if (lane < CH) part[wave][ch * 8 + j] = p[j];
+            for (int w = 0; w < kSelWaves; ++w) p += part[w][t];
+            pool[t] = p;
         }
-    }
-    __syncthreads();
-    if (t < D) {
-        double p = 0.0;
+        __syncthreads();
+        double m = t < D ? fabs(pool[t]) : 0.0;
+        bool bad = !(m < __builtin_inf());  // a NaN or an infinity
 #pragma unroll
-        for (int w = 0; w < kSelWaves; ++w) p += part[w][t];
-        pool[t] = p;
-    }
-    __syncthreads();
-    double m = t < D ? fabs(pool[t]) : 0.0;
-    bool bad = !(m < __builtin_inf());  // a NaN or an infinity
+        for (int x = 32; x; x >>= 1) m = fmax(m, __shfl_xor(m, x));
+        bad = __any(bad);
+        if (lane == 0) wmax[wave] = bad ? __builtin_inf() : m;
+        __syncthreads();
+        m = 0.0;
 #pragma unroll
-    for (int x = 32; x; x >>= 1) m = fmax(m, __shfl_xor(m, x));
-    bad = __any(bad);
-    if (lane == 0) wmax[wave] = bad ? __builtin_inf() : m;
-    __syncthreads();
-    m = 0.0;
-#pragma unroll
-    for (int w = 0; w < kSelWaves; ++w) m = fmax(m, wmax[w]);
-    if (t < D) qi[t] = m > 0.0 && m < __builtin_inf() ? static_cast<int16_t>(rint(pool[t] * 1023.0 / m)) : int16_t{0};
-    __syncthreads();
+        for (int w = 0; w < kSelWaves; ++w) m = fmax(m, wmax[w]);
+        if (t < D) qi[t] = m > 0.0 && m < __builtin_inf() ? static_cast<int16_t>(rint(pool[t] * 1023.0 / m)) : int16_t{0};
+        __syncthreads();
 
-    const uint4 qw = *reinterpret_cast<const uint4*>(qi + ch * 8);
-    const int own = first < 0 ? 0 : block_of(first);
-    // The blocks' pages first, so that nothing but the sums' own latency stands in the way of kBatch of them at once.
-    for (int b = t; b < seen; b += THREADS) keys[b] = static_cast<uint32_t>(s.page(i, b, c.pages));
-    __syncthreads();
-    const int waves_up = (seen + GROUPS - 1) / GROUPS * GROUPS;  // whole groups, so that every lane takes part
-    for (int b0 = grp; b0 < waves_up; b0 += GROUPS * kBatch) {
-        uint4 k[kBatch];
+        const uint4 qw = *reinterpret_cast<const uint4*>(qi + ch * 8);
+        const int own = first < 0 ? 0 : block_of(first);
+        // The blocks' pages first, so that nothing but the sums' own latency stands in the way of kBatch of them at once.
+        for (int b = low + t; b < high; b += THREADS) keys[b - low] = static_cast<uint32_t>(s.page(i, b, c.pages));
+        __syncthreads();
+        const int up = low + (high - low + GROUPS - 1) / GROUPS * GROUPS;  // whole groups, so that every lane takes part
+        for (int b0 = low + grp; b0 < up; b0 += GROUPS * kBatch) {
+            uint4 k[kBatch];
 #pragma unroll
-        for (int x = 0; x < kBatch; ++x) {
-            const int b = b0 + x * GROUPS, page = b < seen ? static_cast<int>(keys[b]) : -1;
-            // (a page that is not there: page 0's, not used)
-            k[x] = *reinterpret_cast<const uint4*>(c.ksum + (static_cast<int64_t>(page < 0 ? 0 : page) * c.heads + h) * D + ch * 8);
-        }
-        // every lane of a group has the sums; lane x makes the key of the group's block x
-        const int b = b0 + ch * GROUPS, page = ch < kBatch && b < seen ? static_cast<int>(keys[b]) : -1;
-        const float ks = page < 0 ? 0.0f : c.ks[static_cast<int64_t>(page) * c.heads + h];
-        int mine = 0;
+            for (int x = 0; x < kBatch; ++x) {
+                const int b = b0 + x * GROUPS, page = b < high ? static_cast<int>(keys[b - low]) : -1;
+                // (a page that is not there: page 0's, not used)
+                k[x] = *reinterpret_cast<const uint4*>(c.ksum + (static_cast<int64_t>(page < 0 ? 0 : page) * c.heads + h) * D + ch * 8);
+            }
+            // every lane of a group has the sums; lane x makes the key of the group's block x
+            const int b = b0 + ch * GROUPS, page = ch < kBatch && b < high ? static_cast<int>(keys[b - low]) : -1;
+            const float ks = page < 0 ? 0.0f : c.ks[static_cast<int64_t>(page) * c.heads + h];
+            int mine = 0;
 #pragma unroll
-        for (int x = 0; x < kBatch; ++x) {
-            int dot = __builtin_amdgcn_sdot2(__builtin_bit_cast(s16x2, qw.x), __builtin_bit_cast(s16x2, k[x].x), 0, false);
-            dot = __builtin_amdgcn_sdot2(__builtin_bit_cast(s16x2, qw.y), __builtin_bit_cast(s16x2, k[x].y), dot, false);
-            dot = __builtin_amdgcn_sdot2(__builtin_bit_cast(s16x2, qw.z), __builtin_bit_cast(s16x2, k[x].z), dot, false);
-            dot = __builtin_amdgcn_sdot2(__builtin_bit_cast(s16x2, qw.w), __builtin_bit_cast(s16x2, k[x].w), dot, false);
-            dot = lane_sum<CH>(dot);
-            mine = ch == x ? dot : mine;
+            for (int x = 0; x < kBatch; ++x) {
+                int dot = __builtin_amdgcn_sdot2(__builtin_bit_cast(s16x2, qw.x), __builtin_bit_cast(s16x2, k[x].x), 0, false);
+                dot = __builtin_amdgcn_sdot2(__builtin_bit_cast(s16x2, qw.y), __builtin_bit_cast(s16x2, k[x].y), dot, false);
+                dot = __builtin_amdgcn_sdot2(__builtin_bit_cast(s16x2, qw.z), __builtin_bit_cast(s16x2, k[x].z), dot, false);
+                dot = __builtin_amdgcn_sdot2(__builtin_bit_cast(s16x2, qw.w), __builtin_bit_cast(s16x2, k[x].w), dot, false);
+                dot = lane_sum<CH>(dot);
+                mine = ch == x ? dot : mine;
+            }
+            if (ch < kBatch && b < high) {
+                const int held = len - b * kKvBlock < kKvBlock ? len - b * kKvBlock : kKvBlock;
+                const float score = static_cast<float>(mine) * (ks / static_cast<float>(held));
+                const uint32_t key = page < 0 ? 0u : causal && b >= own ? 0xFFFFFFFFu : key_of(score);
+                if constexpr (PART == kScores) my_keys[b] = key;
+                else keys[b] = key;
+            }
         }
-        if (ch < kBatch && b < seen) {
-            const int held = len - b * kKvBlock < kKvBlock ? len - b * kKvBlock : kKvBlock;
-            const float score = static_cast<float>(mine) * (ks / static_cast<float>(held));
-            keys[b] = page < 0 ? 0u : causal && b >= own ? 0xFFFFFFFFu : key_of(score);
-        }
+        if constexpr (PART == kScores) return;
     }
     __syncthreads();
 
@@ -231,9 +248,35 @@ __global__ __launch_bounds__(THREADS) void kv_select_kernel(const uint16_t* __re
 
 using namespace h3mi;
 
+namespace {
+
+// Whether the tiles are few and their tables long: 32 tiles of 2048 blocks 21 us in one launch.
+bool scores_apart(int64_t groups, int64_t blocks) { return 2 * groups <= cu_count() && blocks >= 2 * kChunk; }
+
+int64_t key_bytes(int64_t groups, int64_t blocks) { return scores_apart(groups, blocks) ? groups * blocks * 4 : 0; }
+
+template <int D>
+void launch(Part part, int threads, int64_t groups, size_t lds, hipStream_t st, const uint16_t* q, int64_t ld, int64_t bs, const KvCache& c,
+            const KvSeqs& s, int rows, int heads, int top, int causal, int tiles, int chunks, uint32_t* keys, int32_t* out) {
+    const auto fn = part == kScores ? kv_select_kernel<D, 256, kScores>
+                    : part == kSelection ? kv_select_kernel<D, 1024, kSelection>
+                    : threads == 1024 ? kv_select_kernel<D, 1024, kWhole> : kv_select_kernel<D, 256, kWhole>;
+    hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(groups)), dim3(threads), static_cast<unsigned>(lds), st, q, ld, bs, c, s, rows, heads, top,
+                       causal, tiles, chunks, keys, out);
+}
+
+}  // namespace
+
+extern "C" int64_t h3mi_kv_select_workspace(int64_t n, int64_t rows, int64_t kv_heads, int64_t blocks) {
+    int64_t groups;
+    if (n <= 0 || rows <= 0 || kv_heads <= 0 || blocks <= 0 || blocks > kMaxSelect || rows > (1 << 30)) return 0;
+    if (!launchable(n, (rows + kKvTile - 1) / kKvTile, kv_heads, 1024, &groups)) return 0;
+    return key_bytes(groups, blocks);
+}
+
 extern "C" int h3mi_kv_select(const uint16_t* q, int64_t rows, int64_t heads, int64_t ld_q, int64_t bs_q,
                               const h3mi_kv_cache* cache, const h3mi_kv_seqs* seqs, int64_t top, int causal, int32_t* blocks,
-                              void* stream) {
+                              void* workspace, int64_t workspace_bytes, void* stream) {
     if (int e = kv_check("kv_select", cache, seqs)) return e;
     if (heads <= 0 || heads > 65536 || heads % cache->heads)
         return fail(H3MI_EINVAL, "kv_select: heads=%lld must be a multiple of the cache's %lld", (long long)heads, (long long)cache->heads);
@@ -245,17 +288,25 @@ extern "C" int h3mi_kv_select(const uint16_t* q, int64_t rows, int64_t heads, in
     if (!blocks) return fail(H3MI_EINVAL, "kv_select: null blocks");
     if (!aligned(blocks, 4)) return fail(H3MI_EALIGN, "kv_select: blocks must be 4-byte aligned");
     const int64_t tiles = (rows + kKvTile - 1) / kKvTile;
-    const int D = static_cast<int>(cache->dim);
     int64_t groups;
     if (!launchable(seqs->n, tiles, cache->heads, 1024, &groups)) return fail(H3MI_EINVAL, "kv_select: too many rows for one call");
-    // one workgroup a CU or less: more of its own waves (2048 blocks, 32 groups: 21.0 us against 26; 150 blocks, 240 groups
-    // 11.2 against 8.3, 609 blocks, 1064 groups 25.3 against 29.3 with 512)
-    // (whose partial sums leave LDS for 16384 blocks' keys at every dim)
-    const int threads = 2 * groups <= cu_count() && seqs->blocks <= kMaxSelect / 2 ? 1024 : 256;
-    const auto fn = threads == 1024 ? (D == 64 ? kv_select_kernel<64, 1024> : D == 128 ? kv_select_kernel<128, 1024> : kv_select_kernel<256, 1024>)
-                                    : (D == 64 ? kv_select_kernel<64, 256> : D == 128 ? kv_select_kernel<128, 256> : kv_select_kernel<256, 256>);
-    hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(groups)), dim3(threads), static_cast<unsigned>(seqs->blocks * 4),
-                       as_stream(stream), q, ld_q, bs_q, kv_cache(*cache), kv_seqs(*seqs), static_cast<int>(rows),
-                       static_cast<int>(heads), static_cast<int>(top), causal, static_cast<int>(tiles), blocks);
-    return check_launch("kv_select");
+    const int64_t need = key_bytes(groups, seqs->blocks);
+    if (need > 0 && (!workspace || workspace_bytes < need))
+        return fail(H3MI_EINVAL, "kv_select: workspace of %lld bytes, %lld needed", (long long)(workspace ? workspace_bytes : 0), (long long)need);
+    if (!aligned(workspace, 4)) return fail(H3MI_EALIGN, "kv_select: workspace must be 4-byte aligned");
+    const auto go = cache->dim == 64 ? launch<64> : cache->dim == 128 ? launch<128> : launch<256>;
+    const auto run = [&](Part part, int threads, int64_t in_launch, int64_t chunks, int64_t keys_held) {
+        go(part, threads, in_launch, keys_held * 4, as_stream(stream), q, ld_q, bs_q, kv_cache(*cache), kv_seqs(*seqs), static_cast<int>(rows),
+           static_cast<int>(heads), static_cast<int>(top), causal, static_cast<int>(tiles), static_cast<int>(chunks),
+           static_cast<uint32_t*>(workspace), blocks);
+        return check_launch("kv_select");
+    };
+    if (need > 0) {
+        const int64_t chunks = (seqs->blocks + kChunk - 1) / kChunk;
+        if (int e = run(kScores, 256, groups * chunks, chunks, kChunk)) return e;
+        return run(kSelection, 1024, groups, 1, seqs->blocks);
+    }
+    // few workgroups: more of their own waves (150 blocks, 240 groups 11.2 us so, 8.3 with 256 threads; 609 blocks, 1064
+    // groups 25.3 with 256, 29.3 with 512)
+    return run(kWhole, 2 * groups <= cu_count() ? 1024 : 256, groups, 1, seqs->blocks);
 }

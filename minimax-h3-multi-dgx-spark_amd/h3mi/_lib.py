@@ -64,7 +64,8 @@ SIGNATURES = {
     "h3mi_gate_norm_mod_quant_i8": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _F, _P],
     "h3mi_kv_write_i8": [_P, _P, _I, _I, _I, _I, _I, _KC, _KS, _P],
     "h3mi_kv_read_bf16": [_P, _P, _P, _I, _KC, _KS, _P],
-    "h3mi_kv_select": [_P, _I, _I, _I, _I, _KC, _KS, _I, _C, _P, _P],
+    "h3mi_kv_select_workspace": [_I, _I, _I, _I],
+    "h3mi_kv_select": [_P, _I, _I, _I, _I, _KC, _KS, _I, _C, _P, _P, _I, _P],
     "h3mi_kv_attention_workspace": [_I, _I, _I, _I, _I, _I, _I],
     "h3mi_kv_attention_bf16": [_P, _I, _I, _I, _I, _KC, _KS, _F, _C, _P, _I, _P, _P, _I, _P],
     "h3mi_norm_order_info": [_C, ctypes.POINTER(_C), ctypes.POINTER(_C), ctypes.POINTER(_C)],
@@ -72,7 +73,7 @@ SIGNATURES = {
     "h3mi_debug_bf16_rne": [_P, _P, _I, _P],
     "h3mi_debug_buffer_lds_load": [_P, _I, _P, ctypes.c_int32, ctypes.c_int32, _P, _P],
 }
-_RESTYPE = {"h3mi_last_error": ctypes.c_char_p, "h3mi_kv_attention_workspace": _I}
+_RESTYPE = {"h3mi_last_error": ctypes.c_char_p, "h3mi_kv_attention_workspace": _I, "h3mi_kv_select_workspace": _I}
 
 
 class H3miError(RuntimeError):

@@ -161,9 +161,11 @@ def kv_select(q, cache, tables, lens, top, causal=False, counts=None):
     rows, ld, bs = _rows(q, cache, s.n, "q")
     top = int(top)
     out = torch.empty((s.n, -(-rows // KV_TILE), c.heads, max(top, 0)), dtype=torch.int32, device=q.device)
+    need = lib.h3mi_kv_select_workspace(s.n, rows, c.heads, s.blocks)
+    work = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
     with torch.cuda.device(q.device):
         check(lib.h3mi_kv_select(ptr(q), rows, q.shape[2], ld, bs, ctypes.byref(c), ctypes.byref(s), top, int(bool(causal)),
-                                 ptr(out), stream_of(q)))
+                                 ptr(out), ptr(work), need, stream_of(q)))
     return out
 
 

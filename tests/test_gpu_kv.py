@@ -325,6 +325,20 @@ def test_select(heads, kv, dim, causal, rows, lens, counts, top):
     assert np.array_equal(got.cpu().numpy(), want)
 
 
+@pytest.mark.parametrize("heads,kv,dim", [(2, 2, 64), (10, 2, 128), (2, 1, 256)])
+@pytest.mark.parametrize("rows,causal,top", [(1, True, 60), (4, False, 1), (130, True, 300), (1, False, 700)])
+def test_select_over_long_tables(heads, kv, dim, rows, causal, top):
+    """Few tiles over long tables, whose scores are a launch of their own: uneven sequences, pages that are not there."""
+    rng = np.random.default_rng(rows + top)
+    blocks = 700
+    ref, tables, q = _case(rng, heads, kv, dim, 3, rows, blocks, seed=top)
+    tables[1, 100:110] = -1
+    tables[1, 255:258] = 10 ** 7
+    lens, counts = [blocks * 64 - 7, 513 * 64, 3000], [rows, rows, max(rows - 3, 0)]
+    got = _h().kv_select(_bf(q), ref.to(), _i32(tables), _i32(lens), top, causal=causal, counts=_i32(counts))
+    assert np.array_equal(got.cpu().numpy(), R.select(ref, q.astype(np.float64), tables, lens, counts, top, causal))
+
+
 def test_select_ties_and_specials():
     """Equal scores take the lowest blocks; NaN scales come last; a query of zeros, NaN or infinities scores all alike."""
     rng = np.random.default_rng(31)
@@ -479,6 +493,8 @@ def test_another_stream(rows):
         for _ in range(20):
             assert torch.equal(h.kv_attention(x, c, t, lens), want)
             assert torch.equal(h.kv_select(x, c, t, lens, 9), blocks)
+            wide = t.repeat(1, 5)  # scores in a launch of their own
+            assert torch.equal(h.kv_select(x, c, wide, lens, 9), blocks)
     torch.cuda.current_stream().wait_stream(side)
 
 

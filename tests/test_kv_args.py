@@ -21,7 +21,8 @@ def _call(fn, cache=None, seqs=None, **kw):
     elif fn == "read":
         rc = L.h3mi_kv_read_bf16(P(a["p"]), P(a["p2"]), P(a["starts"]), a["length"], c, s, None)
     elif fn == "select":
-        rc = L.h3mi_kv_select(P(a["p"]), a["rows"], a["heads"], a["ld"], a["bs"], c, s, a["top"], 0, P(a["out"]), None)
+        rc = L.h3mi_kv_select(P(a["p"]), a["rows"], a["heads"], a["ld"], a["bs"], c, s, a["top"], 0, P(a["out"]), P(a["work"]),
+                              a["size"], None)
     else:
         rc = L.h3mi_kv_attention_bf16(P(a["p"]), a["rows"], a["heads"], a["ld"], a["bs"], c, s, ctypes.c_float(a["scale"]), 0,
                                       P(a["blocks"]), a["top"], P(a["out"]), P(a["work"]), a["size"], None)
@@ -87,7 +88,7 @@ def test_null_structures(fn):
     L = _lib.lib
     rc = {"write": lambda: L.h3mi_kv_write_i8(P(4096), P(8192), 1, 256, 256, 256, 256, None, None, None),
           "read": lambda: L.h3mi_kv_read_bf16(P(4096), P(8192), None, 1, None, None, None),
-          "select": lambda: L.h3mi_kv_select(P(4096), 1, 2, 256, 256, None, None, 1, 0, P(8192), None),
+          "select": lambda: L.h3mi_kv_select(P(4096), 1, 2, 256, 256, None, None, 1, 0, P(8192), None, 0, None),
           "attention": lambda: L.h3mi_kv_attention_bf16(P(4096), 1, 2, 256, 256, None, None, ctypes.c_float(1), 0, None, 0, P(8192), None, 0, None)}[fn]()
     assert rc == 1 and "null cache or sequences" in L.h3mi_last_error().decode()
 
@@ -107,6 +108,19 @@ def test_workspace(rows, heads, kv, dim, blocks, top):
         assert rc == 1 and "workspace" in m
     rc, m = _call("attention", cache, seqs, work=(1 << 30) + 8, size=need, **kw)
     assert rc == 2 and "workspace" in m
+
+
+def test_workspace_of_a_selection():
+    from h3mi import _lib
+    f = _lib.lib.h3mi_kv_select_workspace
+    need = f(4, 1, 8, 2048)
+    assert need == 4 * 8 * 2048 * 4
+    assert f(4, 1, 8, 100) == 0 and f(1, 2401, 56, 2048) == 0 and f(0, 1, 8, 2048) == 0 and f(1, 1, 8, 32769) == 0 and f(1 << 62, 1, 8, 2048) == 0
+    kw = dict(rows=1, heads=8, ld=1024, bs=1024)
+    for work, size in ((None, need), (1 << 30, need - 1)):
+        rc, m = _call("select", dict(heads=8, v=1 << 40), dict(n=4, blocks=2048), work=work, size=size, **kw)
+        assert rc == 1 and "workspace" in m
+    assert _call("select", dict(heads=8, v=1 << 40), dict(n=4, blocks=2048), work=(1 << 30) + 2, size=need, **kw)[0] == 2
 
 
 @pytest.mark.parametrize("a", [(0, 1, 2, 2, 128, 5, 0), (1, 0, 2, 2, 128, 5, 0), (-1, 1, 2, 2, 128, 5, 0), (1, 1, 3, 2, 128, 5, 0),
