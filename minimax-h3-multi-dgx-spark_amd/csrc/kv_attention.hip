@@ -140,10 +140,7 @@ struct TileShape {
     static constexpr int kGroups = W == 8 ? 2 : 1;
     // MFMAs that an operand is read ahead; 8 waves step together, and 4 there cost them 0.5%, 8 elsewhere gain nothing
     static constexpr int kAhead = W == 8 ? 8 : 4;
-    // A thread's pieces of K (and of V): 16 bytes, or 8 where that would leave threads without one.
-    using Piece = std::conditional_t<(kKvBlock * D >= 16 * kThreads), uint4, uint2>;
-    static constexpr int kPiece = sizeof(Piece);
-    static constexpr int kLoads = kKvBlock * D / kPiece / kThreads;
+    static constexpr int kLoads = kKvBlock * D / 16 / kThreads;  // 16-byte pieces of K (and of V) a thread
 };
 
 // The items of a launch: tiles of the queries of a head, or (pack > 1) of the queries of all
@@ -236,27 +233,22 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv_tile_kernel(Queri
     const int to = static_cast<int>(static_cast<int64_t>(total) * (split + 1) / splits);
 
     // Bytes of a block into registers, and as bf16 into LDS: 8 of them a chunk.
-    using Piece = typename T::Piece;
-    Piece kr[T::kLoads], vr[T::kLoads];
-    auto load = [&](const int8_t* from_pages, int page, Piece (&to_regs)[T::kLoads]) __attribute__((always_inline)) {
+    uint4 kr[T::kLoads], vr[T::kLoads];
+    auto load = [&](const int8_t* from_pages, int page, uint4 (&to_regs)[T::kLoads]) __attribute__((always_inline)) {
         const int8_t* const at = from_pages + (static_cast<int64_t>(page) * c.heads + h) * (kKvBlock * D);  // uniform
 #pragma unroll
-        for (int j = 0; j < T::kLoads; ++j) to_regs[j] = *reinterpret_cast<const Piece*>(at + static_cast<uint32_t>(t + j * T::kThreads) * T::kPiece);
+        for (int j = 0; j < T::kLoads; ++j) to_regs[j] = *reinterpret_cast<const uint4*>(at + static_cast<uint32_t>(t + j * T::kThreads) * 16);
     };
-    auto stage = [&](uint8_t* buf, const Piece (&regs)[T::kLoads], auto chunks, auto swap) __attribute__((always_inline)) {
-        constexpr int CH = chunks, PC = T::kPiece / 8;  // chunks of a row, of a piece
+    auto stage = [&](uint8_t* buf, const uint4 (&regs)[T::kLoads], auto chunks, auto swap) __attribute__((always_inline)) {
+        constexpr int CH = chunks;
 #pragma unroll
         for (int j = 0; j < T::kLoads; ++j) {
-            const int piece = t + j * T::kThreads, line = piece / (CH / PC), ch = piece % (CH / PC) * PC;
+            const int piece = t + j * T::kThreads, line = piece / (CH / 2), ch = piece % (CH / 2) * 2;
             // token bits 2 and 3 change places: an MFMA row's registers are then runs of 8 tokens
             const int row = swap ? (line & ~12) | ((line & 4) << 1) | ((line & 8) >> 1) : line;
             uint8_t* const to_row = buf + row * (CH * 16);
-            if constexpr (PC == 2) {
-                *reinterpret_cast<uint4*>(to_row + chunk_at<CH>(row, ch) * 16) = ints_bf16(make_uint2(regs[j].x, regs[j].y));
-                *reinterpret_cast<uint4*>(to_row + chunk_at<CH>(row, ch + 1) * 16) = ints_bf16(make_uint2(regs[j].z, regs[j].w));
-            } else {
-                *reinterpret_cast<uint4*>(to_row + chunk_at<CH>(row, ch) * 16) = ints_bf16(regs[j]);
-            }
+            *reinterpret_cast<uint4*>(to_row + chunk_at<CH>(row, ch) * 16) = ints_bf16(make_uint2(regs[j].x, regs[j].y));
+            *reinterpret_cast<uint4*>(to_row + chunk_at<CH>(row, ch + 1) * 16) = ints_bf16(make_uint2(regs[j].z, regs[j].w));
         }
     };
     auto stage_k = [&](int which) __attribute__((always_inline)) {
@@ -271,6 +263,9 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv_tile_kernel(Queri
         wg_barrier();
         __builtin_amdgcn_sched_barrier(0);
     };
+    // A wave without a query that sees anything converts its share of the blocks and no more.  (Not among 8 waves of 128
+    // elements, whose registers the branch would overflow: 2000 rows 139 -> 158 us; of 256 it made 404 us 354.)
+    const bool working = (W == 8 && D == 128) || uniform(wave_last) >= 0;
     const int behind = T::kGroups == 2 && __builtin_amdgcn_readfirstlane(wave) >= W / 2;
 
     for (int x0 = from; x0 < to; x0 += T::kThreads) {
@@ -419,11 +414,13 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv_tile_kernel(Queri
             const int2 after = entry[next_k + 1];
             const int block = entry[y + 1].y;
             const Factors next = fact[y + 1];
-            __builtin_amdgcn_s_setprio(1);
-            products(y, std::true_type{}, values);
-            __builtin_amdgcn_s_setprio(0);
+            if (working) {
+                __builtin_amdgcn_s_setprio(1);
+                products(y, std::true_type{}, values);
+                __builtin_amdgcn_s_setprio(0);
+            }
             if constexpr (T::kGroups == 2) arrive();
-            softmax();
+            if (working) softmax();
             if (next_k < n) stage_k(next_k);
             if (next_v < n) stage_v(next_v);
             page_v = page_k;
@@ -434,7 +431,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv_tile_kernel(Queri
         };
         step(0, std::false_type{});
         for (int y = 1; y < n; ++y) step(y, std::true_type{});
-        products(n, std::false_type{}, std::true_type{});
+        if (working) products(n, std::false_type{}, std::true_type{});
         if (T::kGroups == 2 && !behind) arrive();
     }
 
@@ -479,13 +476,15 @@ __device__ __forceinline__ uint4 load_once(const int8_t* p) {
     return __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p)));
 }
 
-constexpr int kFew = 16;      // queries of a kv head's group: the columns of a 16x16 MFMA
+constexpr int kFew = 16;  // queries: the columns of a 16x16 MFMA
 constexpr int kFewWaves = 4;
 
-// A workgroup: one kv head of one sequence, one split of its blocks.  Its waves take whole
-// blocks in turn, straight from memory into the operands' registers (no LDS, no barrier),
-// and are joined once at the end.
-template <int D>
+// A workgroup: up to 16 NQ queries of one kv head's group, one split of its blocks.  Its
+// waves take whole blocks in turn, straight from memory into the operands' registers (no
+// LDS, no barrier; a block's bytes are converted once for all queries), and are joined once
+// at the end.  With a tile's 16 KB at a time a workgroup, 17 rows of 56 heads over 4000
+// tokens waited for memory 272 us; so they take 87.
+template <int D, int NQ>
 __global__ __launch_bounds__(64 * kFewWaves) void kv_few_kernel(Queries q, KvCache c, KvSeqs s, float scale, int causal, Lists list,
                                                                 uint16_t* __restrict__ out, Partial part, int per) {
     constexpr int KL = D / 64;   // 16-byte pieces of a key row a lane
@@ -500,29 +499,33 @@ __global__ __launch_bounds__(64 * kFewWaves) void kv_few_kernel(Queries q, KvCac
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, col = lane & 15, quad = lane >> 4;
 
     const int len = s.len(i), count = s.count(i, q.rows), start = s.end(i) - count;
-    const int row = col / group, hq = h * group + col % group;
     auto last_of = [&](int r) {
         int x = len - 1;
         if (causal && start + r < x) x = start + r;
         return r < count ? x : -1;
     };
-    const int last = col < queries ? last_of(row) : -1;
     const int most = count > 0 ? last_of(count - 1) : -1;
     // below this every query that is one sees a whole block
     const int full = count > 0 ? last_of(0) + 1 : 0;
     const int blocks = most < 0 ? 0 : block_of(most) + 1;
 
-    bf16x8 qf[2 * KL];
-    {
+    // query 16 g + col of each set g
+    int last[NQ];
+    bf16x8 qf[NQ][2 * KL];
+    f32x4 o[NQ][NT];
+    float m[NQ], l[NQ];
+#pragma unroll
+    for (int g = 0; g < NQ; ++g) {
+        const int query = g * kFew + col, row = query / group, hq = h * group + query % group;
+        last[g] = query < queries ? last_of(row) : -1;
         const int64_t at = i * q.bs + static_cast<int64_t>(row) * q.ld + static_cast<int64_t>(hq) * D + quad * 16;
 #pragma unroll
         for (int k = 0; k < 2 * KL; ++k)
-            qf[k] = last >= 0 ? query_frag(q.p + at + (k >> 1) * 64 + (k & 1) * 8, scale) : frag(make_uint4(0, 0, 0, 0));
-    }
-    f32x4 o[NT];
+            qf[g][k] = last[g] >= 0 ? query_frag(q.p + at + (k >> 1) * 64 + (k & 1) * 8, scale) : frag(make_uint4(0, 0, 0, 0));
 #pragma unroll
-    for (int n = 0; n < NT; ++n) o[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    float m = kLowest, l = 0.0f;
+        for (int n = 0; n < NT; ++n) o[g][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        m[g] = kLowest, l[g] = 0.0f;
+    }
 
     const int32_t* const mine = list.p ? list.p + (static_cast<int64_t>(i) * list.tiles * c.heads + h) * list.top : nullptr;
     const int total = blocks == 0 ? 0 : mine ? list.top : blocks;
@@ -575,67 +578,80 @@ __global__ __launch_bounds__(64 * kFewWaves) void kv_few_kernel(Queries q, KvCac
             const float flv = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f.lv), y));
             const float fiv = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f.iv), y));
             const float fvs = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f.vs), y));
-            f32x4 sc[4];
+            f32x4 sc[NQ][4];
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                sc[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int g = 0; g < NQ; ++g) sc[g][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int k = 0; k < KL; ++k) {
                     const uint4 w = kr[u][k];
-                    sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(frag(ints_bf16(make_uint2(w.x, w.y))), qf[2 * k], sc[u], 0, 0, 0);
-                    sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(frag(ints_bf16(make_uint2(w.z, w.w))), qf[2 * k + 1], sc[u], 0, 0, 0);
+                    const bf16x8 lo = frag(ints_bf16(make_uint2(w.x, w.y))), hi = frag(ints_bf16(make_uint2(w.z, w.w)));
+#pragma unroll
+                    for (int g = 0; g < NQ; ++g) {
+                        sc[g][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, qf[g][2 * k], sc[g][u], 0, 0, 0);
+                        sc[g][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, qf[g][2 * k + 1], sc[g][u], 0, 0, 0);
+                    }
                 }
             }
             if (left) load_k(next);
-            // register r of sc[u]: token base + 16 quad + 4 u + r
-            float best = -__builtin_inff();
+            // register r of sc[g][u]: token base + 16 quad + 4 u + r
             const bool mask = base + kKvBlock > full;
+            bf16x8 p[NQ][2];
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    if (mask && base + 16 * quad + 4 * u + r > last) sc[u][r] = -__builtin_inff();
-                    best = fmaxf(best, sc[u][r]);
-                }
-            best = fmaxf(best, __shfl_xor(best, 16));
-            best = fmaxf(best, __shfl_xor(best, 32)) * fc;
-            if (__any(best > m + kSlack)) {
-                const float mn = fmaxf(m, best), fix = exp2_hw(m - mn);
-                m = mn;
-                l *= fix;
-#pragma unroll
-                for (int d = 0; d < NT; ++d) o[d] *= fix;
-            }
-            const float off = flv - m;
-            float sum = 0.0f;
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    sc[u][r] = exp2_hw(__builtin_fmaf(sc[u][r], fc, off));
-                    sum += sc[u][r];
-                }
-            if (fiv != 0.0f) {
-                l = __builtin_fmaf(sum, fiv, l);
-            } else {
-                // a scale that is no ordinary number: what a row does not see must not reach it
+            for (int g = 0; g < NQ; ++g) {
+                float best = -__builtin_inff();
 #pragma unroll
                 for (int u = 0; u < 4; ++u)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const float p = base + 16 * quad + 4 * u + r > last ? 0.0f : sc[u][r];
-                        l += p;
-                        sc[u][r] = p == 0.0f ? 0.0f : p * fvs;
+                        if (mask && base + 16 * quad + 4 * u + r > last[g]) sc[g][u][r] = -__builtin_inff();
+                        best = fmaxf(best, sc[g][u][r]);
                     }
+                best = fmaxf(best, __shfl_xor(best, 16));
+                best = fmaxf(best, __shfl_xor(best, 32)) * fc;
+                if (__any(best > m[g] + kSlack)) {
+                    const float mn = fmaxf(m[g], best), fix = exp2_hw(m[g] - mn);
+                    m[g] = mn;
+                    l[g] *= fix;
+#pragma unroll
+                    for (int d = 0; d < NT; ++d) o[g][d] *= fix;
+                }
+                const float off = flv - m[g];
+                float sum = 0.0f;
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        sc[g][u][r] = exp2_hw(__builtin_fmaf(sc[g][u][r], fc, off));
+                        sum += sc[g][u][r];
+                    }
+                if (fiv != 0.0f) {
+                    l[g] = __builtin_fmaf(sum, fiv, l[g]);
+                } else {
+                    // a scale that is no ordinary number: what a row does not see must not reach it
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const float e = base + 16 * quad + 4 * u + r > last[g] ? 0.0f : sc[g][u][r];
+                            l[g] += e;
+                            sc[g][u][r] = e == 0.0f ? 0.0f : e * fvs;
+                        }
+                }
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    const f32x4 a = sc[g][2 * w], e = sc[g][2 * w + 1];
+                    p[g][w] = frag(make_uint4(bf16x2_bits(a[0], a[1]), bf16x2_bits(a[2], a[3]), bf16x2_bits(e[0], e[1]), bf16x2_bits(e[2], e[3])));
+                }
             }
 #pragma unroll
-            for (int w = 0; w < 2; ++w) {
-                const f32x4 a = sc[2 * w], e = sc[2 * w + 1];
-                const bf16x8 p = frag(make_uint4(bf16x2_bits(a[0], a[1]), bf16x2_bits(a[2], a[3]), bf16x2_bits(e[0], e[1]), bf16x2_bits(e[2], e[3])));
+            for (int d = 0; d < NT; ++d) {
+                const bf16x8 lo = frag(ints_bf16(make_uint2(vr[d].x, vr[d].y))), hi = frag(ints_bf16(make_uint2(vr[d].z, vr[d].w)));
 #pragma unroll
-                for (int d = 0; d < NT; ++d) {
-                    const uint2 v8 = w ? make_uint2(vr[d].z, vr[d].w) : make_uint2(vr[d].x, vr[d].y);
-                    o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(frag(ints_bf16(v8)), p, o[d], 0, 0, 0);
+                for (int g = 0; g < NQ; ++g) {
+                    o[g][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, p[g][0], o[g][d], 0, 0, 0);
+                    o[g][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, p[g][1], o[g][d], 0, 0, 0);
                 }
             }
             if (left) load_v(next);
@@ -643,41 +659,44 @@ __global__ __launch_bounds__(64 * kFewWaves) void kv_few_kernel(Queries q, KvCac
         }
     }
 
-    // register r of o[d]: element 16 d + 4 quad + r of query col
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
-    if (last < 0) {  // padding, or a row that sees nothing: what the registers hold is no result
-        l = 0.0f;
+    // register r of o[g][d]: element 16 d + 4 quad + r of query 16 g + col
 #pragma unroll
-        for (int d = 0; d < NT; ++d) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
-    if (quad == 0) jml[wave][col] = make_float2(m, l);
+    for (int g = 0; g < NQ; ++g) {
+        if (g * kFew >= queries) break;
+        l[g] += __shfl_xor(l[g], 16);
+        l[g] += __shfl_xor(l[g], 32);
+        const bool sees = last[g] >= 0;  // else padding, or a row that sees nothing: what the registers hold is no result
+        if (g > 0) __syncthreads();
+        if (quad == 0) jml[wave][col] = make_float2(m[g], sees ? l[g] : 0.0f);
 #pragma unroll
-    for (int d = 0; d < NT; ++d)
-        *reinterpret_cast<float4*>(&jo[wave][col][16 * d + 4 * quad]) = make_float4(o[d][0], o[d][1], o[d][2], o[d][3]);
-    __syncthreads();
-    for (int e = t; e < queries * (D / 4); e += 64 * kFewWaves) {
-        const int qn = e / (D / 4), d = e % (D / 4) * 4;
-        float top = kLowest;
+        for (int d = 0; d < NT; ++d)
+            *reinterpret_cast<float4*>(&jo[wave][col][16 * d + 4 * quad]) =
+                sees ? make_float4(o[g][d][0], o[g][d][1], o[g][d][2], o[g][d][3]) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        __syncthreads();
+        const int here = queries - g * kFew < kFew ? queries - g * kFew : kFew;
+        for (int e = t; e < here * (D / 4); e += 64 * kFewWaves) {
+            const int qn = e / (D / 4), d = e % (D / 4) * 4, query = g * kFew + qn;
+            float top = kLowest;
 #pragma unroll
-        for (int w = 0; w < kFewWaves; ++w) top = fmaxf(top, jml[w][qn].x);
-        float sum = 0.0f, a[4] = {};
+            for (int w = 0; w < kFewWaves; ++w) top = fmaxf(top, jml[w][qn].x);
+            float sum = 0.0f, a[4] = {};
 #pragma unroll
-        for (int w = 0; w < kFewWaves; ++w) {
-            const float2 ml = jml[w][qn];
-            const float fix = exp2_hw(ml.x - top);
-            sum += ml.y * fix;
-            const float4 x = *reinterpret_cast<const float4*>(&jo[w][qn][d]);
-            a[0] += x.x * fix, a[1] += x.y * fix, a[2] += x.z * fix, a[3] += x.w * fix;
-        }
-        const int64_t query = (static_cast<int64_t>(i) * q.rows + qn / group) * q.heads + h * group + qn % group;
-        if (part.splits > 1) {
-            const int64_t at = part.at(nh, split, qn);
-            if (d == 0) part.ml[at] = make_float2(top, sum);
-            *reinterpret_cast<float4*>(part.o + at * D + d) = make_float4(a[0], a[1], a[2], a[3]);
-        } else {
-            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-            *reinterpret_cast<uint2*>(out + query * D + d) = make_uint2(bf16x2_bits(a[0] * inv, a[1] * inv), bf16x2_bits(a[2] * inv, a[3] * inv));
+            for (int w = 0; w < kFewWaves; ++w) {
+                const float2 ml = jml[w][qn];
+                const float fix = exp2_hw(ml.x - top);
+                sum += ml.y * fix;
+                const float4 x = *reinterpret_cast<const float4*>(&jo[w][qn][d]);
+                a[0] += x.x * fix, a[1] += x.y * fix, a[2] += x.z * fix, a[3] += x.w * fix;
+            }
+            if (part.splits > 1) {
+                const int64_t at = part.at(nh, split, query);
+                if (d == 0) part.ml[at] = make_float2(top, sum);
+                *reinterpret_cast<float4*>(part.o + at * D + d) = make_float4(a[0], a[1], a[2], a[3]);
+            } else {
+                const int64_t to_row = (static_cast<int64_t>(i) * q.rows + query / group) * q.heads + h * group + query % group;
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                *reinterpret_cast<uint2*>(out + to_row * D + d) = make_uint2(bf16x2_bits(a[0] * inv, a[1] * inv), bf16x2_bits(a[2] * inv, a[3] * inv));
+            }
         }
     }
 }
@@ -735,6 +754,10 @@ __global__ __launch_bounds__(256) void kv_join_kernel(Partial part, Queries q, I
 
 // ------------------------------------------------------------------ what a call runs
 
+// Queries of a kv head's group that kv_few_kernel holds in registers: 64 of 64 elements, 32 of 128 (64 spilled, and took
+// 230 us where 32 take 87), 16 of 256.
+constexpr int64_t few_queries(int64_t dim) { return 64 * kFew / dim * 4; }
+
 struct Plan {
     bool few, flat;
     int waves;          // of a tile's workgroup
@@ -750,7 +773,7 @@ Plan plan_of(int64_t n, int64_t rows, int64_t heads, int64_t kv, int64_t dim, in
     Plan p = {};
     const int64_t cus = cu_count(), group = heads / kv;
     const int64_t longest = top > 0 ? top : blocks;  // blocks that a query may read
-    p.few = rows * group <= kFew;
+    p.few = rows * group <= few_queries(dim);
     if (p.few) {
         p.pack = static_cast<int>(group);
         p.rows = rows * group;
@@ -769,10 +792,13 @@ Plan plan_of(int64_t n, int64_t rows, int64_t heads, int64_t kv, int64_t dim, in
     // Rows that leave a tile part empty share it with the other heads of their group (a list is a kv head's).
     p.pack = rows < kKvTile ? static_cast<int>(group) : 1;
     p.heads = heads / p.pack;
-    const int64_t queries = rows * p.pack, tiles8 = (queries + 255) / 256;
-    p.waves = dim == 256 || top > 0 || n * p.heads * tiles8 < cus ? 4 : 8;
+    // Tiles of 4 waves, two a CU, balance themselves; 8 waves in step are ahead where the work is long and even: 128
+    // elements, 128 blocks and 1024 rows on (4800 x 19721 2661 us, 2746 with 4; 2000 x 9000 562 and 583; but 2000 x 2000
+    // causal 138 and 104, 4800 x 19200 of 64 elements 927 and 837).  A list is 128 rows'.
+    const int64_t queries = rows * p.pack, tiles8 = (queries + 255) / 256, tiles4 = (queries + 127) / 128;
+    p.waves = dim == 128 && top == 0 && blocks >= 128 && queries >= 1024 && n * p.heads * tiles8 >= cus ? 8 : 4;
     p.rows = 32 * p.waves;
-    p.tiles = (queries + p.rows - 1) / p.rows;
+    p.tiles = p.waves == 8 ? tiles8 : tiles4;
     p.items = n * p.heads * p.tiles;
     const int64_t slots = (p.waves == 8 || dim == 256 ? 1 : 2) * cus;
     p.flat = p.items <= slots;
@@ -857,13 +883,15 @@ extern "C" int h3mi_kv_attention_bf16(const uint16_t* q, int64_t rows, int64_t h
     if (p.few) {
         int64_t groups;
         if (!launchable(p.items, p.splits, 1, 64 * kFewWaves, &groups)) return fail(H3MI_EINVAL, "kv_attention: too many rows for one call");
-        const auto fn = dim == 64 ? kv_few_kernel<64> : dim == 128 ? kv_few_kernel<128> : kv_few_kernel<256>;
+        const int sets = static_cast<int>((p.rows + kFew - 1) / kFew);
+        const auto fn = dim == 64    ? (sets == 1 ? kv_few_kernel<64, 1> : sets == 2 ? kv_few_kernel<64, 2> : kv_few_kernel<64, 4>)
+                        : dim == 128 ? (sets == 1 ? kv_few_kernel<128, 1> : kv_few_kernel<128, 2>)
+                                     : kv_few_kernel<256, 1>;
         hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(groups)), dim3(64 * kFewWaves), 0, st, qs, c, s, scale, causal, list, out, part,
                            p.per);
         rc = check_launch("kv_attention");
     } else if (dim == 64) {
-        rc = p.waves == 8 ? launch_tiles<64, 8>(items, qs, c, s, scale, causal, list, out, part, st)
-                          : launch_tiles<64, 4>(items, qs, c, s, scale, causal, list, out, part, st);
+        rc = launch_tiles<64, 4>(items, qs, c, s, scale, causal, list, out, part, st);
     } else if (dim == 128) {
         rc = p.waves == 8 ? launch_tiles<128, 8>(items, qs, c, s, scale, causal, list, out, part, st)
                           : launch_tiles<128, 4>(items, qs, c, s, scale, causal, list, out, part, st);
