@@ -275,6 +275,69 @@ def test_attention_long(rows, n, heads, kv, tokens, causal):
     _check(ref, q, tables, lens, None, causal)
 
 
+def _check_on_gpu(c, q, table, end, causal, out):
+    """out [rows, heads, dim] of one sequence whose rows are its last, against 64 bits on the GPU, head by head."""
+    rows, heads, dim = q.shape
+    group = heads // c.k.shape[1]
+    half = torch.finfo(torch.bfloat16).eps / 2
+    page = table.long()
+    at = torch.arange(end, device=DEV)
+    for h in range(heads):
+        k = (c.k[page, h // group].double() * c.k_scale[page, h // group].double()[:, None, None]).reshape(-1, dim)[:end]
+        v = (c.v[page, h // group].double() * c.v_scale[page, h // group].double()[:, None, None]).transpose(1, 2).reshape(-1, dim)[:end]
+        x = q[:, h].double() @ k.t() * dim ** -0.5
+        if causal:
+            x.masked_fill_(at > (end - rows + torch.arange(rows, device=DEV))[:, None], -float("inf"))
+        p = torch.softmax(x, 1)
+        want, mag = p @ v, p @ v.abs()
+        top = (q[:, h].double().abs() @ k.abs().t() * dim ** -0.5).amax(1, keepdim=True)
+        # kv_ref.bound, on the GPU
+        bound = half * (mag * (1 + half) + want.abs()) * (1 + 1e-3) + 2 * mag * ((dim + 8) * 2.0 ** -24 * (top + 4)) + 1e-30
+        assert ((out[:, h].double() - want).abs() <= bound).all(), h
+
+
+@pytest.mark.parametrize("heads,kv,dim,rows,tokens", [
+    (52, 52, 128, 1100, 33000),   # 8 waves a tile, more blocks than are looked up at once
+    (52, 52, 128, 1030, 8200),    # 8 waves, 129 blocks
+    (60, 12, 64, 1300, 17000),    # 4 waves, more blocks than are looked up at once, the last round split
+    (18, 18, 256, 1900, 16500),
+    (300, 300, 128, 70, 17000),   # one tile a head
+])
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_large(heads, kv, dim, rows, tokens, causal):
+    h = _h()
+    g = torch.Generator(device=DEV).manual_seed(tokens)
+    blocks = -(-tokens // 64)
+    shared = 40  # heads' pages: blocks of one cache in many places
+    c = h.KVCache(torch.randint(-127, 128, (shared, kv, 64, dim), generator=g, device=DEV, dtype=torch.int8),
+                  torch.randint(-127, 128, (shared, kv, dim, 64), generator=g, device=DEV, dtype=torch.int8),
+                  torch.rand(shared, kv, generator=g, device=DEV) * 0.02 + 0.005, torch.rand(shared, kv, generator=g, device=DEV) * 0.02 + 0.005,
+                  torch.zeros(shared, kv, dim, dtype=torch.int16, device=DEV))
+    q = torch.randn(1, rows, heads, dim, generator=g, device=DEV).to(torch.bfloat16)
+    tables = torch.randint(0, shared, (1, blocks), generator=g, device=DEV, dtype=torch.int32)
+    out = h.kv_attention(q, c, tables, _i32([tokens]), causal=causal)
+    _check_on_gpu(c, q[0], tables[0], tokens, causal, out[0])
+
+
+@pytest.mark.parametrize("rows,dim", [(1, 128), (20, 128), (50, 64)])
+def test_attention_few_rows_unsplit(rows, dim):
+    """Few rows of so many sequences that a workgroup takes a whole sequence: more blocks than are looked up at once."""
+    h = _h()
+    n, kv, tokens, shared = 70, 8, 17000, 30
+    g = torch.Generator(device=DEV).manual_seed(rows)
+    c = h.KVCache(torch.randint(-127, 128, (shared, kv, 64, dim), generator=g, device=DEV, dtype=torch.int8),
+                  torch.randint(-127, 128, (shared, kv, dim, 64), generator=g, device=DEV, dtype=torch.int8),
+                  torch.rand(shared, kv, generator=g, device=DEV) * 0.02 + 0.005, torch.rand(shared, kv, generator=g, device=DEV) * 0.02 + 0.005,
+                  torch.zeros(shared, kv, dim, dtype=torch.int16, device=DEV))
+    q = torch.randn(n, rows, kv, dim, generator=g, device=DEV).to(torch.bfloat16)
+    tables = torch.randint(0, shared, (n, 266), generator=g, device=DEV, dtype=torch.int32)
+    lens = torch.randint(rows, tokens + 1, (n,), generator=g, device=DEV, dtype=torch.int32)
+    lens[0] = tokens
+    out = h.kv_attention(q, c, tables, lens, causal=True)
+    for i in (0, 1, n - 1):
+        _check_on_gpu(c, q[i], tables[i], int(lens[i]), True, out[i])
+
+
 def test_offsets_past_32_bits():
     """Pages whose bytes lie past 2^31 and whose elements past 2^32 in the pool, and rows past 2^31 elements."""
     h = _h()
