@@ -119,7 +119,7 @@ struct Partial {
 // waves the second four run half a step behind the first, with a barrier after each half:
 // of the two waves on a SIMD one is in its products while the other is in its softmax.  They
 // convert their share of a block one step earlier in turn, so that it is there in time.
-// (With 4 waves a barrier a step; two workgroups share a CU.)  Rows are
+// (With 4 waves a barrier a step; workgroups that share a CU fall out of step by themselves.)  Rows are
 // 16-byte chunks whose index is XORed with row bits, so that 16 lanes of an access lie on
 // the 16 different 16-byte groups of LDS's 256 bytes of banks, both for the writes (rows)
 // and for the MFMA operands' reads (columns).
@@ -174,8 +174,9 @@ struct Items {
     }
 };
 
+// (64 elements leave registers and LDS for three workgroups a CU: 4800 x 19200 831 us with two, 689 so.)
 template <int D, int W>
-__global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv_tile_kernel(Queries q, KvCache c, KvSeqs s, float scale, int causal,
+__global__ __launch_bounds__(64 * W, D == 256 ? 1 : D == 64 ? 3 : 2) void kv_tile_kernel(Queries q, KvCache c, KvSeqs s, float scale, int causal,
                                                                           Lists list, uint16_t* __restrict__ out, Partial part,
                                                                           Items items) {
     using T = TileShape<D, W>;
@@ -315,19 +316,19 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv_tile_kernel(Queri
             constexpr int NK = keys ? D / 8 : 0, N = NK + (values ? 4 * NT : 0);
             const uint8_t* const kb = smem + (y & 1) * T::kKeyBytes;
             const uint8_t* const vb = smem + (3 - (y & 1)) * T::kKeyBytes;
-            // At 256 elements a row's chunk 2 k + half is found from chunk `half` by an XOR, opaque, so that the loop does not
-            // keep a register for every k (1200 rows over 9000 tokens 458 -> 434 us; at 128, where they fit, the XORs took
-            // 2000 rows from 137 to 142 us).
+            // At 64 and 256 elements a row's chunk 2 k + half is found from chunk `half` by an XOR, opaque, so that the loop
+            // does not keep a register for every k (256: 1200 rows over 9000 tokens 458 -> 434 us; 64, 500 rows: 23.7 -> 22.0;
+            // at 128, where they fit, the XORs took 2000 rows from 137 to 142 us).
             uint32_t kx = col * (D * 2) + chunk_at<KC>(col, half) * 16, vx = col * (kKvBlock * 2) + chunk_at<VC>(col, half) * 16;
-            if constexpr (D == 256) asm("" : "+v"(kx), "+v"(vx));
+            if constexpr (D != 128) asm("" : "+v"(kx), "+v"(vx));
             auto fetch = [&](int x) __attribute__((always_inline)) {
                 if (x < NK) {
                     const int row = x % 2 * 32 + col;
-                    const uint32_t at = D == 256 ? (kx ^ (x / 2 * 32)) + x % 2 * (32 * D * 2) : row * (D * 2) + chunk_at<KC>(row, x / 2 * 2 + half) * 16;
+                    const uint32_t at = D != 128 ? (kx ^ (x / 2 * 32)) + x % 2 * (32 * D * 2) : row * (D * 2) + chunk_at<KC>(row, x / 2 * 2 + half) * 16;
                     return frag(*reinterpret_cast<const uint4*>(kb + at));
                 }
                 const int d = (x - NK) % NT, w = (x - NK) / NT, row = d * 32 + col;
-                const uint32_t at = D == 256 ? (vx ^ (w * 32)) + d * (32 * kKvBlock * 2) : row * (kKvBlock * 2) + chunk_at<VC>(row, 2 * w + half) * 16;
+                const uint32_t at = D != 128 ? (vx ^ (w * 32)) + d * (32 * kKvBlock * 2) : row * (kKvBlock * 2) + chunk_at<VC>(row, 2 * w + half) * 16;
                 return frag(*reinterpret_cast<const uint4*>(vb + at));
             };
             bf16x8 a[T::kAhead];
@@ -800,7 +801,7 @@ Plan plan_of(int64_t n, int64_t rows, int64_t heads, int64_t kv, int64_t dim, in
     p.rows = 32 * p.waves;
     p.tiles = p.waves == 8 ? tiles8 : tiles4;
     p.items = n * p.heads * p.tiles;
-    const int64_t slots = (p.waves == 8 || dim == 256 ? 1 : 2) * cus;
+    const int64_t slots = (p.waves == 8 || dim == 256 ? 1 : dim == 64 ? 3 : 2) * cus;
     p.flat = p.items <= slots;
     p.whole = p.items / slots * slots;
     const int64_t rest = p.items - p.whole;
