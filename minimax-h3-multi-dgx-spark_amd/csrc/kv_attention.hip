@@ -801,7 +801,7 @@ Plan plan_of(int64_t n, int64_t rows, int64_t heads, int64_t kv, int64_t dim, in
     p.rows = 32 * p.waves;
     p.tiles = p.waves == 8 ? tiles8 : tiles4;
     p.items = n * p.heads * p.tiles;
-    const int64_t slots = (p.waves == 8 || dim == 256 ? 1 : dim == 64 ? 3 : 2) * cus;
+    const int64_t slots = (p.waves == 8 || dim == 256 ? 1 : dim == 64 ? 3 : 2) * (cus < 8 ? 8 : cus / 8 * 8);  // whole XCDs' worth
     p.flat = p.items <= slots;
     p.whole = p.items / slots * slots;
     const int64_t rest = p.items - p.whole;
@@ -868,6 +868,9 @@ extern "C" int h3mi_kv_attention_bf16(const uint16_t* q, int64_t rows, int64_t h
     const int64_t part_rows = p.part_rows(), need = part_rows * (dim * 4 + 8);
     const int64_t rest = (p.items - p.whole) * p.splits;
     if (p.items > (1 << 30) || rest > (1 << 30)) return fail(H3MI_EINVAL, "kv_attention: too many rows for one call");
+    const size_t bytes = static_cast<size_t>(n) * rows * heads * dim * 2;
+    if (kv_overlaps(out, bytes, q, n, rows, heads, dim, ld_q, bs_q) || kv_overlaps(out, bytes, *cache))
+        return fail(H3MI_EALIAS, "kv_attention: out overlaps q or the cache");
     if (need > 0 && (!workspace || workspace_bytes < need))
         return fail(H3MI_EINVAL, "kv_attention: workspace of %lld bytes, %lld needed", (long long)(workspace ? workspace_bytes : 0), (long long)need);
     if (!aligned(workspace, 16)) return fail(H3MI_EALIGN, "kv_attention: workspace must be 16-byte aligned");

@@ -47,6 +47,18 @@ int kv_check_rows(const char* what, const char* name, const uint16_t* p, int64_t
     return H3MI_OK;
 }
 
+bool kv_overlaps(const void* out, size_t bytes, const uint16_t* p, int64_t n, int64_t rows, int64_t heads, int64_t dim, int64_t ld, int64_t bs) {
+    if (n == 0 || rows == 0) return false;
+    const size_t span = static_cast<size_t>(n - 1) * bs + static_cast<size_t>(rows - 1) * ld + static_cast<size_t>(heads) * dim;
+    return overlap(out, bytes, p, 2 * span);
+}
+
+bool kv_overlaps(const void* out, size_t bytes, const h3mi_kv_cache& c) {
+    const size_t tiles = static_cast<size_t>(c.pages) * c.heads, kv = tiles * c.dim * kKvBlock;
+    return overlap(out, bytes, c.k, kv) || overlap(out, bytes, c.v, kv) || overlap(out, bytes, c.k_scale, 4 * tiles) ||
+           overlap(out, bytes, c.v_scale, 4 * tiles) || overlap(out, bytes, c.k_sum, 2 * tiles * c.dim);
+}
+
 namespace {
 
 constexpr int64_t kMemoryCache = int64_t{256} << 20;  // bytes that the memory-side cache holds
@@ -337,6 +349,13 @@ extern "C" int h3mi_kv_write_i8(const uint16_t* k, const uint16_t* v, int64_t ro
     const int D = static_cast<int>(cache->dim);
     int64_t groups;
     if (!launchable(seqs->n, touched, cache->heads, 2 * D, &groups)) return fail(H3MI_EINVAL, "kv_write: too many tokens for one call");
+    for (int x = 0; x < 2; ++x) {
+        const size_t bytes = static_cast<size_t>(cache->pages) * cache->heads * cache->dim * kKvBlock;
+        const int8_t* const pages = x ? cache->v : cache->k;
+        if (kv_overlaps(pages, bytes, k, seqs->n, rows, cache->heads, cache->dim, ld_k, bs_k) ||
+            kv_overlaps(pages, bytes, v, seqs->n, rows, cache->heads, cache->dim, ld_v, bs_v))
+            return fail(H3MI_EALIAS, "kv_write: the rows overlap the cache");
+    }
     const bool stream_in = seqs->n * rows * cache->heads * D * 4 > kMemoryCache;
     const auto fn = stream_in ? (D == 64 ? kv_write_kernel<64, true> : D == 128 ? kv_write_kernel<128, true> : kv_write_kernel<256, true>)
                               : (D == 64 ? kv_write_kernel<64, false> : D == 128 ? kv_write_kernel<128, false> : kv_write_kernel<256, false>);
@@ -357,6 +376,9 @@ extern "C" int h3mi_kv_read_bf16(uint16_t* k, uint16_t* v, const int32_t* starts
     const int64_t touched = starts ? (length + 2 * kKvBlock - 2) / kKvBlock : (length + kKvBlock - 1) / kKvBlock;
     int64_t groups;
     if (!launchable(seqs->n, touched, cache->heads, 2 * D, &groups)) return fail(H3MI_EINVAL, "kv_read: too many tokens for one call");
+    const size_t bytes = static_cast<size_t>(seqs->n) * length * cache->heads * cache->dim * 2;
+    if (overlap(k, bytes, v, bytes) || kv_overlaps(k, bytes, *cache) || kv_overlaps(v, bytes, *cache))
+        return fail(H3MI_EALIAS, "kv_read: k, v and the cache overlap");
     const auto fn = D == 64 ? kv_read_kernel<64> : D == 128 ? kv_read_kernel<128> : kv_read_kernel<256>;
     hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(groups)), dim3(2 * D), 0, as_stream(stream), k, v, starts,
                        kv_cache(*cache), kv_seqs(*seqs), static_cast<int>(length), static_cast<int>(touched));

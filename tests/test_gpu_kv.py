@@ -227,6 +227,21 @@ def test_attention_poisoned_block():
         assert np.isfinite(out[0, :, 0]).all() and np.isfinite(out[0, at < 192, 1]).all() and np.isnan(out[0, at >= 192, 1]).all()
 
 
+@pytest.mark.parametrize("rows", [3, 20, 150])
+def test_attention_poisoned_query(rows):
+    """A NaN or an infinity in a query stays in its row and head."""
+    h = _h()
+    rng = np.random.default_rng(12)
+    ref, tables, q = _case(rng, 4, 2, 128, 1, rows, 6, seed=12)
+    c, t, lens = ref.to(), _i32(tables), _i32([380])
+    good = _np(h.kv_attention(_bf(q), c, t, lens))
+    q[0, 1, 2, 5], q[0, 2, 0, 9] = np.nan, np.inf
+    bad = _np(h.kv_attention(_bf(q), c, t, lens))
+    hit = np.zeros(good.shape, bool)
+    hit[0, 1, 2], hit[0, 2, 0] = True, True
+    assert np.isnan(bad[hit]).all() and np.array_equal(bad[~hit], good[~hit])
+
+
 @pytest.mark.parametrize("scale", [0.0, 1.0, -0.3, 30.0])
 @pytest.mark.parametrize("rows", [2, 150])
 def test_attention_scales(scale, rows):

@@ -61,6 +61,10 @@ def test_rows(fn, kw, code, msg):
     ("attention", dict(heads=5), 1, "multiple of the cache's"), ("select", dict(top=0), 1, "top=0"), ("select", dict(top=32769), 1, "top=32769"),
     ("select", dict(out=None), 1, "null blocks"), ("select", dict(out=2), 2, "aligned"), ("attention", dict(out=None), 1, "null out"),
     ("attention", dict(out=8), 2, "aligned"), ("attention", dict(scale=float("nan")), 1, "scale"), ("attention", dict(scale=float("inf")), 1, "scale"),
+    ("attention", dict(out=1 << 20), 3, "overlaps"), ("attention", dict(out=(1 << 20) + 2048), 3, "overlaps"),
+    ("attention", dict(out=1 << 19), 3, "overlaps"), ("attention", dict(out=20480), 3, "overlaps"), ("select", dict(out=1 << 20), 3, "overlaps"),
+    ("select", dict(out=12288), 3, "overlaps"), ("read", dict(p2=1 << 20), 3, "overlap"), ("read", dict(p=1 << 19), 3, "overlap"),
+    ("write", dict(p=1 << 19), 3, "overlap"), ("write", dict(p2=(1 << 19) + 4096), 3, "overlap"),
     ("attention", dict(blocks=4096, top=0), 1, "top=0"), ("attention", dict(blocks=4096, top=1 << 25), 1, "top="), ("attention", dict(blocks=4098), 2, "aligned"),
 ])
 def test_each(fn, kw, code, msg):
@@ -100,7 +104,7 @@ def test_workspace(rows, heads, kv, dim, blocks, top):
     from h3mi import _lib
     need = _lib.lib.h3mi_kv_attention_workspace(1, rows, heads, kv, dim, blocks, top)
     assert need > 0 and need % (dim * 4 + 8) == 0
-    kw = dict(rows=rows, heads=heads, ld=heads * dim, bs=rows * heads * dim, blocks=4096 if top else None, top=top)
+    kw = dict(rows=rows, heads=heads, ld=heads * dim, bs=rows * heads * dim, blocks=4096 if top else None, top=top, p=1 << 41, out=1 << 43)
     seqs = dict(n=1, blocks=blocks)
     cache = dict(heads=kv, dim=dim, v=1 << 40)
     for work, size in ((None, need), (1 << 30, need - 1), (1 << 30, 0)):
@@ -116,7 +120,7 @@ def test_workspace_of_a_selection():
     need = f(4, 1, 8, 2048)
     assert need == 4 * 8 * 2048 * 4
     assert f(4, 1, 8, 100) == 0 and f(1, 2401, 56, 2048) == 0 and f(0, 1, 8, 2048) == 0 and f(1, 1, 8, 32769) == 0 and f(1 << 62, 1, 8, 2048) == 0
-    kw = dict(rows=1, heads=8, ld=1024, bs=1024)
+    kw = dict(rows=1, heads=8, ld=1024, bs=1024, p=1 << 41, out=1 << 43)
     for work, size in ((None, need), (1 << 30, need - 1)):
         rc, m = _call("select", dict(heads=8, v=1 << 40), dict(n=4, blocks=2048), work=work, size=size, **kw)
         assert rc == 1 and "workspace" in m
