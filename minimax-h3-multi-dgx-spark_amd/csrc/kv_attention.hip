@@ -706,12 +706,15 @@ __global__ __launch_bounds__(64 * kFewWaves) void kv_few_kernel(Queries q, KvCac
 
 constexpr int kMaxSplits = 64;  // a lane of the join's wave each
 
-// A wave a row of an item: D / 4 lanes a row of sums, 256 / D splits at once.
-template <int D>
+// D / 4 lanes take a row of an item. FEW: at most kFewSplits splits, whose sums a lane adds up; else a wave a row, 256 / D
+// splits at once.  (Two splits of 30720 rows of 64 elements: a wave a row 17.8 us, so 5.9.)
+constexpr int kFewSplits = 8;
+
+template <int D, bool FEW>
 __global__ __launch_bounds__(256) void kv_join_kernel(Partial part, Queries q, Items items, uint32_t all,
                                                       uint16_t* __restrict__ out) {
     constexpr int L = D / 4, SG = 64 / L;
-    const uint32_t x = blockIdx.x * 4 + (threadIdx.x >> 6);
+    const uint32_t x = FEW ? blockIdx.x * (256 / L) + threadIdx.x / L : blockIdx.x * 4 + (threadIdx.x >> 6);
     if (x >= all) return;
     const int lane = threadIdx.x & 63, d = lane % L * 4, sg = lane / L;
     const uint32_t per = part.rows;
@@ -721,36 +724,56 @@ __global__ __launch_bounds__(256) void kv_join_kernel(Partial part, Queries q, I
     const int y = tile * part.rows + r, row = y / items.pack;
     if (row >= q.rows) return;
     const int64_t query = (static_cast<int64_t>(i) * q.rows + row) * q.heads + head * items.pack + y % items.pack;
-    const float2 ml = lane < part.splits ? part.ml[part.at(item, lane, r)] : make_float2(kLowest, 0.0f);
-    float top = ml.x;
+    float sum = 0.0f, a[4] = {};
+    if constexpr (FEW) {
+        float2 ml[kFewSplits];
+        float4 v[kFewSplits];
+        float top = kLowest;
 #pragma unroll
-    for (int y = 32; y; y >>= 1) top = fmaxf(top, __shfl_xor(top, y));
-    const float fix = ml.y == 0.0f ? 0.0f : exp2_hw(ml.x - top);
-    float sum = ml.y * fix;
-#pragma unroll
-    for (int y = 32; y; y >>= 1) sum += __shfl_xor(sum, y);
-    float a[4] = {};
-    for (int y = 0; y < part.splits; y += 4 * SG) {
-        float f[4];
-        float4 v[4];
-#pragma unroll
-        for (int z = 0; z < 4; ++z) {
-            const int sp = y + z * SG + sg;
-            f[z] = __shfl(fix, sp & 63);
-            if (sp >= part.splits) f[z] = 0.0f;
-            v[z] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (f[z] != 0.0f) v[z] = *reinterpret_cast<const float4*>(part.o + part.at(item, sp, r) * D + d);
+        for (int z = 0; z < kFewSplits; ++z) {
+            ml[z] = z < part.splits ? part.ml[part.at(item, z, r)] : make_float2(kLowest, 0.0f);
+            // a split without a token wrote no sums: its l of 0 leaves them out below
+            v[z] = z < part.splits ? *reinterpret_cast<const float4*>(part.o + part.at(item, z, r) * D + d) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            top = fmaxf(top, ml[z].x);
         }
 #pragma unroll
-        for (int z = 0; z < 4; ++z) a[0] += v[z].x * f[z], a[1] += v[z].y * f[z], a[2] += v[z].z * f[z], a[3] += v[z].w * f[z];
+        for (int z = 0; z < kFewSplits; ++z) {
+            if (ml[z].y == 0.0f) continue;
+            const float f = exp2_hw(ml[z].x - top);
+            sum += ml[z].y * f;
+            a[0] += v[z].x * f, a[1] += v[z].y * f, a[2] += v[z].z * f, a[3] += v[z].w * f;
+        }
+    } else {
+        const float2 ml = lane < part.splits ? part.ml[part.at(item, lane, r)] : make_float2(kLowest, 0.0f);
+        float top = ml.x;
+#pragma unroll
+        for (int y2 = 32; y2; y2 >>= 1) top = fmaxf(top, __shfl_xor(top, y2));
+        const float fix = ml.y == 0.0f ? 0.0f : exp2_hw(ml.x - top);
+        sum = ml.y * fix;
+#pragma unroll
+        for (int y2 = 32; y2; y2 >>= 1) sum += __shfl_xor(sum, y2);
+        for (int s0 = 0; s0 < part.splits; s0 += 4 * SG) {
+            float f[4];
+            float4 v[4];
+#pragma unroll
+            for (int z = 0; z < 4; ++z) {
+                const int sp = s0 + z * SG + sg;
+                f[z] = __shfl(fix, sp & 63);
+                if (sp >= part.splits) f[z] = 0.0f;
+                v[z] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (f[z] != 0.0f) v[z] = *reinterpret_cast<const float4*>(part.o + part.at(item, sp, r) * D + d);
+            }
+#pragma unroll
+            for (int z = 0; z < 4; ++z) a[0] += v[z].x * f[z], a[1] += v[z].y * f[z], a[2] += v[z].z * f[z], a[3] += v[z].w * f[z];
+        }
+#pragma unroll
+        for (int y2 = 32; y2 >= L; y2 >>= 1)
+#pragma unroll
+            for (int z = 0; z < 4; ++z) a[z] += __shfl_xor(a[z], y2);
+        if (sg != 0) return;
     }
-#pragma unroll
-    for (int y = 32; y >= L; y >>= 1)
-#pragma unroll
-        for (int z = 0; z < 4; ++z) a[z] += __shfl_xor(a[z], y);
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    if (sg == 0)
-        *reinterpret_cast<uint2*>(out + query * D + d) = make_uint2(bf16x2_bits(a[0] * inv, a[1] * inv), bf16x2_bits(a[2] * inv, a[3] * inv));
+    *reinterpret_cast<uint2*>(out + query * D + d) = make_uint2(bf16x2_bits(a[0] * inv, a[1] * inv), bf16x2_bits(a[2] * inv, a[3] * inv));
 }
 
 // ------------------------------------------------------------------ what a call runs
@@ -806,8 +829,9 @@ Plan plan_of(int64_t n, int64_t rows, int64_t heads, int64_t kv, int64_t dim, in
     p.whole = p.items / slots * slots;
     const int64_t rest = p.items - p.whole;
     // A split pays for its join (5 us and the sums' bytes) by the blocks that it saves (1.3 us each, alone on a CU): a CU
-    // each, or a slot each where lists are long.
-    int64_t splits = rest > 0 ? (longest >= 64 ? slots : cus) / rest : 1;
+    // each, or a slot each where lists are long (240 tiles of 38 blocks 47.9 us unsplit, 44.0 so; 168 tiles of 15 blocks
+    // 27.9 us, and 35.9 split).
+    int64_t splits = rest > 0 ? (longest >= 24 ? slots : cus) / rest : 1;
     if (splits > longest / 4) splits = longest / 4;
     if (splits > kMaxSplits) splits = kMaxSplits;
     if (splits <= 1) p.whole = p.items / 8 * 8, splits = 1;
@@ -905,8 +929,11 @@ extern "C" int h3mi_kv_attention_bf16(const uint16_t* q, int64_t rows, int64_t h
     if (rc || p.splits == 1) return rc;
     const int64_t all = (p.items - p.whole) * p.rows;
     int64_t groups;
-    if (!launchable((all + 3) / 4, 1, 1, 256, &groups)) return fail(H3MI_EINVAL, "kv_attention: too many rows for one call");
-    const auto join = dim == 64 ? kv_join_kernel<64> : dim == 128 ? kv_join_kernel<128> : kv_join_kernel<256>;
+    const bool few = p.splits <= kFewSplits;
+    const int64_t a_group = few ? 1024 / dim : 4;
+    if (!launchable((all + a_group - 1) / a_group, 1, 1, 256, &groups)) return fail(H3MI_EINVAL, "kv_attention: too many rows for one call");
+    const auto join = few ? (dim == 64 ? kv_join_kernel<64, true> : dim == 128 ? kv_join_kernel<128, true> : kv_join_kernel<256, true>)
+                          : (dim == 64 ? kv_join_kernel<64, false> : dim == 128 ? kv_join_kernel<128, false> : kv_join_kernel<256, false>);
     hipLaunchKernelGGL(join, dim3(static_cast<unsigned>(groups)), dim3(256), 0, st, part, qs, items,
                        static_cast<uint32_t>(all), out);
     return check_launch("kv_attention");
