@@ -87,7 +87,8 @@ struct Factors {
 __device__ __forceinline__ Factors factors(float ks, float vs, float scale) {
     const float c = ks * fabsf(scale);
     const bool fold = vs >= kFoldLow && vs <= kFoldHigh && __builtin_isfinite(c);
-    return {c < 0x1p-126f ? 0x1p-126f : c, fold ? log2f(vs) : 0.0f, fold ? 1.0f / vs : 0.0f, vs};
+    // (both within an ulp, of a scale far from where they flush)
+    return {c < 0x1p-126f ? 0x1p-126f : c, fold ? __builtin_amdgcn_logf(vs) : 0.0f, fold ? __builtin_amdgcn_rcpf(vs) : 0.0f, vs};
 }
 
 struct Queries {
@@ -150,6 +151,7 @@ struct TileShape {
 struct Items {
     int tiles, heads;  // of a head (or a kv head's group); heads (groups) of a sequence
     int pack, rows;    // query heads and queries of an item
+    uint32_t per_pack; // ceil(2^32 / pack)
     int count, whole, chunk, rest_chunk;
     bool flat, last_first;
     // Consecutive items on one XCD, whose L2 then holds their head's blocks.  flat (one round, every workgroup at once):
@@ -164,6 +166,9 @@ struct Items {
         split = x % splits;
         return whole + x / splits;
     }
+    // x / pack: x < 128 pack where pack > 1, so that x times what per_pack is over 2^32 / pack stays below 2^32 / pack for
+    // pack <= kMaxPack.
+    __device__ __forceinline__ int row_of(int x) const { return pack == 1 ? x : static_cast<int>(__umulhi(static_cast<uint32_t>(x), per_pack)); }
     // Of causal items those of a head's last rows, the longest, come first: first of all in a flat launch.
     __device__ __forceinline__ void place(int item, int& seq, int& head, int& tile) const {
         const int all = count / tiles, nh = flat ? item % all : item / tiles;
@@ -198,10 +203,10 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : D == 64 ? 3 : 2) void kv_til
     const int len = s.len(i), count = s.count(i, q.rows), start = s.end(i) - count, queries = count * items.pack;
     // this lane's query, its row and its head
     const int r0 = tile * T::kRows, w0 = r0 + wave * 32, query = w0 + col;
-    const int row = query / items.pack, hq = head * items.pack + query % items.pack;
+    const int row = items.row_of(query), hq = head * items.pack + query - row * items.pack;
     // the last token that this lane's query, the wave's last and the workgroup's last see
     auto last_of = [&](int x) {
-        const int y = start + x / items.pack, most = causal && y < len - 1 ? y : len - 1;
+        const int y = start + items.row_of(x), most = causal && y < len - 1 ? y : len - 1;
         return x < queries ? most : -1;
     };
     const int last = last_of(query);
@@ -228,10 +233,12 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : D == 64 ? 3 : 2) void kv_til
     float m = kLowest, l = 0.0f;
 
     const int32_t* const mine =
-        list.p ? list.p + ((static_cast<int64_t>(i) * list.tiles + r0 / items.pack / kKvTile) * c.heads + h) * list.top : nullptr;
+        list.p ? list.p + ((static_cast<int64_t>(i) * list.tiles + items.row_of(r0) / kKvTile) * c.heads + h) * list.top : nullptr;
     const int total = blocks == 0 ? 0 : mine ? list.top : blocks;
-    const int from = static_cast<int>(static_cast<int64_t>(total) * split / splits);
-    const int to = static_cast<int>(static_cast<int64_t>(total) * (split + 1) / splits);
+    // an even share: total < 2^25, splits <= 64
+    const uint32_t share = static_cast<uint32_t>(total), of = static_cast<uint32_t>(splits);
+    const int from = splits == 1 ? 0 : static_cast<int>(share * split / of);
+    const int to = splits == 1 ? total : static_cast<int>(share * (split + 1) / of);
 
     // Bytes of a block into registers, and as bf16 into LDS: 8 of them a chunk.
     uint4 kr[T::kLoads], vr[T::kLoads];
@@ -721,9 +728,9 @@ __global__ __launch_bounds__(256) void kv_join_kernel(Partial part, Queries q, I
     const int item = static_cast<int>(x / per), r = static_cast<int>(x % per);
     int i, head, tile;
     items.place(items.whole + item, i, head, tile);
-    const int y = tile * part.rows + r, row = y / items.pack;
+    const int y = tile * part.rows + r, row = items.row_of(y);
     if (row >= q.rows) return;
-    const int64_t query = (static_cast<int64_t>(i) * q.rows + row) * q.heads + head * items.pack + y % items.pack;
+    const int64_t query = (static_cast<int64_t>(i) * q.rows + row) * q.heads + head * items.pack + y - row * items.pack;
     float sum = 0.0f, a[4] = {};
     if constexpr (FEW) {
         float2 ml[kFewSplits];
@@ -782,6 +789,8 @@ __global__ __launch_bounds__(256) void kv_join_kernel(Partial part, Queries q, I
 // 230 us where 32 take 87), 16 of 256.
 constexpr int64_t few_queries(int64_t dim) { return 64 * kFew / dim * 4; }
 
+constexpr int64_t kMaxPack = 4096;
+
 struct Plan {
     bool few, flat;
     int waves;          // of a tile's workgroup
@@ -814,7 +823,7 @@ Plan plan_of(int64_t n, int64_t rows, int64_t heads, int64_t kv, int64_t dim, in
         return p;
     }
     // Rows that leave a tile part empty share it with the other heads of their group (a list is a kv head's).
-    p.pack = rows < kKvTile ? static_cast<int>(group) : 1;
+    p.pack = rows < kKvTile && group <= kMaxPack ? static_cast<int>(group) : 1;
     p.heads = heads / p.pack;
     // Tiles of 4 waves, two a CU, balance themselves; 8 waves in step are ahead where the work is long and even: 128
     // elements, 128 blocks and 1024 rows on (4800 x 19721 2661 us, 2746 with 4; 2000 x 9000 562 and 583; but 2000 x 2000
@@ -901,7 +910,8 @@ extern "C" int h3mi_kv_attention_bf16(const uint16_t* q, int64_t rows, int64_t h
     const Queries qs = {q, ld_q, bs_q, static_cast<int>(rows), static_cast<int>(heads)};
     const Lists list = {blocks, static_cast<int>(top), static_cast<int>((rows + kKvTile - 1) / kKvTile)};
     Partial part = {static_cast<float*>(workspace), nullptr, p.splits, static_cast<int>(p.rows)};
-    const Items items = {static_cast<int>(p.tiles), static_cast<int>(p.heads), p.pack, static_cast<int>(p.rows), static_cast<int>(p.items),
+    const Items items = {static_cast<int>(p.tiles), static_cast<int>(p.heads), p.pack, static_cast<int>(p.rows),
+                         p.pack == 1 ? 0u : static_cast<uint32_t>(((uint64_t{1} << 32) + p.pack - 1) / p.pack), static_cast<int>(p.items),
                          static_cast<int>(p.whole), static_cast<int>(p.whole / 8), static_cast<int>((rest + 7) / 8), p.flat, causal != 0 && !p.few};
     if (need > 0) part.ml = reinterpret_cast<float2*>(part.o + part_rows * dim);
     const KvCache c = kv_cache(*cache);
