@@ -113,17 +113,24 @@ struct Partial {
 
 // ------------------------------------------------------------------ tiles of queries
 
-// W waves of 32 query rows of one head.  The block's keys and values go through LDS as
-// bf16, converted once a workgroup, in two buffers each.  A wave's step y has two halves:
-// the products of block y's keys and of block y - 1's values (MFMA, while a later block's
-// bytes are loaded), then block y's softmax and that later block's conversion (VALU).  Of 8
-// waves the second four run half a step behind the first, with a barrier after each half:
-// of the two waves on a SIMD one is in its products while the other is in its softmax.  They
+// W waves of 32 query rows.  The block's keys and values go through LDS as bf16, converted
+// once a workgroup, in two buffers each.  A wave's step y has two halves: the products of
+// block y's keys and of block y - 1's values (MFMA, while a later block's bytes are loaded),
+// then block y's softmax and that later block's conversion (VALU).  With 4 waves there is a
+// barrier a step, and the workgroups that share a CU fall out of step by themselves.  Of 8
+// waves the second four run half a step behind the first, with a barrier after each half: of
+// the two waves on a SIMD one is in its products while the other is in its softmax; they
 // convert their share of a block one step earlier in turn, so that it is there in time.
-// (With 4 waves a barrier a step; workgroups that share a CU fall out of step by themselves.)  Rows are
-// 16-byte chunks whose index is XORed with row bits, so that 16 lanes of an access lie on
-// the 16 different 16-byte groups of LDS's 256 bytes of banks, both for the writes (rows)
-// and for the MFMA operands' reads (columns).
+//
+// Rows in LDS are 16-byte chunks whose index is XORed with row bits, so that 16 lanes of an
+// access lie on the 16 different 16-byte groups of LDS's 256 bytes of banks, both for the
+// writes (rows) and for the MFMA operands' reads (columns); by three row bits instead of four
+// 43% of LDS's cycles were conflicts, and 2.88 ms were 2.63.
+//
+// Measured: 4800 rows over 19721 tokens of 56 x 128 in 2.63 ms, 1030 TFLOP/s, 84% of what a
+// large bf16 product reaches on the card; the power limit holds it there (1.98 GHz, 46% of
+// MFMA issue).  56 heads of 2401 rows over lists of 100 blocks in 0.49 ms, 900 TFLOP/s.
+
 // The place of chunk ch of a row of CH chunks (8: two rows share the banks).
 template <int CH>
 __device__ __forceinline__ int chunk_at(int row, int ch) {
@@ -490,8 +497,9 @@ constexpr int kFewWaves = 4;
 // A workgroup: up to 16 NQ queries of one kv head's group, one split of its blocks.  Its
 // waves take whole blocks in turn, straight from memory into the operands' registers (no
 // LDS, no barrier; a block's bytes are converted once for all queries), and are joined once
-// at the end.  With a tile's 16 KB at a time a workgroup, 17 rows of 56 heads over 4000
-// tokens waited for memory 272 us; so they take 87.
+// at the end.  HBM bounds it: a query of 56 heads over 19721 tokens takes 47 us, 6.0 TB/s, 17
+// to 32 rows of 8 x 56 heads over 4000 tokens 87 us, where the 40 that go by tiles, 16 KB a
+// workgroup at a time, take 129.
 template <int D, int NQ>
 __global__ __launch_bounds__(64 * kFewWaves) void kv_few_kernel(Queries q, KvCache c, KvSeqs s, float scale, int causal, Lists list,
                                                                 uint16_t* __restrict__ out, Partial part, int per) {

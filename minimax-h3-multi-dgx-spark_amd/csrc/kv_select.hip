@@ -11,7 +11,8 @@
 // ordered 32-bit keys in LDS, finds the last selected key by four passes over 8 bits of
 // it, and writes the selected blocks in order.  Few tiles over long tables, whose scoring
 // would wait on a few CUs' loads, score in a launch of their own, a workgroup for every
-// kChunk blocks, and the keys pass through memory.
+// kChunk blocks, and the keys pass through memory.  1064 tiles of 609 blocks take 25 us, half
+// of it the queries' pooling; 32 tiles of 2048 blocks 15 us in two launches.
 #include "kv.h"
 
 namespace h3mi {
@@ -250,7 +251,7 @@ using namespace h3mi;
 
 namespace {
 
-// Whether the tiles are few and their tables long: 32 tiles of 2048 blocks 21 us in one launch.
+// Whether the tiles are few and their tables long: 32 tiles of 2048 blocks 21 us in one launch, 15 in two.
 bool scores_apart(int64_t groups, int64_t blocks) { return 2 * groups <= cu_count() && blocks >= 2 * kChunk; }
 
 int64_t key_bytes(int64_t groups, int64_t blocks) { return scores_apart(groups, blocks) ? groups * blocks * 4 : 0; }
