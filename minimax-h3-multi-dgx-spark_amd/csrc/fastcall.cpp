@@ -531,7 +531,7 @@ PyObject* kv_attention(PyObject*, PyObject* const* v, Py_ssize_t n) {
     if (v[7] != Py_None) {
         list = a.typed(v[7], c10::kInt);
         if (!a.ok || list->dim() != 4 || !list->is_contiguous() || list->size(0) != kv.s.n ||
-            list->size(1) != (q.rows + H3MI_KV_TILE - 1) / H3MI_KV_TILE || list->size(2) != kv.c.heads)
+            list->size(1) != (q.rows + H3MI_KV_TILE - 1) / H3MI_KV_TILE || list->size(2) != kv.c.heads || list->size(3) < 1)
             Py_RETURN_NONE;
         top = list->size(3);
     }

@@ -161,9 +161,9 @@ def kv_select(q, cache, tables, lens, top, causal=False, counts=None):
     rows, ld, bs = _rows(q, cache, s.n, "q")
     top = int(top)
     out = torch.empty((s.n, -(-rows // KV_TILE), c.heads, max(top, 0)), dtype=torch.int32, device=q.device)
-    need = lib.h3mi_kv_select_workspace(s.n, rows, c.heads, s.blocks)
-    work = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
     with torch.cuda.device(q.device):
+        need = lib.h3mi_kv_select_workspace(s.n, rows, c.heads, s.blocks)
+        work = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
         check(lib.h3mi_kv_select(ptr(q), rows, q.shape[2], ld, bs, ctypes.byref(c), ctypes.byref(s), top, int(bool(causal)),
                                  ptr(out), ptr(work), need, stream_of(q)))
     return out
@@ -186,11 +186,13 @@ def kv_attention(q, cache, tables, lens, causal=False, counts=None, scale=None, 
     if blocks is not None:
         top = blocks.shape[-1]
         _ints(blocks, (s.n, -(-rows // KV_TILE), c.heads, top), "blocks")
+        if top < 1:  # an empty tensor has no address, which would say: all blocks
+            raise ValueError("blocks must name at least one block a tile (-1: none)")
         same_gpu(q, blocks=blocks)
     out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
-    need = lib.h3mi_kv_attention_workspace(s.n, rows, heads, c.heads, c.dim, s.blocks, top)
-    work = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
     with torch.cuda.device(q.device):
+        need = lib.h3mi_kv_attention_workspace(s.n, rows, heads, c.heads, c.dim, s.blocks, top)
+        work = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
         check(lib.h3mi_kv_attention_bf16(ptr(q), rows, heads, ld, bs, ctypes.byref(c), ctypes.byref(s),
                                          float(c.dim ** -0.5 if scale is None else scale), int(bool(causal)), ptr(blocks), top,
                                          ptr(out), ptr(work), max(need, 0), stream_of(q)))

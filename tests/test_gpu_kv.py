@@ -652,3 +652,14 @@ def test_refusals_of_the_python_functions():
     assert h.kv_attention(q, c, t[:, :0].contiguous(), lens).abs().max() == 0
     assert (h.kv_select(q, c, t[:, :0].contiguous(), lens, 3) == -1).all()
     assert h.kv_read(c, t, lens, 0)[0].shape == (1, 0, 2, 64)
+
+
+def test_lists_of_no_entry_are_refused():
+    """An empty list's tensor has no address, and must not be taken for no list."""
+    h = _h()
+    c, t, lens = h.kv_cache(4, 2, 64), _i32([[0, 1]]), _i32([100])
+    q = torch.zeros(1, 10, 4, 64, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(ValueError, match="at least one"):
+        h.kv_attention(q, c, t, lens, blocks=torch.empty(1, 1, 2, 0, dtype=torch.int32, device=DEV))
+    assert h.kv_attention(q[:, :0], c, t, lens, blocks=torch.empty(1, 0, 2, 3, dtype=torch.int32, device=DEV)).shape == (1, 0, 4, 64)
+    assert h.kv_attention(q, c, t, lens, blocks=torch.full((1, 1, 2, 1), -1, dtype=torch.int32, device=DEV)).abs().max() == 0
