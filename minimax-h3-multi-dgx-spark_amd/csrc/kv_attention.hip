@@ -910,7 +910,7 @@ extern "C" int h3mi_kv_attention_bf16(const uint16_t* q, int64_t rows, int64_t h
     const int64_t rest = (p.items - p.whole) * p.splits;
     if (p.items > (1 << 30) || rest > (1 << 30)) return fail(H3MI_EINVAL, "kv_attention: too many rows for one call");
     const size_t bytes = static_cast<size_t>(n) * rows * heads * dim * 2;
-    if (kv_overlaps(out, bytes, q, n, rows, heads, dim, ld_q, bs_q) || kv_overlaps(out, bytes, *cache))
+    if (overlap(out, bytes, q, kv_span(n, rows, heads, dim, ld_q, bs_q)) || kv_overlaps(out, bytes, *cache))
         return fail(H3MI_EALIAS, "kv_attention: out overlaps q or the cache");
     if (need > 0 && (!workspace || workspace_bytes < need))
         return fail(H3MI_EINVAL, "kv_attention: workspace of %lld bytes, %lld needed", (long long)(workspace ? workspace_bytes : 0), (long long)need);

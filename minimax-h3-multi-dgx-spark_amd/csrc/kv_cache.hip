@@ -47,10 +47,9 @@ int kv_check_rows(const char* what, const char* name, const uint16_t* p, int64_t
     return H3MI_OK;
 }
 
-bool kv_overlaps(const void* out, size_t bytes, const uint16_t* p, int64_t n, int64_t rows, int64_t heads, int64_t dim, int64_t ld, int64_t bs) {
-    if (n == 0 || rows == 0) return false;
-    const size_t span = static_cast<size_t>(n - 1) * bs + static_cast<size_t>(rows - 1) * ld + static_cast<size_t>(heads) * dim;
-    return overlap(out, bytes, p, 2 * span);
+size_t kv_span(int64_t n, int64_t rows, int64_t heads, int64_t dim, int64_t ld, int64_t bs) {
+    if (n == 0 || rows == 0) return 0;
+    return 2 * (static_cast<size_t>(n - 1) * bs + static_cast<size_t>(rows - 1) * ld + static_cast<size_t>(heads) * dim);
 }
 
 bool kv_overlaps(const void* out, size_t bytes, const h3mi_kv_cache& c) {
@@ -350,11 +349,8 @@ extern "C" int h3mi_kv_write_i8(const uint16_t* k, const uint16_t* v, int64_t ro
     int64_t groups;
     if (!launchable(seqs->n, touched, cache->heads, 2 * D, &groups)) return fail(H3MI_EINVAL, "kv_write: too many tokens for one call");
     for (int x = 0; x < 2; ++x) {
-        const size_t bytes = static_cast<size_t>(cache->pages) * cache->heads * cache->dim * kKvBlock;
-        const int8_t* const pages = x ? cache->v : cache->k;
-        if (kv_overlaps(pages, bytes, k, seqs->n, rows, cache->heads, cache->dim, ld_k, bs_k) ||
-            kv_overlaps(pages, bytes, v, seqs->n, rows, cache->heads, cache->dim, ld_v, bs_v))
-            return fail(H3MI_EALIAS, "kv_write: the rows overlap the cache");
+        const size_t bytes = kv_span(seqs->n, rows, cache->heads, cache->dim, x ? ld_v : ld_k, x ? bs_v : bs_k);
+        if (kv_overlaps(x ? v : k, bytes, *cache)) return fail(H3MI_EALIAS, "kv_write: the rows overlap the cache");
     }
     const bool stream_in = seqs->n * rows * cache->heads * D * 4 > kMemoryCache;
     const auto fn = stream_in ? (D == 64 ? kv_write_kernel<64, true> : D == 128 ? kv_write_kernel<128, true> : kv_write_kernel<256, true>)

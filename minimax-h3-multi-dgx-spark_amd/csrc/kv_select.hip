@@ -292,7 +292,7 @@ extern "C" int h3mi_kv_select(const uint16_t* q, int64_t rows, int64_t heads, in
     int64_t groups;
     if (!launchable(seqs->n, tiles, cache->heads, 1024, &groups)) return fail(H3MI_EINVAL, "kv_select: too many rows for one call");
     const size_t bytes = static_cast<size_t>(groups) * top * 4;
-    if (kv_overlaps(blocks, bytes, q, seqs->n, rows, heads, cache->dim, ld_q, bs_q) || kv_overlaps(blocks, bytes, *cache))
+    if (overlap(blocks, bytes, q, kv_span(seqs->n, rows, heads, cache->dim, ld_q, bs_q)) || kv_overlaps(blocks, bytes, *cache))
         return fail(H3MI_EALIAS, "kv_select: blocks overlaps q or the cache");
     const int64_t need = key_bytes(groups, seqs->blocks);
     if (need > 0 && (!workspace || workspace_bytes < need))

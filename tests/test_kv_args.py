@@ -148,3 +148,10 @@ def test_cpu_tensors_are_refused():
             f()
     with pytest.raises(ValueError, match="dim"):
         h3mi.kv_cache(2, 2, 100, device="cpu")
+
+
+@pytest.mark.parametrize("at", [12288, 16384, 20480])
+@pytest.mark.parametrize("name", ["p", "p2"])
+def test_written_rows_over_the_scales_and_sums(name, at):
+    rc, m = _call("write", dict(k=1 << 23, v=1 << 24), **{name: at})
+    assert rc == 3 and "overlap" in m, (rc, m)
