@@ -493,233 +493,296 @@ __device__ __forceinline__ uint4 load_once(const int8_t* p) {
 
 constexpr int kFew = 16;  // queries: the columns of a 16x16 MFMA
 constexpr int kFewWaves = 4;
+constexpr int kFewThreads = 64 * kFewWaves;
 
-// A workgroup: up to 16 NQ queries of one kv head's group, one split of its blocks.  Its
+// How a launch's workgroups share the blocks of all sequences of a kv head, laid end to end: even shares, whatever the
+// sequences' lengths, `shares` for each kv head (0: a workgroup a sequence and kv head).  A piece, what a share has of one
+// sequence, leaves partial sums: sequence i's piece of share w is piece w + i, as from one piece to the next either the
+// share or the sequence is another.  spans[i]: the first and the last share with blocks of sequence i.
+struct Shares {
+    int shares;
+    int2* spans;
+};
+
+// A workgroup: up to 16 NQ queries of one kv head's group, one share of the blocks.  Its
 // waves take whole blocks in turn, straight from memory into the operands' registers (no
 // LDS, no barrier; a block's bytes are converted once for all queries), and are joined once
-// at the end.  HBM bounds it: a query of 56 heads over 19721 tokens takes 47 us, 6.0 TB/s, 17
+// for each sequence.  HBM bounds it: a query of 56 heads over 19721 tokens takes 47 us, 6.0 TB/s, 17
 // to 32 rows of 8 x 56 heads over 4000 tokens 87 us, where the 40 that go by tiles, 16 KB a
-// workgroup at a time, take 129.
+// workgroup at a time, take 129; 16 sequences of 1 to 32768 tokens of 8 heads (780 MB) 128, where
+// shares of their own for each, a quarter of the longest, took 146.
 template <int D, int NQ>
 __global__ __launch_bounds__(64 * kFewWaves) void kv_few_kernel(Queries q, KvCache c, KvSeqs s, float scale, int causal, Lists list,
-                                                                uint16_t* __restrict__ out, Partial part, int per) {
+                                                                uint16_t* __restrict__ out, Partial part, Shares shares) {
     constexpr int KL = D / 64;   // 16-byte pieces of a key row a lane
     constexpr int NT = D / 16;   // tiles of 16 elements of the output
     __shared__ float jo[kFewWaves][kFew][D + 4];
     __shared__ float2 jml[kFewWaves][kFew];
+    __shared__ int ends[kFewThreads + 1];  // blocks of the sequences up to each
+    __shared__ int wave_sum[kFewWaves];
 
-    const int split = blockIdx.x % part.splits;
-    const int nh = blockIdx.x / part.splits;
-    const int h = nh % c.heads, i = nh / c.heads;
+    const int h = blockIdx.x % c.heads, w = blockIdx.x / c.heads;
     const int group = q.heads / c.heads, queries = q.rows * group;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, col = lane & 15, quad = lane >> 4;
 
-    const int len = s.len(i), count = s.count(i, q.rows), start = s.end(i) - count;
-    auto last_of = [&](int r) {
-        int x = len - 1;
-        if (causal && start + r < x) x = start + r;
-        return r < count ? x : -1;
-    };
-    const int most = count > 0 ? last_of(count - 1) : -1;
-    // below this every query that is one sees a whole block
-    const int full = count > 0 ? last_of(0) + 1 : 0;
-    const int blocks = most < 0 ? 0 : block_of(most) + 1;
-
-    // query 16 g + col of each set g
-    int last[NQ];
-    bf16x8 qf[NQ][2 * KL];
-    f32x4 o[NQ][NT];
-    float m[NQ], l[NQ];
-#pragma unroll
-    for (int g = 0; g < NQ; ++g) {
-        const int query = g * kFew + col, row = query / group, hq = h * group + query % group;
-        last[g] = query < queries ? last_of(row) : -1;
-        const int64_t at = i * q.bs + static_cast<int64_t>(row) * q.ld + static_cast<int64_t>(hq) * D + quad * 16;
-#pragma unroll
-        for (int k = 0; k < 2 * KL; ++k)
-            qf[g][k] = last[g] >= 0 ? query_frag(q.p + at + (k >> 1) * 64 + (k & 1) * 8, scale) : frag(make_uint4(0, 0, 0, 0));
-#pragma unroll
-        for (int n = 0; n < NT; ++n) o[g][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        m[g] = kLowest, l[g] = 0.0f;
-    }
-
-    const int32_t* const mine = list.p ? list.p + (static_cast<int64_t>(i) * list.tiles * c.heads + h) * list.top : nullptr;
-    const int total = blocks == 0 ? 0 : mine ? list.top : blocks;
-    // splits of a fixed length, so that those of uneven sequences are even
-    const int from = split * per < total ? split * per : total;
-    const int to = from + per < total ? from + per : total;
-    if (part.splits > 1 && from >= to) {
-        if (t < queries) part.ml[part.at(nh, split, t)] = make_float2(kLowest, 0.0f);
-        return;
-    }
-
-    uint4 kr[4][KL], vr[NT];
-    auto load_k = [&](int page) {
-        const int8_t* const p = c.k + (static_cast<int64_t>(page) * c.heads + h) * (kKvBlock * D);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int tok = 16 * (col >> 2) + 4 * u + (col & 3);
-#pragma unroll
-            for (int k = 0; k < KL; ++k) kr[u][k] = load_once(p + tok * D + 64 * k + 16 * quad);
+    // what sequence i's queries see: tokens, its first row's token and its rows
+    struct Seen {
+        int len, start, count;
+        __device__ __forceinline__ int last_of(int r, int causal) const {
+            int x = len - 1;
+            if (causal && start + r < x) x = start + r;
+            return r < count ? x : -1;
         }
     };
-    auto load_v = [&](int page) {
-        const int8_t* const p = c.v + (static_cast<int64_t>(page) * c.heads + h) * (kKvBlock * D);
-#pragma unroll
-        for (int d = 0; d < NT; ++d) vr[d] = load_once(p + (16 * d + col) * kKvBlock + 16 * quad);
+    auto seen_of = [&](int i) {
+        const int count = s.count(i, q.rows);
+        return Seen{s.len(i), s.end(i) - count, count};
     };
-
-    // a lane holds the page and the factors of one of the wave's next 64 blocks
-    for (int x0 = from; x0 < to; x0 += 64 * kFewWaves) {
-        const int x = x0 + lane * kFewWaves + wave;
-        const int b = x < to ? (mine ? mine[x] : x) : -1;
-        const int page = b >= 0 && b < blocks ? s.page(i, b, c.pages) : -1;
-        uint64_t left = __ballot(page >= 0);
-        if (!left) continue;
-        Factors f = {};
-        if (page >= 0) {
-            const int64_t p = static_cast<int64_t>(page) * c.heads + h;
-            f = factors(c.ks[p], c.vs[p], scale * kLog2e);
+    auto blocks_of = [&](const Seen& n) {
+        const int most = n.count > 0 ? n.last_of(n.count - 1, causal) : -1;
+        return most < 0 ? 0 : block_of(most) + 1;
+    };
+    int i = w, at = 0, share_end = 0;
+    if (shares.shares) {
+        const int mine = t < s.n ? blocks_of(seen_of(t)) : 0;
+        int sum = mine > 0 && list.p ? list.top : mine;
+        const int own = sum;
+#pragma unroll
+        for (int x = 1; x < 64; x <<= 1) {
+            const int o = __shfl_up(sum, x);
+            if (lane >= x) sum += o;
         }
-        int y = __builtin_ctzll(left);
-        int now = __builtin_amdgcn_readlane(page, y);
-        load_k(now);
-        load_v(now);
-        while (left) {
-            left &= left - 1;
-            const int z = left ? __builtin_ctzll(left) : y;
-            const int next = __builtin_amdgcn_readlane(page, z);
-            const int base = __builtin_amdgcn_readlane(b, y) * kKvBlock;
-            const float fc = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f.c), y));
-            const float flv = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f.lv), y));
-            const float fiv = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f.iv), y));
-            const float fvs = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f.vs), y));
-            f32x4 sc[NQ][4];
+        if (lane == 63) wave_sum[wave] = sum;
+        __syncthreads();
+        int all = 0;
+#pragma unroll
+        for (int x = 0; x < kFewWaves; ++x) {
+            if (x < wave) sum += wave_sum[x];
+            all += wave_sum[x];
+        }
+        ends[t + 1] = sum;
+        if (t == 0) ends[0] = 0;
+        __syncthreads();
+        const int per = all == 0 ? 1 : static_cast<int>((static_cast<uint32_t>(all) + shares.shares - 1) / shares.shares);
+        if (blockIdx.x == 0 && t < s.n)
+            shares.spans[t] = own == 0 ? make_int2(0, -1) : make_int2((sum - own) / per, (sum - 1) / per);
+        at = uniform(w * per);
+        share_end = uniform(at + per < all ? at + per : all);
+        if (at >= all) return;
+        // the sequence of the share's first block
+        for (int x = 0; x < s.n; x += 64) {
+            const uint64_t past = __ballot(x + lane < s.n && ends[x + lane + 1] > at);
+            if (past) {
+                i = x + __builtin_ctzll(past);
+                break;
+            }
+        }
+    }
+
+    for (bool again = false;; again = true) {
+        const Seen seq = seen_of(i);
+        const int blocks = blocks_of(seq);
+        // below this every query that is one sees a whole block
+        const int full = seq.count > 0 ? seq.last_of(0, causal) + 1 : 0;
+        // query 16 g + col of each set g
+        int last[NQ];
+        bf16x8 qf[NQ][2 * KL];
+        f32x4 o[NQ][NT];
+        float m[NQ], l[NQ];
+#pragma unroll
+        for (int g = 0; g < NQ; ++g) {
+            const int query = g * kFew + col, row = query / group, hq = h * group + query % group;
+            last[g] = query < queries ? seq.last_of(row, causal) : -1;
+            const int64_t to_q = i * q.bs + static_cast<int64_t>(row) * q.ld + static_cast<int64_t>(hq) * D + quad * 16;
+#pragma unroll
+            for (int k = 0; k < 2 * KL; ++k)
+                qf[g][k] = last[g] >= 0 ? query_frag(q.p + to_q + (k >> 1) * 64 + (k & 1) * 8, scale) : frag(make_uint4(0, 0, 0, 0));
+#pragma unroll
+            for (int n = 0; n < NT; ++n) o[g][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            m[g] = kLowest, l[g] = 0.0f;
+        }
+
+        const int32_t* const mine = list.p ? list.p + (static_cast<int64_t>(i) * list.tiles * c.heads + h) * list.top : nullptr;
+        const int total = blocks == 0 ? 0 : mine ? list.top : blocks;
+        int from = 0, to = total;
+        if (shares.shares) {
+            const int begin = uniform(ends[i]), last_end = uniform(ends[i + 1]), end = last_end < share_end ? last_end : share_end;
+            from = at - begin, to = end - begin;
+            at = end;
+        }
+
+        uint4 kr[4][KL], vr[NT];
+        auto load_k = [&](int page) {
+            const int8_t* const p = c.k + (static_cast<int64_t>(page) * c.heads + h) * (kKvBlock * D);
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
+                const int tok = 16 * (col >> 2) + 4 * u + (col & 3);
 #pragma unroll
-                for (int g = 0; g < NQ; ++g) sc[g][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int k = 0; k < KL; ++k) {
-                    const uint4 w = kr[u][k];
-                    const bf16x8 lo = frag(ints_bf16(make_uint2(w.x, w.y))), hi = frag(ints_bf16(make_uint2(w.z, w.w)));
-#pragma unroll
-                    for (int g = 0; g < NQ; ++g) {
-                        sc[g][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, qf[g][2 * k], sc[g][u], 0, 0, 0);
-                        sc[g][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, qf[g][2 * k + 1], sc[g][u], 0, 0, 0);
-                    }
-                }
+                for (int k = 0; k < KL; ++k) kr[u][k] = load_once(p + tok * D + 64 * k + 16 * quad);
             }
-            if (left) load_k(next);
-            // register r of sc[g][u]: token base + 16 quad + 4 u + r
-            const bool mask = base + kKvBlock > full;
-            bf16x8 p[NQ][2];
+        };
+        auto load_v = [&](int page) {
+            const int8_t* const p = c.v + (static_cast<int64_t>(page) * c.heads + h) * (kKvBlock * D);
 #pragma unroll
-            for (int g = 0; g < NQ; ++g) {
-                float best = -__builtin_inff();
+            for (int d = 0; d < NT; ++d) vr[d] = load_once(p + (16 * d + col) * kKvBlock + 16 * quad);
+        };
+
+        // a lane holds the page and the factors of one of the wave's next 64 blocks
+        for (int x0 = from; x0 < to; x0 += 64 * kFewWaves) {
+            const int x = x0 + lane * kFewWaves + wave;
+            const int b = x < to ? (mine ? mine[x] : x) : -1;
+            const int page = b >= 0 && b < blocks ? s.page(i, b, c.pages) : -1;
+            uint64_t left = __ballot(page >= 0);
+            if (!left) continue;
+            Factors f = {};
+            if (page >= 0) {
+                const int64_t p = static_cast<int64_t>(page) * c.heads + h;
+                f = factors(c.ks[p], c.vs[p], scale * kLog2e);
+            }
+            int y = __builtin_ctzll(left);
+            int now = __builtin_amdgcn_readlane(page, y);
+            load_k(now);
+            load_v(now);
+            while (left) {
+                left &= left - 1;
+                const int z = left ? __builtin_ctzll(left) : y;
+                const int next = __builtin_amdgcn_readlane(page, z);
+                const int base = __builtin_amdgcn_readlane(b, y) * kKvBlock;
+                const float fc = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f.c), y));
+                const float flv = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f.lv), y));
+                const float fiv = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f.iv), y));
+                const float fvs = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f.vs), y));
+                f32x4 sc[NQ][4];
 #pragma unroll
-                for (int u = 0; u < 4; ++u)
+                for (int u = 0; u < 4; ++u) {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        if (mask && base + 16 * quad + 4 * u + r > last[g]) sc[g][u][r] = -__builtin_inff();
-                        best = fmaxf(best, sc[g][u][r]);
+                    for (int g = 0; g < NQ; ++g) sc[g][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int k = 0; k < KL; ++k) {
+                        const uint4 w = kr[u][k];
+                        const bf16x8 lo = frag(ints_bf16(make_uint2(w.x, w.y))), hi = frag(ints_bf16(make_uint2(w.z, w.w)));
+#pragma unroll
+                        for (int g = 0; g < NQ; ++g) {
+                            sc[g][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, qf[g][2 * k], sc[g][u], 0, 0, 0);
+                            sc[g][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, qf[g][2 * k + 1], sc[g][u], 0, 0, 0);
+                        }
                     }
-                best = fmaxf(best, __shfl_xor(best, 16));
-                best = fmaxf(best, __shfl_xor(best, 32)) * fc;
-                if (__any(best > m[g] + kSlack)) {
-                    const float mn = fmaxf(m[g], best), fix = exp2_hw(m[g] - mn);
-                    m[g] = mn;
-                    l[g] *= fix;
-#pragma unroll
-                    for (int d = 0; d < NT; ++d) o[g][d] *= fix;
                 }
-                const float off = flv - m[g];
-                float sum = 0.0f;
+                if (left) load_k(next);
+                // register r of sc[g][u]: token base + 16 quad + 4 u + r
+                const bool mask = base + kKvBlock > full;
+                bf16x8 p[NQ][2];
 #pragma unroll
-                for (int u = 0; u < 4; ++u)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        sc[g][u][r] = exp2_hw(__builtin_fmaf(sc[g][u][r], fc, off));
-                        sum += sc[g][u][r];
-                    }
-                if (fiv != 0.0f) {
-                    l[g] = __builtin_fmaf(sum, fiv, l[g]);
-                } else {
-                    // a scale that is no ordinary number: what a row does not see must not reach it
+                for (int g = 0; g < NQ; ++g) {
+                    float best = -__builtin_inff();
 #pragma unroll
                     for (int u = 0; u < 4; ++u)
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
-                            const float e = base + 16 * quad + 4 * u + r > last[g] ? 0.0f : sc[g][u][r];
-                            l[g] += e;
-                            sc[g][u][r] = e == 0.0f ? 0.0f : e * fvs;
+                            if (mask && base + 16 * quad + 4 * u + r > last[g]) sc[g][u][r] = -__builtin_inff();
+                            best = fmaxf(best, sc[g][u][r]);
                         }
+                    best = fmaxf(best, __shfl_xor(best, 16));
+                    best = fmaxf(best, __shfl_xor(best, 32)) * fc;
+                    if (__any(best > m[g] + kSlack)) {
+                        const float mn = fmaxf(m[g], best), fix = exp2_hw(m[g] - mn);
+                        m[g] = mn;
+                        l[g] *= fix;
+#pragma unroll
+                        for (int d = 0; d < NT; ++d) o[g][d] *= fix;
+                    }
+                    const float off = flv - m[g];
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            sc[g][u][r] = exp2_hw(__builtin_fmaf(sc[g][u][r], fc, off));
+                            sum += sc[g][u][r];
+                        }
+                    if (fiv != 0.0f) {
+                        l[g] = __builtin_fmaf(sum, fiv, l[g]);
+                    } else {
+                        // a scale that is no ordinary number: what a row does not see must not reach it
+#pragma unroll
+                        for (int u = 0; u < 4; ++u)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                const float e = base + 16 * quad + 4 * u + r > last[g] ? 0.0f : sc[g][u][r];
+                                l[g] += e;
+                                sc[g][u][r] = e == 0.0f ? 0.0f : e * fvs;
+                            }
+                    }
+#pragma unroll
+                    for (int w = 0; w < 2; ++w) {
+                        const f32x4 a = sc[g][2 * w], e = sc[g][2 * w + 1];
+                        p[g][w] = frag(make_uint4(bf16x2_bits(a[0], a[1]), bf16x2_bits(a[2], a[3]), bf16x2_bits(e[0], e[1]), bf16x2_bits(e[2], e[3])));
+                    }
                 }
 #pragma unroll
-                for (int w = 0; w < 2; ++w) {
-                    const f32x4 a = sc[g][2 * w], e = sc[g][2 * w + 1];
-                    p[g][w] = frag(make_uint4(bf16x2_bits(a[0], a[1]), bf16x2_bits(a[2], a[3]), bf16x2_bits(e[0], e[1]), bf16x2_bits(e[2], e[3])));
+                for (int d = 0; d < NT; ++d) {
+                    const bf16x8 lo = frag(ints_bf16(make_uint2(vr[d].x, vr[d].y))), hi = frag(ints_bf16(make_uint2(vr[d].z, vr[d].w)));
+#pragma unroll
+                    for (int g = 0; g < NQ; ++g) {
+                        o[g][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, p[g][0], o[g][d], 0, 0, 0);
+                        o[g][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, p[g][1], o[g][d], 0, 0, 0);
+                    }
                 }
+                if (left) load_v(next);
+                y = z;
             }
-#pragma unroll
-            for (int d = 0; d < NT; ++d) {
-                const bf16x8 lo = frag(ints_bf16(make_uint2(vr[d].x, vr[d].y))), hi = frag(ints_bf16(make_uint2(vr[d].z, vr[d].w)));
-#pragma unroll
-                for (int g = 0; g < NQ; ++g) {
-                    o[g][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, p[g][0], o[g][d], 0, 0, 0);
-                    o[g][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, p[g][1], o[g][d], 0, 0, 0);
-                }
-            }
-            if (left) load_v(next);
-            y = z;
         }
-    }
 
-    // register r of o[g][d]: element 16 d + 4 quad + r of query 16 g + col
+        // register r of o[g][d]: element 16 d + 4 quad + r of query 16 g + col
 #pragma unroll
-    for (int g = 0; g < NQ; ++g) {
-        if (g * kFew >= queries) break;
-        l[g] += __shfl_xor(l[g], 16);
-        l[g] += __shfl_xor(l[g], 32);
-        const bool sees = last[g] >= 0;  // else padding, or a row that sees nothing: what the registers hold is no result
-        if (g > 0) __syncthreads();
-        if (quad == 0) jml[wave][col] = make_float2(m[g], sees ? l[g] : 0.0f);
+        for (int g = 0; g < NQ; ++g) {
+            if (g * kFew >= queries) break;
+            l[g] += __shfl_xor(l[g], 16);
+            l[g] += __shfl_xor(l[g], 32);
+            const bool sees = last[g] >= 0;  // else padding, or a row that sees nothing: what the registers hold is no result
+            if (g > 0 || again) __syncthreads();
+            if (quad == 0) jml[wave][col] = make_float2(m[g], sees ? l[g] : 0.0f);
 #pragma unroll
-        for (int d = 0; d < NT; ++d)
-            *reinterpret_cast<float4*>(&jo[wave][col][16 * d + 4 * quad]) =
-                sees ? make_float4(o[g][d][0], o[g][d][1], o[g][d][2], o[g][d][3]) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        __syncthreads();
-        const int here = queries - g * kFew < kFew ? queries - g * kFew : kFew;
-        for (int e = t; e < here * (D / 4); e += 64 * kFewWaves) {
-            const int qn = e / (D / 4), d = e % (D / 4) * 4, query = g * kFew + qn;
-            float top = kLowest;
+            for (int d = 0; d < NT; ++d)
+                *reinterpret_cast<float4*>(&jo[wave][col][16 * d + 4 * quad]) =
+                    sees ? make_float4(o[g][d][0], o[g][d][1], o[g][d][2], o[g][d][3]) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            __syncthreads();
+            const int here = queries - g * kFew < kFew ? queries - g * kFew : kFew;
+            for (int e = t; e < here * (D / 4); e += 64 * kFewWaves) {
+                const int qn = e / (D / 4), d = e % (D / 4) * 4, query = g * kFew + qn;
+                float top = kLowest;
 #pragma unroll
-            for (int w = 0; w < kFewWaves; ++w) top = fmaxf(top, jml[w][qn].x);
-            float sum = 0.0f, a[4] = {};
+                for (int w = 0; w < kFewWaves; ++w) top = fmaxf(top, jml[w][qn].x);
+                float sum = 0.0f, a[4] = {};
 #pragma unroll
-            for (int w = 0; w < kFewWaves; ++w) {
-                const float2 ml = jml[w][qn];
-                const float fix = exp2_hw(ml.x - top);
-                sum += ml.y * fix;
-                const float4 x = *reinterpret_cast<const float4*>(&jo[w][qn][d]);
-                a[0] += x.x * fix, a[1] += x.y * fix, a[2] += x.z * fix, a[3] += x.w * fix;
-            }
-            if (part.splits > 1) {
-                const int64_t at = part.at(nh, split, query);
-                if (d == 0) part.ml[at] = make_float2(top, sum);
-                *reinterpret_cast<float4*>(part.o + at * D + d) = make_float4(a[0], a[1], a[2], a[3]);
-            } else {
-                const int64_t to_row = (static_cast<int64_t>(i) * q.rows + query / group) * q.heads + h * group + query % group;
-                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                *reinterpret_cast<uint2*>(out + to_row * D + d) = make_uint2(bf16x2_bits(a[0] * inv, a[1] * inv), bf16x2_bits(a[2] * inv, a[3] * inv));
+                for (int w = 0; w < kFewWaves; ++w) {
+                    const float2 ml = jml[w][qn];
+                    const float fix = exp2_hw(ml.x - top);
+                    sum += ml.y * fix;
+                    const float4 x = *reinterpret_cast<const float4*>(&jo[w][qn][d]);
+                    a[0] += x.x * fix, a[1] += x.y * fix, a[2] += x.z * fix, a[3] += x.w * fix;
+                }
+                if (shares.shares) {
+                    const int64_t to_part = part.at(h, w + i, query);
+                    if (d == 0) part.ml[to_part] = make_float2(top, sum);
+                    *reinterpret_cast<float4*>(part.o + to_part * D + d) = make_float4(a[0], a[1], a[2], a[3]);
+                } else {
+                    const int64_t to_row = (static_cast<int64_t>(i) * q.rows + query / group) * q.heads + h * group + query % group;
+                    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                    *reinterpret_cast<uint2*>(out + to_row * D + d) = make_uint2(bf16x2_bits(a[0] * inv, a[1] * inv), bf16x2_bits(a[2] * inv, a[3] * inv));
+                }
             }
         }
+        if (at >= share_end) return;
+        // the next sequence that has blocks: there is one, as the share goes on
+        do ++i;
+        while (uniform(ends[i + 1]) == at);
     }
 }
 
 // ------------------------------------------------------------------ joining splits
 
-constexpr int kMaxSplits = 64;  // a lane of the join's wave each
+constexpr int kMaxSplits = 64;  // of a tile, a lane of the join's wave each
 
 // D / 4 lanes take a row of an item. FEW: at most kFewSplits splits, whose sums a lane adds up; else a wave a row, 256 / D
 // splits at once.  (Two splits of 30720 rows of 64 elements: a wave a row 17.8 us, so 5.9.)
@@ -791,6 +854,64 @@ __global__ __launch_bounds__(256) void kv_join_kernel(Partial part, Queries q, I
     *reinterpret_cast<uint2*>(out + query * D + d) = make_uint2(bf16x2_bits(a[0] * inv, a[1] * inv), bf16x2_bits(a[2] * inv, a[3] * inv));
 }
 
+// A row of kv_few_kernel's pieces: a workgroup, D / 4 lanes for every 1024 / D-th piece, as one sequence may have most of
+// the launch's.
+template <int D>
+__global__ __launch_bounds__(256) void kv_join_pieces_kernel(Partial part, Shares shares, Queries q, int kv, uint16_t* __restrict__ out) {
+    constexpr int L = D / 4, G = 256 / L, kAhead = 4;
+    __shared__ float4 sums[G][L];
+    __shared__ float2 parts[G];
+    const int t = threadIdx.x, d = t % L * 4, g = t / L;
+    // rows in the order of sequences, kv heads, queries of a group
+    const int query = blockIdx.x % part.rows, nh = blockIdx.x / part.rows, h = nh % kv, i = nh / kv;
+    const int2 span = shares.spans[i];
+    float top = kLowest, sum = 0.0f, a[4] = {};
+    for (int w0 = span.x + g; w0 <= span.y; w0 += G * kAhead) {
+        float2 ml[kAhead];
+        float4 v[kAhead];
+        float best = top;
+#pragma unroll
+        for (int x = 0; x < kAhead; ++x) {
+            const int w = w0 + x * G;
+            const int64_t at = part.at(h, w + i, query);
+            ml[x] = make_float2(kLowest, 0.0f);
+            v[x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (w <= span.y) ml[x] = part.ml[at], v[x] = *reinterpret_cast<const float4*>(part.o + at * D + d);
+        }
+#pragma unroll
+        for (int x = 0; x < kAhead; ++x) best = fmaxf(best, ml[x].x);
+        const float fix = exp2_hw(top - best);
+        top = best;
+        sum *= fix;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) a[j] *= fix;
+#pragma unroll
+        for (int x = 0; x < kAhead; ++x) {
+            const float f = exp2_hw(ml[x].x - top);
+            sum += ml[x].y * f;
+            a[0] += v[x].x * f, a[1] += v[x].y * f, a[2] += v[x].z * f, a[3] += v[x].w * f;
+        }
+    }
+    sums[g][t % L] = make_float4(a[0], a[1], a[2], a[3]);
+    if (t % L == 0) parts[g] = make_float2(top, sum);
+    __syncthreads();
+    if (g > 0) return;
+#pragma unroll
+    for (int x = 0; x < G; ++x) top = fmaxf(top, parts[x].x);
+    sum = a[0] = a[1] = a[2] = a[3] = 0.0f;
+#pragma unroll
+    for (int x = 0; x < G; ++x) {
+        const float4 v = sums[x][t];
+        const float f = exp2_hw(parts[x].x - top);
+        sum += parts[x].y * f;
+        a[0] += v.x * f, a[1] += v.y * f, a[2] += v.z * f, a[3] += v.w * f;
+    }
+    const int group = q.heads / kv;
+    const int64_t to_row = (static_cast<int64_t>(i) * q.rows + query / group) * q.heads + h * group + query % group;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    *reinterpret_cast<uint2*>(out + to_row * D + d) = make_uint2(bf16x2_bits(a[0] * inv, a[1] * inv), bf16x2_bits(a[2] * inv, a[3] * inv));
+}
+
 // ------------------------------------------------------------------ what a call runs
 
 // Queries of a kv head's group that kv_few_kernel holds in registers: 64 of 64 elements, 32 of 128 (64 spilled, and took
@@ -803,10 +924,12 @@ struct Plan {
     bool few, flat;
     int waves;          // of a tile's workgroup
     int pack;           // query heads of an item
-    int splits, per;    // of a split item; blocks of a split (few)
+    int splits;         // of a split item
+    int shares;         // of a kv head's blocks (few), 0: none
     int64_t rows;       // queries of an item
     int64_t heads, tiles, items, whole;  // items of one workgroup each come first
-    int64_t part_rows() const { return splits > 1 ? (items - whole) * splits * rows : 0; }
+    int64_t spans;          // rows' worth of the shares' spans
+    int64_t part_rows() const { return shares ? heads * (shares + items / heads) * rows + spans : splits > 1 ? (items - whole) * splits * rows : 0; }
 };
 
 // Sizes checked by the caller.
@@ -821,13 +944,15 @@ Plan plan_of(int64_t n, int64_t rows, int64_t heads, int64_t kv, int64_t dim, in
         p.heads = kv;
         p.tiles = 1;
         p.items = n * kv;
-        // two workgroups a CU: 145 us for 16 uneven sequences against 151 with four, a single query's 51 against 54
-        int64_t splits = 2 * cus / p.items;
-        if (splits > longest / (2 * kFewWaves)) splits = longest / (2 * kFewWaves);
-        if (splits > kMaxSplits) splits = kMaxSplits;
-        if (splits < 1) splits = 1;
-        p.per = static_cast<int>((longest + splits - 1) / splits);
-        p.splits = p.per > 0 ? static_cast<int>((longest + p.per - 1) / p.per) : 1;
+        p.splits = 1;
+        // As many workgroups as the CUs hold at once, by the registers that the queries take, of at least two blocks a wave,
+        // where they are half as many again as the sequences: a piece and its place in the join cost 3 us (448 workgroups of
+        // 17 rows unsplit 88 us, 512 shares 108; but 8 x 20 heads of 256 unsplit 68 us, 240 shares 55).
+        int64_t shares = ((p.rows + kFew - 1) / kFew * dim >= 256 ? 1 : 2) * cus / kv;
+        if (n <= kFewThreads && n * longest < (int64_t{1} << 30)) {
+            if (shares > n * longest / (2 * kFewWaves)) shares = n * longest / (2 * kFewWaves);
+            if (shares > n && 2 * shares >= 3 * n) p.shares = static_cast<int>(shares), p.spans = (8 * n + 4 * dim + 7) / (4 * dim + 8);
+        }
         return p;
     }
     // Rows that leave a tile part empty share it with the other heads of their group (a list is a kv head's).
@@ -917,25 +1042,31 @@ extern "C" int h3mi_kv_attention_bf16(const uint16_t* q, int64_t rows, int64_t h
     if (!aligned(workspace, 16)) return fail(H3MI_EALIGN, "kv_attention: workspace must be 16-byte aligned");
     const Queries qs = {q, ld_q, bs_q, static_cast<int>(rows), static_cast<int>(heads)};
     const Lists list = {blocks, static_cast<int>(top), static_cast<int>((rows + kKvTile - 1) / kKvTile)};
-    Partial part = {static_cast<float*>(workspace), nullptr, p.splits, static_cast<int>(p.rows)};
+    Partial part = {static_cast<float*>(workspace), nullptr, p.shares ? p.shares + static_cast<int>(n) : p.splits, static_cast<int>(p.rows)};
     const Items items = {static_cast<int>(p.tiles), static_cast<int>(p.heads), p.pack, static_cast<int>(p.rows),
                          p.pack == 1 ? 0u : static_cast<uint32_t>(((uint64_t{1} << 32) + p.pack - 1) / p.pack), static_cast<int>(p.items),
-                         static_cast<int>(p.whole), static_cast<int>(p.whole / 8), static_cast<int>((rest + 7) / 8), p.flat, causal != 0 && !p.few};
-    if (need > 0) part.ml = reinterpret_cast<float2*>(part.o + part_rows * dim);
+                         static_cast<int>(p.whole), static_cast<int>(p.whole / 8), static_cast<int>((rest + 7) / 8), p.flat, causal != 0};
+    if (need > 0) part.ml = reinterpret_cast<float2*>(part.o + (part_rows - p.spans) * dim);
     const KvCache c = kv_cache(*cache);
     const KvSeqs s = kv_seqs(*seqs);
     const hipStream_t st = as_stream(stream);
     int rc;
     if (p.few) {
         int64_t groups;
-        if (!launchable(p.items, p.splits, 1, 64 * kFewWaves, &groups)) return fail(H3MI_EINVAL, "kv_attention: too many rows for one call");
+        const Shares shares = {p.shares, p.shares ? reinterpret_cast<int2*>(part.ml + part_rows - p.spans) : nullptr};
+        if (!launchable(p.shares ? p.shares * p.heads : p.items, 1, 1, kFewThreads, &groups)) return fail(H3MI_EINVAL, "kv_attention: too many rows for one call");
         const int sets = static_cast<int>((p.rows + kFew - 1) / kFew);
         const auto fn = dim == 64    ? (sets == 1 ? kv_few_kernel<64, 1> : sets == 2 ? kv_few_kernel<64, 2> : kv_few_kernel<64, 4>)
                         : dim == 128 ? (sets == 1 ? kv_few_kernel<128, 1> : kv_few_kernel<128, 2>)
                                      : kv_few_kernel<256, 1>;
-        hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(groups)), dim3(64 * kFewWaves), 0, st, qs, c, s, scale, causal, list, out, part,
-                           p.per);
+        hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(groups)), dim3(kFewThreads), 0, st, qs, c, s, scale, causal, list, out, part,
+                           shares);
         rc = check_launch("kv_attention");
+        if (rc || !p.shares) return rc;
+        if (!launchable(p.items, p.rows, 1, 256, &groups)) return fail(H3MI_EINVAL, "kv_attention: too many rows for one call");
+        const auto join = dim == 64 ? kv_join_pieces_kernel<64> : dim == 128 ? kv_join_pieces_kernel<128> : kv_join_pieces_kernel<256>;
+        hipLaunchKernelGGL(join, dim3(static_cast<unsigned>(groups)), dim3(256), 0, st, part, shares, qs, c.heads, out);
+        return check_launch("kv_attention");
     } else if (dim == 64) {
         rc = launch_tiles<64, 4>(items, qs, c, s, scale, causal, list, out, part, st);
     } else if (dim == 128) {

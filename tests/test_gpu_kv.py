@@ -663,3 +663,64 @@ def test_lists_of_no_entry_are_refused():
         h.kv_attention(q, c, t, lens, blocks=torch.empty(1, 1, 2, 0, dtype=torch.int32, device=DEV))
     assert h.kv_attention(q[:, :0], c, t, lens, blocks=torch.empty(1, 0, 2, 3, dtype=torch.int32, device=DEV)).shape == (1, 0, 4, 64)
     assert h.kv_attention(q, c, t, lens, blocks=torch.full((1, 1, 2, 1), -1, dtype=torch.int32, device=DEV)).abs().max() == 0
+
+
+# ------------------------------------------------------------------ few queries of uneven sequences
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(3, 3, 64), (10, 2, 128), (2, 2, 256), (24, 1, 128), (40, 1, 64)])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("lens,counts", [
+    ([0, 700, 0, 64, 3000, 0], None), ([3000, 1], None), ([1, 3000], None), ([0, 0, 0], None), ([5, 0, 64, 65], [1, 0, 1, 1]),
+    ([3000, 2000, 130, 0], [1, 0, 1, 1]), ([64 * 9] * 5, None), ([1 << 30, 900, -4], None)])
+def test_attention_few_uneven(heads, kv, dim, causal, lens, counts):
+    rng = np.random.default_rng(sum(map(abs, lens)) % 1000 + dim)
+    ref, tables, q = _case(rng, heads, kv, dim, len(lens), 1, 47, seed=7)
+    _check(ref, q, tables, lens, counts, causal)
+
+
+@pytest.mark.parametrize("n", [255, 256, 257, 300])
+def test_attention_few_many_sequences(n):
+    """As many sequences as a workgroup can lay end to end, and more."""
+    rng = np.random.default_rng(n)
+    lens = rng.integers(0, 20 * 64 + 1, n)
+    lens[rng.random(n) < 0.3] = 0
+    ref, tables, q = _case(rng, 2, 1, 64, n, 1, 20, seed=3)
+    _check(ref, q, tables, lens, None, True)
+
+
+@pytest.mark.parametrize("rows,heads,kv,dim", [(1, 4, 2, 64), (3, 10, 2, 128), (2, 2, 2, 256)])
+def test_sparse_attention_few_uneven(rows, heads, kv, dim):
+    """Lists over uneven sequences, some without a token, some shorter than the list."""
+    rng = np.random.default_rng(rows + dim)
+    n, blocks, top = 7, 60, 24
+    lens = [3840, 0, 100, 2000, 64 * 24, 0, 1]
+    ref, tables, q = _case(rng, heads, kv, dim, n, rows, blocks, seed=rows)
+    lists = np.full((n, 1, kv, top), -1, np.int32)
+    for i in range(n):
+        for h in range(kv):
+            lists[i, 0, h, :] = rng.permutation(blocks)[:top]
+    _check(ref, q, tables, lens, None, True, blocks=lists)
+
+
+@pytest.mark.parametrize("rows,kv,dim", [(1, 2, 64), (2, 8, 128), (1, 3, 256)])
+def test_few_uneven_captured_and_replayed(rows, kv, dim):
+    """A captured call follows the lengths that it finds, as an eager call does."""
+    h = _h()
+    rng = np.random.default_rng(rows)
+    n, blocks = 6, 80
+    ref, tables, q = _case(rng, 2 * kv, kv, dim, n, rows, blocks, seed=9)
+    c, t, x, lens = ref.to(), _i32(tables), _bf(q), _i32([64 * blocks] * n)
+    call = lambda: h.kv_attention(x, c, t, lens, causal=True)  # noqa: E731
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for r in range(6):
+        lens.copy_(_i32(rng.integers(0, 64 * blocks + 1, n) * (rng.random(n) < 0.8)))
+        graph.replay()
+        want = call()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), r
+        _check(ref, q, tables, lens.cpu().numpy(), None, True)
