@@ -534,6 +534,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void kv_few_kernel(Queries q, KvCac
             return r < count ? x : -1;
         }
     };
+    __shared__ Seen seen[kFewThreads];
     auto seen_of = [&](int i) {
         const int count = s.count(i, q.rows);
         return Seen{s.len(i), s.end(i) - count, count};
@@ -544,25 +545,25 @@ __global__ __launch_bounds__(64 * kFewWaves) void kv_few_kernel(Queries q, KvCac
     };
     int i = w, at = 0, share_end = 0;
     if (shares.shares) {
-        const int mine = t < s.n ? blocks_of(seen_of(t)) : 0;
-        int sum = mine > 0 && list.p ? list.top : mine;
+        Seen mine = {};
+        if (t < s.n) mine = seen_of(t);
+        seen[t] = mine;
+        int sum = blocks_of(mine);
+        if (sum > 0 && list.p) sum = list.top;
         const int own = sum;
-#pragma unroll
-        for (int x = 1; x < 64; x <<= 1) {
+        for (int x = 1; x < 64 && x < s.n; x <<= 1) {
             const int o = __shfl_up(sum, x);
             if (lane >= x) sum += o;
         }
-        if (lane == 63) wave_sum[wave] = sum;
-        __syncthreads();
-        int all = 0;
-#pragma unroll
-        for (int x = 0; x < kFewWaves; ++x) {
-            if (x < wave) sum += wave_sum[x];
-            all += wave_sum[x];
+        if (s.n > 64) {
+            if (lane == 63) wave_sum[wave] = sum;
+            __syncthreads();
+            for (int x = 0; x < wave; ++x) sum += wave_sum[x];
         }
-        ends[t + 1] = sum;
+        if (t < s.n) ends[t + 1] = sum;
         if (t == 0) ends[0] = 0;
         __syncthreads();
+        const int all = uniform(ends[s.n]);
         const int per = all == 0 ? 1 : static_cast<int>((static_cast<uint32_t>(all) + shares.shares - 1) / shares.shares);
         if (blockIdx.x == 0 && t < s.n)
             shares.spans[t] = own == 0 ? make_int2(0, -1) : make_int2((sum - own) / per, (sum - 1) / per);
@@ -580,7 +581,13 @@ __global__ __launch_bounds__(64 * kFewWaves) void kv_few_kernel(Queries q, KvCac
     }
 
     for (bool again = false;; again = true) {
-        const Seen seq = seen_of(i);
+        Seen seq;
+        if (shares.shares) {
+            const Seen x = seen[i];
+            seq = {uniform(x.len), uniform(x.start), uniform(x.count)};
+        } else {
+            seq = seen_of(i);
+        }
         const int blocks = blocks_of(seq);
         // below this every query that is one sees a whole block
         const int full = seq.count > 0 ? seq.last_of(0, causal) + 1 : 0;
