@@ -406,16 +406,17 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : D == 64 ? 3 : 2) void kv_til
                 }
                 l = __builtin_fmaf(sum, f.iv, l);
             } else {
-                // a scale that is no ordinary number: what a row does not see must not reach it
+                // a scale that is no ordinary number: what a row does not see must not reach it, and a NaN or an infinity
+                // must where a probability underflows
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
                     float x[8];
 #pragma unroll
                     for (int r = 0; r < 8; ++r) {
-                        x[r] = exp2_hw(__builtin_fmaf(sc[w / 2][w % 2 * 8 + r], f.c, off));
-                        if (base + 16 * w + 8 * half + r > last) x[r] = 0.0f;
+                        const uint32_t sees = (base + 16 * w + 8 * half + r - 1 - last) >> 31;  // all bits, or none
+                        x[r] = __uint_as_float(__float_as_uint(exp2_hw(__builtin_fmaf(sc[w / 2][w % 2 * 8 + r], f.c, off))) & sees);
                         l += x[r];
-                        x[r] = x[r] == 0.0f ? 0.0f : x[r] * f.vs;
+                        x[r] = __uint_as_float(__float_as_uint(x[r] * f.vs) & sees);
                     }
                     p[w] = pack(x);
                 }
@@ -710,14 +711,15 @@ __global__ __launch_bounds__(64 * kFewWaves) void kv_few_kernel(Queries q, KvCac
                     if (fiv != 0.0f) {
                         l[g] = __builtin_fmaf(sum, fiv, l[g]);
                     } else {
-                        // a scale that is no ordinary number: what a row does not see must not reach it
+                        // a scale that is no ordinary number: what a row does not see must not reach it, and a NaN or an
+                        // infinity must where a probability underflows
 #pragma unroll
                         for (int u = 0; u < 4; ++u)
 #pragma unroll
                             for (int r = 0; r < 4; ++r) {
-                                const float e = base + 16 * quad + 4 * u + r > last[g] ? 0.0f : sc[g][u][r];
-                                l[g] += e;
-                                sc[g][u][r] = e == 0.0f ? 0.0f : e * fvs;
+                                const bool sees = base + 16 * quad + 4 * u + r <= last[g];
+                                l[g] += sees ? sc[g][u][r] : 0.0f;
+                                sc[g][u][r] = sees ? sc[g][u][r] * fvs : 0.0f;
                             }
                     }
 #pragma unroll

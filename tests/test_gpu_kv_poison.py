@@ -1,0 +1,75 @@
+"""Blocks that a NaN or an infinity was written to: every row that sees one is NaN, however little the block weighs in it, and
+no other row is, in each of the kernels and of the joins of their parts."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+# rows, blocks: what runs, for 2 heads of 128 elements of one sequence (parts: partial rows that its workspace holds, 0 for
+# none; the pieces' join takes two rows' worth of spans at most)
+PLANS = {
+    "few": (1, 6), "few, 32 rows": (32, 6), "few, pieces joined": (1, 64), "few, 20 rows, pieces joined": (20, 64),
+    "tiles": (300, 6), "tiles, 6 splits": (300, 24),
+}
+SPLITS = {"tiles, 6 splits": 6}
+
+
+def _parts(n, rows, heads, kv, dim, blocks, top=0):
+    from h3mi import _lib
+    need = _lib.lib.h3mi_kv_attention_workspace(n, rows, heads, kv, dim, blocks, top)
+    assert need % (dim * 4 + 8) == 0
+    return need // (dim * 4 + 8)
+
+
+def _check_plan(name):
+    rows, blocks = PLANS[name]
+    parts = _parts(1, rows, 2, 2, 128, blocks)
+    if name in SPLITS:
+        assert parts == 2 * -(-rows // 128) * SPLITS[name] * 128
+    else:
+        assert (parts > 0) == ("joined" in name)
+
+
+def _levels(blocks, hot, bad, low):
+    """Which way each block's keys point: the hot one along the query, the bad one against it, the others neither way, or
+    (low) against it too."""
+    to = torch.full((blocks,), -1.0 if low else 0.0)
+    to[hot], to[bad] = 1.0, -1.0
+    return to
+
+
+@pytest.mark.parametrize("what", ["k", "v"])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("low", [False, True])
+@pytest.mark.parametrize("plan", list(PLANS))
+def test_a_poisoned_block_reaches_every_row_that_sees_it(plan, low, value, what):
+    """Scores 1448 apart: the block's probabilities are 0 in 32 bits, within its split and against the others."""
+    import h3mi
+    _check_plan(plan)
+    rows, blocks = PLANS[plan]
+    bad, hot, end = blocks - 2, 1, blocks * 64
+    g = torch.Generator().manual_seed(rows + blocks)
+    k = torch.randn(1, end, 2, 128, generator=g) * 0.01 + 8 * _levels(blocks, hot, bad, low).repeat_interleave(64)[None, :, None, None]
+    v = torch.randn(1, end, 2, 128, generator=g)
+    (k if what == "k" else v)[0, bad * 64 + 5, 1, 7] = value
+    q = torch.randn(1, rows, 2, 128, generator=g) * 0.01 + 8
+    k, v, q = (t.to(torch.bfloat16).to(DEV) for t in (k, v, q))
+    tables = torch.randperm(blocks, generator=g).to(torch.int32)[None].to(DEV)
+    lens = torch.tensor([end], dtype=torch.int32, device=DEV)
+    cache = h3mi.kv_write_(h3mi.kv_cache(blocks, 2, 128), k, v, tables, lens)
+    bad_row = torch.zeros(1, rows, 2, 128, dtype=torch.bool)
+    for causal in (False, True):
+        bad_row[:, :, 1] = True
+        if causal:  # rows before the bad block, of which 300 rows have some
+            bad_row[:, end - rows + torch.arange(rows) < bad * 64, 1] = False
+        out = h3mi.kv_attention(q, cache, tables, lens, causal=causal).float().cpu()
+        assert torch.equal(out.isnan(), bad_row), causal
+    # a list without it
+    take = torch.tensor([b for b in range(blocks) if b != bad], dtype=torch.int32, device=DEV)
+    lists = take.repeat(1, -(-rows // 128), 2, 1)
+    assert h3mi.kv_attention(q, cache, tables, lens, blocks=lists).isfinite().all()
+    # and one with it
+    lists[..., blocks - 2] = bad
+    got = h3mi.kv_attention(q, cache, tables, lens, blocks=lists).isnan().cpu()
+    assert got[:, :, 1].all() and not got[:, :, 0].any()
