@@ -836,6 +836,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(Partial part, Queries q, I
 #pragma unroll
         for (int y2 = 32; y2; y2 >>= 1) top = fmaxf(top, __shfl_xor(top, y2));
         const float fix = ml.y == 0.0f ? 0.0f : exp2_hw(ml.x - top);
+        const uint64_t held = __ballot(ml.y != 0.0f);  // the splits that wrote sums
         sum = ml.y * fix;
 #pragma unroll
         for (int y2 = 32; y2; y2 >>= 1) sum += __shfl_xor(sum, y2);
@@ -846,9 +847,9 @@ __global__ __launch_bounds__(256) void kv_join_kernel(Partial part, Queries q, I
             for (int z = 0; z < 4; ++z) {
                 const int sp = s0 + z * SG + sg;
                 f[z] = __shfl(fix, sp & 63);
-                if (sp >= part.splits) f[z] = 0.0f;
                 v[z] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (f[z] != 0.0f) v[z] = *reinterpret_cast<const float4*>(part.o + part.at(item, sp, r) * D + d);
+                // (what a factor of 0 makes of a NaN or an infinity is part of the sum)
+                if (held >> (sp & 63) & 1) v[z] = *reinterpret_cast<const float4*>(part.o + part.at(item, sp, r) * D + d);
             }
 #pragma unroll
             for (int z = 0; z < 4; ++z) a[0] += v[z].x * f[z], a[1] += v[z].y * f[z], a[2] += v[z].z * f[z], a[3] += v[z].w * f[z];

@@ -10,9 +10,9 @@ DEV = "cuda"
 # none; the pieces' join takes two rows' worth of spans at most)
 PLANS = {
     "few": (1, 6), "few, 32 rows": (32, 6), "few, pieces joined": (1, 64), "few, 20 rows, pieces joined": (20, 64),
-    "tiles": (300, 6), "tiles, 6 splits": (300, 24),
+    "tiles": (300, 6), "tiles, 6 splits": (300, 24), "tiles, 16 splits": (300, 64), "tiles, 64 splits": (200, 300),
 }
-SPLITS = {"tiles, 6 splits": 6}
+SPLITS = {"tiles, 6 splits": 6, "tiles, 16 splits": 16, "tiles, 64 splits": 64}
 
 
 def _parts(n, rows, heads, kv, dim, blocks, top=0):
