@@ -262,7 +262,8 @@ typedef struct h3mi_kv_seqs {
  * A value's error is at most one step s' (half of one if its scale never grew).
  * A block with a NaN or an infinity reads back as NaN.  Tokens of a written block
  * behind the sequence's end become 0; other blocks are left as they were.  k_sum is
- * renewed.  The pages that a call writes have to be distinct.  dim 64, 128 or 256. */
+ * renewed.  The pages that a call writes have to be distinct, and none of the cache's
+ * tensors may overlap another, tables, lens or counts.  dim 64, 128 or 256. */
 int h3mi_kv_write_i8(const uint16_t* k, const uint16_t* v, int64_t rows, int64_t ld_k, int64_t bs_k,
                      int64_t ld_v, int64_t bs_v, const h3mi_kv_cache* cache, const h3mi_kv_seqs* seqs,
                      void* stream);

@@ -17,6 +17,10 @@ int kv_check_rows(const char* what, const char* name, const uint16_t* p, int64_t
 size_t kv_span(int64_t n, int64_t rows, int64_t heads, int64_t dim, int64_t ld, int64_t bs);
 // Whether `bytes` at p overlap the cache's keys, values, scales or sums.
 bool kv_overlaps(const void* p, size_t bytes, const h3mi_kv_cache& c);
+// Whether two of the cache's keys, values, scales and sums overlap.
+bool kv_self_overlaps(const h3mi_kv_cache& c);
+// Whether `bytes` at p overlap the sequences' tables, lens or counts.
+bool kv_seqs_overlap(const void* p, size_t bytes, const h3mi_kv_seqs& s);
 // groups = a b c workgroups, if HIP takes a launch of so many with `threads` threads each: it refuses 2^32 threads and more.
 inline bool launchable(int64_t a, int64_t b, int64_t c, int64_t threads, int64_t* groups) {
     int64_t g, all;

@@ -52,10 +52,41 @@ size_t kv_span(int64_t n, int64_t rows, int64_t heads, int64_t dim, int64_t ld, 
     return 2 * (static_cast<size_t>(n - 1) * bs + static_cast<size_t>(rows - 1) * ld + static_cast<size_t>(heads) * dim);
 }
 
+namespace {
+
+struct Span {
+    const void* p;
+    size_t bytes;
+};
+
+// The cache's keys, values, scales and sums.
+struct Spans {
+    Span s[5];
+    explicit Spans(const h3mi_kv_cache& c) {
+        const size_t tiles = static_cast<size_t>(c.pages) * c.heads, kv = tiles * c.dim * kKvBlock;
+        s[0] = {c.k, kv}, s[1] = {c.v, kv}, s[2] = {c.k_scale, 4 * tiles}, s[3] = {c.v_scale, 4 * tiles}, s[4] = {c.k_sum, 2 * tiles * c.dim};
+    }
+};
+
+}  // namespace
+
 bool kv_overlaps(const void* out, size_t bytes, const h3mi_kv_cache& c) {
-    const size_t tiles = static_cast<size_t>(c.pages) * c.heads, kv = tiles * c.dim * kKvBlock;
-    return overlap(out, bytes, c.k, kv) || overlap(out, bytes, c.v, kv) || overlap(out, bytes, c.k_scale, 4 * tiles) ||
-           overlap(out, bytes, c.v_scale, 4 * tiles) || overlap(out, bytes, c.k_sum, 2 * tiles * c.dim);
+    for (const Span& x : Spans(c).s)
+        if (overlap(out, bytes, x.p, x.bytes)) return true;
+    return false;
+}
+
+bool kv_self_overlaps(const h3mi_kv_cache& c) {
+    const Spans all(c);
+    for (int x = 1; x < 5; ++x)
+        for (int y = 0; y < x; ++y)
+            if (overlap(all.s[x].p, all.s[x].bytes, all.s[y].p, all.s[y].bytes)) return true;
+    return false;
+}
+
+bool kv_seqs_overlap(const void* p, size_t bytes, const h3mi_kv_seqs& s) {
+    const size_t each = 4 * static_cast<size_t>(s.n);
+    return (s.blocks && overlap(p, bytes, s.tables, each * s.blocks)) || overlap(p, bytes, s.lens, each) || (s.counts && overlap(p, bytes, s.counts, each));
 }
 
 namespace {
@@ -352,6 +383,9 @@ extern "C" int h3mi_kv_write_i8(const uint16_t* k, const uint16_t* v, int64_t ro
         const size_t bytes = kv_span(seqs->n, rows, cache->heads, cache->dim, x ? ld_v : ld_k, x ? bs_v : bs_k);
         if (kv_overlaps(x ? v : k, bytes, *cache)) return fail(H3MI_EALIAS, "kv_write: the rows overlap the cache");
     }
+    if (kv_self_overlaps(*cache)) return fail(H3MI_EALIAS, "kv_write: the cache's tensors overlap");
+    for (const Span& x : Spans(*cache).s)
+        if (kv_seqs_overlap(x.p, x.bytes, *seqs)) return fail(H3MI_EALIAS, "kv_write: tables, lens or counts overlap the cache");
     const bool stream_in = seqs->n * rows * cache->heads * D * 4 > kMemoryCache;
     const auto fn = stream_in ? (D == 64 ? kv_write_kernel<64, true> : D == 128 ? kv_write_kernel<128, true> : kv_write_kernel<256, true>)
                               : (D == 64 ? kv_write_kernel<64, false> : D == 128 ? kv_write_kernel<128, false> : kv_write_kernel<256, false>);

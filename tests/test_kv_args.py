@@ -155,3 +155,26 @@ def test_cpu_tensors_are_refused():
 def test_written_rows_over_the_scales_and_sums(name, at):
     rc, m = _call("write", dict(k=1 << 23, v=1 << 24), **{name: at})
     assert rc == 3 and "overlap" in m, (rc, m)
+
+
+# a cache, sequences and rows that do not overlap
+APART = dict(k=1 << 23, v=1 << 24, k_scale=1 << 25, v_scale=1 << 26, k_sum=1 << 27)
+APART_SEQS = dict(tables=1 << 28, lens=1 << 29, counts=1 << 30)
+
+
+@pytest.mark.parametrize("cache", [
+    dict(v_scale=1 << 25), dict(v_scale=(1 << 25) + 76), dict(k_scale=(1 << 26) + 4), dict(k_sum=1 << 25), dict(k_sum=(1 << 23) + 4096),
+    dict(k_scale=(1 << 24) + 163836), dict(v_scale=(1 << 27) + 5116),
+])
+def test_written_cache_over_itself(cache):
+    """Two workgroups, or two of a thread's stores, would write the same bytes."""
+    rc, m = _call("write", {**APART, **cache}, APART_SEQS)
+    assert rc == 3 and "the cache's tensors overlap" in m, (rc, m)
+
+
+@pytest.mark.parametrize("seqs", [
+    dict(tables=1 << 23), dict(tables=(1 << 25) - 36), dict(lens=1 << 26), dict(lens=(1 << 27) + 5116), dict(counts=(1 << 24) + 8),
+])
+def test_written_cache_over_the_sequences(seqs):
+    rc, m = _call("write", APART, {**APART_SEQS, **seqs})
+    assert rc == 3 and "tables, lens or counts overlap the cache" in m, (rc, m)
