@@ -1047,6 +1047,9 @@ extern "C" int h3mi_kv_attention_bf16(const uint16_t* q, int64_t rows, int64_t h
     const size_t bytes = static_cast<size_t>(n) * rows * heads * dim * 2;
     if (overlap(out, bytes, q, kv_span(n, rows, heads, dim, ld_q, bs_q)) || kv_overlaps(out, bytes, *cache))
         return fail(H3MI_EALIAS, "kv_attention: out overlaps q or the cache");
+    const size_t list_bytes = static_cast<size_t>(n) * ((rows + kKvTile - 1) / kKvTile) * cache->heads * top * 4;
+    if (kv_seqs_overlap(out, bytes, *seqs) || (blocks && overlap(out, bytes, blocks, list_bytes)))
+        return fail(H3MI_EALIAS, "kv_attention: out overlaps tables, lens, counts or blocks");
     if (need > 0 && (!workspace || workspace_bytes < need))
         return fail(H3MI_EINVAL, "kv_attention: workspace of %lld bytes, %lld needed", (long long)(workspace ? workspace_bytes : 0), (long long)need);
     if (!aligned(workspace, 16)) return fail(H3MI_EALIGN, "kv_attention: workspace must be 16-byte aligned");

@@ -409,6 +409,9 @@ extern "C" int h3mi_kv_read_bf16(uint16_t* k, uint16_t* v, const int32_t* starts
     const size_t bytes = static_cast<size_t>(seqs->n) * length * cache->heads * cache->dim * 2;
     if (overlap(k, bytes, v, bytes) || kv_overlaps(k, bytes, *cache) || kv_overlaps(v, bytes, *cache))
         return fail(H3MI_EALIAS, "kv_read: k, v and the cache overlap");
+    for (const uint16_t* x : {k, v})
+        if (kv_seqs_overlap(x, bytes, *seqs) || (starts && overlap(x, bytes, starts, 4 * static_cast<size_t>(seqs->n))))
+            return fail(H3MI_EALIAS, "kv_read: k or v overlaps tables, lens, counts or starts");
     const auto fn = D == 64 ? kv_read_kernel<64> : D == 128 ? kv_read_kernel<128> : kv_read_kernel<256>;
     hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(groups)), dim3(2 * D), 0, as_stream(stream), k, v, starts,
                        kv_cache(*cache), kv_seqs(*seqs), static_cast<int>(length), static_cast<int>(touched));

@@ -306,6 +306,7 @@ extern "C" int h3mi_kv_select(const uint16_t* q, int64_t rows, int64_t heads, in
     const size_t bytes = static_cast<size_t>(groups) * top * 4;
     if (overlap(blocks, bytes, q, kv_span(seqs->n, rows, heads, cache->dim, ld_q, bs_q)) || kv_overlaps(blocks, bytes, *cache))
         return fail(H3MI_EALIAS, "kv_select: blocks overlaps q or the cache");
+    if (kv_seqs_overlap(blocks, bytes, *seqs)) return fail(H3MI_EALIAS, "kv_select: blocks overlaps tables, lens or counts");
     const int64_t need = key_bytes(groups, seqs->blocks);
     if (need > 0 && (!workspace || workspace_bytes < need))
         return fail(H3MI_EINVAL, "kv_select: workspace of %lld bytes, %lld needed", (long long)(workspace ? workspace_bytes : 0), (long long)need);

@@ -178,3 +178,17 @@ def test_written_cache_over_itself(cache):
 def test_written_cache_over_the_sequences(seqs):
     rc, m = _call("write", APART, {**APART_SEQS, **seqs})
     assert rc == 3 and "tables, lens or counts overlap the cache" in m, (rc, m)
+
+
+@pytest.mark.parametrize("fn,kw,msg", [
+    ("read", dict(p=1 << 28), "tables, lens"), ("read", dict(p2=1 << 29), "tables, lens"), ("read", dict(p2=(1 << 28) - 2 * 9 * 256 * 2 + 16), "tables, lens"),
+    ("read", dict(p=(1 << 31) - 16, starts=1 << 31), "starts"), ("read", dict(p2=1 << 31, starts=1 << 31), "starts"),
+    ("select", dict(out=1 << 28), "tables, lens"), ("select", dict(out=(1 << 29) - 8), "tables, lens"), ("select", dict(out=(1 << 30) + 4), "tables, lens"),
+    ("attention", dict(out=1 << 28), "tables, lens"), ("attention", dict(out=(1 << 29) - 16), "tables, lens"), ("attention", dict(out=1 << 30), "tables, lens"),
+    ("attention", dict(out=1 << 31, blocks=1 << 31), "blocks"), ("attention", dict(out=(1 << 31) - 8192 + 16, blocks=1 << 31), "blocks"),
+    ("attention", dict(out=(1 << 31) + 32, blocks=1 << 31), "blocks"),
+])
+def test_outputs_over_what_is_read(fn, kw, msg):
+    """A workgroup's output would change what another has yet to read."""
+    rc, m = _call(fn, APART, APART_SEQS, **kw)
+    assert rc == 3 and "overlap" in m and msg in m, (rc, m)
