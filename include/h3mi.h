@@ -225,7 +225,8 @@ int h3mi_rms_rope_split_half_bf16(uint16_t* q, uint16_t* k, const uint16_t* tab,
  * A cache is a pool of pages, one block of tokens a page.  A sequence's block b is
  * page tables[b]; pages of different sequences need not be distinct for reading.
  * A page index outside [0, pages) is a block that is not there: writes to it are
- * dropped, reads of it give zeros, attention and selection pass over it. */
+ * dropped, reads of it give zeros, attention and selection pass over it.
+ * Outputs and workspaces must not overlap the cache, another input or each other. */
 #define H3MI_KV_BLOCK 64   /* tokens of a block */
 #define H3MI_KV_TILE 128   /* query rows that share a selection of blocks */
 

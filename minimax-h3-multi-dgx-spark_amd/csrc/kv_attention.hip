@@ -1053,6 +1053,10 @@ extern "C" int h3mi_kv_attention_bf16(const uint16_t* q, int64_t rows, int64_t h
     if (need > 0 && (!workspace || workspace_bytes < need))
         return fail(H3MI_EINVAL, "kv_attention: workspace of %lld bytes, %lld needed", (long long)(workspace ? workspace_bytes : 0), (long long)need);
     if (!aligned(workspace, 16)) return fail(H3MI_EALIGN, "kv_attention: workspace must be 16-byte aligned");
+    if (need > 0 && (overlap(workspace, need, out, bytes) || overlap(workspace, need, q, kv_span(n, rows, heads, dim, ld_q, bs_q)) ||
+                     kv_overlaps(workspace, need, *cache) || kv_seqs_overlap(workspace, need, *seqs) ||
+                     (blocks && overlap(workspace, need, blocks, list_bytes))))
+        return fail(H3MI_EALIAS, "kv_attention: the workspace overlaps out or an input");
     const Queries qs = {q, ld_q, bs_q, static_cast<int>(rows), static_cast<int>(heads)};
     const Lists list = {blocks, static_cast<int>(top), static_cast<int>((rows + kKvTile - 1) / kKvTile)};
     Partial part = {static_cast<float*>(workspace), nullptr, p.shares ? p.shares + static_cast<int>(n) : p.splits, static_cast<int>(p.rows)};

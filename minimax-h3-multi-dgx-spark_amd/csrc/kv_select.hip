@@ -311,6 +311,9 @@ extern "C" int h3mi_kv_select(const uint16_t* q, int64_t rows, int64_t heads, in
     if (need > 0 && (!workspace || workspace_bytes < need))
         return fail(H3MI_EINVAL, "kv_select: workspace of %lld bytes, %lld needed", (long long)(workspace ? workspace_bytes : 0), (long long)need);
     if (!aligned(workspace, 4)) return fail(H3MI_EALIGN, "kv_select: workspace must be 4-byte aligned");
+    if (need > 0 && (overlap(workspace, need, blocks, bytes) || overlap(workspace, need, q, kv_span(seqs->n, rows, heads, cache->dim, ld_q, bs_q)) ||
+                     kv_overlaps(workspace, need, *cache) || kv_seqs_overlap(workspace, need, *seqs)))
+        return fail(H3MI_EALIAS, "kv_select: the workspace overlaps blocks or an input");
     const auto go = cache->dim == 64 ? launch<64> : cache->dim == 128 ? launch<128> : launch<256>;
     const auto run = [&](Part part, int threads, int64_t in_launch, int64_t chunks, int64_t keys_held) {
         go(part, threads, in_launch, keys_held * 4, as_stream(stream), q, ld_q, bs_q, kv_cache(*cache), kv_seqs(*seqs), static_cast<int>(rows),

@@ -192,3 +192,21 @@ def test_outputs_over_what_is_read(fn, kw, msg):
     """A workgroup's output would change what another has yet to read."""
     rc, m = _call(fn, APART, APART_SEQS, **kw)
     assert rc == 3 and "overlap" in m and msg in m, (rc, m)
+
+
+@pytest.mark.parametrize("fn,at", [(fn, at) for fn in ("select", "attention") for at in (
+    "p", "out", "k", "v", "k_scale", "v_scale", "k_sum", "tables", "lens", "counts")] + [("attention", "blocks")])
+def test_workspace_over_what_a_call_reads_or_writes(fn, at):
+    from h3mi import _lib
+    seqs = dict(APART_SEQS, n=4, blocks=2048)
+    cache = dict(APART, k=1 << 33, v=1 << 34, heads=8)
+    kw = dict(rows=1, heads=8, ld=1024, bs=1024, p=1 << 35, out=1 << 36, top=64 if fn == "attention" else 3)
+    if fn == "attention" and at == "blocks":
+        kw["blocks"] = 1 << 37
+    need = _lib.lib.h3mi_kv_select_workspace(4, 1, 8, 2048) if fn == "select" else \
+        _lib.lib.h3mi_kv_attention_workspace(4, 1, 8, 8, 128, 2048, 64 if "blocks" in kw else 0)
+    assert need > 0
+    where = {**cache, **seqs, **kw}[at]
+    for work in (where, where - (need - 1) // 16 * 16):
+        rc, m = _call(fn, cache, seqs, work=work, size=need, **kw)
+        assert rc == 3 and "workspace overlaps" in m, (rc, m)
