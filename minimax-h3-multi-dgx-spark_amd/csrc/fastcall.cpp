@@ -420,7 +420,7 @@ struct KvRows {
         if (!a.ok) return;
         const int64_t D = kv.c.dim;
         if (t->dim() != 4 || t->size(0) != kv.s.n || t->size(3) != D || t->stride(3) != 1 || (t->size(2) > 1 && t->stride(2) != D) ||
-            (t->requires_grad() && c10::GradMode::is_enabled())) {
+            (t->requires_grad() && c10::GradMode::is_enabled()) || t->_fw_grad(0).defined()) {
             a.ok = false;
             return;
         }

@@ -25,6 +25,7 @@ import ctypes
 import typing
 
 import torch
+from torch.autograd import forward_ad
 
 from ._lib import KvCacheC, KvSeqsC, _fast, check, lib, ptr, same_gpu, stream_of
 
@@ -103,6 +104,8 @@ def _rows(t, c, n, name, heads=None):
 def _no_grad(*ts):
     if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
         raise RuntimeError("attention over an 8-bit cache has no gradient: call it under torch.no_grad()")
+    if any(forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise RuntimeError("attention over an 8-bit cache has no forward-mode gradient: call it with the primal tensors")
 
 
 def kv_write_(cache, k, v, tables, lens, counts=None):

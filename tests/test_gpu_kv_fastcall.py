@@ -94,3 +94,22 @@ def test_native_path_is_taken():
     assert _fast.kv_select(x, cache, t, lens, 1, False, None) is not None
     assert _fast.kv_attention(x, cache, t, lens, False, None, None, None) is not None
     assert _fast.kv_attention(x.requires_grad_(), cache, t, lens, False, None, None, None) is None
+
+
+def test_tangents_are_left_to_the_python_path(monkeypatch):
+    from torch.autograd import forward_ad as fwd
+
+    import h3mi
+    full = h3mi.kv_cache(2, 2, 64)
+    t, lens = torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.ones(1, dtype=torch.int32, device="cuda")
+    x = torch.ones(1, 1, 2, 64, dtype=torch.bfloat16, device="cuda")
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        forms = [lambda h: tuple(h.kv_write_(full, dual, x, t, lens)), lambda h: tuple(h.kv_write_(full, x, dual, t, lens)),
+                 lambda h: h.kv_select(dual, full, t, lens, 1), lambda h: h.kv_attention(dual, full, t, lens)]
+        for f in forms:
+            assert _both(monkeypatch, f) == (RuntimeError, RuntimeError)
+        a, b = _both(monkeypatch, lambda h: h.kv_attention(fwd.unpack_dual(dual).primal, full, t, lens))
+        assert _same(a, b)
+    a, b = _both(monkeypatch, lambda h: h.kv_attention(dual, full, t, lens))
+    assert torch.is_tensor(a) and _same(a, b)

@@ -210,3 +210,32 @@ def test_workspace_over_what_a_call_reads_or_writes(fn, at):
     for work in (where, where - (need - 1) // 16 * 16):
         rc, m = _call(fn, cache, seqs, work=work, size=need, **kw)
         assert rc == 3 and "workspace overlaps" in m, (rc, m)
+
+
+def test_tangents_are_refused():
+    """As a gradient is: a dual tensor's tangent would be dropped.  Its primal and a dual of a level that has ended pass on."""
+    import torch
+    from torch.autograd import forward_ad as fwd
+
+    import h3mi
+    c = h3mi.kv_cache(2, 2, 64, device="cpu")
+    t, lens = torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    x = torch.zeros(1, 1, 2, 64, dtype=torch.bfloat16)
+
+    def calls(y):
+        return (lambda: h3mi.kv_write_(c, y, x, t, lens), lambda: h3mi.kv_write_(c, x, y, t, lens), lambda: h3mi.kv_select(y, c, t, lens, 1),
+                lambda: h3mi.kv_attention(y, c, t, lens))
+
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        for f in calls(dual):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                f()
+            with pytest.raises(RuntimeError, match="forward-mode"), torch.no_grad():
+                f()
+        for f in calls(fwd.unpack_dual(dual).primal):
+            with pytest.raises(ValueError, match="GPU"):
+                f()
+    for f in calls(dual):
+        with pytest.raises(ValueError, match="GPU"):
+            f()
