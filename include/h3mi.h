@@ -301,7 +301,9 @@ int h3mi_kv_select(const uint16_t* q, int64_t rows, int64_t heads, int64_t ld_q,
  * that comes twice counts twice).  Rows that
  * see no token, and rows behind counts, are 0.  Sums and statistics are fp32, the
  * products' operands bf16 (8-bit keys and values are exact in it, probabilities
- * are rounded to it).
+ * times their block's value scale are rounded to it: below 2^-126 to multiples of
+ * 2^-133).  Sums are formed before they are divided, against a reference that the
+ * largest score may pass by 2^8: values above 2^120 / tokens can make them infinite.
  * workspace: h3mi_kv_attention_workspace bytes of device memory, 16-byte aligned
  * (NULL where that is 0), for this call alone until it has run. */
 int64_t h3mi_kv_attention_workspace(int64_t n, int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim,
