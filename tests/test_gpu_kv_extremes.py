@@ -47,3 +47,24 @@ def test_value_scales_at_the_ends_of_fp32(rows, blocks, steep, scale):
     bound += 2.0 ** -134
     assert (np.abs(out - want) <= bound).all(), (np.abs(out - want) / bound).max()
     assert (bound < 0.6 * np.abs(want)).all() if scale >= 2.0 ** -130 else True  # zeros would not do
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3, 1.0, 30.0])
+@pytest.mark.parametrize("rows,blocks", [(1, 64), (20, 64), (200, 24), (200, 64)])
+def test_scales_of_scores_over_joined_parts(rows, blocks, scale):
+    """A scale of 0 is the mean of the values, a negative one turns the scores round, a steep one leaves a token or two."""
+    import h3mi
+    from h3mi import _lib
+    rng = np.random.default_rng(rows * blocks)
+    heads, dim = 2, 128
+    assert _lib.lib.h3mi_kv_attention_workspace(1, rows, heads, heads, dim, blocks, 0) > 0
+    ref = R.Cache(blocks, heads, dim, seed=blocks)
+    ref.ks *= 0.2
+    ref.ks[3], ref.k[3] = 0, 0
+    ref.vs[5], ref.v[5] = 0, 0
+    tables = rng.permutation(blocks)[None].astype(np.int32)
+    end = blocks * 64 - 9
+    q = torch.from_numpy(rng.standard_normal((1, rows, heads, dim))).to(torch.bfloat16)
+    out = h3mi.kv_attention(q.to(DEV), ref.to(), _i32(tables), _i32([end]), scale=scale).double().cpu().numpy()
+    want, mag, top = R.attention(ref, q.double().numpy(), tables, [end], [rows], False, scale)
+    assert (np.abs(out - want) <= R.bound(want, mag, top, dim)).all()

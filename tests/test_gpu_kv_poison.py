@@ -73,3 +73,24 @@ def test_a_poisoned_block_reaches_every_row_that_sees_it(plan, low, value, what)
     lists[..., blocks - 2] = bad
     got = h3mi.kv_attention(q, cache, tables, lens, blocks=lists).isnan().cpu()
     assert got[:, :, 1].all() and not got[:, :, 0].any()
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("plan", list(PLANS))
+def test_a_poisoned_query_stays_in_its_row_and_head(plan, value):
+    import h3mi
+    _check_plan(plan)
+    rows, blocks = PLANS[plan]
+    g = torch.Generator(device=DEV).manual_seed(rows * blocks)
+    draw = lambda *s: torch.randn(*s, generator=g, device=DEV).to(torch.bfloat16)  # noqa: E731
+    tables = torch.randperm(blocks, generator=g, device=DEV).to(torch.int32)[None]
+    lens = torch.tensor([blocks * 64 - 3], dtype=torch.int32, device=DEV)
+    cache = h3mi.kv_write_(h3mi.kv_cache(blocks, 2, 128), draw(1, blocks * 64 - 3, 2, 128), draw(1, blocks * 64 - 3, 2, 128), tables, lens)
+    q = draw(1, rows, 2, 128)
+    hit = torch.zeros(rows, 2, dtype=torch.bool, device=DEV)
+    hit[rows // 2, 1] = hit[0, 0] = True
+    bad = q.clone()
+    bad[0, :, :, 17] = torch.where(hit, torch.tensor(value, device=DEV, dtype=torch.bfloat16), q[0, :, :, 17])
+    for causal in (False, True):
+        want, got = (h3mi.kv_attention(x, cache, tables, lens, causal=causal)[0] for x in (q, bad))
+        assert got[hit].isnan().all() and want.isfinite().all() and torch.equal(got[~hit], want[~hit])
