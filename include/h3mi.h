@@ -261,7 +261,8 @@ typedef struct h3mi_kv_seqs {
  *   q = clamp(rne(x / s'), -127, 127), and the tokens the block held before become
  *   rne(q 2^-k) (0 where s' starts anew); 0 everywhere where s' is 0 or not finite.
  * A value's error is at most one step s' (half of one if its scale never grew).
- * A block with a NaN or an infinity reads back as NaN.  Tokens of a written block
+ * A block with a NaN or an infinity reads back as NaN until its first token is written
+ * again.  Tokens of a written block
  * behind the sequence's end become 0; other blocks are left as they were.  k_sum is
  * renewed.  The pages that a call writes have to be distinct, and none of the cache's
  * tensors may overlap another, tables, lens or counts.  dim 64, 128 or 256. */
@@ -282,12 +283,14 @@ int h3mi_kv_read_bf16(uint16_t* k, uint16_t* v, const int32_t* starts, int64_t l
  *   (64-bit), qi = rne(1023 P / max |P|)  (0 where max |P| is 0 or not finite),
  *   score_b = f32(sum_d qi[d] k_sum_b[d]) * (k_scale_b / tokens of block b),
  * the mean key's product with the mean query but for a factor that is the tile's.
- * It is a whole number's rounding, so no order of summing changes a selection.
+ * It is a whole number's rounding, so no order of summing changes a selection (where
+ * the largest element of a tile's queries is below 2^(38 - log2(heads / kv heads)) times
+ * the least that is not 0; of others P may be off in the last of its 53 bits).
  * causal: the blocks with the tile's own tokens come first, later ones are not
  * seen.  Equal scores: the lowest block first; NaN scores come last.  A tile with no
  * rows of its own selects nothing.  top in [1, 32768], seqs->blocks <= 32768.
- * workspace: h3mi_kv_select_workspace bytes of device memory, 4-byte aligned (NULL
- * where that is 0), for this call alone until it has run. */
+ * workspace: h3mi_kv_select_workspace bytes (for the current device) of device memory,
+ * 4-byte aligned (NULL where that is 0), for this call alone until it has run. */
 int64_t h3mi_kv_select_workspace(int64_t n, int64_t rows, int64_t kv_heads, int64_t blocks);
 int h3mi_kv_select(const uint16_t* q, int64_t rows, int64_t heads, int64_t ld_q, int64_t bs_q,
                    const h3mi_kv_cache* cache, const h3mi_kv_seqs* seqs, int64_t top, int causal,
@@ -304,8 +307,8 @@ int h3mi_kv_select(const uint16_t* q, int64_t rows, int64_t heads, int64_t ld_q,
  * times their block's value scale are rounded to it: below 2^-126 to multiples of
  * 2^-133).  Sums are formed before they are divided, against a reference that the
  * largest score may pass by 2^8: values above 2^120 / tokens can make them infinite.
- * workspace: h3mi_kv_attention_workspace bytes of device memory, 16-byte aligned
- * (NULL where that is 0), for this call alone until it has run. */
+ * workspace: h3mi_kv_attention_workspace bytes (for the current device) of device
+ * memory, 16-byte aligned (NULL where that is 0), for this call alone until it has run. */
 int64_t h3mi_kv_attention_workspace(int64_t n, int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim,
                                     int64_t blocks, int64_t top);
 int h3mi_kv_attention_bf16(const uint16_t* q, int64_t rows, int64_t heads, int64_t ld_q, int64_t bs_q,

@@ -7,7 +7,9 @@
 // scale is a factor of its scores (one fma with the subtraction of m), and its value scale
 // a term of the exponent, p v_scale = 2^(x - m + log2 v_scale), which costs nothing per
 // score; l takes the sum times 1 / v_scale.  Scores and sums are fp32; a probability is
-// rounded once, to the bf16 that the second product multiplies.
+// rounded once, to the bf16 that the second product multiplies.  That is off by 2^-8 of it at
+// most, as the output's own rounding is: outputs are 1.8e-3 off (rms) where probabilities in
+// 32 bits leave 1.7e-3, and a second MFMA for the remainder would add half of all products.
 //
 // Both products are formed transposed, S^T = K Q^T and O^T = V^T P^T: a query is then a
 // column, whose scores lie in the registers of two (four) lanes, so that the maximum needs
@@ -17,7 +19,8 @@
 // its rows are runs of tokens too.  P never leaves the registers.
 //
 // Two kernels: tiles of 128 or 256 query rows of a head, bound by the MFMAs and the
-// softmax, and up to 16 queries of a kv head's group, bound by the cache's bytes.
+// softmax, and up to 64, 32 or 16 queries (of 64, 128, 256 elements) of a kv head's group,
+// bound by the cache's bytes.
 #include <type_traits>
 
 #include "kv.h"
@@ -127,9 +130,9 @@ struct Partial {
 // writes (rows) and for the MFMA operands' reads (columns); by three row bits instead of four
 // 43% of LDS's cycles were conflicts, and 2.88 ms were 2.63.
 //
-// Measured: 4800 rows over 19721 tokens of 56 x 128 in 2.63 ms, 1030 TFLOP/s, 84% of what a
+// Measured: 4800 rows over 19721 tokens of 56 x 128 in 2.6 ms, 1040 TFLOP/s, 86% of what a
 // large bf16 product reaches on the card; the power limit holds it there (1.98 GHz, 46% of
-// MFMA issue).  56 heads of 2401 rows over lists of 100 blocks in 0.49 ms, 900 TFLOP/s.
+// MFMA issue).  56 heads of 2401 rows over lists of 100 blocks in 0.51 ms, 860 TFLOP/s.
 
 // The place of chunk ch of a row of CH chunks (8: two rows share the banks).
 template <int CH>
@@ -186,7 +189,7 @@ struct Items {
     }
 };
 
-// (64 elements leave registers and LDS for three workgroups a CU: 4800 x 19200 831 us with two, 689 so.)
+// (64 elements leave registers, 164 of 168, and LDS for three workgroups a CU: 4800 x 19200 831 us with two, 680 so.)
 template <int D, int W>
 __global__ __launch_bounds__(64 * W, D == 256 ? 1 : D == 64 ? 3 : 2) void kv_tile_kernel(Queries q, KvCache c, KvSeqs s, float scale, int causal,
                                                                           Lists list, uint16_t* __restrict__ out, Partial part,
@@ -508,10 +511,11 @@ struct Shares {
 // A workgroup: up to 16 NQ queries of one kv head's group, one share of the blocks.  Its
 // waves take whole blocks in turn, straight from memory into the operands' registers (no
 // LDS, no barrier; a block's bytes are converted once for all queries), and are joined once
-// for each sequence.  HBM bounds it: a query of 56 heads over 19721 tokens takes 47 us, 6.0 TB/s, 17
+// for each sequence.  HBM bounds it: a query of 56 heads over 19721 tokens takes 50 us, 5.7 TB/s, 17
 // to 32 rows of 8 x 56 heads over 4000 tokens 87 us, where the 40 that go by tiles, 16 KB a
 // workgroup at a time, take 129; 16 sequences of 1 to 32768 tokens of 8 heads (780 MB) 128, where
-// shares of their own for each, a quarter of the longest, took 146.
+// shares of their own for each, a quarter of the longest, took 146.  Without shares (plan_of) a
+// workgroup reads a whole sequence, and the launch takes as long as the longest.
 template <int D, int NQ>
 __global__ __launch_bounds__(64 * kFewWaves) void kv_few_kernel(Queries q, KvCache c, KvSeqs s, float scale, int causal, Lists list,
                                                                 uint16_t* __restrict__ out, Partial part, Shares shares) {

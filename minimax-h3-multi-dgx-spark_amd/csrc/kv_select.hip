@@ -3,16 +3,21 @@
 // A tile's score of a block is a product of whole numbers (the pooled queries as 11-bit
 // integers, the sum of the block's 8-bit keys as 16-bit ones), exact in int32: |qi| <=
 // 1023, |k_sum| <= 64 * 127 and dim <= 256 keep it below 2^31.  The pooled queries are
-// summed in 64 bits, where bf16 values within a factor of 2^30 of each other add
-// exactly.  So neither the order of a sum nor the split of the work changes a selection.
+// summed in 64 bits: the sum of N bf16 values (128 rows of the heads of a group) is exact
+// where the largest is below 2^(45 - log2 N) times the least that is not 0, 2^38 for one
+// head, 2^30 to 256 heads.  So neither the order of a sum nor the split of the work changes
+// a selection; of values further apart the last bits of 53 may, and with them a selection
+// whose scores lie next to each other.
 //
 // A workgroup takes one tile of one kv head: it pools the queries, scores every block
 // (dim / 8 lanes a block, 16 bytes of k_sum each, v_dot2_i32_i16), keeps the scores as
 // ordered 32-bit keys in LDS, finds the last selected key by up to four passes over 8 bits
 // of it, and writes the selected blocks in order.  Few tiles over long tables, whose scoring
 // would wait on a few CUs' loads, score in a launch of their own, a workgroup for every
-// kChunk blocks, and the keys pass through memory.  1064 tiles of 609 blocks take 24 us, half
-// of it the queries' pooling; 32 tiles of 2048 blocks 15 us in two launches.
+// kChunk blocks, and the keys pass through memory.  1064 tiles of 609 blocks take 28 us (25
+// again and again, its inputs in the caches; 34 MB of queries and 9 MB of sums would be 9), half
+// of it the queries' pooling, and then each tile reads all the sums of its head; 32 tiles of
+// 2048 blocks 15 us in two launches.
 #include "kv.h"
 
 namespace h3mi {

@@ -2,9 +2,10 @@
 
 No counterpart in the reference, which computes its attention in the host program
 (comfyui_nodes/minimax-h3-sp/minimax_sp/sp_forward.py:276-318).  Keys and values
-that outlive a call (a prompt's and reference frames' over the denoising steps, the
-finished chunks' of a long clip, the tokens before a step's) stay in a KVCache, at
-half of bf16's size:
+that outlive a call (the finished chunks' of a long clip, the tokens before a step's,
+a prompt's or reference frames' whose own rows attend to nothing that changes) stay in
+a KVCache, at half of bf16's size.  Rows of one bidirectional sequence change with
+every denoising step, its text rows among them: their keys are written anew for each.
 
   kv_cache(pages, heads, dim)                          an empty pool of pages of 64 tokens
   kv_write_(cache, k, v, tables, lens)                 quantize new tokens into it
@@ -17,8 +18,10 @@ tables int32 [n, blocks] gives the page of each block of 64 tokens of n sequence
 lens int32 [n] their tokens, those of the call among them; counts int32 [n] says how
 many of a call's rows a sequence has (the rest is padding), and row r of sequence i is
 token lens[i] - counts[i] + r.  All stay on the GPU and are read there, so that a
-captured call follows them.  Rows are [n, rows, heads, dim] bf16 with contiguous heads
-and any token stride: views of a projection's output serve, as after
+captured call follows them.  How a call's work is split goes by the tables' width, so
+tables no wider than the sequences need serve best.  Rows are [n, rows, heads, dim] bf16
+with contiguous heads, 16-byte aligned, with token and sequence strides that are multiples
+of 8 elements and no shorter than a row: views of a projection's output serve, as after
 rms_rope_split_half_.
 """
 import ctypes
@@ -113,7 +116,8 @@ def kv_write_(cache, k, v, tables, lens, counts=None):
 
     A block's scale is max|x| / 127 of its first write.  A later write of tokens that do not fit doubles it as often
     as they need and halves the block's older 8-bit values as often, so that an error stays within one step.  A NaN or
-    an infinity makes its block read back as NaN.  The pages that a call writes have to be distinct."""
+    an infinity makes its block read back as NaN until the block's first token is written again.  The pages that a call
+    writes have to be distinct."""
     done = _fast.kv_write_(cache, k, v, tables, lens, counts)
     if done is not None:
         return done
@@ -154,7 +158,8 @@ def kv_select(q, cache, tables, lens, top, causal=False, counts=None):
 
     A block's score is the product of its mean key with the mean of the tile's queries (of all heads that share the kv
     head), formed from 8-bit keys and 11-bit queries in whole numbers.  With causal, the blocks of the tile's own tokens
-    are taken first and later ones never.  Equal scores go to the lowest block."""
+    are taken first and later ones never.  Equal scores go to the lowest block: of a tile with a NaN or an infinity in any
+    of its queries all scores are equal."""
     out = _fast.kv_select(q, cache, tables, lens, top, causal, counts)
     if out is not None:
         return out
