@@ -128,10 +128,11 @@ struct Partial {
 // Rows in LDS are 16-byte chunks whose index is XORed with row bits, so that 16 lanes of an
 // access lie on the 16 different 16-byte groups of LDS's 256 bytes of banks, both for the
 // writes (rows) and for the MFMA operands' reads (columns); by three row bits instead of four
-// 43% of LDS's cycles were conflicts, and 2.88 ms were 2.63.
+// 43% of LDS's cycles were conflicts, and 2.88 ms were 2.63.  (16% are now, with
+// threads that stage two neighbouring chunks, which took the 256-element kernel from 434 us to 404.)
 //
 // Measured: 4800 rows over 19721 tokens of 56 x 128 in 2.6 ms, 1040 TFLOP/s, 86% of what a
-// large bf16 product reaches on the card; the power limit holds it there (1.98 GHz, 46% of
+// large bf16 product reaches on the card; the power limit holds it there (1.93 GHz, 52% of
 // MFMA issue).  56 heads of 2401 rows over lists of 100 blocks in 0.51 ms, 860 TFLOP/s.
 
 // The place of chunk ch of a row of CH chunks (8: two rows share the banks).
