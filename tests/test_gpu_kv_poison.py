@@ -94,3 +94,29 @@ def test_a_poisoned_query_stays_in_its_row_and_head(plan, value):
     for causal in (False, True):
         want, got = (h3mi.kv_attention(x, cache, tables, lens, causal=causal)[0] for x in (q, bad))
         assert got[hit].isnan().all() and want.isfinite().all() and torch.equal(got[~hit], want[~hit])
+
+
+@pytest.mark.parametrize("rows,blocks", [(8, 6), (8, 64), (300, 6), (300, 64)])
+def test_rows_behind_a_sequences_own_are_not_read(rows, blocks):
+    """NaN in the padding of a batch changes no page, no selection and no output."""
+    import h3mi
+    g = torch.Generator(device=DEV).manual_seed(rows + blocks)
+    draw = lambda *s: torch.randn(*s, generator=g, device=DEV).to(torch.bfloat16)  # noqa: E731
+    n = 3
+    counts = torch.tensor([rows, rows // 2 + 1, 0], dtype=torch.int32, device=DEV)
+    lens = torch.tensor([blocks * 64, blocks * 40 + 7, 0], dtype=torch.int32, device=DEV)
+    tables = torch.randperm(n * blocks, generator=g, device=DEV).reshape(n, blocks).to(torch.int32)
+    k, v, before = draw(n, rows, 2, 128), draw(n, rows, 2, 128), draw(n, blocks * 64, 2, 128)
+    q = draw(n, rows, 4, 128)
+    pad = (torch.arange(rows, device=DEV) >= counts[:, None])[..., None, None]
+    got = []
+    for fill in (0.0, float("nan")):
+        kx, vx, qx = (torch.where(pad, torch.tensor(fill, dtype=torch.bfloat16, device=DEV), x) for x in (k, v, q))
+        c = h3mi.kv_write_(h3mi.kv_cache(n * blocks, 2, 128), before, before, tables, lens)
+        h3mi.kv_write_(c, kx, vx, tables, lens, counts=counts)
+        pick = h3mi.kv_select(qx, c, tables, lens, 3, causal=True, counts=counts)
+        got.append([*c, pick, h3mi.kv_attention(qx, c, tables, lens, causal=True, counts=counts),
+                    h3mi.kv_attention(qx, c, tables, lens, counts=counts, blocks=pick)])
+    for a, b in zip(*got):
+        assert torch.equal(a, b) and (not a.is_floating_point() or a.isfinite().all())
+    assert (got[0][6][pad.expand(n, rows, 4, 128)] == 0).all()
