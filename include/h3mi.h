@@ -316,6 +316,45 @@ int h3mi_kv_attention_bf16(const uint16_t* q, int64_t rows, int64_t heads, int64
                            const int32_t* blocks, int64_t top, uint16_t* out, void* workspace,
                            int64_t workspace_bytes, void* stream);
 
+/* The key/value cache in 4 bits: 17/32 of the 8-bit cache's bytes.  An element is a
+ * sign (bit 3) and the place of its magnitude among 0, 0.5, 1, 1.5, 2, 3, 4, 6 (bits
+ * 0 to 2), times the 2^(code - 127) of its group of 32 elements of the token; codes of
+ * 253 and more stand for no number. */
+#define H3MI_KV_GROUP 32   /* elements that share a scale */
+
+typedef struct h3mi_kv_cache4 {
+    uint8_t* k;        /* [pages, heads, 64, dim / 2]: element 2 j in the low half of byte j */
+    uint8_t* v;        /* as k */
+    uint8_t* k_scale;  /* [pages, heads, dim / 32, 64] */
+    uint8_t* v_scale;  /* as k_scale */
+    int64_t pages, heads, dim;
+} h3mi_kv_cache4;
+
+/* Quantizes k and v into the cache, as h3mi_kv_write_i8 takes them.  A group's code is
+ * e + 127 for the least e of -125 .. 125 with max |x| <= 7 2^e, and x 2^-e is rounded to
+ * the nearest of the values, between two to the one with the even place (above 7 2^125
+ * to 6 2^125).  A group with a NaN or an infinity gets 255 and reads back as NaNs.  The
+ * call's tokens alone are written: nothing that the cache held is rounded again, and what
+ * a page holds behind a sequence's end stays.  The tokens that a call writes have to be
+ * distinct, and none of the cache's tensors (16-byte aligned) may overlap another, tables,
+ * lens or counts.  dim 64, 128 or 256. */
+int h3mi_kv_write_mx4(const uint16_t* k, const uint16_t* v, int64_t rows, int64_t ld_k, int64_t bs_k,
+                      int64_t ld_v, int64_t bs_v, const h3mi_kv_cache4* cache, const h3mi_kv_seqs* seqs,
+                      void* stream);
+
+/* As h3mi_kv_read_bf16; the values are bf16 numbers, so nothing is rounded. */
+int h3mi_kv_read_mx4_bf16(uint16_t* k, uint16_t* v, const int32_t* starts, int64_t length,
+                          const h3mi_kv_cache4* cache, const h3mi_kv_seqs* seqs, void* stream);
+
+/* As h3mi_kv_attention_bf16, with the workspace that h3mi_kv_attention_workspace gives.
+ * Keys and values are exact in the products.  A value group that stands for no number
+ * makes NaNs of its 32 elements of the rows that see its token, a key group of all of
+ * theirs. */
+int h3mi_kv_attention_mx4_bf16(const uint16_t* q, int64_t rows, int64_t heads, int64_t ld_q, int64_t bs_q,
+                               const h3mi_kv_cache4* cache, const h3mi_kv_seqs* seqs, float scale, int causal,
+                               const int32_t* blocks, int64_t top, uint16_t* out, void* workspace,
+                               int64_t workspace_bytes, void* stream);
+
 /* (numx, vec, warp) of an order; returns H3MI_EINVAL for an unknown order. */
 int h3mi_norm_order_info(int order, int* numx, int* vec, int* warp);
 

@@ -371,25 +371,37 @@ PyObject* rms_rope_(PyObject*, PyObject* const* v, Py_ssize_t n) {
     H3MI_END
 }
 
-// A KVCache and the sequences of a call.
+// A KVCache or (four) a KVCache4, and the sequences of a call.
 struct Kv {
-    h3mi_kv_cache c = {};
+    bool four = false;
+    h3mi_kv_cache c = {};  // four: its sizes alone
+    h3mi_kv_cache4 c4 = {};
     h3mi_kv_seqs s = {};
     Kv(Args& a, PyObject* cache, PyObject* tables, PyObject* lens, PyObject* counts) {
         if (!a.ok) return;
         a.ok = false;
-        if (!PyTuple_Check(cache) || PyTuple_GET_SIZE(cache) != 5) return;
+        if (!PyTuple_Check(cache)) return;
+        const Py_ssize_t size = PyTuple_GET_SIZE(cache);
+        if (size != 4 && size != 5) return;
+        four = size == 4;
         a.ok = true;
-        const at::Tensor* k = a.typed(PyTuple_GET_ITEM(cache, 0), c10::kChar);
+        const at::Tensor* k = a.typed(PyTuple_GET_ITEM(cache, 0), four ? c10::kByte : c10::kChar);
         if (!a.ok || k->dim() != 4 || k->size(2) != H3MI_KV_BLOCK || !k->is_contiguous()) {
             a.ok = false;
             return;
         }
-        const int64_t P = k->size(0), H = k->size(1), D = k->size(3);
-        const at::Tensor* v = shaped(a, PyTuple_GET_ITEM(cache, 1), c10::kChar, {P, H, D, H3MI_KV_BLOCK});
-        const at::Tensor* ks = shaped(a, PyTuple_GET_ITEM(cache, 2), c10::kFloat, {P, H});
-        const at::Tensor* vs = shaped(a, PyTuple_GET_ITEM(cache, 3), c10::kFloat, {P, H});
-        const at::Tensor* sum = shaped(a, PyTuple_GET_ITEM(cache, 4), c10::kShort, {P, H, D});
+        const int64_t P = k->size(0), H = k->size(1), D = k->size(3) * (four ? 2 : 1);
+        const at::Tensor *v, *ks, *vs, *sum = nullptr;
+        if (four) {
+            v = shaped(a, PyTuple_GET_ITEM(cache, 1), c10::kByte, {P, H, H3MI_KV_BLOCK, D / 2});
+            ks = shaped(a, PyTuple_GET_ITEM(cache, 2), c10::kByte, {P, H, D / H3MI_KV_GROUP, H3MI_KV_BLOCK});
+            vs = shaped(a, PyTuple_GET_ITEM(cache, 3), c10::kByte, {P, H, D / H3MI_KV_GROUP, H3MI_KV_BLOCK});
+        } else {
+            v = shaped(a, PyTuple_GET_ITEM(cache, 1), c10::kChar, {P, H, D, H3MI_KV_BLOCK});
+            ks = shaped(a, PyTuple_GET_ITEM(cache, 2), c10::kFloat, {P, H});
+            vs = shaped(a, PyTuple_GET_ITEM(cache, 3), c10::kFloat, {P, H});
+            sum = shaped(a, PyTuple_GET_ITEM(cache, 4), c10::kShort, {P, H, D});
+        }
         const at::Tensor* tab = a.typed(tables, c10::kInt);
         if (!a.ok || tab->dim() != 2 || !tab->is_contiguous() || a.dev.index() != c10::hip::current_device()) {
             a.ok = false;
@@ -398,7 +410,12 @@ struct Kv {
         const at::Tensor* l = shaped(a, lens, c10::kInt, {tab->size(0)});
         const at::Tensor* n = counts == Py_None ? nullptr : shaped(a, counts, c10::kInt, {tab->size(0)});
         if (!a.ok) return;
-        c = {i8(k), i8(v), mf32(ks), mf32(vs), static_cast<int16_t*>(sum->data_ptr()), P, H, D};
+        if (four) {
+            c4 = {u8(k), u8(v), u8(ks), u8(vs), P, H, D};
+            c.pages = P, c.heads = H, c.dim = D;
+        } else {
+            c = {i8(k), i8(v), mf32(ks), mf32(vs), static_cast<int16_t*>(sum->data_ptr()), P, H, D};
+        }
         s = {i32(tab), i32(l), n ? i32(n) : nullptr, tab->size(0), tab->size(1)};
     }
     static const at::Tensor* shaped(Args& a, PyObject* o, c10::ScalarType type, std::initializer_list<int64_t> size) {
@@ -406,6 +423,7 @@ struct Kv {
         if (t && (t->sizes() != at::IntArrayRef(size) || !t->is_contiguous())) a.ok = false;
         return t;
     }
+    static uint8_t* u8(const at::Tensor* t) { return static_cast<uint8_t*>(t->data_ptr()); }
     static int8_t* i8(const at::Tensor* t) { return static_cast<int8_t*>(t->data_ptr()); }
     static float* mf32(const at::Tensor* t) { return static_cast<float*>(t->data_ptr()); }
     static const int32_t* i32(const at::Tensor* t) { return static_cast<const int32_t*>(t->data_ptr()); }
@@ -456,7 +474,8 @@ PyObject* kv_write_(PyObject*, PyObject* const* v, Py_ssize_t n) {
     int rc;
     {
         pybind11::gil_scoped_release nogil;
-        rc = h3mi_kv_write_i8(u16(k.t), u16(x.t), k.rows, k.ld, k.bs, x.ld, x.bs, &kv.c, &kv.s, a.stream());
+        rc = kv.four ? h3mi_kv_write_mx4(u16(k.t), u16(x.t), k.rows, k.ld, k.bs, x.ld, x.bs, &kv.c4, &kv.s, a.stream())
+                     : h3mi_kv_write_i8(u16(k.t), u16(x.t), k.rows, k.ld, k.bs, x.ld, x.bs, &kv.c, &kv.s, a.stream());
     }
     if (rc) return raise_status(rc);
     Py_INCREF(v[0]);
@@ -480,7 +499,9 @@ PyObject* kv_read(PyObject*, PyObject* const* v, Py_ssize_t n) {
         pybind11::gil_scoped_release nogil;
         k = a.empty({kv.s.n, length, kv.c.heads, kv.c.dim}, c10::kBFloat16);
         x = a.empty({kv.s.n, length, kv.c.heads, kv.c.dim}, c10::kBFloat16);
-        rc = h3mi_kv_read_bf16(mu16(k), mu16(x), starts ? Kv::i32(starts) : nullptr, length, &kv.c, &kv.s, a.stream());
+        const int32_t* const from = starts ? Kv::i32(starts) : nullptr;
+        rc = kv.four ? h3mi_kv_read_mx4_bf16(mu16(k), mu16(x), from, length, &kv.c4, &kv.s, a.stream())
+                     : h3mi_kv_read_bf16(mu16(k), mu16(x), from, length, &kv.c, &kv.s, a.stream());
     }
     return rc ? raise_status(rc) : pair(k, x);
     H3MI_END
@@ -496,7 +517,7 @@ PyObject* kv_select(PyObject*, PyObject* const* v, Py_ssize_t n) {
     const KvRows q(a, v[0], kv);
     int64_t top = 0;
     int causal = 0;
-    if (!a.ok || !whole(v[4], &top) || top < 1 || !truth(v[5], &causal)) Py_RETURN_NONE;
+    if (!a.ok || kv.four || !whole(v[4], &top) || top < 1 || !truth(v[5], &causal)) Py_RETURN_NONE;
     at::Tensor out, work;
     int rc;
     {
@@ -542,8 +563,11 @@ PyObject* kv_attention(PyObject*, PyObject* const* v, Py_ssize_t n) {
         out = a.empty(q.t->sizes(), c10::kBFloat16);
         const int64_t need = h3mi_kv_attention_workspace(kv.s.n, q.rows, q.heads, kv.c.heads, kv.c.dim, kv.s.blocks, top);
         if (need > 0) work = a.empty({need}, c10::kByte);
-        rc = h3mi_kv_attention_bf16(u16(q.t), q.rows, q.heads, q.ld, q.bs, &kv.c, &kv.s, static_cast<float>(scale), causal,
-                                    list ? Kv::i32(list) : nullptr, top, mu16(out), need > 0 ? work.data_ptr() : nullptr, need, a.stream());
+        const auto attend = [&](const auto fn, const auto* c) {
+            return fn(u16(q.t), q.rows, q.heads, q.ld, q.bs, c, &kv.s, static_cast<float>(scale), causal, list ? Kv::i32(list) : nullptr,
+                      top, mu16(out), need > 0 ? work.data_ptr() : nullptr, need, a.stream());
+        };
+        rc = kv.four ? attend(&h3mi_kv_attention_mx4_bf16, &kv.c4) : attend(&h3mi_kv_attention_bf16, &kv.c);
     }
     return rc ? raise_status(rc) : THPVariable_Wrap(out);
     H3MI_END

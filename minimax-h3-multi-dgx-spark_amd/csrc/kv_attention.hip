@@ -94,6 +94,12 @@ __device__ __forceinline__ Factors factors(float ks, float vs, float scale) {
     return {c < 0x1p-126f ? 0x1p-126f : c, fold ? __builtin_amdgcn_logf(vs) : 0.0f, fold ? __builtin_amdgcn_rcpf(vs) : 0.0f, vs};
 }
 
+// Whether one of four scale codes stands for no number: bytes of kFourBad and more.
+__device__ __forceinline__ bool four_bad(uint32_t codes) {
+    static_assert(kFourBad == 253, "125 + 3 = 2^7");
+    return (((codes & 0x7F7F7F7Fu) + 0x03030303u) & codes & 0x80808080u) != 0;
+}
+
 struct Queries {
     const uint16_t* p;
     int64_t ld, bs;
@@ -155,6 +161,117 @@ struct TileShape {
     static constexpr int kLoads = kKvBlock * D / 16 / kThreads;  // 16-byte pieces of K (and of V) a thread
 };
 
+// What a thread loads and stages of a block in 4 bits.  Keys: pieces of 16 elements of a token, half a group's, as in 8 bits.
+// Values lie as they were written, token by token, and the second product wants runs of tokens: a thread takes 8 elements of
+// 4 (2) neighbouring tokens, whose pairs of elements, converted (one instruction for two, exact), change places with a permute
+// each and are 8 (4) bytes of 8 rows in LDS.
+template <int D, int W>
+struct FourTile {
+    static constexpr int G = D / kFourGroup, kThreads = 64 * W;
+    static constexpr int kPieces = kKvBlock * D / 16 / kThreads;
+    static constexpr int kEach = kKvBlock * D / kThreads;     // elements a thread
+    static constexpr int kTok = kEach >= 32 ? 4 : 2, kUnits = kEach / (8 * kTok);
+
+    struct Keys {
+        uint2 w[kPieces];
+        uint8_t code[kPieces];
+        __device__ __forceinline__ void load(const KvCache4& c, int64_t tile, int t) {
+            const uint8_t* const at = c.k + tile * (kKvBlock * D / 2);
+            const uint8_t* const codes = c.ks + tile * (kKvBlock * G);
+#pragma unroll
+            for (int j = 0; j < kPieces; ++j) {
+                const uint32_t piece = t + j * kThreads, line = piece / (D / 16), g = piece % (D / 16) / 2;
+                w[j] = *reinterpret_cast<const uint2*>(at + piece * 8);
+                code[j] = codes[g * kKvBlock + line];
+            }
+        }
+        __device__ __forceinline__ void stage(uint8_t* buf, int t) const {
+            constexpr int CH = D / 8;
+#pragma unroll
+            for (int j = 0; j < kPieces; ++j) {
+                const int piece = t + j * kThreads, line = piece / (CH / 2), ch = piece % (CH / 2) * 2;
+                // token bits 2 and 3 change places, as in 8 bits
+                const int row = (line & ~12) | ((line & 4) << 1) | ((line & 8) >> 1);
+                uint8_t* const to_row = buf + row * (CH * 16);
+                // (a NaN of every element: a factor of 2^128 is none, whatever is not 0 times it)
+                const bool bad = code[j] >= kFourBad;
+                const float f = four_scale(bad ? 255 : code[j]);
+                const uint32_t some = bad ? 0x11111111u : 0u;
+                *reinterpret_cast<uint4*>(to_row + chunk_at<CH>(row, ch) * 16) = four_bf16x8(w[j].x | some, f);
+                *reinterpret_cast<uint4*>(to_row + chunk_at<CH>(row, ch + 1) * 16) = four_bf16x8(w[j].y | some, f);
+            }
+        }
+    };
+
+    // The place of chunk ch (8 tokens) of element `row` in LDS: two rows on the 256 bytes of banks, 16-byte chunks whose index is
+    // XORed so that 16 lanes lie on different ones where they read neighbouring rows; where 32 (64) lanes write all tokens of
+    // rows r and r + 8, bit 3 puts these on the two halves.
+    static __device__ __forceinline__ uint32_t value_at(int row, int ch) {
+        return (row >> 1) * 256 + (((((row & 1) << 3) | ch) ^ ((row >> 1) & 7) ^ (row & 8)) * 16);
+    }
+
+    struct Values {
+        uint32_t w[kUnits][kTok], codes[kUnits];
+        // A unit's 8 elements and its first token: all tokens of two neighbouring runs of elements, then of the next two.
+        static __device__ __forceinline__ void place(uint32_t unit, uint32_t& ch, uint32_t& tok) {
+            tok = (unit >> 1) % (kKvBlock / kTok) * kTok;
+            ch = unit / (2 * kKvBlock / kTok) * 2 + (unit & 1);
+        }
+        __device__ __forceinline__ void load(const KvCache4& c, int64_t tile, int t) {
+            const uint8_t* const at = c.v + tile * (kKvBlock * D / 2);
+            const uint8_t* const from = c.vs + tile * (kKvBlock * G);
+#pragma unroll
+            for (int j = 0; j < kUnits; ++j) {
+                uint32_t ch, tok;
+                place(t + j * kThreads, ch, tok);
+#pragma unroll
+                for (int x = 0; x < kTok; ++x) w[j][x] = *reinterpret_cast<const uint32_t*>(at + (tok + x) * (D / 2) + ch * 4);
+                const uint8_t* const p = from + ch / 4 * kKvBlock + tok;
+                if constexpr (kTok == 4) codes[j] = *reinterpret_cast<const uint32_t*>(p);
+                else codes[j] = *reinterpret_cast<const uint16_t*>(p);
+            }
+        }
+        __device__ __forceinline__ void stage(uint8_t* buf, int t, int* poison) {
+#pragma unroll
+            for (int j = 0; j < kUnits; ++j) {
+                uint32_t ch, tok;
+                place(t + j * kThreads, ch, tok);
+                // value_at(8 ch + 2 e + z, tok / 8) = (to ^ (16 e + 128 z)) + 256 e, opaque, so that the loop does not keep eight
+                uint32_t to = ch * 1024 + ((tok / 8) ^ (12 * (ch & 1))) * 16 + tok % 8 * 2;
+                asm("" : "+v"(to));
+                if (four_bad(codes[j])) {
+#pragma unroll
+                    for (int x = 0; x < kTok; ++x) {
+                        if ((codes[j] >> (8 * x) & 255) < kFourBad) continue;
+                        w[j][x] = 0;
+                        codes[j] &= ~(255u << (8 * x));
+                    }
+                    *poison = 1;
+                }
+                float f[kTok];
+#pragma unroll
+                for (int x = 0; x < kTok; ++x) f[x] = four_scale(codes[j] >> (8 * x) & 255);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    uint32_t y[kTok];
+#pragma unroll
+                    for (int x = 0; x < kTok; ++x)
+                        y[x] = e == 0 ? four_bf16<0>(w[j][x], f[x]) : e == 1 ? four_bf16<1>(w[j][x], f[x]) : e == 2 ? four_bf16<2>(w[j][x], f[x]) : four_bf16<3>(w[j][x], f[x]);
+#pragma unroll
+                    for (int z = 0; z < 2; ++z) {
+                        const uint32_t sel = z ? 0x07060302u : 0x05040100u;
+                        uint8_t* const p = buf + (to ^ (16 * e + 128 * z)) + 256 * e;
+                        if constexpr (kTok == 4)
+                            *reinterpret_cast<uint2*>(p) = make_uint2(__builtin_amdgcn_perm(y[1], y[0], sel), __builtin_amdgcn_perm(y[kTok - 1], y[kTok - 2], sel));
+                        else
+                            *reinterpret_cast<uint32_t*>(p) = __builtin_amdgcn_perm(y[1], y[0], sel);
+                    }
+                }
+            }
+        }
+    };
+};
+
 // The items of a launch: tiles of the queries of a head, or (pack > 1) of the queries of all
 // heads that share a kv head, in the order of rows, then heads.  The first `whole` take one
 // workgroup each, a multiple of what the card holds at once; the rest, which would leave a
@@ -191,17 +308,19 @@ struct Items {
 };
 
 // (64 elements leave registers, 164 of 168, and LDS for three workgroups a CU: 4800 x 19200 831 us with two, 680 so.)
-template <int D, int W>
-__global__ __launch_bounds__(64 * W, D == 256 ? 1 : D == 64 ? 3 : 2) void kv_tile_kernel(Queries q, KvCache c, KvSeqs s, float scale, int causal,
+template <class C, int D, int W>
+__global__ __launch_bounds__(64 * W, D == 256 ? 1 : D == 64 ? 3 : 2) void kv_tile_kernel(Queries q, C c, KvSeqs s, float scale, int causal,
                                                                           Lists list, uint16_t* __restrict__ out, Partial part,
                                                                           Items items) {
     using T = TileShape<D, W>;
+    constexpr bool kFour = std::is_same_v<C, KvCache4>;
     constexpr int NT = D / 32;            // tiles of 32 elements of the output
     constexpr int KC = D / 8, VC = 8;     // 16-byte chunks of a row of K, of V
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     __shared__ int2 entry[T::kThreads + 3];  // (page, block) of the blocks at hand
-    __shared__ Factors fact[T::kThreads + 1];
+    __shared__ Factors fact[kFour ? 1 : T::kThreads + 1];
     __shared__ int wcount[W];
+    __shared__ int poison;  // kFour: a value's scale stands for no number
 
     int split, splits;
     const int item = items.of(blockIdx.x, part.splits, split, splits);
@@ -252,13 +371,21 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : D == 64 ? 3 : 2) void kv_til
     const int to = splits == 1 ? total : static_cast<int>(share * (split + 1) / of);
 
     // Bytes of a block into registers, and as bf16 into LDS: 8 of them a chunk.
-    uint4 kr[T::kLoads], vr[T::kLoads];
-    auto load = [&](const int8_t* from_pages, int page, uint4 (&to_regs)[T::kLoads]) __attribute__((always_inline)) {
-        const int8_t* const at = from_pages + (static_cast<int64_t>(page) * c.heads + h) * (kKvBlock * D);  // uniform
+    using Four = FourTile<D, W>;
+    std::conditional_t<kFour, typename Four::Keys, uint4[T::kLoads]> kr;
+    std::conditional_t<kFour, typename Four::Values, uint4[T::kLoads]> vr;
+    if (kFour && t == 0) poison = 0;  // (barriers follow before it is set)
+    auto load = [&](const auto* from_pages, int page, auto& to_regs) __attribute__((always_inline)) {
+        const int64_t tile_of = static_cast<int64_t>(page) * c.heads + h;  // uniform
+        if constexpr (kFour) {
+            to_regs.load(c, tile_of, t);
+        } else {
+            const int8_t* const at = from_pages + tile_of * (kKvBlock * D);
 #pragma unroll
-        for (int j = 0; j < T::kLoads; ++j) to_regs[j] = *reinterpret_cast<const uint4*>(at + static_cast<uint32_t>(t + j * T::kThreads) * 16);
+            for (int j = 0; j < T::kLoads; ++j) to_regs[j] = *reinterpret_cast<const uint4*>(at + static_cast<uint32_t>(t + j * T::kThreads) * 16);
+        }
     };
-    auto stage = [&](uint8_t* buf, const uint4 (&regs)[T::kLoads], auto chunks, auto swap) __attribute__((always_inline)) {
+    auto stage = [&](uint8_t* buf, const auto& regs, auto chunks, auto swap) __attribute__((always_inline)) {
         constexpr int CH = chunks;
 #pragma unroll
         for (int j = 0; j < T::kLoads; ++j) {
@@ -271,10 +398,12 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : D == 64 ? 3 : 2) void kv_til
         }
     };
     auto stage_k = [&](int which) __attribute__((always_inline)) {
-        stage(smem + (which & 1) * T::kKeyBytes, kr, std::integral_constant<int, KC>{}, std::true_type{});
+        if constexpr (kFour) kr.stage(smem + (which & 1) * T::kKeyBytes, t);
+        else stage(smem + (which & 1) * T::kKeyBytes, kr, std::integral_constant<int, KC>{}, std::true_type{});
     };
     auto stage_v = [&](int which) __attribute__((always_inline)) {
-        stage(smem + (2 + (which & 1)) * T::kKeyBytes, vr, std::integral_constant<int, VC>{}, std::false_type{});
+        if constexpr (kFour) vr.stage(smem + (2 + (which & 1)) * T::kKeyBytes, t, &poison);
+        else stage(smem + (2 + (which & 1)) * T::kKeyBytes, vr, std::integral_constant<int, VC>{}, std::false_type{});
     };
     auto arrive = [&]() __attribute__((always_inline)) {
         wait_lgkm0();
@@ -300,10 +429,11 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : D == 64 ? 3 : 2) void kv_til
             int at = __popcll(got & ((uint64_t{1} << lane) - 1));
             for (int w = 0; w < wave; ++w) at += wcount[w];
             if (page >= 0) {
-                const int64_t p = static_cast<int64_t>(page) * c.heads + h;
-                const Factors f = factors(c.ks[p], c.vs[p], scale * kLog2e);
                 entry[at] = make_int2(page, b);
-                fact[at] = f;
+                if constexpr (!kFour) {
+                    const int64_t p = static_cast<int64_t>(page) * c.heads + h;
+                    fact[at] = factors(c.ks[p], c.vs[p], scale * kLog2e);
+                }
             }
         }
         __syncthreads();
@@ -325,8 +455,9 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : D == 64 ? 3 : 2) void kv_til
         }
         // What a step needs to know of its blocks is read a step ahead: the pages that it loads, and its own block and factors.
         int page_k = uniform(entry[1 + behind].x), page_v = uniform(entry[behind].x), base = uniform(entry[0].y) * kKvBlock;
-        Factors f = fact[0];
-        f = {uniform(f.c), uniform(f.lv), uniform(f.iv), uniform(f.vs)};
+        // (4 bits: the same for all)
+        Factors f = kFour ? factors(1.0f, 1.0f, scale * kLog2e) : fact[0];
+        if constexpr (!kFour) f = {uniform(f.c), uniform(f.lv), uniform(f.iv), uniform(f.vs)};
         // Step y's halves.  The products take their operands from LDS kAhead MFMAs ahead.
         bf16x8 p[4];
         f32x16 sc[2];
@@ -337,7 +468,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : D == 64 ? 3 : 2) void kv_til
             // At 64 and 256 elements a row's chunk 2 k + half is found from chunk `half` by an XOR, opaque, so that the loop
             // does not keep a register for every k (256: 1200 rows over 9000 tokens 458 -> 434 us; 64, 500 rows: 23.7 -> 22.0;
             // at 128, where they fit, the XORs took 2000 rows from 137 to 142 us).
-            uint32_t kx = col * (D * 2) + chunk_at<KC>(col, half) * 16, vx = col * (kKvBlock * 2) + chunk_at<VC>(col, half) * 16;
+            uint32_t kx = col * (D * 2) + chunk_at<KC>(col, half) * 16, vx = kFour ? Four::value_at(col, half) : col * (kKvBlock * 2) + chunk_at<VC>(col, half) * 16;
             if constexpr (D != 128) asm("" : "+v"(kx), "+v"(vx));
             auto fetch = [&](int x) __attribute__((always_inline)) {
                 if (x < NK) {
@@ -346,6 +477,10 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : D == 64 ? 3 : 2) void kv_til
                     return frag(*reinterpret_cast<const uint4*>(kb + at));
                 }
                 const int d = (x - NK) % NT, w = (x - NK) / NT, row = d * 32 + col;
+                if constexpr (kFour) {
+                    const uint32_t at = D != 128 ? (vx ^ (w * 32)) + d * (32 * kKvBlock * 2) : Four::value_at(row, 2 * w + half);
+                    return frag(*reinterpret_cast<const uint4*>(vb + at));
+                }
                 const uint32_t at = D != 128 ? (vx ^ (w * 32)) + d * (32 * kKvBlock * 2) : row * (kKvBlock * 2) + chunk_at<VC>(row, 2 * w + half) * 16;
                 return frag(*reinterpret_cast<const uint4*>(vb + at));
             };
@@ -395,8 +530,8 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : D == 64 ? 3 : 2) void kv_til
 #pragma unroll
                     for (int r = 0; r < 16; ++r) o[d][r] *= fix;
             }
-            const float off = f.lv - m;
-            if (f.iv != 0.0f) {
+            const float off = kFour ? -m : f.lv - m;
+            if (kFour || f.iv != 0.0f) {
                 float sum = 0.0f;
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
@@ -408,7 +543,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : D == 64 ? 3 : 2) void kv_til
                     }
                     p[w] = pack(x);
                 }
-                l = __builtin_fmaf(sum, f.iv, l);
+                l = kFour ? l + sum : __builtin_fmaf(sum, f.iv, l);
             } else {
                 // a scale that is no ordinary number: what a row does not see must not reach it, and a NaN or an infinity
                 // must where a probability underflows
@@ -433,7 +568,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : D == 64 ? 3 : 2) void kv_til
             // (past the last block: whatever the arrays hold, which is then not used)
             const int2 after = entry[next_k + 1];
             const int block = entry[y + 1].y;
-            const Factors next = fact[y + 1];
+            const Factors next = kFour ? f : fact[y + 1];
             if (working) {
                 __builtin_amdgcn_s_setprio(1);
                 products(y, std::true_type{}, values);
@@ -446,13 +581,34 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : D == 64 ? 3 : 2) void kv_til
             page_v = page_k;
             page_k = uniform(after.x);
             base = uniform(block) * kKvBlock;
-            f = {uniform(next.c), uniform(next.lv), uniform(next.iv), uniform(next.vs)};
+            if constexpr (!kFour) f = {uniform(next.c), uniform(next.lv), uniform(next.iv), uniform(next.vs)};
             arrive();
         };
         step(0, std::false_type{});
         for (int y = 1; y < n; ++y) step(y, std::true_type{});
         if (working) products(n, std::false_type{}, std::true_type{});
         if (T::kGroups == 2 && !behind) arrive();
+    }
+
+    // 4 bits: the values of a token whose scale stands for no number went in as zeros; they make NaNs of their elements,
+    // 32 of the output, in the rows that see the token.  Its blocks are looked through again, in a launch that met one.
+    if constexpr (kFour) {
+        if (poison) {
+            for (int x = from; x < to; ++x) {
+                const int b = mine ? mine[x] : x;
+                const int page = b >= 0 && b < blocks ? s.page(i, b, c.pages) : -1;
+                if (page < 0) continue;
+                const uint8_t* const codes = c.vs + (static_cast<int64_t>(page) * c.heads + h) * (NT * kKvBlock);
+#pragma unroll
+                for (int d = 0; d < NT; ++d) {
+                    bool hit = false;
+#pragma unroll 1
+                    for (int x2 = 0; x2 < kKvBlock; ++x2) hit |= codes[d * kKvBlock + x2] >= kFourBad && b * kKvBlock + x2 <= last;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[d][r] = hit ? __builtin_nanf("") : o[d][r];
+                }
+            }
+        }
     }
 
     l += __shfl_xor(l, 32);
@@ -489,12 +645,127 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : D == 64 ? 3 : 2) void kv_til
 
 // ------------------------------------------------------------------ few queries
 
-typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
-
 // A load of what no other workgroup reads, past the caches: 537 MB of cache in 87 us against 99.
 __device__ __forceinline__ uint4 load_once(const int8_t* p) {
     return __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p)));
 }
+
+template <class T>
+__device__ __forceinline__ T load_past(const uint8_t* p) {
+    if constexpr (sizeof(T) == 16) return __builtin_bit_cast(T, __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p)));
+    else if constexpr (sizeof(T) == 8) return __builtin_bit_cast(T, __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p)));
+    else return __builtin_nontemporal_load(reinterpret_cast<const T*>(p));
+}
+
+// What a lane (column col, lanes 16 quad ..) loads of a block in 4 bits, and the operands that it makes of them.  Of the keys,
+// rows of the first product's MFMAs: token 4 col + u for MFMA set u, a quarter of each 128 elements (of 64), one scale each
+// (half of one).  Of the values: D / 16 neighbouring elements of 16 neighbouring tokens, whose pairs change places by a permute
+// each; MFMA e takes element e of each lane's.
+template <int D>
+struct FourFew {
+    static constexpr int G = D / kFourGroup;
+    static constexpr int kRun = D >= 128 ? 32 : 16;       // neighbouring elements of a key
+    static constexpr int kRuns = D / (4 * kRun);
+    static constexpr int kWords = kRun / 8;               // words of a run
+    static constexpr int kWide = D / 16;                  // neighbouring elements of a value
+    static constexpr int kBytes = kWide / 2;
+
+    // first of the 8 elements of first-product operand k
+    static __device__ __forceinline__ int element(int quad, int k) { return k / kWords * (4 * kRun) + quad * kRun + k % kWords * 8; }
+    // the element of register r of output tile e
+    static __device__ __forceinline__ int out_element(int quad, int r, int e) { return kWide * (4 * quad + r) + e; }
+
+    struct Keys {
+        uint32_t w[4][kRuns * kWords], codes[kRuns];  // codes: of the four tokens
+        __device__ __forceinline__ void load(const KvCache4& c, int64_t tile, int col, int quad) {
+            const uint8_t* const p = c.k + tile * (kKvBlock * D / 2);
+#pragma unroll
+            for (int n = 0; n < kRuns; ++n)
+                codes[n] = load_past<uint32_t>(c.ks + tile * (kKvBlock * G) + element(quad, n * kWords) / kFourGroup * kKvBlock + 4 * col);
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int n = 0; n < kRuns; ++n) {
+                    const uint8_t* const at = p + (4 * col + u) * (D / 2) + element(quad, n * kWords) / 2;
+                    if constexpr (kWords == 4) {
+                        const uint4 x = load_past<uint4>(at);
+                        w[u][4 * n] = x.x, w[u][4 * n + 1] = x.y, w[u][4 * n + 2] = x.z, w[u][4 * n + 3] = x.w;
+                    } else {
+                        const uint2 x = load_past<uint2>(at);
+                        w[u][2 * n] = x.x, w[u][2 * n + 1] = x.y;
+                    }
+                }
+        }
+        __device__ __forceinline__ bf16x8 operand(int u, int k) const {
+            const uint32_t code = codes[k / kWords] >> (8 * u) & 255;
+            // (a NaN of every element: a factor of 2^128 is none, whatever is not 0 times it)
+            const bool bad = code >= kFourBad;
+            return frag(four_bf16x8(w[u][k] | (bad ? 0x11111111u : 0u), four_scale(bad ? 255 : code)));
+        }
+    };
+
+    struct Values {
+        static constexpr int N = kBytes < 4 ? 1 : kBytes / 4;
+        uint32_t w[16][N];
+        uint4 codes;
+        __device__ __forceinline__ void load(const KvCache4& c, int64_t tile, int col, int quad) {
+            const uint8_t* const p = c.v + tile * (kKvBlock * D / 2) + 16 * quad * (D / 2) + col * kBytes;
+            codes = load_past<uint4>(c.vs + tile * (kKvBlock * G) + kWide * col / kFourGroup * kKvBlock + 16 * quad);
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+                if constexpr (kBytes == 2) {
+                    w[x][0] = load_past<uint16_t>(p + x * (D / 2));
+                } else if constexpr (kBytes == 4) {
+                    w[x][0] = load_past<uint32_t>(p + x * (D / 2));
+                } else {
+                    const uint2 y = load_past<uint2>(p + x * (D / 2));
+                    w[x][0] = y.x, w[x][N - 1] = y.y;
+                }
+            }
+        }
+        // Zeros for the values of tokens whose scale stands for no number; whether there are any.
+        __device__ __forceinline__ bool clean() {
+            uint32_t cw[4] = {codes.x, codes.y, codes.z, codes.w};
+            bool any = false;
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+                if (!four_bad(cw[y])) continue;
+                any = true;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    if ((cw[y] >> (8 * x) & 255) < kFourBad) continue;
+                    cw[y] &= ~(255u << (8 * x));
+#pragma unroll
+                    for (int n = 0; n < N; ++n) w[4 * y + x][n] = 0;
+                }
+            }
+            codes = make_uint4(cw[0], cw[1], cw[2], cw[3]);
+            return any;
+        }
+        // The second product's operands of elements 2 e and 2 e + 1 (a[0], a[1]) with each half of the tokens' probabilities:
+        // half h, register j has token 4 (j % 4) + 2 h + j / 4 of the lane's 16.
+        __device__ __forceinline__ void operands(int e, bf16x8 (&a)[2][2]) const {
+            const uint32_t cw[4] = {codes.x, codes.y, codes.z, codes.w};
+            uint32_t y[16];
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+                const float f = four_scale(cw[x / 4] >> (8 * (x % 4)) & 255);
+                const uint32_t v = w[x][e / 4];
+                y[x] = e % 4 == 0 ? four_bf16<0>(v, f) : e % 4 == 1 ? four_bf16<1>(v, f) : e % 4 == 2 ? four_bf16<2>(v, f) : four_bf16<3>(v, f);
+            }
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+                const uint32_t sel = z ? 0x07060302u : 0x05040100u;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int s = 2 * h;
+                    a[z][h] = frag(make_uint4(__builtin_amdgcn_perm(y[4 + s], y[s], sel), __builtin_amdgcn_perm(y[12 + s], y[8 + s], sel),
+                                              __builtin_amdgcn_perm(y[5 + s], y[1 + s], sel), __builtin_amdgcn_perm(y[13 + s], y[9 + s], sel)));
+                }
+            }
+        }
+    };
+};
 
 constexpr int kFew = 16;  // queries: the columns of a 16x16 MFMA
 constexpr int kFewWaves = 4;
@@ -517,9 +788,11 @@ struct Shares {
 // workgroup at a time, take 129; 16 sequences of 1 to 32768 tokens of 8 heads (780 MB) 128, where
 // shares of their own for each, a quarter of the longest, took 146.  Without shares (plan_of) a
 // workgroup reads a whole sequence, and the launch takes as long as the longest.
-template <int D, int NQ>
-__global__ __launch_bounds__(64 * kFewWaves) void kv_few_kernel(Queries q, KvCache c, KvSeqs s, float scale, int causal, Lists list,
+template <class C, int D, int NQ>
+__global__ __launch_bounds__(64 * kFewWaves) void kv_few_kernel(Queries q, C c, KvSeqs s, float scale, int causal, Lists list,
                                                                 uint16_t* __restrict__ out, Partial part, Shares shares) {
+    constexpr bool kFour = std::is_same_v<C, KvCache4>;
+    using Four = FourFew<D>;
     constexpr int KL = D / 64;   // 16-byte pieces of a key row a lane
     constexpr int NT = D / 16;   // tiles of 16 elements of the output
     __shared__ float jo[kFewWaves][kFew][D + 4];
@@ -609,7 +882,9 @@ __global__ __launch_bounds__(64 * kFewWaves) void kv_few_kernel(Queries q, KvCac
             const int64_t to_q = i * q.bs + static_cast<int64_t>(row) * q.ld + static_cast<int64_t>(hq) * D + quad * 16;
 #pragma unroll
             for (int k = 0; k < 2 * KL; ++k)
-                qf[g][k] = last[g] >= 0 ? query_frag(q.p + to_q + (k >> 1) * 64 + (k & 1) * 8, scale) : frag(make_uint4(0, 0, 0, 0));
+                qf[g][k] = last[g] < 0 ? frag(make_uint4(0, 0, 0, 0))
+                           : kFour     ? query_frag(q.p + to_q - quad * 16 + Four::element(quad, k), scale)
+                                       : query_frag(q.p + to_q + (k >> 1) * 64 + (k & 1) * 8, scale);
 #pragma unroll
             for (int n = 0; n < NT; ++n) o[g][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
             m[g] = kLowest, l[g] = 0.0f;
@@ -624,8 +899,14 @@ __global__ __launch_bounds__(64 * kFewWaves) void kv_few_kernel(Queries q, KvCac
             at = end;
         }
 
-        uint4 kr[4][KL], vr[NT];
+        std::conditional_t<kFour, typename Four::Keys, uint4[4][KL]> kr;
+        std::conditional_t<kFour, typename Four::Values, uint4[NT]> vr;
+        bool poison = false;  // kFour: a value's scale stands for no number
         auto load_k = [&](int page) {
+            if constexpr (kFour) {
+                kr.load(c, static_cast<int64_t>(page) * c.heads + h, col, quad);
+                return;
+            } else {
             const int8_t* const p = c.k + (static_cast<int64_t>(page) * c.heads + h) * (kKvBlock * D);
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
@@ -633,11 +914,16 @@ __global__ __launch_bounds__(64 * kFewWaves) void kv_few_kernel(Queries q, KvCac
 #pragma unroll
                 for (int k = 0; k < KL; ++k) kr[u][k] = load_once(p + tok * D + 64 * k + 16 * quad);
             }
+            }
         };
         auto load_v = [&](int page) {
+            if constexpr (kFour) {
+                vr.load(c, static_cast<int64_t>(page) * c.heads + h, col, quad);
+            } else {
             const int8_t* const p = c.v + (static_cast<int64_t>(page) * c.heads + h) * (kKvBlock * D);
 #pragma unroll
             for (int d = 0; d < NT; ++d) vr[d] = load_once(p + (16 * d + col) * kKvBlock + 16 * quad);
+            }
         };
 
         // a lane holds the page and the factors of one of the wave's next 64 blocks
@@ -648,7 +934,9 @@ __global__ __launch_bounds__(64 * kFewWaves) void kv_few_kernel(Queries q, KvCac
             uint64_t left = __ballot(page >= 0);
             if (!left) continue;
             Factors f = {};
-            if (page >= 0) {
+            if constexpr (kFour) {
+                f = factors(1.0f, 1.0f, scale * kLog2e);
+            } else if (page >= 0) {
                 const int64_t p = static_cast<int64_t>(page) * c.heads + h;
                 f = factors(c.ks[p], c.vs[p], scale * kLog2e);
             }
@@ -661,15 +949,23 @@ __global__ __launch_bounds__(64 * kFewWaves) void kv_few_kernel(Queries q, KvCac
                 const int z = left ? __builtin_ctzll(left) : y;
                 const int next = __builtin_amdgcn_readlane(page, z);
                 const int base = __builtin_amdgcn_readlane(b, y) * kKvBlock;
-                const float fc = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f.c), y));
-                const float flv = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f.lv), y));
-                const float fiv = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f.iv), y));
-                const float fvs = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f.vs), y));
+                const float fc = kFour ? f.c : __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f.c), y));
+                const float flv = kFour ? 0.0f : __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f.lv), y));
+                const float fiv = kFour ? 1.0f : __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f.iv), y));
+                const float fvs = kFour ? 1.0f : __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f.vs), y));
                 f32x4 sc[NQ][4];
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
 #pragma unroll
                     for (int g = 0; g < NQ; ++g) sc[g][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                    if constexpr (kFour) {
+#pragma unroll
+                        for (int k = 0; k < D / 32; ++k) {
+                            const bf16x8 a = kr.operand(u, k);
+#pragma unroll
+                            for (int g = 0; g < NQ; ++g) sc[g][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, qf[g][k], sc[g][u], 0, 0, 0);
+                        }
+                    } else
 #pragma unroll
                     for (int k = 0; k < KL; ++k) {
                         const uint4 w = kr[u][k];
@@ -682,7 +978,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void kv_few_kernel(Queries q, KvCac
                     }
                 }
                 if (left) load_k(next);
-                // register r of sc[g][u]: token base + 16 quad + 4 u + r
+                // register r of sc[g][u]: token base + 16 quad + 4 u + r (4 bits: 4 r + u)
                 const bool mask = base + kKvBlock > full;
                 bf16x8 p[NQ][2];
 #pragma unroll
@@ -692,7 +988,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void kv_few_kernel(Queries q, KvCac
                     for (int u = 0; u < 4; ++u)
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
-                            if (mask && base + 16 * quad + 4 * u + r > last[g]) sc[g][u][r] = -__builtin_inff();
+                            if (mask && base + 16 * quad + (kFour ? 4 * r + u : 4 * u + r) > last[g]) sc[g][u][r] = -__builtin_inff();
                             best = fmaxf(best, sc[g][u][r]);
                         }
                     best = fmaxf(best, __shfl_xor(best, 16));
@@ -713,8 +1009,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void kv_few_kernel(Queries q, KvCac
                             sc[g][u][r] = exp2_hw(__builtin_fmaf(sc[g][u][r], fc, off));
                             sum += sc[g][u][r];
                         }
-                    if (fiv != 0.0f) {
-                        l[g] = __builtin_fmaf(sum, fiv, l[g]);
+                    if (kFour || fiv != 0.0f) {
+                        l[g] = kFour ? l[g] + sum : __builtin_fmaf(sum, fiv, l[g]);
                     } else {
                         // a scale that is no ordinary number: what a row does not see must not reach it, and a NaN or an
                         // infinity must where a probability underflows
@@ -733,6 +1029,21 @@ __global__ __launch_bounds__(64 * kFewWaves) void kv_few_kernel(Queries q, KvCac
                         p[g][w] = frag(make_uint4(bf16x2_bits(a[0], a[1]), bf16x2_bits(a[2], a[3]), bf16x2_bits(e[0], e[1]), bf16x2_bits(e[2], e[3])));
                     }
                 }
+                if constexpr (kFour) {
+                    poison |= vr.clean();
+#pragma unroll
+                    for (int e = 0; e < NT / 2; ++e) {
+                        bf16x8 a[2][2];
+                        vr.operands(e, a);
+#pragma unroll
+                        for (int z = 0; z < 2; ++z)
+#pragma unroll
+                            for (int g = 0; g < NQ; ++g) {
+                                o[g][2 * e + z] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[z][0], p[g][0], o[g][2 * e + z], 0, 0, 0);
+                                o[g][2 * e + z] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[z][1], p[g][1], o[g][2 * e + z], 0, 0, 0);
+                            }
+                    }
+                } else
 #pragma unroll
                 for (int d = 0; d < NT; ++d) {
                     const bf16x8 lo = frag(ints_bf16(make_uint2(vr[d].x, vr[d].y))), hi = frag(ints_bf16(make_uint2(vr[d].z, vr[d].w)));
@@ -747,7 +1058,30 @@ __global__ __launch_bounds__(64 * kFewWaves) void kv_few_kernel(Queries q, KvCac
             }
         }
 
-        // register r of o[g][d]: element 16 d + 4 quad + r of query 16 g + col
+        // as in kv_tile_kernel: a wave that has met such a value looks through its blocks again
+        if constexpr (kFour) {
+            if (__any(poison)) {
+                for (int x = from + wave; x < to; x += kFewWaves) {
+                    const int b = mine ? mine[x] : x;
+                    const int page = b >= 0 && b < blocks ? s.page(i, b, c.pages) : -1;
+                    if (page < 0) continue;
+                    const uint8_t* const codes = c.vs + (static_cast<int64_t>(page) * c.heads + h) * (D / kFourGroup * kKvBlock);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        int first = 0x7FFFFFFF;  // token with such a scale of this register's elements
+#pragma unroll 1
+                        for (int x2 = kKvBlock - 1; x2 >= 0; --x2)
+                            if (codes[Four::out_element(quad, r, 0) / kFourGroup * kKvBlock + x2] >= kFourBad) first = b * kKvBlock + x2;
+#pragma unroll
+                        for (int g = 0; g < NQ; ++g)
+#pragma unroll
+                            for (int e = 0; e < NT; ++e) o[g][e][r] = first <= last[g] ? __builtin_nanf("") : o[g][e][r];
+                    }
+                }
+            }
+        }
+
+        // register r of o[g][d]: element 16 d + 4 quad + r of query 16 g + col (4 bits: out_element)
 #pragma unroll
         for (int g = 0; g < NQ; ++g) {
             if (g * kFew >= queries) break;
@@ -756,6 +1090,14 @@ __global__ __launch_bounds__(64 * kFewWaves) void kv_few_kernel(Queries q, KvCac
             const bool sees = last[g] >= 0;  // else padding, or a row that sees nothing: what the registers hold is no result
             if (g > 0 || again) __syncthreads();
             if (quad == 0) jml[wave][col] = make_float2(m[g], sees ? l[g] : 0.0f);
+            if constexpr (kFour) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int e = 0; e < NT; e += 4)
+                        *reinterpret_cast<float4*>(&jo[wave][col][Four::out_element(quad, r, e)]) =
+                            sees ? make_float4(o[g][e][r], o[g][e + 1][r], o[g][e + 2][r], o[g][e + 3][r]) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            } else
 #pragma unroll
             for (int d = 0; d < NT; ++d)
                 *reinterpret_cast<float4*>(&jo[wave][col][16 * d + 4 * quad]) =
@@ -1015,24 +1357,24 @@ extern "C" int64_t h3mi_kv_attention_workspace(int64_t n, int64_t rows, int64_t 
 
 namespace {
 
-template <int D, int W>
-int launch_tiles(const Items& items, const Queries& q, const KvCache& c, const KvSeqs& s, float scale, int causal, const Lists& list,
+template <class C, int D, int W>
+int launch_tiles(const Items& items, const Queries& q, const C& c, const KvSeqs& s, float scale, int causal, const Lists& list,
                  uint16_t* out, const Partial& part, hipStream_t stream) {
     int64_t groups;
     if (!launchable(items.whole + int64_t{8} * items.rest_chunk, 1, 1, 64 * W, &groups))
         return fail(H3MI_EINVAL, "kv_attention: too many rows for one call");
-    const auto fn = kv_tile_kernel<D, W>;
+    const auto fn = kv_tile_kernel<C, D, W>;
     constexpr int lds = TileShape<D, W>::kLds;
     hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(groups)), dim3(64 * W), lds, stream, q, c, s, scale, causal, list, out, part, items);
     return check_launch("kv_attention");
 }
 
-}  // namespace
-
-extern "C" int h3mi_kv_attention_bf16(const uint16_t* q, int64_t rows, int64_t heads, int64_t ld_q, int64_t bs_q,
-                                      const h3mi_kv_cache* cache, const h3mi_kv_seqs* seqs, float scale, int causal,
-                                      const int32_t* blocks, int64_t top, uint16_t* out, void* workspace,
-                                      int64_t workspace_bytes, void* stream) {
+// A call over a cache of 8 or of 4 bits.
+template <class Cache>
+int attention(const uint16_t* q, int64_t rows, int64_t heads, int64_t ld_q, int64_t bs_q, const Cache* cache, const h3mi_kv_seqs* seqs,
+              float scale, int causal, const int32_t* blocks, int64_t top, uint16_t* out, void* workspace, int64_t workspace_bytes,
+              void* stream) {
+    using C = decltype(kv_cache(*cache));
     if (int e = kv_check("kv_attention", cache, seqs)) return e;
     if (heads <= 0 || heads > 65536 || heads % cache->heads)
         return fail(H3MI_EINVAL, "kv_attention: heads=%lld must be a multiple of the cache's %lld", (long long)heads, (long long)cache->heads);
@@ -1069,7 +1411,7 @@ extern "C" int h3mi_kv_attention_bf16(const uint16_t* q, int64_t rows, int64_t h
                          p.pack == 1 ? 0u : static_cast<uint32_t>(((uint64_t{1} << 32) + p.pack - 1) / p.pack), static_cast<int>(p.items),
                          static_cast<int>(p.whole), static_cast<int>(p.whole / 8), static_cast<int>((rest + 7) / 8), p.flat, causal != 0};
     if (need > 0) part.ml = reinterpret_cast<float2*>(part.o + (part_rows - p.spans) * dim);
-    const KvCache c = kv_cache(*cache);
+    const C c = kv_cache(*cache);
     const KvSeqs s = kv_seqs(*seqs);
     const hipStream_t st = as_stream(stream);
     int rc;
@@ -1078,9 +1420,9 @@ extern "C" int h3mi_kv_attention_bf16(const uint16_t* q, int64_t rows, int64_t h
         const Shares shares = {p.shares, p.shares ? reinterpret_cast<int2*>(part.ml + part_rows - p.spans) : nullptr};
         if (!launchable(p.shares ? p.shares * p.heads : p.items, 1, 1, kFewThreads, &groups)) return fail(H3MI_EINVAL, "kv_attention: too many rows for one call");
         const int sets = static_cast<int>((p.rows + kFew - 1) / kFew);
-        const auto fn = dim == 64    ? (sets == 1 ? kv_few_kernel<64, 1> : sets == 2 ? kv_few_kernel<64, 2> : kv_few_kernel<64, 4>)
-                        : dim == 128 ? (sets == 1 ? kv_few_kernel<128, 1> : kv_few_kernel<128, 2>)
-                                     : kv_few_kernel<256, 1>;
+        const auto fn = dim == 64    ? (sets == 1 ? kv_few_kernel<C, 64, 1> : sets == 2 ? kv_few_kernel<C, 64, 2> : kv_few_kernel<C, 64, 4>)
+                        : dim == 128 ? (sets == 1 ? kv_few_kernel<C, 128, 1> : kv_few_kernel<C, 128, 2>)
+                                     : kv_few_kernel<C, 256, 1>;
         hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(groups)), dim3(kFewThreads), 0, st, qs, c, s, scale, causal, list, out, part,
                            shares);
         rc = check_launch("kv_attention");
@@ -1090,12 +1432,12 @@ extern "C" int h3mi_kv_attention_bf16(const uint16_t* q, int64_t rows, int64_t h
         hipLaunchKernelGGL(join, dim3(static_cast<unsigned>(groups)), dim3(256), 0, st, part, shares, qs, c.heads, out);
         return check_launch("kv_attention");
     } else if (dim == 64) {
-        rc = launch_tiles<64, 4>(items, qs, c, s, scale, causal, list, out, part, st);
+        rc = launch_tiles<C, 64, 4>(items, qs, c, s, scale, causal, list, out, part, st);
     } else if (dim == 128) {
-        rc = p.waves == 8 ? launch_tiles<128, 8>(items, qs, c, s, scale, causal, list, out, part, st)
-                          : launch_tiles<128, 4>(items, qs, c, s, scale, causal, list, out, part, st);
+        rc = p.waves == 8 ? launch_tiles<C, 128, 8>(items, qs, c, s, scale, causal, list, out, part, st)
+                          : launch_tiles<C, 128, 4>(items, qs, c, s, scale, causal, list, out, part, st);
     } else {
-        rc = launch_tiles<256, 4>(items, qs, c, s, scale, causal, list, out, part, st);
+        rc = launch_tiles<C, 256, 4>(items, qs, c, s, scale, causal, list, out, part, st);
     }
     if (rc || p.splits == 1) return rc;
     const int64_t all = (p.items - p.whole) * p.rows;
@@ -1108,4 +1450,20 @@ extern "C" int h3mi_kv_attention_bf16(const uint16_t* q, int64_t rows, int64_t h
     hipLaunchKernelGGL(join, dim3(static_cast<unsigned>(groups)), dim3(256), 0, st, part, qs, items,
                        static_cast<uint32_t>(all), out);
     return check_launch("kv_attention");
+}
+
+}  // namespace
+
+extern "C" int h3mi_kv_attention_bf16(const uint16_t* q, int64_t rows, int64_t heads, int64_t ld_q, int64_t bs_q,
+                                      const h3mi_kv_cache* cache, const h3mi_kv_seqs* seqs, float scale, int causal,
+                                      const int32_t* blocks, int64_t top, uint16_t* out, void* workspace,
+                                      int64_t workspace_bytes, void* stream) {
+    return attention(q, rows, heads, ld_q, bs_q, cache, seqs, scale, causal, blocks, top, out, workspace, workspace_bytes, stream);
+}
+
+extern "C" int h3mi_kv_attention_mx4_bf16(const uint16_t* q, int64_t rows, int64_t heads, int64_t ld_q, int64_t bs_q,
+                                          const h3mi_kv_cache4* cache, const h3mi_kv_seqs* seqs, float scale, int causal,
+                                          const int32_t* blocks, int64_t top, uint16_t* out, void* workspace,
+                                          int64_t workspace_bytes, void* stream) {
+    return attention(q, rows, heads, ld_q, bs_q, cache, seqs, scale, causal, blocks, top, out, workspace, workspace_bytes, stream);
 }

@@ -15,14 +15,29 @@
 
 namespace h3mi {
 
-int kv_check(const char* what, const h3mi_kv_cache* c, const h3mi_kv_seqs* s) {
-    if (!c || !s) return fail(H3MI_EINVAL, "%s: null cache or sequences", what);
-    if (c->dim != 64 && c->dim != 128 && c->dim != 256)
-        return fail(H3MI_EINVAL, "%s: dim=%lld must be 64, 128 or 256", what, (long long)c->dim);
-    if (c->heads <= 0 || c->heads > 65536 || c->pages < 0 || c->pages > 0x7FFFFFFF)
-        return fail(H3MI_EINVAL, "%s: bad cache sizes heads=%lld pages=%lld", what, (long long)c->heads, (long long)c->pages);
+namespace {
+
+int check_sizes(const char* what, int64_t pages, int64_t heads, int64_t dim, const h3mi_kv_seqs* s) {
+    if (dim != 64 && dim != 128 && dim != 256)
+        return fail(H3MI_EINVAL, "%s: dim=%lld must be 64, 128 or 256", what, (long long)dim);
+    if (heads <= 0 || heads > 65536 || pages < 0 || pages > 0x7FFFFFFF)
+        return fail(H3MI_EINVAL, "%s: bad cache sizes heads=%lld pages=%lld", what, (long long)heads, (long long)pages);
     if (s->n < 0 || s->n > 0x7FFFFFFF || s->blocks < 0 || s->blocks >= (int64_t{1} << 25))
         return fail(H3MI_EINVAL, "%s: bad sequences n=%lld blocks=%lld", what, (long long)s->n, (long long)s->blocks);
+    return H3MI_OK;
+}
+
+int check_seqs(const char* what, const h3mi_kv_seqs* s) {
+    if (!aligned(s->tables, 4) || !aligned(s->lens, 4) || !aligned(s->counts, 4))
+        return fail(H3MI_EALIGN, "%s: tables, lens and counts must be 4-byte aligned", what);
+    return H3MI_OK;
+}
+
+}  // namespace
+
+int kv_check(const char* what, const h3mi_kv_cache* c, const h3mi_kv_seqs* s) {
+    if (!c || !s) return fail(H3MI_EINVAL, "%s: null cache or sequences", what);
+    if (int e = check_sizes(what, c->pages, c->heads, c->dim, s)) return e;
     if (s->n == 0) return H3MI_OK;
     if (c->pages > 0 && (!c->k || !c->v || !c->k_scale || !c->v_scale || !c->k_sum))
         return fail(H3MI_EINVAL, "%s: null cache pointer", what);
@@ -31,9 +46,19 @@ int kv_check(const char* what, const h3mi_kv_cache* c, const h3mi_kv_seqs* s) {
         return fail(H3MI_EALIGN, "%s: the cache must be 16-byte aligned", what);
     const size_t bytes = static_cast<size_t>(c->pages) * c->heads * c->dim * kKvBlock;
     if (overlap(c->k, bytes, c->v, bytes)) return fail(H3MI_EALIAS, "%s: the cache's k and v overlap", what);
-    if (!aligned(s->tables, 4) || !aligned(s->lens, 4) || !aligned(s->counts, 4))
-        return fail(H3MI_EALIGN, "%s: tables, lens and counts must be 4-byte aligned", what);
-    return H3MI_OK;
+    return check_seqs(what, s);
+}
+
+int kv_check(const char* what, const h3mi_kv_cache4* c, const h3mi_kv_seqs* s) {
+    if (!c || !s) return fail(H3MI_EINVAL, "%s: null cache or sequences", what);
+    if (int e = check_sizes(what, c->pages, c->heads, c->dim, s)) return e;
+    if (s->n == 0) return H3MI_OK;
+    if (c->pages > 0 && (!c->k || !c->v || !c->k_scale || !c->v_scale)) return fail(H3MI_EINVAL, "%s: null cache pointer", what);
+    if (!s->lens || (s->blocks > 0 && !s->tables)) return fail(H3MI_EINVAL, "%s: null tables or lens", what);
+    if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->k_scale, 16) || !aligned(c->v_scale, 16))
+        return fail(H3MI_EALIGN, "%s: the cache must be 16-byte aligned", what);
+    if (kv_self_overlaps(*c)) return fail(H3MI_EALIAS, "%s: the cache's tensors overlap", what);
+    return check_seqs(what, s);
 }
 
 int kv_check_rows(const char* what, const char* name, const uint16_t* p, int64_t rows, int64_t heads, int64_t dim,
@@ -60,30 +85,44 @@ struct Span {
     size_t bytes;
 };
 
-// The cache's keys, values, scales and sums.
+// A cache's tensors.
 struct Spans {
     Span s[5];
-    explicit Spans(const h3mi_kv_cache& c) {
+    int count;
+    explicit Spans(const h3mi_kv_cache& c) : count(5) {
         const size_t tiles = static_cast<size_t>(c.pages) * c.heads, kv = tiles * c.dim * kKvBlock;
         s[0] = {c.k, kv}, s[1] = {c.v, kv}, s[2] = {c.k_scale, 4 * tiles}, s[3] = {c.v_scale, 4 * tiles}, s[4] = {c.k_sum, 2 * tiles * c.dim};
+    }
+    explicit Spans(const h3mi_kv_cache4& c) : count(4) {
+        const size_t all = static_cast<size_t>(c.pages) * c.heads * c.dim * kKvBlock;
+        s[0] = {c.k, all / 2}, s[1] = {c.v, all / 2}, s[2] = {c.k_scale, all / kFourGroup}, s[3] = {c.v_scale, all / kFourGroup};
+    }
+    bool meet(const void* p, size_t bytes) const {
+        for (int x = 0; x < count; ++x)
+            if (overlap(p, bytes, s[x].p, s[x].bytes)) return true;
+        return false;
+    }
+    bool meet_each_other() const {
+        for (int x = 1; x < count; ++x)
+            for (int y = 0; y < x; ++y)
+                if (overlap(s[x].p, s[x].bytes, s[y].p, s[y].bytes)) return true;
+        return false;
+    }
+    bool meet(const h3mi_kv_seqs& q) const {
+        for (int x = 0; x < count; ++x)
+            if (kv_seqs_overlap(s[x].p, s[x].bytes, q)) return true;
+        return false;
     }
 };
 
 }  // namespace
 
-bool kv_overlaps(const void* out, size_t bytes, const h3mi_kv_cache& c) {
-    for (const Span& x : Spans(c).s)
-        if (overlap(out, bytes, x.p, x.bytes)) return true;
-    return false;
-}
-
-bool kv_self_overlaps(const h3mi_kv_cache& c) {
-    const Spans all(c);
-    for (int x = 1; x < 5; ++x)
-        for (int y = 0; y < x; ++y)
-            if (overlap(all.s[x].p, all.s[x].bytes, all.s[y].p, all.s[y].bytes)) return true;
-    return false;
-}
+bool kv_overlaps(const void* p, size_t bytes, const h3mi_kv_cache& c) { return Spans(c).meet(p, bytes); }
+bool kv_overlaps(const void* p, size_t bytes, const h3mi_kv_cache4& c) { return Spans(c).meet(p, bytes); }
+bool kv_self_overlaps(const h3mi_kv_cache& c) { return Spans(c).meet_each_other(); }
+bool kv_self_overlaps(const h3mi_kv_cache4& c) { return Spans(c).meet_each_other(); }
+bool kv_seqs_overlap(const h3mi_kv_cache& c, const h3mi_kv_seqs& s) { return Spans(c).meet(s); }
+bool kv_seqs_overlap(const h3mi_kv_cache4& c, const h3mi_kv_seqs& s) { return Spans(c).meet(s); }
 
 bool kv_seqs_overlap(const void* p, size_t bytes, const h3mi_kv_seqs& s) {
     const size_t each = 4 * static_cast<size_t>(s.n);
@@ -92,33 +131,9 @@ bool kv_seqs_overlap(const void* p, size_t bytes, const h3mi_kv_seqs& s) {
 
 namespace {
 
-constexpr int64_t kMemoryCache = int64_t{256} << 20;  // bytes that the memory-side cache holds
-
 // Words of a head's transposed block in LDS: 16 words of 4 tokens a row, one row's
 // words off the next's banks.
 constexpr int kVtStride = 17;
-
-typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
-typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
-
-__device__ __forceinline__ void store_past(void* p, uint4 v) {
-    __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v), static_cast<u32x4*>(p));
-}
-__device__ __forceinline__ void store_past(void* p, uint2 v) {
-    __builtin_nontemporal_store(__builtin_bit_cast(u32x2, v), static_cast<u32x2*>(p));
-}
-
-template <bool STREAM>
-__device__ __forceinline__ uint4 load_row(const uint16_t* p) {
-    if constexpr (STREAM) return __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p)));
-    return *reinterpret_cast<const uint4*>(p);
-}
-
-// The larger of packed 16-bit magnitudes (bit patterns of |bf16|, so a NaN wins).
-__device__ __forceinline__ uint32_t max_mag(uint32_t a, uint32_t b) {
-    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
-    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
-}
 
 // A block's new scale and what becomes of its old values: old ints times mul, 0 if it is 0.
 struct Scale {
@@ -167,11 +182,6 @@ __device__ __forceinline__ void transpose4(const uint2 (&t)[4], uint32_t (&w)[8]
         w[4 * p + 3] = __builtin_amdgcn_perm(cd1, ab1, 0x07060302u);
     }
 }
-
-struct Rows {
-    const uint16_t* p;
-    int64_t ld, bs;
-};
 
 // One workgroup: one of the blocks that a sequence's new tokens touch, one head.  2 D threads.
 // STREAM: the rows are loaded past the caches as well (a clip of 19200 tokens 150 us against
@@ -385,8 +395,7 @@ extern "C" int h3mi_kv_write_i8(const uint16_t* k, const uint16_t* v, int64_t ro
         if (kv_overlaps(x ? v : k, bytes, *cache)) return fail(H3MI_EALIAS, "kv_write: the rows overlap the cache");
     }
     if (kv_self_overlaps(*cache)) return fail(H3MI_EALIAS, "kv_write: the cache's tensors overlap");
-    for (const Span& x : Spans(*cache).s)
-        if (kv_seqs_overlap(x.p, x.bytes, *seqs)) return fail(H3MI_EALIAS, "kv_write: tables, lens or counts overlap the cache");
+    if (kv_seqs_overlap(*cache, *seqs)) return fail(H3MI_EALIAS, "kv_write: tables, lens or counts overlap the cache");
     const bool stream_in = seqs->n * rows * cache->heads * D * 4 > kMemoryCache;
     const auto fn = stream_in ? (D == 64 ? kv_write_kernel<64, true> : D == 128 ? kv_write_kernel<128, true> : kv_write_kernel<256, true>)
                               : (D == 64 ? kv_write_kernel<64, false> : D == 128 ? kv_write_kernel<128, false> : kv_write_kernel<256, false>);

@@ -35,12 +35,17 @@ class KvCacheC(ctypes.Structure):
     _fields_ = [("k", _P), ("v", _P), ("k_scale", _P), ("v_scale", _P), ("k_sum", _P), ("pages", _I), ("heads", _I), ("dim", _I)]
 
 
+class KvCache4C(ctypes.Structure):
+    """h3mi_kv_cache4"""
+    _fields_ = [("k", _P), ("v", _P), ("k_scale", _P), ("v_scale", _P), ("pages", _I), ("heads", _I), ("dim", _I)]
+
+
 class KvSeqsC(ctypes.Structure):
     """h3mi_kv_seqs"""
     _fields_ = [("tables", _P), ("lens", _P), ("counts", _P), ("n", _I), ("blocks", _I)]
 
 
-_KC, _KS = ctypes.POINTER(KvCacheC), ctypes.POINTER(KvSeqsC)
+_KC, _KC4, _KS = ctypes.POINTER(KvCacheC), ctypes.POINTER(KvCache4C), ctypes.POINTER(KvSeqsC)
 
 # name -> argtypes (restype int unless listed in _RESTYPE)
 SIGNATURES = {
@@ -68,6 +73,9 @@ SIGNATURES = {
     "h3mi_kv_select": [_P, _I, _I, _I, _I, _KC, _KS, _I, _C, _P, _P, _I, _P],
     "h3mi_kv_attention_workspace": [_I, _I, _I, _I, _I, _I, _I],
     "h3mi_kv_attention_bf16": [_P, _I, _I, _I, _I, _KC, _KS, _F, _C, _P, _I, _P, _P, _I, _P],
+    "h3mi_kv_write_mx4": [_P, _P, _I, _I, _I, _I, _I, _KC4, _KS, _P],
+    "h3mi_kv_read_mx4_bf16": [_P, _P, _P, _I, _KC4, _KS, _P],
+    "h3mi_kv_attention_mx4_bf16": [_P, _I, _I, _I, _I, _KC4, _KS, _F, _C, _P, _I, _P, _P, _I, _P],
     "h3mi_norm_order_info": [_C, ctypes.POINTER(_C), ctypes.POINTER(_C), ctypes.POINTER(_C)],
     "h3mi_debug_rsqrt_f32": [_P, _P, _I, _C, _P],
     "h3mi_debug_bf16_rne": [_P, _P, _I, _P],

@@ -1,17 +1,17 @@
-"""Keys and values held in 8 bits, and attention over them (HIP, gfx950).
+"""Keys and values held in 8 or in 4 bits, and attention over them (HIP, gfx950).
 
 No counterpart in the reference, which computes its attention in the host program
 (comfyui_nodes/minimax-h3-sp/minimax_sp/sp_forward.py:276-318).  Keys and values
 that outlive a call (the finished chunks' of a long clip, the tokens before a step's,
 a prompt's or reference frames' whose own rows attend to nothing that changes) stay in
-a KVCache, at half of bf16's size.  Rows of one bidirectional sequence change with
+a KVCache, at half of bf16's size, or in a KVCache4, at 17/64 of it.  Rows of one bidirectional sequence change with
 every denoising step, its text rows among them: their keys are written anew for each.
 
-  kv_cache(pages, heads, dim)                          an empty pool of pages of 64 tokens
+  kv_cache(pages, heads, dim, bits=8)                  an empty pool of pages of 64 tokens
   kv_write_(cache, k, v, tables, lens)                 quantize new tokens into it
   kv_read(cache, tables, lens, length)                 tokens back as bf16
   kv_attention(q, cache, tables, lens, causal)         attention over all of it
-  kv_select(q, cache, tables, lens, top, causal)       the blocks worth attending to,
+  kv_select(q, cache, tables, lens, top, causal)       the blocks worth attending to (8 bits),
   kv_attention(..., blocks=...)                        and attention over those alone
 
 tables int32 [n, blocks] gives the page of each block of 64 tokens of n sequences and
@@ -30,10 +30,11 @@ import typing
 import torch
 from torch.autograd import forward_ad
 
-from ._lib import KvCacheC, KvSeqsC, _fast, check, lib, ptr, same_gpu, stream_of
+from ._lib import KvCache4C, KvCacheC, KvSeqsC, _fast, check, lib, ptr, same_gpu, stream_of
 
-KV_BLOCK = 64   # tokens of a block, one scale per block and head, and of a page
+KV_BLOCK = 64   # tokens of a block, and of a page; in 8 bits one scale per block and head
 KV_TILE = 128   # query rows that share a selection
+KV_GROUP = 32   # elements of a token that share a scale in 4 bits
 
 
 class KVCache(typing.NamedTuple):
@@ -45,10 +46,24 @@ class KVCache(typing.NamedTuple):
     k_sum: torch.Tensor    # int16 [pages, heads, dim]: sum of the block's 8-bit keys
 
 
-def kv_cache(pages, heads, dim, device="cuda"):
-    """An empty KVCache (zeros)."""
+class KVCache4(typing.NamedTuple):
+    """A pool of pages in 4 bits: a sign and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6, times a power of two for every 32
+    elements of a token."""
+    k: torch.Tensor        # uint8 [pages, heads, 64, dim / 2]: element 2 j in the low half of byte j
+    v: torch.Tensor        # uint8 [pages, heads, 64, dim / 2]
+    k_scale: torch.Tensor  # uint8 [pages, heads, dim / 32, 64]: e + 127 of 2^e; 253 and more: not a number
+    v_scale: torch.Tensor  # uint8 [pages, heads, dim / 32, 64]
+
+
+def kv_cache(pages, heads, dim, device="cuda", bits=8):
+    """An empty KVCache (bits=8) or KVCache4 (bits=4): zeros."""
     if dim not in (64, 128, 256):
         raise ValueError("dim must be 64, 128 or 256")
+    if bits not in (4, 8):
+        raise ValueError("bits must be 8 or 4")
+    if bits == 4:
+        values, scales = ((pages, heads, KV_BLOCK, dim // 2), (pages, heads, dim // KV_GROUP, KV_BLOCK))
+        return KVCache4(*(torch.zeros(shape, dtype=torch.uint8, device=device) for shape in (values, values, scales, scales)))
     z = lambda *s, t: torch.zeros(*s, dtype=t, device=device)  # noqa: E731
     return KVCache(z(pages, heads, KV_BLOCK, dim, t=torch.int8), z(pages, heads, dim, KV_BLOCK, t=torch.int8),
                    z(pages, heads, t=torch.float32), z(pages, heads, t=torch.float32), z(pages, heads, dim, t=torch.int16))
@@ -59,7 +74,26 @@ def kv_cache(pages, heads, dim, device="cuda"):
 # other form.
 
 
+def _cache4(c):
+    k = c.k
+    if k.dim() != 4 or k.shape[2] != KV_BLOCK or k.dtype != torch.uint8:
+        raise ValueError(f"cache.k must be uint8 [pages, heads, {KV_BLOCK}, dim / 2]")
+    pages, heads, _, half = k.shape
+    dim = 2 * half
+    for name, shape in (("v", (pages, heads, KV_BLOCK, half)), ("k_scale", (pages, heads, dim // KV_GROUP, KV_BLOCK)),
+                        ("v_scale", (pages, heads, dim // KV_GROUP, KV_BLOCK))):
+        t = getattr(c, name)
+        if t.shape != shape or t.dtype != torch.uint8:
+            raise ValueError(f"cache.{name} must be {torch.uint8} {list(shape)}")
+    if not all(t.is_contiguous() for t in c):
+        raise ValueError("the cache's tensors must be contiguous")
+    same_gpu(k, **{name: t for name, t in zip(c._fields[1:], c[1:])})
+    return KvCache4C(*(t.data_ptr() for t in c), pages, heads, dim)
+
+
 def _cache(c):
+    if isinstance(c, KVCache4):
+        return _cache4(c)
     k = c.k
     if k.dim() != 4 or k.shape[2] != KV_BLOCK or k.dtype != torch.int8:
         raise ValueError(f"cache.k must be int8 [pages, heads, {KV_BLOCK}, dim]")
@@ -96,8 +130,9 @@ def _rows(t, c, n, name, heads=None):
     if t.dtype != torch.bfloat16 or t.dim() != 4:
         raise ValueError(f"{name} must be bfloat16 [n, rows, heads, dim]")
     _, rows, h, d = t.shape
-    if t.shape[0] != n or d != c.k.shape[3] or (heads is not None and h != heads):
-        raise ValueError(f"{name} must be [{n}, rows, {'heads' if heads is None else heads}, {c.k.shape[3]}]")
+    dim = c.k.shape[3] * (2 if isinstance(c, KVCache4) else 1)
+    if t.shape[0] != n or d != dim or (heads is not None and h != heads):
+        raise ValueError(f"{name} must be [{n}, rows, {'heads' if heads is None else heads}, {dim}]")
     if t.numel() and (t.stride(3) != 1 or (h > 1 and t.stride(2) != d)):
         raise ValueError(f"{name}: heads must be contiguous (strides [*, *, dim, 1])")
     same_gpu(c.k, **{name: t})
@@ -106,18 +141,23 @@ def _rows(t, c, n, name, heads=None):
 
 def _no_grad(*ts):
     if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
-        raise RuntimeError("attention over an 8-bit cache has no gradient: call it under torch.no_grad()")
+        raise RuntimeError("a cache of 8 or 4 bits has no gradient: call it under torch.no_grad()")
     if any(forward_ad.unpack_dual(t).tangent is not None for t in ts):
-        raise RuntimeError("attention over an 8-bit cache has no forward-mode gradient: call it with the primal tensors")
+        raise RuntimeError("a cache of 8 or 4 bits has no forward-mode gradient: call it with the primal tensors")
 
 
 def kv_write_(cache, k, v, tables, lens, counts=None):
     """Quantizes k and v, the last counts[i] tokens of each sequence, into the cache's pages; returns the cache.
 
-    A block's scale is max|x| / 127 of its first write.  A later write of tokens that do not fit doubles it as often
+    8 bits: a block's scale is max|x| / 127 of its first write.  A later write of tokens that do not fit doubles it as often
     as they need and halves the block's older 8-bit values as often, so that an error stays within one step.  A NaN or
     an infinity makes its block read back as NaN until the block's first token is written again.  The pages that a call
-    writes have to be distinct."""
+    writes have to be distinct.
+
+    4 bits: every 32 elements of a token have a power of two of their own, the least with which they fit, and are off by
+    half a step at most (a sixteenth of the largest of them, a seventh of it where that lies just above 5 steps): nothing
+    written before changes.  A NaN or an infinity makes its 32 elements read back as NaN.  The tokens that a call writes
+    have to be distinct."""
     done = _fast.kv_write_(cache, k, v, tables, lens, counts)
     if done is not None:
         return done
@@ -129,7 +169,8 @@ def kv_write_(cache, k, v, tables, lens, counts=None):
     if rv != rows:
         raise ValueError("k and v must have the same number of rows")
     with torch.cuda.device(k.device):
-        check(lib.h3mi_kv_write_i8(ptr(k), ptr(v), rows, ldk, bsk, ldv, bsv, ctypes.byref(c), ctypes.byref(s), stream_of(k)))
+        write = lib.h3mi_kv_write_mx4 if isinstance(cache, KVCache4) else lib.h3mi_kv_write_i8
+        check(write(ptr(k), ptr(v), rows, ldk, bsk, ldv, bsv, ctypes.byref(c), ctypes.byref(s), stream_of(k)))
     return cache
 
 
@@ -148,7 +189,8 @@ def kv_read(cache, tables, lens, length, starts=None):
     k = torch.empty((s.n, length, c.heads, c.dim), dtype=torch.bfloat16, device=cache.k.device)
     v = torch.empty_like(k)
     with torch.cuda.device(k.device):
-        check(lib.h3mi_kv_read_bf16(ptr(k), ptr(v), ptr(starts), length, ctypes.byref(c), ctypes.byref(s), stream_of(k)))
+        read = lib.h3mi_kv_read_mx4_bf16 if isinstance(cache, KVCache4) else lib.h3mi_kv_read_bf16
+        check(read(ptr(k), ptr(v), ptr(starts), length, ctypes.byref(c), ctypes.byref(s), stream_of(k)))
     return k, v
 
 
@@ -164,6 +206,8 @@ def kv_select(q, cache, tables, lens, top, causal=False, counts=None):
     if out is not None:
         return out
     _no_grad(q)
+    if isinstance(cache, KVCache4):
+        raise ValueError("kv_select takes an 8-bit cache: one of 4 bits holds no sums of its blocks' keys")
     c = _cache(cache)
     s = _seqs(cache, tables, lens, counts)
     rows, ld, bs = _rows(q, cache, s.n, "q")
@@ -201,7 +245,7 @@ def kv_attention(q, cache, tables, lens, causal=False, counts=None, scale=None, 
     with torch.cuda.device(q.device):
         need = lib.h3mi_kv_attention_workspace(s.n, rows, heads, c.heads, c.dim, s.blocks, top)
         work = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
-        check(lib.h3mi_kv_attention_bf16(ptr(q), rows, heads, ld, bs, ctypes.byref(c), ctypes.byref(s),
-                                         float(c.dim ** -0.5 if scale is None else scale), int(bool(causal)), ptr(blocks), top,
-                                         ptr(out), ptr(work), max(need, 0), stream_of(q)))
+        attend = lib.h3mi_kv_attention_mx4_bf16 if isinstance(cache, KVCache4) else lib.h3mi_kv_attention_bf16
+        check(attend(ptr(q), rows, heads, ld, bs, ctypes.byref(c), ctypes.byref(s), float(c.dim ** -0.5 if scale is None else scale),
+                     int(bool(causal)), ptr(blocks), top, ptr(out), ptr(work), max(need, 0), stream_of(q)))
     return out
