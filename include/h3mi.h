@@ -355,6 +355,56 @@ int h3mi_kv_attention_mx4_bf16(const uint16_t* q, int64_t rows, int64_t heads, i
                                const int32_t* blocks, int64_t top, uint16_t* out, void* workspace,
                                int64_t workspace_bytes, void* stream);
 
+/* Free pages: a stack, free[0 .. count - 1], taken from its end. */
+typedef struct h3mi_kv_pool {
+    int32_t* free;   /* [pages], at most 2^30 */
+    int32_t* count;  /* [1]; taken as 0 .. pages */
+    int64_t pages;
+} h3mi_kv_pool;
+
+/* Room for counts[i] (NULL: rows; taken as 0 .. rows) more tokens of each sequence:
+ *   held = ceil(lens[i] / 64), want = ceil((lens[i] + counts[i]) / 64) - held (0 where the
+ *   table has not so many blocks), upto = the sum of want up to sequence i
+ *   granted[i] = counts[i] where the table has the blocks and want = 0 or upto <= count, else 0
+ * A sequence that is granted takes pages off the stack for its blocks held, held + 1, ..,
+ * sequence by sequence, and lens[i] grows by its counts; of others nothing changes (a
+ * length below 0 becomes 0).  So sequences are served in order until one is not; from
+ * there on those that need no page.  count falls by what was taken.
+ * positions int32 [n, rows]: lens[i] before + r where r < granted[i], else -1;
+ * slots int64 [n, rows]: 64 page + position % 64, -1 where there is no such row or its
+ * page is none of the pool's.  n * rows < 2^31.  Calls on one pool run in order: on one
+ * stream, or on several that wait for each other.  No two of the tensors may overlap. */
+int h3mi_kv_extend(const h3mi_kv_pool* pool, int32_t* tables, int32_t* lens, const int32_t* counts, int64_t n,
+                   int64_t blocks, int64_t rows, int32_t* granted, int32_t* positions, int64_t* slots,
+                   void* stream);
+
+/* Drops tokens: sequence i keeps its first keep[i] (NULL: none; taken as 0 .. lens[i]).
+ * The pages of blocks wholly behind go back onto the stack, in the order of sequences,
+ * then blocks; their table entries become -1 and lens[i] becomes what was kept.  Entries
+ * that are no page of the pool are passed over, and pages past a full stack dropped. */
+int h3mi_kv_release(const h3mi_kv_pool* pool, int32_t* tables, int32_t* lens, const int32_t* keep, int64_t n,
+                    int64_t blocks, void* stream);
+
+/* Rows of [n, rows, heads, dim] bf16, heads contiguous, strides in elements. */
+typedef struct h3mi_rope_rows {
+    const uint16_t* in;
+    uint16_t* out;   /* in place: in, with the same strides */
+    int64_t heads, ld_in, bs_in, ld_out, bs_out;
+} h3mi_rope_rows;
+
+/* Rotary positions.  Of each head's first rot elements the pairs (a, b), (i, i + rot / 2)
+ * or (2 i, 2 i + 1) if interleaved, become bf16(a c - b s), bf16(a s + b c) with
+ * c = amplitude cos(p w), s = amplitude sin(p w) (inverse: -s), p = positions[n, rows]
+ * and w = freqs[i] radians (fp64 [rot / 2]); p w is formed and reduced in 64 bits, sine,
+ * cosine, products and sums in 32.  The rest of a head is left as it is (copied to out),
+ * and so are rows with p < 0.  inverse is the transpose: what a gradient goes through.
+ * k NULL: none.  dim a multiple of 8 up to 512, rot even, 2 to dim; pointers 16-byte
+ * aligned, strides multiples of 8 and no shorter than a row.  q and k may be views of
+ * one buffer whose rows do not overlap, but not of what else the call reads or writes. */
+int h3mi_rope_bf16(const h3mi_rope_rows* q, const h3mi_rope_rows* k, const int32_t* positions, const double* freqs,
+                   int64_t n, int64_t rows, int64_t dim, int64_t rot, int interleaved, int inverse, float amplitude,
+                   void* stream);
+
 /* (numx, vec, warp) of an order; returns H3MI_EINVAL for an unknown order. */
 int h3mi_norm_order_info(int order, int* numx, int* vec, int* warp);
 

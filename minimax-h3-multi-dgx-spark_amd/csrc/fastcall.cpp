@@ -573,6 +573,144 @@ PyObject* kv_attention(PyObject*, PyObject* const* v, Py_ssize_t n) {
     H3MI_END
 }
 
+// A KVPool, tables and lens.
+struct Pool {
+    h3mi_kv_pool p = {};
+    int32_t *tables = nullptr, *lens = nullptr;
+    int64_t n = 0, blocks = 0;
+    Pool(Args& a, PyObject* pool, PyObject* to, PyObject* lo) {
+        a.ok = a.ok && PyTuple_Check(pool) && PyTuple_GET_SIZE(pool) == 2;
+        if (!a.ok) return;
+        const at::Tensor* t = a.typed(to, c10::kInt);
+        if (!a.ok || t->dim() != 2 || !t->is_contiguous() || a.dev.index() != c10::hip::current_device()) {
+            a.ok = false;
+            return;
+        }
+        n = t->size(0), blocks = t->size(1);
+        const at::Tensor* free = a.typed(PyTuple_GET_ITEM(pool, 0), c10::kInt);
+        if (a.ok && (free->dim() != 1 || !free->is_contiguous())) a.ok = false;
+        const at::Tensor* count = Kv::shaped(a, PyTuple_GET_ITEM(pool, 1), c10::kInt, {1});
+        const at::Tensor* l = Kv::shaped(a, lo, c10::kInt, {n});
+        if (!a.ok) return;
+        p = {i32(free), i32(count), free->numel()};
+        tables = i32(t), lens = i32(l);
+    }
+    static int32_t* i32(const at::Tensor* t) { return static_cast<int32_t*>(t->data_ptr()); }
+};
+
+// (pool, tables, lens, rows, counts) -> (granted, positions, slots)
+PyObject* kv_extend_(PyObject*, PyObject* const* v, Py_ssize_t n) {
+    H3MI_BEGIN
+    H3MI_ARGS(5)
+    Args a;
+    const Pool p(a, v[0], v[1], v[2]);
+    int64_t rows = 0;
+    if (!a.ok || !whole(v[3], &rows) || rows < 1) Py_RETURN_NONE;
+    const at::Tensor* counts = v[4] == Py_None ? nullptr : Kv::shaped(a, v[4], c10::kInt, {p.n});
+    if (!a.ok) Py_RETURN_NONE;
+    at::Tensor granted, positions, slots;
+    int rc;
+    {
+        pybind11::gil_scoped_release nogil;
+        granted = a.empty({p.n}, c10::kInt);
+        positions = a.empty({p.n, rows}, c10::kInt);
+        slots = a.empty({p.n, rows}, c10::kLong);
+        rc = h3mi_kv_extend(&p.p, p.tables, p.lens, counts ? Kv::i32(counts) : nullptr, p.n, p.blocks, rows, Pool::i32(&granted),
+                            Pool::i32(&positions), static_cast<int64_t*>(slots.data_ptr()), a.stream());
+    }
+    if (rc) return raise_status(rc);
+    PyObject *x = THPVariable_Wrap(granted), *y = x ? THPVariable_Wrap(positions) : nullptr, *z = y ? THPVariable_Wrap(slots) : nullptr;
+    PyObject* r = z ? PyTuple_Pack(3, x, y, z) : nullptr;
+    Py_XDECREF(x);
+    Py_XDECREF(y);
+    Py_XDECREF(z);
+    return r;
+    H3MI_END
+}
+
+// (pool, tables, lens, keep) -> pool
+PyObject* kv_release_(PyObject*, PyObject* const* v, Py_ssize_t n) {
+    H3MI_BEGIN
+    H3MI_ARGS(4)
+    Args a;
+    const Pool p(a, v[0], v[1], v[2]);
+    if (!a.ok) Py_RETURN_NONE;
+    const at::Tensor* keep = v[3] == Py_None ? nullptr : Kv::shaped(a, v[3], c10::kInt, {p.n});
+    if (!a.ok) Py_RETURN_NONE;
+    int rc;
+    {
+        pybind11::gil_scoped_release nogil;
+        rc = h3mi_kv_release(&p.p, p.tables, p.lens, keep ? Kv::i32(keep) : nullptr, p.n, p.blocks, a.stream());
+    }
+    if (rc) return raise_status(rc);
+    Py_INCREF(v[0]);
+    return v[0];
+    H3MI_END
+}
+
+// [n, rows, heads, dim] that are turned, with contiguous heads, that no gradient is wanted of
+struct Turned {
+    const at::Tensor* t = nullptr;
+    h3mi_rope_rows x = {};
+    Turned(Args& a, PyObject* o, int64_t n, int64_t rows, int64_t dim) {
+        if (a.ok) t = a.typed(o, c10::kBFloat16);
+        if (!a.ok) return;
+        if (t->dim() != 4 || t->size(0) != n || t->size(1) != rows || (dim && t->size(3) != dim) || t->stride(3) != 1 ||
+            (t->size(2) > 1 && t->stride(2) != t->size(3)) || (t->requires_grad() && c10::GradMode::is_enabled()) || t->_fw_grad(0).defined()) {
+            a.ok = false;
+            return;
+        }
+        const int64_t e = t->size(2) * t->size(3);
+        x = {u16(t), mu16(*t), t->size(2), rows > 1 ? t->stride(1) : e, n > 1 ? t->stride(0) : rows * e, 0, 0};
+        x.ld_out = x.ld_in, x.bs_out = x.bs_in;
+    }
+    at::Tensor fresh(const Args& a) {
+        const at::Tensor o = a.empty(t->sizes(), c10::kBFloat16);
+        x.out = mu16(o), x.ld_out = t->size(2) * t->size(3), x.bs_out = t->size(1) * x.ld_out;
+        return o;
+    }
+};
+
+// (q, k, positions, freqs, interleaved, inverse, amplitude, in place) -> (q, k)
+PyObject* rope(PyObject*, PyObject* const* v, Py_ssize_t n) {
+    H3MI_BEGIN
+    H3MI_ARGS(8)
+    Args a;
+    const at::Tensor* pos = a.typed(v[2], c10::kInt);
+    const at::Tensor* freqs = a.typed(v[3], c10::kDouble);
+    int interleaved = 0, inverse = 0;
+    double amplitude = 0.0;
+    if (!a.ok || pos->dim() != 2 || !pos->is_contiguous() || freqs->dim() != 1 || !freqs->is_contiguous() ||
+        a.dev.index() != c10::hip::current_device() || !truth(v[4], &interleaved) || !truth(v[5], &inverse) || !number(v[6], &amplitude))
+        Py_RETURN_NONE;
+    const int64_t N = pos->size(0), rows = pos->size(1);
+    Turned q(a, v[0], N, rows, 0);
+    if (!a.ok) Py_RETURN_NONE;
+    const bool two = v[1] != Py_None, in_place = v[7] == Py_True;
+    const int64_t dim = q.t->size(3);
+    Turned k = two ? Turned(a, v[1], N, rows, dim) : q;
+    if (!a.ok) Py_RETURN_NONE;
+    at::Tensor qo, ko;
+    int rc;
+    {
+        pybind11::gil_scoped_release nogil;
+        if (!in_place) {
+            qo = q.fresh(a);
+            if (two) ko = k.fresh(a);
+        }
+        rc = h3mi_rope_bf16(&q.x, two ? &k.x : nullptr, Kv::i32(pos), static_cast<const double*>(freqs->data_ptr()), N, rows, dim,
+                            2 * freqs->numel(), interleaved, inverse, static_cast<float>(amplitude), a.stream());
+    }
+    if (rc) return raise_status(rc);
+    if (in_place) return PyTuple_Pack(2, v[0], v[1]);
+    if (two) return pair(qo, ko);
+    PyObject* x = THPVariable_Wrap(qo);
+    PyObject* r = x ? PyTuple_Pack(2, x, Py_None) : nullptr;
+    Py_XDECREF(x);
+    return r;
+    H3MI_END
+}
+
 // (set,): set False forgets the last GEMM's shape; returns it, or None
 PyObject* last_shape(PyObject*, PyObject* const* v, Py_ssize_t n) {
     H3MI_ARGS(1)
@@ -595,6 +733,7 @@ PyMethodDef kMethods[] = {
     H3MI_FN("norm_mod", &norm_any<false>), H3MI_FN("gate_norm_mod_", &norm_any<true>), H3MI_FN("gate_", &gate_),
     H3MI_FN("rms_rope_", &rms_rope_), H3MI_FN("last_shape", &last_shape), H3MI_FN("kv_write_", &kv_write_),
     H3MI_FN("kv_read", &kv_read), H3MI_FN("kv_select", &kv_select), H3MI_FN("kv_attention", &kv_attention),
+    H3MI_FN("kv_extend_", &kv_extend_), H3MI_FN("kv_release_", &kv_release_), H3MI_FN("rope", &rope),
     {"set_error", set_error, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_fast", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

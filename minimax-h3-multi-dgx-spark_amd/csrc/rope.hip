@@ -1,0 +1,274 @@
+// Rotary positions: pairs (a, b) of a head's first `rot` elements become, with w = freqs[pair],
+//   (a c - b s, a s + b c),  c = amplitude cos(p w), s = amplitude sin(p w)   (inverse: s negated)
+// for a row at position p.  The transpose of that matrix, which a gradient is multiplied by, is
+// the inverse.  Pairs are (i, i + rot / 2), or (2 i, 2 i + 1) where they are interleaved.
+//
+// p w is formed in turns in 64 bits and reduced there, as p has up to 31 bits and a bf16 result
+// wants the angle to a few thousandths whatever p is; what is left, half a turn at most, goes
+// through fp32 sine and cosine.  Products and sums are fp32, and a result is rounded once.
+//
+// It moves 4 bytes a turned element and does 3 operations with it, so HBM bounds it, and the
+// sines, one for each row and pair whatever the heads, are formed once for a workgroup's share of
+// the row's heads and kept in LDS.  A workgroup takes a few whole rows, or where there are few
+// rows a share of one's heads.  A thread takes 8 pairs of a head (4 interleaved ones): 16-byte
+// accesses whose lanes lie side by side.
+#include "common.h"
+
+namespace h3mi {
+namespace {
+
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+
+struct RopeRows {
+    const uint16_t* in;
+    uint16_t* out;
+    int heads;
+    int64_t ld_in, bs_in, ld_out, bs_out;
+};
+
+struct RopeCall {
+    RopeRows q, k;  // k.heads 0: none
+    const int32_t* positions;
+    const double* freqs;
+    uint32_t rows, all;   // of a sequence; of all
+    int dim, rot, tokens; // tokens: rows of a workgroup
+    int parts;            // workgroups of such rows
+    int turned, units;    // units of a head: turned ones, and with those that are copied (at most 256)
+    float amplitude, sign;
+    bool in_place;
+};
+
+constexpr int kRopeThreads = 256;
+constexpr int kRopeAhead = 4;   // units that a thread has in flight
+constexpr int kRopeTokens = 16;
+
+enum RopeForm { kHalves, kPairs, kOne };
+
+// What a thread holds of a unit: 8 elements and their partners 8 chunks on (kHalves), 8 elements (kPairs), two (kOne).
+template <RopeForm F>
+struct Unit {
+    uint4 a, b;
+};
+
+__device__ __forceinline__ void turn(float x, float y, float2 cs, float& u, float& v) {
+    u = __builtin_fmaf(x, cs.x, -(y * cs.y));
+    v = __builtin_fmaf(x, cs.y, y * cs.x);
+}
+
+// tab: (c, s) of the unit's first pair
+template <RopeForm F>
+__device__ __forceinline__ void turn(Unit<F>& x, const float2* tab) {
+    if constexpr (F == kHalves) {
+        uint32_t* const a = &x.a.x;
+        uint32_t* const b = &x.b.x;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float u0, v0, u1, v1;
+            turn(bf16_lo(a[j]), bf16_lo(b[j]), tab[2 * j], u0, v0);
+            turn(bf16_hi(a[j]), bf16_hi(b[j]), tab[2 * j + 1], u1, v1);
+            a[j] = bf16x2_bits(u0, u1);
+            b[j] = bf16x2_bits(v0, v1);
+        }
+    } else if constexpr (F == kPairs) {
+        uint32_t* const a = &x.a.x;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float u, v;
+            turn(bf16_lo(a[j]), bf16_hi(a[j]), tab[j], u, v);
+            a[j] = bf16x2_bits(u, v);
+        }
+    } else {
+        float u, v;
+        turn(bf16_f32(x.a.x), bf16_f32(x.b.x), tab[0], u, v);
+        x.a.x = bf16_bits(u);
+        x.b.x = bf16_bits(v);
+    }
+}
+
+template <RopeForm F>
+__global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeCall c, int interleaved) {
+    extern __shared__ float2 tab[];  // [tokens, rot / 2]: (c, s)
+    __shared__ bool real[kRopeTokens];  // rows that a position was given for
+    const int half = c.rot / 2, t = threadIdx.x;
+    const uint32_t first = blockIdx.x / c.parts * c.tokens, left = c.all - first;
+    const int part = blockIdx.x % c.parts, tokens = left < static_cast<uint32_t>(c.tokens) ? static_cast<int>(left) : c.tokens;
+    if (t < tokens) real[t] = c.positions[first + t] >= 0;
+    for (int x = t; x < tokens * half; x += kRopeThreads) {
+        const int tok = x / half, i = x - tok * half, p = c.positions[first + tok];
+        float2 cs = make_float2(1.0f, 0.0f);
+        if (p >= 0) {
+            constexpr double kTurn = 0.15915494309189533577;  // 1 / (2 pi)
+            double a = p * (c.freqs[i] * kTurn);
+            a -= __builtin_rint(a);
+            float s, o;
+            sincospif(2.0f * static_cast<float>(a), &s, &o);
+            cs = make_float2(o * c.amplitude, s * c.sign);
+        }
+        tab[x] = cs;
+    }
+    __syncthreads();
+
+    // (row, head) pairs of the workgroup's share, kRopeThreads / units at a time
+    const int heads = c.q.heads + c.k.heads, share = (heads + c.parts - 1) / c.parts;
+    const int h0 = part * share, h1 = h0 + share < heads ? h0 + share : heads, mine = h1 - h0;
+    if (mine <= 0) return;
+    const int lanes = kRopeThreads / c.units, unit = t % c.units, lane = t / c.units;
+    if (lane >= lanes) return;
+    const bool turned = unit < c.turned;
+    // elements of the unit: a at `at`, b at `at + apart`
+    int at, apart = 0;
+    if (turned) {
+        at = F == kOne ? (interleaved ? 2 * unit : unit) : 8 * unit;
+        apart = F == kPairs ? 0 : F == kOne && interleaved ? 1 : half;
+    } else {
+        at = F == kOne ? c.rot + 2 * (unit - c.turned) : c.rot + 8 * (unit - c.turned) * (F == kHalves ? 2 : 1);
+        apart = F == kOne ? 1 : 8;
+    }
+    // (the last copied unit of kHalves may have 8 elements alone)
+    const bool two = F == kOne || (F == kHalves && at + apart < c.dim);
+    for (int x0 = lane; x0 < tokens * mine; x0 += lanes * kRopeAhead) {
+        Unit<F> y[kRopeAhead];
+        uint16_t* to[kRopeAhead];
+        int tok[kRopeAhead];
+#pragma unroll
+        for (int j = 0; j < kRopeAhead; ++j) {
+            const int x = x0 + j * lanes;
+            to[j] = nullptr;
+            if (x >= tokens * mine) continue;
+            tok[j] = x / mine;
+            const int h = h0 + x - tok[j] * mine;
+            const uint32_t row = first + tok[j], i = row / c.rows, r = row - i * c.rows;
+            if (c.in_place && !real[tok[j]]) continue;
+            const bool of_q = h < c.q.heads;
+            const RopeRows& z = of_q ? c.q : c.k;
+            const int64_t el = static_cast<int64_t>(of_q ? h : h - c.q.heads) * c.dim + at;
+            const uint16_t* const from = z.in + i * z.bs_in + r * z.ld_in + el;
+            to[j] = z.out + i * z.bs_out + r * z.ld_out + el;
+            if (!(turned && real[tok[j]])) tok[j] = -1;
+            if constexpr (F == kOne) {
+                y[j].a.x = from[0];
+                y[j].b.x = from[apart];
+            } else {
+                y[j].a = *reinterpret_cast<const uint4*>(from);
+                if (two) y[j].b = *reinterpret_cast<const uint4*>(from + apart);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kRopeAhead; ++j) {
+            if (!to[j]) continue;
+            if (tok[j] >= 0) turn<F>(y[j], tab + tok[j] * half + unit * (F == kHalves ? 8 : F == kPairs ? 4 : 1));
+            if constexpr (F == kOne) {
+                to[j][0] = static_cast<uint16_t>(y[j].a.x);
+                to[j][apart] = static_cast<uint16_t>(y[j].b.x);
+            } else {
+                *reinterpret_cast<uint4*>(to[j]) = y[j].a;
+                if (two) *reinterpret_cast<uint4*>(to[j] + apart) = y[j].b;
+            }
+        }
+    }
+}
+
+size_t span_of(const h3mi_rope_rows& x, bool out, int64_t n, int64_t rows, int64_t dim) {
+    const int64_t ld = out ? x.ld_out : x.ld_in, bs = out ? x.bs_out : x.bs_in;
+    return 2 * (static_cast<size_t>(n - 1) * bs + static_cast<size_t>(rows - 1) * ld + static_cast<size_t>(x.heads) * dim);
+}
+
+int check_rows(const char* name, const h3mi_rope_rows& x, int64_t n, int64_t rows, int64_t dim) {
+    const int64_t e = x.heads * dim;
+    if (!x.in || !x.out) return fail(H3MI_EINVAL, "rope: null %s", name);
+    if (x.heads <= 0 || x.heads > 65536) return fail(H3MI_EINVAL, "rope: %s has %lld heads", name, (long long)x.heads);
+    for (int64_t ld : {x.ld_in, x.ld_out})
+        if (rows > 1 && ld < e) return fail(H3MI_EINVAL, "rope: %s strides are shorter than a row", name);
+    for (int64_t bs : {x.bs_in, x.bs_out})
+        if (n > 1 && bs < e) return fail(H3MI_EINVAL, "rope: %s strides are shorter than a row", name);
+    if (!aligned(x.in, 16) || !aligned(x.out, 16) || (rows > 1 && (x.ld_in % 8 || x.ld_out % 8)) || (n > 1 && (x.bs_in % 8 || x.bs_out % 8)))
+        return fail(H3MI_EALIGN, "rope: %s must be 16-byte aligned with strides that are multiples of 8", name);
+    // rows that overlap would be turned twice
+    if (n > 1 && rows > 1 && x.bs_out < (rows - 1) * x.ld_out + e && x.ld_out < (n - 1) * x.bs_out + e)
+        return fail(H3MI_EALIAS, "rope: rows of %s overlap", name);
+    if (x.in == x.out && ((rows > 1 && x.ld_in != x.ld_out) || (n > 1 && x.bs_in != x.bs_out)))
+        return fail(H3MI_EALIAS, "rope: %s in place with other strides", name);
+    if (x.in != x.out && overlap(x.in, span_of(x, false, n, rows, dim), x.out, span_of(x, true, n, rows, dim)))
+        return fail(H3MI_EALIAS, "rope: %s overlaps its result", name);
+    return H3MI_OK;
+}
+
+// Whether rows of a and b share an element.  Rows of equal strides, as views of one projection's output, may lie between
+// each other's.
+bool rows_meet(const uint16_t* a, int64_t ha, int64_t lda, int64_t bsa, const uint16_t* b, int64_t hb, int64_t ldb, int64_t bsb,
+               int64_t n, int64_t rows, int64_t dim) {
+    const h3mi_rope_rows x = {a, nullptr, ha, lda, bsa, 0, 0}, y = {b, nullptr, hb, ldb, bsb, 0, 0};
+    if (!overlap(a, span_of(x, false, n, rows, dim), b, span_of(y, false, n, rows, dim))) return false;
+    if ((rows > 1 && lda != ldb) || (n > 1 && bsa != bsb) || (rows == 1 && n == 1)) return true;
+    const int64_t step = rows == 1 ? bsa : n == 1 || lda < bsa ? lda : bsa;
+    if (n > 1 && rows > 1 && (lda < bsa ? bsa : lda) % step) return true;
+    int64_t d = (reinterpret_cast<intptr_t>(b) - reinterpret_cast<intptr_t>(a)) / 2 % step;
+    if (d < 0) d += step;
+    return d < ha * dim || d + hb * dim > step;
+}
+
+}  // namespace
+}  // namespace h3mi
+
+using namespace h3mi;
+
+extern "C" int h3mi_rope_bf16(const h3mi_rope_rows* q, const h3mi_rope_rows* k, const int32_t* positions, const double* freqs,
+                              int64_t n, int64_t rows, int64_t dim, int64_t rot, int interleaved, int inverse, float amplitude,
+                              void* stream) {
+    if (!q) return fail(H3MI_EINVAL, "rope: null q");
+    if (dim < 8 || dim > 512 || dim % 8) return fail(H3MI_EINVAL, "rope: dim=%lld must be a multiple of 8 up to 512", (long long)dim);
+    if (rot < 2 || rot > dim || rot % 2) return fail(H3MI_EINVAL, "rope: rot=%lld must be even, 2 to dim", (long long)rot);
+    if (n < 0 || rows < 0 || n > 0x7FFFFFFF || rows > 0x7FFFFFFF || n * rows > 0x7FFFFFFF)
+        return fail(H3MI_EINVAL, "rope: bad sizes n=%lld rows=%lld", (long long)n, (long long)rows);
+    if (!(amplitude - amplitude == 0.0f)) return fail(H3MI_EINVAL, "rope: amplitude is not finite");
+    if (n == 0 || rows == 0) return ok();
+    if (!positions || !freqs) return fail(H3MI_EINVAL, "rope: null positions or freqs");
+    if (!aligned(positions, 4) || !aligned(freqs, 8)) return fail(H3MI_EALIGN, "rope: positions must be 4-byte aligned, freqs 8-byte");
+    if (int e = check_rows("q", *q, n, rows, dim)) return e;
+    if (k)
+        if (int e = check_rows("k", *k, n, rows, dim)) return e;
+    const size_t pos_bytes = 4 * static_cast<size_t>(n) * rows, freq_bytes = 4 * static_cast<size_t>(rot);
+    for (const h3mi_rope_rows* x : {q, k}) {
+        if (!x) continue;
+        if (overlap(x->out, span_of(*x, true, n, rows, dim), positions, pos_bytes) || overlap(x->out, span_of(*x, true, n, rows, dim), freqs, freq_bytes))
+            return fail(H3MI_EALIAS, "rope: a result overlaps positions or freqs");
+    }
+    if (k && (rows_meet(q->out, q->heads, q->ld_out, q->bs_out, k->out, k->heads, k->ld_out, k->bs_out, n, rows, dim) ||
+              (k->in != k->out && rows_meet(q->out, q->heads, q->ld_out, q->bs_out, k->in, k->heads, k->ld_in, k->bs_in, n, rows, dim)) ||
+              (q->in != q->out && rows_meet(k->out, k->heads, k->ld_out, k->bs_out, q->in, q->heads, q->ld_in, q->bs_in, n, rows, dim))))
+        return fail(H3MI_EALIAS, "rope: q and k overlap");
+    if (k && (k->in == k->out) != (q->in == q->out)) return fail(H3MI_EINVAL, "rope: q and k must both be in place, or neither");
+
+    const RopeForm form = interleaved ? (rot % 8 ? kOne : kPairs) : (rot % 16 ? kOne : kHalves);
+    RopeCall c = {};
+    const auto side = [](const h3mi_rope_rows& x) { return RopeRows{x.in, x.out, static_cast<int>(x.heads), x.ld_in, x.bs_in, x.ld_out, x.bs_out}; };
+    c.q = side(*q);
+    if (k) c.k = side(*k);
+    c.positions = positions, c.freqs = freqs;
+    c.rows = static_cast<uint32_t>(rows), c.all = static_cast<uint32_t>(n * rows);
+    c.dim = static_cast<int>(dim), c.rot = static_cast<int>(rot);
+    c.amplitude = amplitude, c.sign = inverse ? -amplitude : amplitude;
+    c.in_place = q->in == q->out;
+    c.turned = static_cast<int>(form == kHalves ? rot / 16 : form == kPairs ? rot / 8 : rot / 2);
+    const int64_t rest = c.in_place ? 0 : dim - rot;
+    c.units = c.turned + static_cast<int>(form == kHalves ? (rest + 15) / 16 : form == kPairs ? rest / 8 : rest / 2);
+    // Rows until a thread has kRopeAhead units, as far as there are workgroups for every CU; else a share of a row's heads.
+    const int64_t heads = q->heads + (k ? k->heads : 0), a_round = kRopeThreads / c.units, want = a_round * kRopeAhead, cus = cu_count();
+    int64_t tokens = want / heads;
+    if (tokens > c.all / (4 * cus)) tokens = c.all / (4 * cus);
+    if (tokens > kRopeTokens) tokens = kRopeTokens;
+    if (tokens < 1) tokens = 1;
+    int64_t parts = 1;
+    if (tokens == 1) {
+        parts = 4 * cus / c.all;
+        if (parts > (heads + a_round - 1) / a_round) parts = (heads + a_round - 1) / a_round;
+        if (parts < (heads + 4 * want - 1) / (4 * want)) parts = (heads + 4 * want - 1) / (4 * want);
+    }
+    c.tokens = static_cast<int>(tokens), c.parts = static_cast<int>(parts);
+    const int64_t groups = (c.all + tokens - 1) / tokens * parts;
+    if (groups * kRopeThreads >= (int64_t{1} << 32)) return fail(H3MI_EINVAL, "rope: too many rows for one call");
+    const size_t lds = static_cast<size_t>(tokens) * (rot / 2) * 8;
+    const auto fn = form == kHalves ? rope_kernel<kHalves> : form == kPairs ? rope_kernel<kPairs> : rope_kernel<kOne>;
+    hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(groups)), dim3(kRopeThreads), lds, as_stream(stream), c, interleaved != 0);
+    return check_launch("rope");
+}

@@ -45,6 +45,17 @@ class KvSeqsC(ctypes.Structure):
     _fields_ = [("tables", _P), ("lens", _P), ("counts", _P), ("n", _I), ("blocks", _I)]
 
 
+class KvPoolC(ctypes.Structure):
+    """h3mi_kv_pool"""
+    _fields_ = [("free", _P), ("count", _P), ("pages", _I)]
+
+
+class RopeRowsC(ctypes.Structure):
+    """h3mi_rope_rows"""
+    _fields_ = [("in_", _P), ("out", _P), ("heads", _I), ("ld_in", _I), ("bs_in", _I), ("ld_out", _I), ("bs_out", _I)]
+
+
+_KP, _RR = ctypes.POINTER(KvPoolC), ctypes.POINTER(RopeRowsC)
 _KC, _KC4, _KS = ctypes.POINTER(KvCacheC), ctypes.POINTER(KvCache4C), ctypes.POINTER(KvSeqsC)
 
 # name -> argtypes (restype int unless listed in _RESTYPE)
@@ -76,6 +87,9 @@ SIGNATURES = {
     "h3mi_kv_write_mx4": [_P, _P, _I, _I, _I, _I, _I, _KC4, _KS, _P],
     "h3mi_kv_read_mx4_bf16": [_P, _P, _P, _I, _KC4, _KS, _P],
     "h3mi_kv_attention_mx4_bf16": [_P, _I, _I, _I, _I, _KC4, _KS, _F, _C, _P, _I, _P, _P, _I, _P],
+    "h3mi_kv_extend": [_KP, _P, _P, _P, _I, _I, _I, _P, _P, _P, _P],
+    "h3mi_kv_release": [_KP, _P, _P, _P, _I, _I, _P],
+    "h3mi_rope_bf16": [_RR, _RR, _P, _P, _I, _I, _I, _I, _C, _C, _F, _P],
     "h3mi_norm_order_info": [_C, ctypes.POINTER(_C), ctypes.POINTER(_C), ctypes.POINTER(_C)],
     "h3mi_debug_rsqrt_f32": [_P, _P, _I, _C, _P],
     "h3mi_debug_bf16_rne": [_P, _P, _I, _P],

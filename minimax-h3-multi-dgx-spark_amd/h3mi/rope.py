@@ -1,6 +1,7 @@
-"""q/k RMSNorm + split-half rotary embedding (HIP, gfx950), in place.
+"""q/k RMSNorm + split-half rotary embedding, in place, and rotary positions of any
+layout from the positions themselves (HIP, gfx950).
 
-Stands in for comfy-kitchen's ck.rms_rope_split_half_ / rms_rope_split_half as
+rms_rope_split_half_ stands in for comfy-kitchen's ck.rms_rope_split_half_ / rms_rope_split_half as
 the reference calls them on the attention's q and k
 (comfyui_nodes/minimax-h3-sp/minimax_sp/sp_forward.py:279-296): q, k
 [1, s, heads, dim] views of the qkv projection, rope_freqs from
@@ -8,10 +9,19 @@ rope_rotation_table (:548) with rot_dim = rope_freqs.shape[-3] * 2.  Each
 (token, head) row becomes the eager F.rms_norm of the row followed by the
 split-half rotation: the pair (y[i], y[i + rot/2]) times the token's 2 x 2
 table entry i, in fp32, rounded to bf16.
-"""
-import torch
 
-from ._lib import RSQRT_HW, RSQRT_RN, _fast, check, lib, ptr, same_gpu, stream_of
+rope_ and rope have no counterpart in the reference, whose tables come from the host
+program: they take the tokens' positions, as kv_extend_ gives them, and the pairs'
+frequencies (rope_frequencies), turn split halves or interleaved pairs of all or a
+part of each head, and turn back.
+"""
+import ctypes
+import math
+
+import torch
+from torch.autograd import forward_ad
+
+from ._lib import RSQRT_HW, RSQRT_RN, RopeRowsC, _fast, check, lib, ptr, same_gpu, stream_of
 
 _MODES = {"hw": RSQRT_HW, "rn": RSQRT_RN}
 
@@ -69,3 +79,93 @@ def rms_rope_split_half(q, k, rope_freqs, qw, kw, epsilon=1e-6, rot_dim=None, rs
     qo = q.contiguous().clone()
     ko = k.contiguous().clone()
     return rms_rope_split_half_(qo, ko, rope_freqs, qw, kw, epsilon, rot_dim, rsqrt)
+
+
+def rope_frequencies(rot_dim, base=10000.0, scaling=None, factor=1.0, window=8192, device="cuda"):
+    """(freqs fp64 [rot_dim / 2], amplitude) for rope_ and rope: base ** (-2 i / rot_dim) radians a token, and 1.
+
+    scaling, for contexts of `factor` (>= 1) times the `window` tokens that the frequencies were made for:
+      "linear"  positions count for 1 / factor: all frequencies are divided by it
+      "ntk"     the base grows by factor ** (rot_dim / (rot_dim - 2)): the slowest pair is divided by factor, the fastest stays
+      "yarn"    pairs that turn less than once in the window are divided by factor, those that turn 32 times and more stay,
+                and those between go from one to the other with their number (rounded outward to whole ones); the amplitude
+                is 1 + 0.1 ln factor (Peng et al., 2023)"""
+    rot_dim, base, factor = int(rot_dim), float(base), float(factor)
+    if rot_dim < 2 or rot_dim % 2:
+        raise ValueError("rot_dim must be even and at least 2")
+    if not (base > 1.0 and math.isfinite(base)) or not (factor >= 1.0 and math.isfinite(factor)) or not window > 0:
+        raise ValueError("base must be above 1, factor at least 1 and window above 0")
+    if scaling not in (None, "linear", "ntk", "yarn"):
+        raise ValueError("scaling must be None, 'linear', 'ntk' or 'yarn'")
+    if scaling == "ntk" and rot_dim > 2:
+        base *= factor ** (rot_dim / (rot_dim - 2))
+    i = torch.arange(rot_dim // 2, dtype=torch.float64)
+    f, amplitude = base ** (-2.0 * i / rot_dim), 1.0
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "yarn" and factor > 1.0:
+        def at(turns):  # the pair, as a real number, that turns so often in the window
+            return rot_dim * math.log(window / (2 * math.pi * turns)) / (2 * math.log(base))
+        lo, hi = max(math.floor(at(32.0)), 0), min(math.ceil(at(1.0)), rot_dim - 1)
+        keep = 1 - ((i - lo) / max(hi - lo, 0.001)).clamp(0, 1)
+        f, amplitude = f * (keep + (1 - keep) / factor), 1 + 0.1 * math.log(factor)
+    return f.to(device), amplitude
+
+
+def _turned(x, positions, dim, name):
+    """(rows, heads, token stride, sequence stride) of [n, rows, heads, dim]."""
+    if x.dtype != torch.bfloat16 or x.dim() != 4:
+        raise ValueError(f"{name} must be bfloat16 [n, rows, heads, dim]")
+    if tuple(x.shape[:2]) != tuple(positions.shape) or x.shape[3] != dim:
+        raise ValueError(f"{name} must be [{positions.shape[0]}, {positions.shape[1]}, heads, {dim}]")
+    n, rows, h, d = x.shape
+    if x.numel() and (x.stride(3) != 1 or (h > 1 and x.stride(2) != d)):
+        raise ValueError(f"{name}: heads must be contiguous (strides [*, *, dim, 1])")
+    if torch.is_grad_enabled() and x.requires_grad:
+        raise RuntimeError("rope records no gradient: call it under torch.no_grad() (a gradient is turned by rope with inverse=True)")
+    if forward_ad.unpack_dual(x).tangent is not None:
+        raise RuntimeError("rope has no forward-mode gradient: call it with the primal tensors")
+    return h, x.stride(1) if rows > 1 else h * d, x.stride(0) if n > 1 else rows * h * d
+
+
+def _rope(q, k, positions, freqs, interleaved, inverse, amplitude, in_place):
+    if positions.dim() != 2 or positions.dtype != torch.int32 or not positions.is_contiguous():
+        raise ValueError("positions must be contiguous int32 [n, rows]")
+    if freqs.dim() != 1 or freqs.dtype != torch.float64 or not freqs.is_contiguous():
+        raise ValueError("freqs must be contiguous float64 [rot / 2]")
+    if q.dim() != 4:
+        raise ValueError("q must be bfloat16 [n, rows, heads, dim]")
+    (n, rows), dim, outs, sides = positions.shape, q.shape[3], [], []
+    for x, name in ((q, "q"), (k, "k")):
+        if x is None:
+            outs.append(None), sides.append(None)
+            continue
+        h, ld, bs = _turned(x, positions, dim, name)
+        same_gpu(positions, **{name: x, "freqs": freqs})
+        out = x if in_place else torch.empty(x.shape, dtype=torch.bfloat16, device=x.device)
+        outs.append(out)
+        sides.append(RopeRowsC(x.data_ptr(), out.data_ptr(), h, ld, bs, *((ld, bs) if in_place else (h * dim, rows * h * dim))))
+    if positions.numel() and any(x is not None and x.shape[2] == 0 for x in (q, k)):
+        raise ValueError("q and k must have heads")
+    with torch.cuda.device(positions.device):
+        check(lib.h3mi_rope_bf16(ctypes.byref(sides[0]), None if k is None else ctypes.byref(sides[1]), ptr(positions), ptr(freqs), n, rows,
+                                 dim, 2 * freqs.numel(), int(bool(interleaved)), int(bool(inverse)), float(amplitude), stream_of(positions)))
+    return tuple(outs)
+
+
+def rope_(q, k, positions, freqs, interleaved=False, inverse=False, amplitude=1.0):
+    """Rotary positions, in place on q and k (k may be None); returns (q, k).
+
+    q, k bf16 [n, rows, heads, dim], each with its own number of heads, views of a projection's output serve; positions int32
+    [n, rows], freqs fp64 [rot / 2] radians a token (rope_frequencies).  The first rot elements of each head are turned, pairs
+    (i, i + rot / 2) or, interleaved, (2 i, 2 i + 1): by position times frequency, formed in 64 bits, and scaled by amplitude.
+    inverse turns back, with the same amplitude: the transpose, which a gradient goes through.  Rows at a position below 0,
+    and the elements from rot on, are left as they are."""
+    done = _fast.rope(q, k, positions, freqs, interleaved, inverse, amplitude, True)
+    return done if done is not None else _rope(q, k, positions, freqs, interleaved, inverse, amplitude, True)
+
+
+def rope(q, k, positions, freqs, interleaved=False, inverse=False, amplitude=1.0):
+    """rope_ into new tensors; returns them."""
+    done = _fast.rope(q, k, positions, freqs, interleaved, inverse, amplitude, False)
+    return done if done is not None else _rope(q, k, positions, freqs, interleaved, inverse, amplitude, False)
