@@ -12,7 +12,9 @@
 // workgroup takes one block of 64 tokens of one head, keys and values: a thread holds 4 tokens of
 // 8 elements, 4 lanes a group, so that a wave's accesses are whole rows of a head, of 128 to 512
 // bytes in bf16 and 32 to 128 in 4 bits.  The scales, bytes 64 apart from group to group, are
-// gathered in LDS and stored four tokens at a time.
+// gathered in LDS and stored four tokens at a time.  4-bit rows are stored through the L2, which makes
+// whole lines of them (a clip of 19200 tokens of 56 x 128 written and read back 264 us past it, 218
+// so); bf16 rows go past it, and large inputs past the memory-side cache, as in 8 bits.
 #include "kv.h"
 
 namespace h3mi {
@@ -78,7 +80,7 @@ __global__ __launch_bounds__(2 * D) void kv4_write_kernel(Rows kin, Rows vin, Kv
             const int tok = 16 * j + line, at = base + tok;
             const int code = four_code(group_max(x[w][j]));
             if (ch % 4 == 0) codes[w][ch / 4][tok] = static_cast<uint8_t>(code);
-            if (at >= start && at < len) store_past(out + tok * (D / 2) + ch * 4, pack_four(x[w][j], code));
+            if (at >= start && at < len) *reinterpret_cast<uint32_t*>(out + tok * (D / 2) + ch * 4) = pack_four(x[w][j], code);
         }
     }
     __syncthreads();
@@ -96,7 +98,9 @@ __global__ __launch_bounds__(2 * D) void kv4_write_kernel(Rows kin, Rows vin, Kv
 }
 
 // One workgroup: one cache block of those that a sequence's tokens starts .. starts + length - 1 lie in, one head.
-template <int D>
+// STREAM: loads past the caches too, where the call's own output is more than the memory-side cache holds (a clip of 19200 tokens
+// of 56 x 128 written and read back 252 us without, 237 so; where nothing came between, and the cache still holds it, 218).
+template <int D, bool STREAM>
 __global__ __launch_bounds__(2 * D) void kv4_read_kernel(uint16_t* __restrict__ kout, uint16_t* __restrict__ vout,
                                                          const int32_t* __restrict__ starts, KvCache4 c, KvSeqs s, int length,
                                                          int touched) {
@@ -119,7 +123,8 @@ __global__ __launch_bounds__(2 * D) void kv4_read_kernel(uint16_t* __restrict__ 
             const int tok = 16 * j + line;
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
-                q[w][j] = *reinterpret_cast<const uint32_t*>((w ? c.v : c.k) + tile * (kKvBlock * D / 2) + tok * (D / 2) + ch * 4);
+                const uint32_t* const p = reinterpret_cast<const uint32_t*>((w ? c.v : c.k) + tile * (kKvBlock * D / 2) + tok * (D / 2) + ch * 4);
+                q[w][j] = STREAM ? __builtin_nontemporal_load(p) : *p;
                 code[w][j] = (w ? c.vs : c.ks)[tile * (G * kKvBlock) + ch / 4 * kKvBlock + tok];
             }
         }
@@ -188,7 +193,9 @@ extern "C" int h3mi_kv_read_mx4_bf16(uint16_t* k, uint16_t* v, const int32_t* st
     for (const uint16_t* x : {k, v})
         if (kv_seqs_overlap(x, bytes, *seqs) || (starts && overlap(x, bytes, starts, 4 * static_cast<size_t>(seqs->n))))
             return fail(H3MI_EALIAS, "kv_read: k or v overlaps tables, lens, counts or starts");
-    const auto fn = D == 64 ? kv4_read_kernel<64> : D == 128 ? kv4_read_kernel<128> : kv4_read_kernel<256>;
+    const bool stream_in = 2 * bytes > static_cast<size_t>(kMemoryCache);
+    const auto fn = stream_in ? (D == 64 ? kv4_read_kernel<64, true> : D == 128 ? kv4_read_kernel<128, true> : kv4_read_kernel<256, true>)
+                              : (D == 64 ? kv4_read_kernel<64, false> : D == 128 ? kv4_read_kernel<128, false> : kv4_read_kernel<256, false>);
     hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(groups)), dim3(2 * D), 0, as_stream(stream), k, v, starts,
                        kv_cache(*cache), kv_seqs(*seqs), static_cast<int>(length), static_cast<int>(touched));
     return check_launch("kv_read");

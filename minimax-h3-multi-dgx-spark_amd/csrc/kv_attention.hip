@@ -788,8 +788,15 @@ struct Shares {
 // workgroup at a time, take 129; 16 sequences of 1 to 32768 tokens of 8 heads (780 MB) 128, where
 // shares of their own for each, a quarter of the longest, took 146.  Without shares (plan_of) a
 // workgroup reads a whole sequence, and the launch takes as long as the longest.
+// Workgroups of a CU that registers are kept for: left to itself the compiler takes some more for 16 queries over 4 bits
+// (a query of 56 heads over 19721 tokens 34.4 us, 33.8 so; three spill, and take 48).
 template <class C, int D, int NQ>
-__global__ __launch_bounds__(64 * kFewWaves) void kv_few_kernel(Queries q, C c, KvSeqs s, float scale, int causal, Lists list,
+constexpr int few_groups() {
+    return std::is_same_v<C, KvCache4> && NQ == 1 && D < 256 ? 2 : 1;
+}
+
+template <class C, int D, int NQ>
+__global__ __launch_bounds__(64 * kFewWaves, (few_groups<C, D, NQ>())) void kv_few_kernel(Queries q, C c, KvSeqs s, float scale, int causal, Lists list,
                                                                 uint16_t* __restrict__ out, Partial part, Shares shares) {
     constexpr bool kFour = std::is_same_v<C, KvCache4>;
     using Four = FourFew<D>;

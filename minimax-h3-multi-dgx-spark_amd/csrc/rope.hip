@@ -12,12 +12,10 @@
 // the row's heads and kept in LDS.  A workgroup takes a few whole rows, or where there are few
 // rows a share of one's heads.  A thread takes 8 pairs of a head (4 interleaved ones): 16-byte
 // accesses whose lanes lie side by side.
-#include "common.h"
+#include "kv.h"
 
 namespace h3mi {
 namespace {
-
-typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 
 struct RopeRows {
     const uint16_t* in;
@@ -39,10 +37,23 @@ struct RopeCall {
 };
 
 constexpr int kRopeThreads = 256;
-constexpr int kRopeAhead = 4;   // units that a thread has in flight
+constexpr int kRopeAhead = 4;   // units that a thread has in flight (2 and 8: 1% and 4% slower)
 constexpr int kRopeTokens = 16;
 
 enum RopeForm { kHalves, kPairs, kOne };
+
+// How rows go through the caches.  kCached: rows in place that the memory-side cache may hold.  kStore: new tensors, written past
+// the L2 (2401 rows of 112 heads, the memory-side cache full of others 31.5 us, 28.6 so; else 24.2 and 24.6).  kPast: rows that
+// are more than that cache holds beside others, read past it too (19200 in place 217 us, 191 so; 2401 of 48 heads of 4 sequences
+// into new tensors 51 and 47; but 4801 rows in place, which it holds, 43 and 52).
+enum RopeWay { kCached, kStore, kPast };
+constexpr int64_t kRopePast = kMemoryCache / 4 * 3;
+
+template <bool PAST>
+__device__ __forceinline__ void store_row(uint16_t* p, uint4 v) {
+    if constexpr (PAST) store_past(p, v);
+    else *reinterpret_cast<uint4*>(p) = v;
+}
 
 // What a thread holds of a unit: 8 elements and their partners 8 chunks on (kHalves), 8 elements (kPairs), two (kOne).
 template <RopeForm F>
@@ -85,7 +96,7 @@ __device__ __forceinline__ void turn(Unit<F>& x, const float2* tab) {
     }
 }
 
-template <RopeForm F>
+template <RopeForm F, RopeWay W>
 __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeCall c, int interleaved) {
     extern __shared__ float2 tab[];  // [tokens, rot / 2]: (c, s)
     __shared__ bool real[kRopeTokens];  // rows that a position was given for
@@ -149,8 +160,8 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeCall c, int inte
                 y[j].a.x = from[0];
                 y[j].b.x = from[apart];
             } else {
-                y[j].a = *reinterpret_cast<const uint4*>(from);
-                if (two) y[j].b = *reinterpret_cast<const uint4*>(from + apart);
+                y[j].a = load_row<W == kPast>(from);
+                if (two) y[j].b = load_row<W == kPast>(from + apart);
             }
         }
 #pragma unroll
@@ -161,8 +172,8 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeCall c, int inte
                 to[j][0] = static_cast<uint16_t>(y[j].a.x);
                 to[j][apart] = static_cast<uint16_t>(y[j].b.x);
             } else {
-                *reinterpret_cast<uint4*>(to[j]) = y[j].a;
-                if (two) *reinterpret_cast<uint4*>(to[j] + apart) = y[j].b;
+                store_row<W != kCached>(to[j], y[j].a);
+                if (two) store_row<W != kCached>(to[j] + apart, y[j].b);
             }
         }
     }
@@ -268,7 +279,10 @@ extern "C" int h3mi_rope_bf16(const h3mi_rope_rows* q, const h3mi_rope_rows* k, 
     const int64_t groups = (c.all + tokens - 1) / tokens * parts;
     if (groups * kRopeThreads >= (int64_t{1} << 32)) return fail(H3MI_EINVAL, "rope: too many rows for one call");
     const size_t lds = static_cast<size_t>(tokens) * (rot / 2) * 8;
-    const auto fn = form == kHalves ? rope_kernel<kHalves> : form == kPairs ? rope_kernel<kPairs> : rope_kernel<kOne>;
+    const RopeWay way = c.all * heads * dim * (c.in_place ? 2 : 4) > kRopePast ? kPast : c.in_place ? kCached : kStore;
+    const auto halves = way == kCached ? rope_kernel<kHalves, kCached> : way == kStore ? rope_kernel<kHalves, kStore> : rope_kernel<kHalves, kPast>;
+    const auto pairs = way == kCached ? rope_kernel<kPairs, kCached> : way == kStore ? rope_kernel<kPairs, kStore> : rope_kernel<kPairs, kPast>;
+    const auto fn = form == kHalves ? halves : form == kPairs ? pairs : rope_kernel<kOne, kCached>;
     hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(groups)), dim3(kRopeThreads), lds, as_stream(stream), c, interleaved != 0);
     return check_launch("rope");
 }
