@@ -77,6 +77,12 @@ __device__ __forceinline__ float max_halves(float v) {
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
+// The larger of lanes l and l ^ 16.
+__device__ __forceinline__ float max_quads(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // What a block's scores and probabilities are multiplied by.
@@ -650,106 +656,179 @@ __device__ __forceinline__ uint4 load_once(const int8_t* p) {
     return __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p)));
 }
 
+// A block's keys (values) in 4 bits and their scales as buffers, which end behind the block: nothing of either is loaded if it
+// is not there.
+struct FourSpan {
+    __amdgpu_buffer_rsrc_t values, codes;
+    // (page < 0: not there)
+    __device__ __forceinline__ FourSpan(const uint8_t* v, const uint8_t* s, int heads, int h, int dim, int page) {
+        const int64_t tile = static_cast<int64_t>(page < 0 ? 0 : page) * heads + h;
+        values = span_bytes(v + tile * (kKvBlock * dim / 2), page < 0 ? 0 : kKvBlock * dim / 2);
+        codes = span_bytes(s + tile * (kKvBlock * dim / kFourGroup), page < 0 ? 0 : kKvBlock * dim / kFourGroup);
+    }
+};
+
+constexpr int kNonTemporal = 2;  // of a buffer load, as load_once (a query of 56 heads over 19721 tokens 34.3 us without, 30.4 so)
+
+// LDS operations of a wave are done in order: what the compiler may not change here.
+__device__ __forceinline__ void wave_order() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("" ::: "memory");
+}
+
 template <class T>
-__device__ __forceinline__ T load_past(const uint8_t* p) {
-    if constexpr (sizeof(T) == 16) return __builtin_bit_cast(T, __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p)));
-    else if constexpr (sizeof(T) == 8) return __builtin_bit_cast(T, __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p)));
-    else return __builtin_nontemporal_load(reinterpret_cast<const T*>(p));
+__device__ __forceinline__ T load_past(__amdgpu_buffer_rsrc_t b, int at) {
+    if constexpr (sizeof(T) == 16) return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b128(b, at, 0, kNonTemporal));
+    else if constexpr (sizeof(T) == 8) return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b64(b, at, 0, kNonTemporal));
+    else if constexpr (sizeof(T) == 4) return __builtin_amdgcn_raw_buffer_load_b32(b, at, 0, kNonTemporal);
+    else return __builtin_amdgcn_raw_buffer_load_b16(b, at, 0, kNonTemporal);
 }
 
 // What a lane (column col, lanes 16 quad ..) loads of a block in 4 bits, and the operands that it makes of them.  Of the keys,
-// rows of the first product's MFMAs: token 4 col + u for MFMA set u, a quarter of each 128 elements (of 64), one scale each
-// (half of one).  Of the values: D / 16 neighbouring elements of 16 neighbouring tokens, whose pairs change places by a permute
-// each; MFMA e takes element e of each lane's.
+// rows of the first product's MFMAs: column 4 q + r has token 16 u + 4 r + q for MFMA set u, of it a quarter of each 128
+// elements (of 64), one scale each (half of one).  So a query's probabilities of tokens 16 u + 4 r + quad are in a lane, and of
+// the values it takes these, D / 16 neighbouring elements each, whose pairs change places by a permute; MFMA e takes element e
+// of each lane's.  Each load's lanes then lie on whole cache lines, which no other load touches (but keys of 256 elements):
+// where two did, the second waited in the L1 for the first's line (43% of cycles).  Scales are loaded once a wave, in order, and
+// go through LDS to the lanes that want them.  A query of 56 heads over 19721 tokens (150 MB) 33.2 us with neighbouring tokens
+// in a lane, 30.4 so, the join's 4.6 among them; 16 sequences of up to 32768 tokens of 8 heads 58.9 and 53.2, 5.7 TB/s.
 template <int D>
 struct FourFew {
-    static constexpr int G = D / kFourGroup;
     static constexpr int kRun = D >= 128 ? 32 : 16;       // neighbouring elements of a key
     static constexpr int kRuns = D / (4 * kRun);
     static constexpr int kWords = kRun / 8;               // words of a run
     static constexpr int kWide = D / 16;                  // neighbouring elements of a value
     static constexpr int kBytes = kWide / 2;
+    static constexpr int kCodes = D / kFourGroup * kKvBlock / 4;  // words of a block's scales
+
+    // A wave's place in LDS for the scales of a block's keys and of its values.
+    struct Scratch {
+        uint32_t k[kCodes], v[kCodes];
+    };
 
     // first of the 8 elements of first-product operand k
     static __device__ __forceinline__ int element(int quad, int k) { return k / kWords * (4 * kRun) + quad * kRun + k % kWords * 8; }
     // the element of register r of output tile e
     static __device__ __forceinline__ int out_element(int quad, int r, int e) { return kWide * (4 * quad + r) + e; }
 
-    struct Keys {
-        uint32_t w[4][kRuns * kWords], codes[kRuns];  // codes: of the four tokens
-        __device__ __forceinline__ void load(const KvCache4& c, int64_t tile, int col, int quad) {
-            const uint8_t* const p = c.k + tile * (kKvBlock * D / 2);
+    // Byte q of a word of scale codes where a factor's exponent is; what else is in it a conversion does not read.
+    static __device__ __forceinline__ float factor(uint32_t word, int q) {
+        return __uint_as_float(__builtin_amdgcn_alignbit(word, word, 8 * q + 9));
+    }
+    static __device__ __forceinline__ bool bad(uint32_t word, int q) { return (word >> (8 * q) & 255) >= kFourBad; }
+
+    // A block's scale codes, a word (two) a lane.
+    struct Codes {
+        static constexpr int N = kCodes > 64 ? kCodes / 64 : 1;
+        uint32_t w[N];
+        __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t b, int lane) {
 #pragma unroll
-            for (int n = 0; n < kRuns; ++n)
-                codes[n] = load_past<uint32_t>(c.ks + tile * (kKvBlock * G) + element(quad, n * kWords) / kFourGroup * kKvBlock + 4 * col);
+            for (int n = 0; n < N; ++n) w[n] = load_past<uint32_t>(b, (n * 64 + lane) * 4);
+        }
+        // Into LDS; whether any of them stands for no number.
+        __device__ __forceinline__ bool put(uint32_t* to, int lane) const {
+            bool any = false;
+            wave_order();
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                if (kCodes >= 64 || lane < kCodes) to[n * 64 + lane] = w[n];
+                any |= four_bad(w[n]);
+            }
+            wave_order();
+            return __any(any);
+        }
+    };
+
+    struct Keys {
+        uint32_t w[4][kRuns * kWords], c[kRuns][4];
+        Codes codes;
+        __device__ __forceinline__ void load(const KvCache4& cache, int h, int page, int col, int quad) {
+            const FourSpan p(cache.k, cache.ks, cache.heads, h, D, page);
+            codes.load(p.codes, 16 * quad + col);
+            const int tok = 4 * (col & 3) + (col >> 2);
 #pragma unroll
             for (int u = 0; u < 4; ++u)
 #pragma unroll
                 for (int n = 0; n < kRuns; ++n) {
-                    const uint8_t* const at = p + (4 * col + u) * (D / 2) + element(quad, n * kWords) / 2;
+                    const int at = (16 * u + tok) * (D / 2) + element(quad, n * kWords) / 2;
                     if constexpr (kWords == 4) {
-                        const uint4 x = load_past<uint4>(at);
+                        const uint4 x = load_past<uint4>(p.values, at);
                         w[u][4 * n] = x.x, w[u][4 * n + 1] = x.y, w[u][4 * n + 2] = x.z, w[u][4 * n + 3] = x.w;
                     } else {
-                        const uint2 x = load_past<uint2>(at);
+                        const uint2 x = load_past<uint2>(p.values, at);
                         w[u][2 * n] = x.x, w[u][2 * n + 1] = x.y;
                     }
                 }
         }
-        __device__ __forceinline__ bf16x8 operand(int u, int k) const {
-            const uint32_t code = codes[k / kWords] >> (8 * u) & 255;
-            // (a NaN of every element: a factor of 2^128 is none, whatever is not 0 times it)
-            const bool bad = code >= kFourBad;
-            return frag(four_bf16x8(w[u][k] | (bad ? 0x11111111u : 0u), four_scale(bad ? 255 : code)));
+        // The scales; NaNs of every element where one stands for no number: a factor of 2^128 is none, whatever is not 0 times it.
+        __device__ __forceinline__ void ready(Scratch& scratch, int col, int quad) {
+            const bool any = codes.put(scratch.k, 16 * quad + col);
+#pragma unroll
+            for (int n = 0; n < kRuns; ++n)
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    c[n][u] = scratch.k[element(quad, n * kWords) / kFourGroup * (kKvBlock / 4) + 4 * u + (col & 3)];
+            if (!any) return;
+#pragma unroll
+            for (int n = 0; n < kRuns; ++n)
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    if (!bad(c[n][u], col >> 2)) continue;
+                    c[n][u] = ~0u;
+#pragma unroll
+                    for (int k = 0; k < kWords; ++k) w[u][n * kWords + k] |= 0x11111111u;
+                }
+        }
+        __device__ __forceinline__ bf16x8 operand(int u, int k, int col) const {
+            return frag(four_bf16x8(w[u][k], factor(c[k / kWords][u], col >> 2)));
         }
     };
 
     struct Values {
         static constexpr int N = kBytes < 4 ? 1 : kBytes / 4;
-        uint32_t w[16][N];
-        uint4 codes;
-        __device__ __forceinline__ void load(const KvCache4& c, int64_t tile, int col, int quad) {
-            const uint8_t* const p = c.v + tile * (kKvBlock * D / 2) + 16 * quad * (D / 2) + col * kBytes;
-            codes = load_past<uint4>(c.vs + tile * (kKvBlock * G) + kWide * col / kFourGroup * kKvBlock + 16 * quad);
+        uint32_t w[16][N], c[16];
+        Codes codes;
+        __device__ __forceinline__ void load(const KvCache4& cache, int h, int page, int col, int quad) {
+            const FourSpan p(cache.v, cache.vs, cache.heads, h, D, page);
+            codes.load(p.codes, 16 * quad + col);
+            const int at = quad * (D / 2) + col * kBytes;
 #pragma unroll
             for (int x = 0; x < 16; ++x) {
                 if constexpr (kBytes == 2) {
-                    w[x][0] = load_past<uint16_t>(p + x * (D / 2));
+                    w[x][0] = load_past<uint16_t>(p.values, at + x * (4 * D / 2));
                 } else if constexpr (kBytes == 4) {
-                    w[x][0] = load_past<uint32_t>(p + x * (D / 2));
+                    w[x][0] = load_past<uint32_t>(p.values, at + x * (4 * D / 2));
                 } else {
-                    const uint2 y = load_past<uint2>(p + x * (D / 2));
+                    const uint2 y = load_past<uint2>(p.values, at + x * (4 * D / 2));
                     w[x][0] = y.x, w[x][N - 1] = y.y;
                 }
             }
         }
-        // Zeros for the values of tokens whose scale stands for no number; whether there are any.
-        __device__ __forceinline__ bool clean() {
-            uint32_t cw[4] = {codes.x, codes.y, codes.z, codes.w};
-            bool any = false;
+        // The scales; zeros for the values of tokens whose scale stands for no number; whether the block has any.
+        __device__ __forceinline__ bool ready(Scratch& scratch, int col, int quad) {
+            const bool any = codes.put(scratch.v, 16 * quad + col);
 #pragma unroll
-            for (int y = 0; y < 4; ++y) {
-                if (!four_bad(cw[y])) continue;
-                any = true;
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    if ((cw[y] >> (8 * x) & 255) < kFourBad) continue;
-                    cw[y] &= ~(255u << (8 * x));
-#pragma unroll
-                    for (int n = 0; n < N; ++n) w[4 * y + x][n] = 0;
-                }
+            for (int x = 0; x < 16; x += 4) {
+                const uint4 y = *reinterpret_cast<const uint4*>(&scratch.v[kWide * col / kFourGroup * (kKvBlock / 4) + x]);
+                c[x] = y.x, c[x + 1] = y.y, c[x + 2] = y.z, c[x + 3] = y.w;
             }
-            codes = make_uint4(cw[0], cw[1], cw[2], cw[3]);
-            return any;
+            if (!any) return false;
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+                if (!bad(c[x], quad)) continue;
+                c[x] = 0;
+#pragma unroll
+                for (int n = 0; n < N; ++n) w[x][n] = 0;
+            }
+            return true;
         }
-        // The second product's operands of elements 2 e and 2 e + 1 (a[0], a[1]) with each half of the tokens' probabilities:
-        // half h, register j has token 4 (j % 4) + 2 h + j / 4 of the lane's 16.
-        __device__ __forceinline__ void operands(int e, bf16x8 (&a)[2][2]) const {
-            const uint32_t cw[4] = {codes.x, codes.y, codes.z, codes.w};
+        // The second product's operands of elements 2 e and 2 e + 1 (a[0], a[1]) with each half of the tokens' probabilities.
+        __device__ __forceinline__ void operands(int e, int quad, bf16x8 (&a)[2][2]) const {
             uint32_t y[16];
 #pragma unroll
             for (int x = 0; x < 16; ++x) {
-                const float f = four_scale(cw[x / 4] >> (8 * (x % 4)) & 255);
+                const float f = factor(c[x], quad);
                 const uint32_t v = w[x][e / 4];
                 y[x] = e % 4 == 0 ? four_bf16<0>(v, f) : e % 4 == 1 ? four_bf16<1>(v, f) : e % 4 == 2 ? four_bf16<2>(v, f) : four_bf16<3>(v, f);
             }
@@ -757,11 +836,9 @@ struct FourFew {
             for (int z = 0; z < 2; ++z) {
                 const uint32_t sel = z ? 0x07060302u : 0x05040100u;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int s = 2 * h;
-                    a[z][h] = frag(make_uint4(__builtin_amdgcn_perm(y[4 + s], y[s], sel), __builtin_amdgcn_perm(y[12 + s], y[8 + s], sel),
-                                              __builtin_amdgcn_perm(y[5 + s], y[1 + s], sel), __builtin_amdgcn_perm(y[13 + s], y[9 + s], sel)));
-                }
+                for (int h = 0; h < 2; ++h)
+                    a[z][h] = frag(make_uint4(__builtin_amdgcn_perm(y[8 * h + 1], y[8 * h], sel), __builtin_amdgcn_perm(y[8 * h + 3], y[8 * h + 2], sel),
+                                              __builtin_amdgcn_perm(y[8 * h + 5], y[8 * h + 4], sel), __builtin_amdgcn_perm(y[8 * h + 7], y[8 * h + 6], sel)));
             }
         }
     };
@@ -788,8 +865,8 @@ struct Shares {
 // workgroup at a time, take 129; 16 sequences of 1 to 32768 tokens of 8 heads (780 MB) 128, where
 // shares of their own for each, a quarter of the longest, took 146.  Without shares (plan_of) a
 // workgroup reads a whole sequence, and the launch takes as long as the longest.
-// Workgroups of a CU that registers are kept for: left to itself the compiler takes some more for 16 queries over 4 bits
-// (a query of 56 heads over 19721 tokens 34.4 us, 33.8 so; three spill, and take 48).
+// Workgroups of a CU that registers are kept for: left to itself the compiler schedules 16 queries over 4 bits a little worse
+// (a query of 56 heads over 19721 tokens 31.1 us, 30.4 so; registers for three spill, 48).
 template <class C, int D, int NQ>
 constexpr int few_groups() {
     return std::is_same_v<C, KvCache4> && NQ == 1 && D < 256 ? 2 : 1;
@@ -804,6 +881,7 @@ __global__ __launch_bounds__(64 * kFewWaves, (few_groups<C, D, NQ>())) void kv_f
     constexpr int NT = D / 16;   // tiles of 16 elements of the output
     __shared__ float jo[kFewWaves][kFew][D + 4];
     __shared__ float2 jml[kFewWaves][kFew];
+    __shared__ __attribute__((aligned(16))) std::conditional_t<kFour, typename Four::Scratch, int> scratch[kFewWaves];
     __shared__ int ends[kFewThreads + 1];  // blocks of the sequences up to each
     __shared__ int wave_sum[kFewWaves];
 
@@ -911,8 +989,7 @@ __global__ __launch_bounds__(64 * kFewWaves, (few_groups<C, D, NQ>())) void kv_f
         bool poison = false;  // kFour: a value's scale stands for no number
         auto load_k = [&](int page) {
             if constexpr (kFour) {
-                kr.load(c, static_cast<int64_t>(page) * c.heads + h, col, quad);
-                return;
+                kr.load(c, h, page, col, quad);
             } else {
             const int8_t* const p = c.k + (static_cast<int64_t>(page) * c.heads + h) * (kKvBlock * D);
 #pragma unroll
@@ -925,7 +1002,7 @@ __global__ __launch_bounds__(64 * kFewWaves, (few_groups<C, D, NQ>())) void kv_f
         };
         auto load_v = [&](int page) {
             if constexpr (kFour) {
-                vr.load(c, static_cast<int64_t>(page) * c.heads + h, col, quad);
+                vr.load(c, h, page, col, quad);
             } else {
             const int8_t* const p = c.v + (static_cast<int64_t>(page) * c.heads + h) * (kKvBlock * D);
 #pragma unroll
@@ -961,6 +1038,7 @@ __global__ __launch_bounds__(64 * kFewWaves, (few_groups<C, D, NQ>())) void kv_f
                 const float fiv = kFour ? 1.0f : __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f.iv), y));
                 const float fvs = kFour ? 1.0f : __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f.vs), y));
                 f32x4 sc[NQ][4];
+                if constexpr (kFour) kr.ready(scratch[wave], col, quad);
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
 #pragma unroll
@@ -968,7 +1046,7 @@ __global__ __launch_bounds__(64 * kFewWaves, (few_groups<C, D, NQ>())) void kv_f
                     if constexpr (kFour) {
 #pragma unroll
                         for (int k = 0; k < D / 32; ++k) {
-                            const bf16x8 a = kr.operand(u, k);
+                            const bf16x8 a = kr.operand(u, k, col);
 #pragma unroll
                             for (int g = 0; g < NQ; ++g) sc[g][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, qf[g][k], sc[g][u], 0, 0, 0);
                         }
@@ -984,22 +1062,41 @@ __global__ __launch_bounds__(64 * kFewWaves, (few_groups<C, D, NQ>())) void kv_f
                         }
                     }
                 }
-                if (left) load_k(next);
-                // register r of sc[g][u]: token base + 16 quad + 4 u + r (4 bits: 4 r + u)
+                // (4 bits: loads that are always issued, of nothing behind the last, let the others' waits count them)
+                if constexpr (kFour) load_k(left ? next : -1);
+                else if (left) load_k(next);
+                // register r of sc[g][u]: token base + 16 quad + 4 u + r (4 bits: 16 u + 4 r + quad)
                 const bool mask = base + kKvBlock > full;
                 bf16x8 p[NQ][2];
 #pragma unroll
                 for (int g = 0; g < NQ; ++g) {
                     float best = -__builtin_inff();
+                    if constexpr (kFour) {
+                        if (mask) {
+                            const int most = last[g] - base - quad;
+#pragma unroll
+                            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                                for (int r = 0; r < 4; ++r) sc[g][u][r] = 16 * u + 4 * r > most ? -__builtin_inff() : sc[g][u][r];
+                        }
+#pragma unroll
+                        for (int u = 0; u < 4; ++u)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) best = fmaxf(best, sc[g][u][r]);
+                    } else
 #pragma unroll
                     for (int u = 0; u < 4; ++u)
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
-                            if (mask && base + 16 * quad + (kFour ? 4 * r + u : 4 * u + r) > last[g]) sc[g][u][r] = -__builtin_inff();
+                            if (mask && base + 16 * quad + 4 * u + r > last[g]) sc[g][u][r] = -__builtin_inff();
                             best = fmaxf(best, sc[g][u][r]);
                         }
-                    best = fmaxf(best, __shfl_xor(best, 16));
-                    best = fmaxf(best, __shfl_xor(best, 32)) * fc;
+                    if constexpr (kFour) {
+                        best = max_halves(max_quads(best)) * fc;
+                    } else {
+                        best = fmaxf(best, __shfl_xor(best, 16));
+                        best = fmaxf(best, __shfl_xor(best, 32)) * fc;
+                    }
                     if (__any(best > m[g] + kSlack)) {
                         const float mn = fmaxf(m[g], best), fix = exp2_hw(m[g] - mn);
                         m[g] = mn;
@@ -1037,11 +1134,11 @@ __global__ __launch_bounds__(64 * kFewWaves, (few_groups<C, D, NQ>())) void kv_f
                     }
                 }
                 if constexpr (kFour) {
-                    poison |= vr.clean();
+                    poison |= vr.ready(scratch[wave], col, quad);
 #pragma unroll
                     for (int e = 0; e < NT / 2; ++e) {
                         bf16x8 a[2][2];
-                        vr.operands(e, a);
+                        vr.operands(e, quad, a);
 #pragma unroll
                         for (int z = 0; z < 2; ++z)
 #pragma unroll
@@ -1060,14 +1157,15 @@ __global__ __launch_bounds__(64 * kFewWaves, (few_groups<C, D, NQ>())) void kv_f
                         o[g][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, p[g][1], o[g][d], 0, 0, 0);
                     }
                 }
-                if (left) load_v(next);
+                if constexpr (kFour) load_v(left ? next : -1);
+                else if (left) load_v(next);
                 y = z;
             }
         }
 
         // as in kv_tile_kernel: a wave that has met such a value looks through its blocks again
         if constexpr (kFour) {
-            if (__any(poison)) {
+            if (poison) {
                 for (int x = from + wave; x < to; x += kFewWaves) {
                     const int b = mine ? mine[x] : x;
                     const int page = b >= 0 && b < blocks ? s.page(i, b, c.pages) : -1;
