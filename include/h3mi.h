@@ -372,7 +372,7 @@ typedef struct h3mi_kv_pool {
  * there on those that need no page.  count falls by what was taken.
  * positions int32 [n, rows]: lens[i] before + r where r < granted[i], else -1;
  * slots int64 [n, rows]: 64 page + position % 64, -1 where there is no such row or its
- * page is none of the pool's.  n * rows < 2^31.  Calls on one pool run in order: on one
+ * page is none of the pool's.  n * rows and n * blocks < 2^31.  Calls on one pool run in order: on one
  * stream, or on several that wait for each other.  No two of the tensors may overlap. */
 int h3mi_kv_extend(const h3mi_kv_pool* pool, int32_t* tables, int32_t* lens, const int32_t* counts, int64_t n,
                    int64_t blocks, int64_t rows, int32_t* granted, int32_t* positions, int64_t* slots,

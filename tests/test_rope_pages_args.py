@@ -70,7 +70,7 @@ def _pages(fn, pool=None, **kw):
 @pytest.mark.parametrize("fn", ["extend", "release"])
 @pytest.mark.parametrize("pool,kw,code,msg", [
     (dict(pages=-1), {}, 1, "pages=-1"), (dict(pages=(1 << 30) + 1), {}, 1, "pages"), (None, dict(n=-1), 1, "n=-1"), (None, dict(blocks=1 << 25), 1, "blocks"),
-    (None, dict(n=0x7FFFFFFF), 1, "n="), (dict(free=None), {}, 1, "null free"), (dict(count=None), {}, 1, "null free or count"), (None, dict(tables=None), 1, "null tables"),
+    (None, dict(n=0x7FFFFFFF), 1, "n="), (None, dict(n=1 << 11, blocks=1 << 20), 1, "2^31 entries"), (dict(free=None), {}, 1, "null free"), (dict(count=None), {}, 1, "null free or count"), (None, dict(tables=None), 1, "null tables"),
     (None, dict(lens=None), 1, "null tables or lens"), (dict(free=(1 << 20) + 2), {}, 2, "4-byte"), (None, dict(lens=(1 << 23) + 1), 2, "4-byte"),
     (None, dict(counts=(1 << 24) + 2), 2, "4-byte"), (dict(free=(1 << 22) + 136), {}, 3, "overlap"), (dict(count=(1 << 20) + 396), {}, 3, "overlap"),
     (None, dict(lens=(1 << 22) + 4), 3, "overlap"), (None, dict(counts=1 << 23), 3, "overlap"), (None, dict(counts=(1 << 20) - 4), 3, "overlap"),
