@@ -347,7 +347,7 @@ def run(st):
     if kind == "rope":
         if own:
             h3mi = _package()
-            f = h3mi.rope_ if case["inplace"] else h3mi.rope
+            f = h3mi.rotary_ if case["inplace"] else h3mi.rotary
             return f(st["q"], st["k"], st["positions"], st["freqs"], interleaved=case["interleaved"], inverse=case["inverse"],
                      amplitude=st["amplitude"])
         return _plain_rope(st)
