@@ -672,7 +672,7 @@ struct Turned {
 };
 
 // (q, k, positions, freqs, interleaved, inverse, amplitude, in place) -> (q, k)
-PyObject* rope(PyObject*, PyObject* const* v, Py_ssize_t n) {
+PyObject* rotary(PyObject*, PyObject* const* v, Py_ssize_t n) {
     H3MI_BEGIN
     H3MI_ARGS(8)
     Args a;
@@ -733,7 +733,7 @@ PyMethodDef kMethods[] = {
     H3MI_FN("norm_mod", &norm_any<false>), H3MI_FN("gate_norm_mod_", &norm_any<true>), H3MI_FN("gate_", &gate_),
     H3MI_FN("rms_rope_", &rms_rope_), H3MI_FN("last_shape", &last_shape), H3MI_FN("kv_write_", &kv_write_),
     H3MI_FN("kv_read", &kv_read), H3MI_FN("kv_select", &kv_select), H3MI_FN("kv_attention", &kv_attention),
-    H3MI_FN("kv_extend_", &kv_extend_), H3MI_FN("kv_release_", &kv_release_), H3MI_FN("rope", &rope),
+    H3MI_FN("kv_extend_", &kv_extend_), H3MI_FN("kv_release_", &kv_release_), H3MI_FN("rotary", &rotary),
     {"set_error", set_error, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_fast", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

@@ -7,7 +7,7 @@ slot of every row, without the host knowing a length:
 
   pool = kv_pool(pages)
   granted, positions, slots = kv_extend_(pool, tables, lens, rows, counts)
-  rope_(q, k, positions, freqs)
+  rotary_(q, k, positions, freqs)
   kv_write_(cache, k, v, tables, lens, counts=granted)
   kv_attention(q, cache, tables, lens, causal=True, counts=granted)
   kv_release_(pool, tables, lens, keep)

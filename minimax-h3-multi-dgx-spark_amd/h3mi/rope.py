@@ -10,9 +10,9 @@ rope_rotation_table (:548) with rot_dim = rope_freqs.shape[-3] * 2.  Each
 split-half rotation: the pair (y[i], y[i + rot/2]) times the token's 2 x 2
 table entry i, in fp32, rounded to bf16.
 
-rope_ and rope have no counterpart in the reference, whose tables come from the host
+rotary_ and rotary have no counterpart in the reference, whose tables come from the host
 program: they take the tokens' positions, as kv_extend_ gives them, and the pairs'
-frequencies (rope_frequencies), turn split halves or interleaved pairs of all or a
+frequencies (rotary_frequencies), turn split halves or interleaved pairs of all or a
 part of each head, and turn back.
 """
 import ctypes
@@ -81,8 +81,8 @@ def rms_rope_split_half(q, k, rope_freqs, qw, kw, epsilon=1e-6, rot_dim=None, rs
     return rms_rope_split_half_(qo, ko, rope_freqs, qw, kw, epsilon, rot_dim, rsqrt)
 
 
-def rope_frequencies(rot_dim, base=10000.0, scaling=None, factor=1.0, window=8192, device="cuda"):
-    """(freqs fp64 [rot_dim / 2], amplitude) for rope_ and rope: base ** (-2 i / rot_dim) radians a token, and 1.
+def rotary_frequencies(rot_dim, base=10000.0, scaling=None, factor=1.0, window=8192, device="cuda"):
+    """(freqs fp64 [rot_dim / 2], amplitude) for rotary_ and rotary: base ** (-2 i / rot_dim) radians a token, and 1.
 
     scaling, for contexts of `factor` (>= 1) times the `window` tokens that the frequencies were made for:
       "linear"  positions count for 1 / factor: all frequencies are divided by it
@@ -122,13 +122,13 @@ def _turned(x, positions, dim, name):
     if x.numel() and (x.stride(3) != 1 or (h > 1 and x.stride(2) != d)):
         raise ValueError(f"{name}: heads must be contiguous (strides [*, *, dim, 1])")
     if torch.is_grad_enabled() and x.requires_grad:
-        raise RuntimeError("rope records no gradient: call it under torch.no_grad() (a gradient is turned by rope with inverse=True)")
+        raise RuntimeError("rotary records no gradient: call it under torch.no_grad() (a gradient is turned by rotary with inverse=True)")
     if forward_ad.unpack_dual(x).tangent is not None:
-        raise RuntimeError("rope has no forward-mode gradient: call it with the primal tensors")
+        raise RuntimeError("rotary has no forward-mode gradient: call it with the primal tensors")
     return h, x.stride(1) if rows > 1 else h * d, x.stride(0) if n > 1 else rows * h * d
 
 
-def _rope(q, k, positions, freqs, interleaved, inverse, amplitude, in_place):
+def _rotary(q, k, positions, freqs, interleaved, inverse, amplitude, in_place):
     if positions.dim() != 2 or positions.dtype != torch.int32 or not positions.is_contiguous():
         raise ValueError("positions must be contiguous int32 [n, rows]")
     if freqs.dim() != 1 or freqs.dtype != torch.float64 or not freqs.is_contiguous():
@@ -153,19 +153,19 @@ def _rope(q, k, positions, freqs, interleaved, inverse, amplitude, in_place):
     return tuple(outs)
 
 
-def rope_(q, k, positions, freqs, interleaved=False, inverse=False, amplitude=1.0):
+def rotary_(q, k, positions, freqs, interleaved=False, inverse=False, amplitude=1.0):
     """Rotary positions, in place on q and k (k may be None); returns (q, k).
 
     q, k bf16 [n, rows, heads, dim], each with its own number of heads, views of a projection's output serve; positions int32
-    [n, rows], freqs fp64 [rot / 2] radians a token (rope_frequencies).  The first rot elements of each head are turned, pairs
+    [n, rows], freqs fp64 [rot / 2] radians a token (rotary_frequencies).  The first rot elements of each head are turned, pairs
     (i, i + rot / 2) or, interleaved, (2 i, 2 i + 1): by position times frequency, formed in 64 bits, and scaled by amplitude.
     inverse turns back, with the same amplitude: the transpose, which a gradient goes through.  Rows at a position below 0,
     and the elements from rot on, are left as they are."""
-    done = _fast.rope(q, k, positions, freqs, interleaved, inverse, amplitude, True)
-    return done if done is not None else _rope(q, k, positions, freqs, interleaved, inverse, amplitude, True)
+    done = _fast.rotary(q, k, positions, freqs, interleaved, inverse, amplitude, True)
+    return done if done is not None else _rotary(q, k, positions, freqs, interleaved, inverse, amplitude, True)
 
 
-def rope(q, k, positions, freqs, interleaved=False, inverse=False, amplitude=1.0):
-    """rope_ into new tensors; returns them."""
-    done = _fast.rope(q, k, positions, freqs, interleaved, inverse, amplitude, False)
-    return done if done is not None else _rope(q, k, positions, freqs, interleaved, inverse, amplitude, False)
+def rotary(q, k, positions, freqs, interleaved=False, inverse=False, amplitude=1.0):
+    """rotary_ into new tensors; returns them."""
+    done = _fast.rotary(q, k, positions, freqs, interleaved, inverse, amplitude, False)
+    return done if done is not None else _rotary(q, k, positions, freqs, interleaved, inverse, amplitude, False)

@@ -59,20 +59,20 @@ def test_rope(dim, rot, interleaved, n, rows, hq, hk):
     positions = torch.from_numpy(rng.integers(0, 200000, (n, 1)) + np.arange(rows)).to(torch.int32)
     positions[:, rows - rows // 3:] = -1
     positions[-1, 0] = 0
-    freqs, amplitude = h.rope_frequencies(rot, scaling="yarn", factor=4.0, device="cpu")
+    freqs, amplitude = h.rotary_frequencies(rot, scaling="yarn", factor=4.0, device="cpu")
     for inverse in (False, True):
         d = qkv.to(DEV)
         q, k = d[:, :, :hq], d[:, :, hq:hq + hk]
         args = (positions.to(DEV), freqs.to(DEV))
-        new = h.rope(q, k, *args, interleaved=interleaved, inverse=inverse, amplitude=amplitude)
+        new = h.rotary(q, k, *args, interleaved=interleaved, inverse=inverse, amplitude=amplitude)
         assert torch.equal(d.cpu(), qkv) and all(t.is_contiguous() for t in new)
-        got = h.rope_(q, k, *args, interleaved=interleaved, inverse=inverse, amplitude=amplitude)
+        got = h.rotary_(q, k, *args, interleaved=interleaved, inverse=inverse, amplitude=amplitude)
         assert got[0] is q and got[1] is k
         for y, z, x in ((q, new[0], qkv[:, :, :hq]), (k, new[1], qkv[:, :, hq:hq + hk])):
             _check(y, x, positions, freqs, interleaved, inverse, amplitude)
             assert torch.equal(y, z)
         assert torch.equal(d[:, :, hq + hk:].cpu(), qkv[:, :, hq + hk:])  # the values between
-        assert torch.equal(h.rope(qkv[:, :, :hq].to(DEV), None, *args, interleaved, inverse, amplitude)[0], new[0])
+        assert torch.equal(h.rotary(qkv[:, :, :hq].to(DEV), None, *args, interleaved, inverse, amplitude)[0], new[0])
 
 
 @pytest.mark.parametrize("interleaved", [False, True])
@@ -83,7 +83,7 @@ def test_far_positions(interleaved):
     positions = torch.tensor([[0, 1, 2, 4095, 131071, 1 << 20, (1 << 24) + 1, (1 << 30) + 1, 2 ** 31 - 1, -1, -2 ** 31]], dtype=torch.int32)
     freqs = torch.from_numpy(np.concatenate([np.linspace(0, math.pi, 60), [1.0, 100.0, 1e-9, -0.5]]))
     x = _bf(rng, 1, 11, 4, 128)
-    _check(h.rope(x.to(DEV), None, positions.to(DEV), freqs.to(DEV), interleaved=interleaved)[0], x, positions, freqs, interleaved, False, 1.0)
+    _check(h.rotary(x.to(DEV), None, positions.to(DEV), freqs.to(DEV), interleaved=interleaved)[0], x, positions, freqs, interleaved, False, 1.0)
 
 
 @pytest.mark.parametrize("n,rows,hq,hk,dim,rot", [(1, 3001, 56, 56, 128, 128), (4, 701, 40, 8, 128, 64), (300, 1, 40, 8, 128, 128), (1, 9001, 1, 1, 64, 64),
@@ -95,8 +95,8 @@ def test_every_split_of_the_rows(n, rows, hq, hk, dim, rot, interleaved):
     rng = np.random.default_rng(rows)
     q, k = _bf(rng, n, rows, hq, dim), _bf(rng, n, rows, hk, dim)
     positions = torch.from_numpy(rng.integers(-1, 5000, (n, rows))).to(torch.int32)
-    freqs, _ = h.rope_frequencies(rot, device="cpu")
-    got = h.rope(q.to(DEV), k.to(DEV), positions.to(DEV), freqs.to(DEV), interleaved=interleaved)
+    freqs, _ = h.rotary_frequencies(rot, device="cpu")
+    got = h.rotary(q.to(DEV), k.to(DEV), positions.to(DEV), freqs.to(DEV), interleaved=interleaved)
     for y, x in zip(got, (q, k)):
         some = rng.choice(rows, min(rows, 60), replace=False)
         _check(y[:, some], x[:, some], positions[:, some], freqs, interleaved, False, 1.0)
@@ -117,13 +117,13 @@ def test_sequences_between_each_other():
     """Strides that run over sequences first, and one row of many sequences."""
     h = _h()
     rng = np.random.default_rng(6)
-    freqs, _ = h.rope_frequencies(128, device="cpu")
+    freqs, _ = h.rotary_frequencies(128, device="cpu")
     for n, rows in ((5, 7), (5, 1), (1, 7)):
         x = _bf(rng, rows, n, 6, 128)
         positions = torch.from_numpy(rng.integers(0, 99, (n, rows))).to(torch.int32)
         d = x.to(DEV)
         t = d.transpose(0, 1)
-        h.rope_(t[:, :, :4], t[:, :, 4:], positions.to(DEV), freqs.to(DEV))
+        h.rotary_(t[:, :, :4], t[:, :, 4:], positions.to(DEV), freqs.to(DEV))
         _check(t, x.transpose(0, 1), positions, freqs, False, False, 1.0)
 
 
@@ -131,12 +131,12 @@ def test_inverse_is_the_gradient():
     """<g, R x> = <R' g, x>, and differences of R along a direction; to the roundings of both sides."""
     h = _h()
     rng = np.random.default_rng(7)
-    freqs, amplitude = h.rope_frequencies(64, scaling="yarn", factor=16.0)
+    freqs, amplitude = h.rotary_frequencies(64, scaling="yarn", factor=16.0)
     positions = torch.from_numpy(rng.integers(0, 99999, (2, 50))).to(torch.int32).to(DEV)
     x, g = (_bf(rng, 2, 50, 3, 128).to(DEV) for _ in range(2))
     for interleaved in (False, True):
-        y = h.rope(x, None, positions, freqs, interleaved, False, amplitude)[0].double()
-        b = h.rope(g, None, positions, freqs, interleaved, True, amplitude)[0].double()
+        y = h.rotary(x, None, positions, freqs, interleaved, False, amplitude)[0].double()
+        b = h.rotary(g, None, positions, freqs, interleaved, True, amplitude)[0].double()
         left, right = (g.double() * y).sum(), (b * x.double()).sum()
         half = 2.0 ** -8
         most = half * ((g.double() * y).abs().sum() + (b * x.double()).abs().sum()) * 1.01
@@ -144,8 +144,8 @@ def test_inverse_is_the_gradient():
         # R is linear: R (x + g) - R x = R g
         both = (x.float() + g.float()).to(torch.bfloat16)
         step = (both.double() - x.double())
-        d = h.rope(both, None, positions, freqs, interleaved, False, amplitude)[0].double() - y
-        want = h.rope(step.to(torch.bfloat16), None, positions, freqs, interleaved, False, amplitude)[0].double()
+        d = h.rotary(both, None, positions, freqs, interleaved, False, amplitude)[0].double() - y
+        want = h.rotary(step.to(torch.bfloat16), None, positions, freqs, interleaved, False, amplitude)[0].double()
         slack = half * (d.abs() + 2 * y.abs() + want.abs() * 2) * 1.01 + half * amplitude * 2 * step.abs().amax(-1, keepdim=True) + 1e-5
         assert ((d - want).abs() <= slack).all()
 
@@ -153,14 +153,14 @@ def test_inverse_is_the_gradient():
 def test_special_values_stay_in_their_pairs():
     h = _h()
     rng = np.random.default_rng(8)
-    freqs, _ = h.rope_frequencies(128)
+    freqs, _ = h.rotary_frequencies(128)
     positions = torch.tensor([[5, -1, 7]], dtype=torch.int32, device=DEV)
     x = _bf(rng, 1, 3, 2, 128).to(DEV)
     for interleaved in (False, True):
-        want = h.rope(x, None, positions, freqs, interleaved)[0]
+        want = h.rotary(x, None, positions, freqs, interleaved)[0]
         bad = x.clone()
         bad[0, 0, 1, 10], bad[0, 1, 0, 3] = float("nan"), float("inf")
-        got = h.rope(bad, None, positions, freqs, interleaved)[0]
+        got = h.rotary(bad, None, positions, freqs, interleaved)[0]
         other = 11 if interleaved else 74
         hit = torch.zeros_like(x, dtype=torch.bool)
         hit[0, 0, 1, 10] = hit[0, 0, 1, other] = True
@@ -172,12 +172,12 @@ def test_special_values_stay_in_their_pairs():
 def test_frequencies():
     h = _h()
     i = np.arange(32)
-    f, amp = h.rope_frequencies(64, base=500.0, device="cpu")
+    f, amp = h.rotary_frequencies(64, base=500.0, device="cpu")
     assert f.dtype == torch.float64 and np.allclose(f, 500.0 ** (-i / 32), rtol=1e-14) and amp == 1.0
-    assert np.allclose(h.rope_frequencies(64, scaling="linear", factor=8.0)[0].cpu(), 10000.0 ** (-i / 32) / 8, rtol=1e-14)
-    f = h.rope_frequencies(64, scaling="ntk", factor=8.0)[0].cpu().numpy()
+    assert np.allclose(h.rotary_frequencies(64, scaling="linear", factor=8.0)[0].cpu(), 10000.0 ** (-i / 32) / 8, rtol=1e-14)
+    f = h.rotary_frequencies(64, scaling="ntk", factor=8.0)[0].cpu().numpy()
     assert f[0] == 1.0 and np.isclose(f[31], 10000.0 ** (-31 / 32) / 8, rtol=1e-12)
-    f, amp = h.rope_frequencies(64, scaling="yarn", factor=8.0, window=4096)
+    f, amp = h.rotary_frequencies(64, scaling="yarn", factor=8.0, window=4096)
     plain, f = 10000.0 ** (-i / 32), f.cpu().numpy()
     turns = 4096 * plain / (2 * math.pi)
     assert np.allclose(f[turns >= 34], plain[turns >= 34]) and np.allclose(f[turns <= 0.7], plain[turns <= 0.7] / 8) and np.isclose(amp, 1 + 0.1 * math.log(8))
@@ -185,36 +185,36 @@ def test_frequencies():
     assert (np.diff(plain / f) >= -128 * 2.0 ** -53).all()
     for kw in (dict(rot_dim=3), dict(rot_dim=0), dict(rot_dim=8, base=1.0), dict(rot_dim=8, factor=0.5), dict(rot_dim=8, scaling="other"), dict(rot_dim=8, window=0)):
         with pytest.raises(ValueError):
-            h.rope_frequencies(**kw)
+            h.rotary_frequencies(**kw)
 
 
 def test_captured_and_streams():
     h = _h()
     rng = np.random.default_rng(9)
-    freqs, _ = h.rope_frequencies(128)
+    freqs, _ = h.rotary_frequencies(128)
     q, k = _bf(rng, 2, 33, 4, 128).to(DEV), _bf(rng, 2, 33, 1, 128).to(DEV)
     positions = torch.zeros(2, 33, dtype=torch.int32, device=DEV)
     side = torch.cuda.Stream()
-    h.rope(q, k, positions, freqs)
+    h.rotary(q, k, positions, freqs)
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
-        out = h.rope(q, k, positions, freqs)
+        out = h.rotary(q, k, positions, freqs)
     for r in range(4):
         positions.random_(-1, 9999)
         q.normal_()
         torch.cuda.synchronize()
         graph.replay()
         with torch.cuda.stream(side):
-            beside = h.rope(q, k, positions, freqs)
-        want = h.rope(q, k, positions, freqs)
+            beside = h.rotary(q, k, positions, freqs)
+        want = h.rotary(q, k, positions, freqs)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) and torch.equal(c, b) for a, b, c in zip(out, want, beside)), r
 
 
 def test_refusals():
     h = _h()
-    freqs, _ = h.rope_frequencies(64)
+    freqs, _ = h.rotary_frequencies(64)
     positions = torch.zeros(2, 3, dtype=torch.int32, device=DEV)
     q = torch.zeros(2, 3, 4, 64, dtype=torch.bfloat16, device=DEV)
     k = q.clone()
@@ -223,25 +223,25 @@ def test_refusals():
                       ((q, k, positions, freqs.float()), "freqs"), ((q, k.cpu(), positions, freqs), "k is on"), ((q.transpose(2, 3), None, positions, freqs), "contiguous"),
                       ((q[..., :32].expand(2, 3, 4, 32), None, positions, freqs[:8]), "contiguous")):
         with pytest.raises(ValueError, match=msg):
-            h.rope(*args)
-    for call, msg in ((lambda: h.rope_(q, q, positions, freqs), "overlap"), (lambda: h.rope_(q, q[:, :, 1:], positions, freqs), "overlap"),
-                      (lambda: h.rope_(q[:1].expand(2, 3, 4, 64), None, positions, freqs), "shorter"),
-                      (lambda: h.rope(q, k, positions, torch.ones(33, dtype=torch.float64, device=DEV)), "rot=66"),
-                      (lambda: h.rope(q, k, positions, freqs, amplitude=float("inf")), "amplitude"),
-                      (lambda: h.rope_(q.view(-1)[4:4 + 2 * 3 * 3 * 64].view(2, 3, 3, 64), None, positions, freqs), "aligned"),
-                      (lambda: h.rope_(q.as_strided((2, 3, 2, 64), (256, 128, 64, 1)), None, positions, freqs), "overlap")):
+            h.rotary(*args)
+    for call, msg in ((lambda: h.rotary_(q, q, positions, freqs), "overlap"), (lambda: h.rotary_(q, q[:, :, 1:], positions, freqs), "overlap"),
+                      (lambda: h.rotary_(q[:1].expand(2, 3, 4, 64), None, positions, freqs), "shorter"),
+                      (lambda: h.rotary(q, k, positions, torch.ones(33, dtype=torch.float64, device=DEV)), "rot=66"),
+                      (lambda: h.rotary(q, k, positions, freqs, amplitude=float("inf")), "amplitude"),
+                      (lambda: h.rotary_(q.view(-1)[4:4 + 2 * 3 * 3 * 64].view(2, 3, 3, 64), None, positions, freqs), "aligned"),
+                      (lambda: h.rotary_(q.as_strided((2, 3, 2, 64), (256, 128, 64, 1)), None, positions, freqs), "overlap")):
         with pytest.raises(h._lib.H3miError, match=msg):
             call()
     with pytest.raises(RuntimeError, match="no gradient"):
-        h.rope(q.requires_grad_(), None, positions, freqs)
+        h.rotary(q.requires_grad_(), None, positions, freqs)
     with torch.no_grad():
-        h.rope(q, None, positions, freqs)
+        h.rotary(q, None, positions, freqs)
 
 
 def test_nothing_to_do():
     h = _h()
-    freqs, _ = h.rope_frequencies(64)
+    freqs, _ = h.rotary_frequencies(64)
     for n, rows in ((0, 3), (2, 0)):
         x = torch.zeros(n, rows, 4, 64, dtype=torch.bfloat16, device=DEV)
-        y, z = h.rope(x, None, torch.zeros(n, rows, dtype=torch.int32, device=DEV), freqs)
+        y, z = h.rotary(x, None, torch.zeros(n, rows, dtype=torch.int32, device=DEV), freqs)
         assert y.shape == x.shape and z is None

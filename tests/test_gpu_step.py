@@ -25,7 +25,7 @@ class Model:
         self.ws = torch.rand(out, generator=g, device=DEV) * 1e-3 + 1e-4
         self.x = torch.zeros(n * rows, width, device=DEV, dtype=torch.bfloat16)
         self.counts, self.keep = (torch.zeros(n, dtype=torch.int32, device=DEV) for _ in range(2))
-        self.freqs, self.amplitude = h3mi.rope_frequencies(rot, scaling="yarn", factor=4.0, window=512)
+        self.freqs, self.amplitude = h3mi.rotary_frequencies(rot, scaling="yarn", factor=4.0, window=512)
         self.interleaved = interleaved
         self.fresh(blocks, pages)
 
@@ -42,7 +42,7 @@ class Model:
         qkv = h3mi.w8a8_linear(self.x, self.w, self.ws).view(self.n, self.rows, -1, self.dim)
         q, k, v = qkv.split([self.heads, self.kv, self.kv], 2)
         before = qkv.clone()
-        h3mi.rope_(q, k, positions, self.freqs, interleaved=self.interleaved, amplitude=self.amplitude)
+        h3mi.rotary_(q, k, positions, self.freqs, interleaved=self.interleaved, amplitude=self.amplitude)
         h3mi.kv_write_(self.cache, k, v, self.tables, self.lens, counts=granted)
         out = h3mi.kv_attention(q, self.cache, self.tables, self.lens, causal=True, counts=granted)
         return out, granted, positions, slots, before, qkv

@@ -109,7 +109,17 @@ def test_cpu_tensors_are_refused():
         with pytest.raises(ValueError, match="GPU"):
             f()
     q = torch.zeros(1, 1, 2, 64, dtype=torch.bfloat16)
-    freqs, _ = h3mi.rope_frequencies(64, device="cpu")
-    for f in (h3mi.rope, h3mi.rope_):
+    freqs, _ = h3mi.rotary_frequencies(64, device="cpu")
+    for f in (h3mi.rotary, h3mi.rotary_):
         with pytest.raises(ValueError, match="GPU"):
             f(q, q.clone(), lens[None], freqs)
+
+
+def test_the_modules_keep_their_names():
+    """No function of the package hides the module that it is in."""
+    import inspect
+
+    import h3mi
+    for name in ("fused", "gemm", "kvcache", "kvpages", "linear", "quant", "rope"):
+        __import__(f"h3mi.{name}")
+        assert inspect.ismodule(getattr(h3mi, name)), name
