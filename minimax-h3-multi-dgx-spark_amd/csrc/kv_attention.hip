@@ -167,13 +167,37 @@ struct TileShape {
     static constexpr int kLoads = kKvBlock * D / 16 / kThreads;  // 16-byte pieces of K (and of V) a thread
 };
 
+// A block's keys (values) in 4 bits and their scales as buffers, which end behind the block: nothing is loaded of one that is not
+// there (page < 0).  (By address 4800 rows over 19721 tokens take 2635 us, so 2650; 300 rows over 4000 tokens 47.3, so 46.2.)
+struct FourPlace {
+    __amdgpu_buffer_rsrc_t values, codes;
+    __device__ __forceinline__ FourPlace(const uint8_t* v, const uint8_t* s, int heads, int h, int dim, int page) {
+        const int64_t tile = static_cast<int64_t>(page < 0 ? 0 : page) * heads + h;
+        values = span_bytes(v + tile * (kKvBlock * dim / 2), page < 0 ? 0 : kKvBlock * dim / 2);
+        codes = span_bytes(s + tile * (kKvBlock * dim / kFourGroup), page < 0 ? 0 : kKvBlock * dim / kFourGroup);
+    }
+};
+
+constexpr int kNonTemporal = 2;  // of a buffer load, as load_once (a query of 56 heads over 19721 tokens 34.3 us without, 30.4 so)
+
+template <class T, int WAY>
+__device__ __forceinline__ T load_from(__amdgpu_buffer_rsrc_t b, int at) {
+    if constexpr (sizeof(T) == 16) return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b128(b, at, 0, WAY));
+    else if constexpr (sizeof(T) == 8) return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b64(b, at, 0, WAY));
+    else if constexpr (sizeof(T) == 4) return __builtin_amdgcn_raw_buffer_load_b32(b, at, 0, WAY);
+    else if constexpr (sizeof(T) == 2) return __builtin_amdgcn_raw_buffer_load_b16(b, at, 0, WAY);
+    else return __builtin_amdgcn_raw_buffer_load_b8(b, at, 0, WAY);
+}
+template <class T>
+__device__ __forceinline__ T load_past(__amdgpu_buffer_rsrc_t b, int at) { return load_from<T, kNonTemporal>(b, at); }
+
 // What a thread loads and stages of a block in 4 bits.  Keys: pieces of 16 elements of a token, half a group's, as in 8 bits.
 // Values lie as they were written, token by token, and the second product wants runs of tokens: a thread takes 8 elements of
 // 4 (2) neighbouring tokens, whose pairs of elements, converted (one instruction for two, exact), change places with a permute
 // each and are 8 (4) bytes of 8 rows in LDS.
 template <int D, int W>
 struct FourTile {
-    static constexpr int G = D / kFourGroup, kThreads = 64 * W;
+    static constexpr int kThreads = 64 * W;
     static constexpr int kPieces = kKvBlock * D / 16 / kThreads;
     static constexpr int kEach = kKvBlock * D / kThreads;     // elements a thread
     static constexpr int kTok = kEach >= 32 ? 4 : 2, kUnits = kEach / (8 * kTok);
@@ -181,14 +205,13 @@ struct FourTile {
     struct Keys {
         uint2 w[kPieces];
         uint8_t code[kPieces];
-        __device__ __forceinline__ void load(const KvCache4& c, int64_t tile, int t) {
-            const uint8_t* const at = c.k + tile * (kKvBlock * D / 2);
-            const uint8_t* const codes = c.ks + tile * (kKvBlock * G);
+        __device__ __forceinline__ void load(const KvCache4& c, int h, int page, int t) {
+            const FourPlace p(c.k, c.ks, c.heads, h, D, page);
 #pragma unroll
             for (int j = 0; j < kPieces; ++j) {
-                const uint32_t piece = t + j * kThreads, line = piece / (D / 16), g = piece % (D / 16) / 2;
-                w[j] = *reinterpret_cast<const uint2*>(at + piece * 8);
-                code[j] = codes[g * kKvBlock + line];
+                const int piece = t + j * kThreads, line = piece / (D / 16), g = piece % (D / 16) / 2;
+                w[j] = load_from<uint2, 0>(p.values, piece * 8);
+                code[j] = load_from<uint8_t, 0>(p.codes, g * kKvBlock + line);
             }
         }
         __device__ __forceinline__ void stage(uint8_t* buf, int t) const {
@@ -223,18 +246,15 @@ struct FourTile {
             tok = (unit >> 1) % (kKvBlock / kTok) * kTok;
             ch = unit / (2 * kKvBlock / kTok) * 2 + (unit & 1);
         }
-        __device__ __forceinline__ void load(const KvCache4& c, int64_t tile, int t) {
-            const uint8_t* const at = c.v + tile * (kKvBlock * D / 2);
-            const uint8_t* const from = c.vs + tile * (kKvBlock * G);
+        __device__ __forceinline__ void load(const KvCache4& c, int h, int page, int t) {
+            const FourPlace p(c.v, c.vs, c.heads, h, D, page);
 #pragma unroll
             for (int j = 0; j < kUnits; ++j) {
                 uint32_t ch, tok;
                 place(t + j * kThreads, ch, tok);
 #pragma unroll
-                for (int x = 0; x < kTok; ++x) w[j][x] = *reinterpret_cast<const uint32_t*>(at + (tok + x) * (D / 2) + ch * 4);
-                const uint8_t* const p = from + ch / 4 * kKvBlock + tok;
-                if constexpr (kTok == 4) codes[j] = *reinterpret_cast<const uint32_t*>(p);
-                else codes[j] = *reinterpret_cast<const uint16_t*>(p);
+                for (int x = 0; x < kTok; ++x) w[j][x] = load_from<uint32_t, 0>(p.values, (tok + x) * (D / 2) + ch * 4);
+                codes[j] = load_from<std::conditional_t<kTok == 4, uint32_t, uint16_t>, 0>(p.codes, ch / 4 * kKvBlock + tok);
             }
         }
         __device__ __forceinline__ void stage(uint8_t* buf, int t, int* poison) {
@@ -320,6 +340,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : D == 64 ? 3 : 2) void kv_til
                                                                           Items items) {
     using T = TileShape<D, W>;
     constexpr bool kFour = std::is_same_v<C, KvCache4>;
+    constexpr bool kFar = kFour && D == 256;
     constexpr int NT = D / 32;            // tiles of 32 elements of the output
     constexpr int KC = D / 8, VC = 8;     // 16-byte chunks of a row of K, of V
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
@@ -382,11 +403,10 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : D == 64 ? 3 : 2) void kv_til
     std::conditional_t<kFour, typename Four::Values, uint4[T::kLoads]> vr;
     if (kFour && t == 0) poison = 0;  // (barriers follow before it is set)
     auto load = [&](const auto* from_pages, int page, auto& to_regs) __attribute__((always_inline)) {
-        const int64_t tile_of = static_cast<int64_t>(page) * c.heads + h;  // uniform
         if constexpr (kFour) {
-            to_regs.load(c, tile_of, t);
+            to_regs.load(c, h, page, t);
         } else {
-            const int8_t* const at = from_pages + tile_of * (kKvBlock * D);
+            const int8_t* const at = from_pages + (static_cast<int64_t>(page) * c.heads + h) * (kKvBlock * D);  // uniform
 #pragma unroll
             for (int j = 0; j < T::kLoads; ++j) to_regs[j] = *reinterpret_cast<const uint4*>(at + static_cast<uint32_t>(t + j * T::kThreads) * 16);
         }
@@ -590,8 +610,45 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : D == 64 ? 3 : 2) void kv_til
             if constexpr (!kFour) f = {uniform(next.c), uniform(next.lv), uniform(next.iv), uniform(next.vs)};
             arrive();
         };
-        step(0, std::false_type{});
-        for (int y = 1; y < n; ++y) step(y, std::true_type{});
+        if constexpr (kFar) {
+            // One wave a SIMD, with registers to spare: the bytes of block y + 2 (values: y + 1) are asked for in step y, into one of
+            // two sets.  Every load is issued, of nothing behind the last block, so that the wait for one does not have to be
+            // for those after it.  (1000 rows of 20 heads over 4000 tokens 190 us a step later, 182 so; of 128 elements, where two
+            // waves are on a SIMD, prompts of 512 rows 22.5 and 23.0.)
+            typename Four::Keys k1;
+            typename Four::Values v1;
+            page_k = n > 2 ? uniform(entry[2].x) : -1, page_v = n > 1 ? uniform(entry[1].x) : -1;
+            load(c.k, page_v, kr);
+            load(c.v, uniform(entry[0].x), vr);
+            auto far_step = [&](int y, auto values, auto& k_to, auto& v_to, auto& k_from, auto& v_from) __attribute__((always_inline)) {
+                load(c.k, page_k, k_to);
+                load(c.v, page_v, v_to);
+                const int2 after = entry[y + 3];
+                const int block = entry[y + 1].y;
+                if (working) {
+                    __builtin_amdgcn_s_setprio(1);
+                    products(y, std::true_type{}, values);
+                    __builtin_amdgcn_s_setprio(0);
+                    softmax();
+                }
+                if (y + 1 < n) k_from.stage(smem + ((y + 1) & 1) * T::kKeyBytes, t);
+                v_from.stage(smem + (2 + (y & 1)) * T::kKeyBytes, t, &poison);
+                page_v = page_k;
+                page_k = y + 3 < n ? uniform(after.x) : -1;
+                base = uniform(block) * kKvBlock;
+                arrive();
+            };
+            far_step(0, std::false_type{}, k1, v1, kr, vr);
+            for (int y = 1; y < n;) {
+                far_step(y, std::true_type{}, kr, vr, k1, v1);
+                if (++y >= n) break;
+                far_step(y, std::true_type{}, k1, v1, kr, vr);
+                ++y;
+            }
+        } else {
+            step(0, std::false_type{});
+            for (int y = 1; y < n; ++y) step(y, std::true_type{});
+        }
         if (working) products(n, std::false_type{}, std::true_type{});
         if (T::kGroups == 2 && !behind) arrive();
     }
@@ -656,33 +713,11 @@ __device__ __forceinline__ uint4 load_once(const int8_t* p) {
     return __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p)));
 }
 
-// A block's keys (values) in 4 bits and their scales as buffers, which end behind the block: nothing of either is loaded if it
-// is not there.
-struct FourSpan {
-    __amdgpu_buffer_rsrc_t values, codes;
-    // (page < 0: not there)
-    __device__ __forceinline__ FourSpan(const uint8_t* v, const uint8_t* s, int heads, int h, int dim, int page) {
-        const int64_t tile = static_cast<int64_t>(page < 0 ? 0 : page) * heads + h;
-        values = span_bytes(v + tile * (kKvBlock * dim / 2), page < 0 ? 0 : kKvBlock * dim / 2);
-        codes = span_bytes(s + tile * (kKvBlock * dim / kFourGroup), page < 0 ? 0 : kKvBlock * dim / kFourGroup);
-    }
-};
-
-constexpr int kNonTemporal = 2;  // of a buffer load, as load_once (a query of 56 heads over 19721 tokens 34.3 us without, 30.4 so)
-
 // LDS operations of a wave are done in order: what the compiler may not change here.
 __device__ __forceinline__ void wave_order() {
     asm volatile("" ::: "memory");
     __builtin_amdgcn_wave_barrier();
     asm volatile("" ::: "memory");
-}
-
-template <class T>
-__device__ __forceinline__ T load_past(__amdgpu_buffer_rsrc_t b, int at) {
-    if constexpr (sizeof(T) == 16) return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b128(b, at, 0, kNonTemporal));
-    else if constexpr (sizeof(T) == 8) return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b64(b, at, 0, kNonTemporal));
-    else if constexpr (sizeof(T) == 4) return __builtin_amdgcn_raw_buffer_load_b32(b, at, 0, kNonTemporal);
-    else return __builtin_amdgcn_raw_buffer_load_b16(b, at, 0, kNonTemporal);
 }
 
 // What a lane (column col, lanes 16 quad ..) loads of a block in 4 bits, and the operands that it makes of them.  Of the keys,
@@ -744,7 +779,7 @@ struct FourFew {
         uint32_t w[4][kRuns * kWords], c[kRuns][4];
         Codes codes;
         __device__ __forceinline__ void load(const KvCache4& cache, int h, int page, int col, int quad) {
-            const FourSpan p(cache.k, cache.ks, cache.heads, h, D, page);
+            const FourPlace p(cache.k, cache.ks, cache.heads, h, D, page);
             codes.load(p.codes, 16 * quad + col);
             const int tok = 4 * (col & 3) + (col >> 2);
 #pragma unroll
@@ -790,7 +825,7 @@ struct FourFew {
         uint32_t w[16][N], c[16];
         Codes codes;
         __device__ __forceinline__ void load(const KvCache4& cache, int h, int page, int col, int quad) {
-            const FourSpan p(cache.v, cache.vs, cache.heads, h, D, page);
+            const FourPlace p(cache.v, cache.vs, cache.heads, h, D, page);
             codes.load(p.codes, 16 * quad + col);
             const int at = quad * (D / 2) + col * kBytes;
 #pragma unroll
