@@ -346,10 +346,12 @@ int h3mi_kv_write_mx4(const uint16_t* k, const uint16_t* v, int64_t rows, int64_
 int h3mi_kv_read_mx4_bf16(uint16_t* k, uint16_t* v, const int32_t* starts, int64_t length,
                           const h3mi_kv_cache4* cache, const h3mi_kv_seqs* seqs, void* stream);
 
-/* As h3mi_kv_attention_bf16, with the workspace that h3mi_kv_attention_workspace gives.
+/* As h3mi_kv_attention_bf16, with a workspace of h3mi_kv_attention_mx4_workspace bytes.
  * Keys and values are exact in the products.  A value group that stands for no number
  * makes NaNs of its 32 elements of the rows that see its token, a key group of all of
  * theirs. */
+int64_t h3mi_kv_attention_mx4_workspace(int64_t n, int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim,
+                                        int64_t blocks, int64_t top);
 int h3mi_kv_attention_mx4_bf16(const uint16_t* q, int64_t rows, int64_t heads, int64_t ld_q, int64_t bs_q,
                                const h3mi_kv_cache4* cache, const h3mi_kv_seqs* seqs, float scale, int causal,
                                const int32_t* blocks, int64_t top, uint16_t* out, void* workspace,

@@ -561,7 +561,8 @@ PyObject* kv_attention(PyObject*, PyObject* const* v, Py_ssize_t n) {
     {
         pybind11::gil_scoped_release nogil;
         out = a.empty(q.t->sizes(), c10::kBFloat16);
-        const int64_t need = h3mi_kv_attention_workspace(kv.s.n, q.rows, q.heads, kv.c.heads, kv.c.dim, kv.s.blocks, top);
+        const auto size = kv.four ? &h3mi_kv_attention_mx4_workspace : &h3mi_kv_attention_workspace;
+        const int64_t need = size(kv.s.n, q.rows, q.heads, kv.c.heads, kv.c.dim, kv.s.blocks, top);
         if (need > 0) work = a.empty({need}, c10::kByte);
         const auto attend = [&](const auto fn, const auto* c) {
             return fn(u16(q.t), q.rows, q.heads, q.ld, q.bs, c, &kv.s, static_cast<float>(scale), causal, list ? Kv::i32(list) : nullptr,

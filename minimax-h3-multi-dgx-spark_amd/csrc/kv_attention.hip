@@ -308,6 +308,7 @@ struct Items {
     uint32_t per_pack; // ceil(2^32 / pack)
     int count, whole, chunk, rest_chunk;
     bool flat, last_first;
+    int seqs;
     // Consecutive items on one XCD, whose L2 then holds their head's blocks.  flat (one round, every workgroup at once):
     // dealt out in order.
     __device__ __forceinline__ int of(int block, int tail_splits, int& split, int& splits) const {
@@ -323,13 +324,22 @@ struct Items {
     // x / pack: x < 128 pack where pack > 1, so that x times what per_pack is over 2^32 / pack stays below 2^32 / pack for
     // pack <= kMaxPack.
     __device__ __forceinline__ int row_of(int x) const { return pack == 1 ? x : static_cast<int>(__umulhi(static_cast<uint32_t>(x), per_pack)); }
-    // Of causal items those of a head's last rows, the longest, come first: first of all in a flat launch.
+    // Of causal items those of a head's last rows, the longest, come first: first of all in a flat launch.  MIX: where items are
+    // dealt out in runs those of a head's sequences are consecutive, not those of a sequence's heads, so that the XCDs' shares are
+    // alike however uneven the sequences are (8 of 1176 rows and up to 10228 tokens 1800 -> 1086 us, 16 of 2560 rows over
+    // themselves of 256 elements 2122 -> 1514).
+    template <bool MIX>
     __device__ __forceinline__ void place(int item, int& seq, int& head, int& tile) const {
         const int all = count / tiles, nh = flat ? item % all : item / tiles;
         tile = flat ? item / all : item % tiles;
         if (last_first) tile = tiles - 1 - tile;
-        seq = nh / heads;
-        head = nh % heads;
+        if (MIX && !flat) {
+            seq = nh % seqs;
+            head = nh / seqs;
+        } else {
+            seq = nh / heads;
+            head = nh % heads;
+        }
     }
 };
 
@@ -353,7 +363,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : D == 64 ? 3 : 2) void kv_til
     const int item = items.of(blockIdx.x, part.splits, split, splits);
     if (item >= items.count) return;
     int i, head, tile;
-    items.place(item, i, head, tile);
+    items.place<kFour>(item, i, head, tile);
     const int h = head * items.pack / (q.heads / c.heads);
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, col = lane & 31, half = lane >> 5;
 
@@ -1284,7 +1294,7 @@ constexpr int kMaxSplits = 64;  // of a tile, a lane of the join's wave each
 // splits at once.  (Two splits of 30720 rows of 64 elements: a wave a row 17.8 us, so 5.9.)
 constexpr int kFewSplits = 8;
 
-template <int D, bool FEW>
+template <int D, bool FEW, bool MIX>
 __global__ __launch_bounds__(256) void kv_join_kernel(Partial part, Queries q, Items items, uint32_t all,
                                                       uint16_t* __restrict__ out) {
     constexpr int L = D / 4, SG = 64 / L;
@@ -1294,7 +1304,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(Partial part, Queries q, I
     const uint32_t per = part.rows;
     const int item = static_cast<int>(x / per), r = static_cast<int>(x % per);
     int i, head, tile;
-    items.place(items.whole + item, i, head, tile);
+    items.place<MIX>(items.whole + item, i, head, tile);
     const int y = tile * part.rows + r, row = items.row_of(y);
     if (row >= q.rows) return;
     const int64_t query = (static_cast<int64_t>(i) * q.rows + row) * q.heads + head * items.pack + y - row * items.pack;
@@ -1429,8 +1439,27 @@ struct Plan {
     int64_t part_rows() const { return shares ? heads * (shares + items / heads) * rows + spans : splits > 1 ? (items - whole) * splits * rows : 0; }
 };
 
-// Sizes checked by the caller.
-Plan plan_of(int64_t n, int64_t rows, int64_t heads, int64_t kv, int64_t dim, int64_t blocks, int64_t top) {
+// How many pieces the blocks of `rest` items are split into over 4 bits: the least of what this makes of the launch, in steps of
+// a block (1 to 2 us).  A piece costs 3 beside its blocks, a join 4 and its bytes, 12 MB a step.  One sequence's items are alike
+// and go in rounds; of several, whose lengths are not known here, the lists are taken to be three quarters of the longest, the
+// pieces to be dealt out evenly, and the last one to come on top.  Against as many as fill one round: 1000 rows of 20 heads of 256
+// over 4000 tokens 182 -> 141 us, 3 sequences of 300 rows and up to 30000 tokens of 24 heads of 64 214 -> 145, of 150 rows and up
+// to 9000 of 56 of 128 231 -> 165; 200 rows of 40 heads over 9000 61.5 -> 62.0.
+int64_t four_splits(int64_t n, int64_t rest, int64_t slots, int64_t longest, int64_t item_bytes) {
+    int64_t best = 1;
+    double least = 0.0;
+    for (int64_t s = 1; s <= kMaxSplits && (s == 1 || longest / s >= 4); ++s) {
+        const int64_t rounds = (rest * s + slots - 1) / slots, piece = (longest + s - 1) / s;
+        double cost = n == 1 ? static_cast<double>(rounds * (piece + 3))
+                             : static_cast<double>(rest) * (0.75 * longest + 3.0 * s) / slots * (rounds > 1) + piece + 3;
+        if (s > 1) cost += 4.0 + static_cast<double>(rest * s * item_bytes) / 12e6;
+        if (s == 1 || cost < least) best = s, least = cost;
+    }
+    return best;
+}
+
+// Sizes checked by the caller.  four: of a cache in 4 bits.
+Plan plan_of(bool four, int64_t n, int64_t rows, int64_t heads, int64_t kv, int64_t dim, int64_t blocks, int64_t top) {
     Plan p = {};
     const int64_t cus = cu_count(), group = heads / kv;
     const int64_t longest = top > 0 ? top : blocks;  // blocks that a query may read
@@ -1473,6 +1502,7 @@ Plan plan_of(int64_t n, int64_t rows, int64_t heads, int64_t kv, int64_t dim, in
     int64_t splits = rest > 0 ? (longest >= 24 ? slots : cus) / rest : 1;
     if (splits > longest / 4) splits = longest / 4;
     if (splits > kMaxSplits) splits = kMaxSplits;
+    if (four && rest > 0) splits = four_splits(n, rest, slots, longest, p.rows * (dim * 4 + 8));
     if (splits <= 1) p.whole = p.items / 8 * 8, splits = 1;
     p.splits = static_cast<int>(splits);
     return p;
@@ -1489,10 +1519,23 @@ bool sizes_ok(int64_t n, int64_t rows, int64_t heads, int64_t kv, int64_t dim, i
 
 using namespace h3mi;
 
+namespace {
+
+int64_t workspace_of(bool four, int64_t n, int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim, int64_t blocks, int64_t top) {
+    if (!sizes_ok(n, rows, heads, kv_heads, dim, blocks, top) || n == 0 || rows == 0) return 0;
+    return plan_of(four, n, rows, heads, kv_heads, dim, blocks, top).part_rows() * (dim * 4 + 8);
+}
+
+}  // namespace
+
 extern "C" int64_t h3mi_kv_attention_workspace(int64_t n, int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim, int64_t blocks,
                                                int64_t top) {
-    if (!sizes_ok(n, rows, heads, kv_heads, dim, blocks, top) || n == 0 || rows == 0) return 0;
-    return plan_of(n, rows, heads, kv_heads, dim, blocks, top).part_rows() * (dim * 4 + 8);
+    return workspace_of(false, n, rows, heads, kv_heads, dim, blocks, top);
+}
+
+extern "C" int64_t h3mi_kv_attention_mx4_workspace(int64_t n, int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim, int64_t blocks,
+                                                   int64_t top) {
+    return workspace_of(true, n, rows, heads, kv_heads, dim, blocks, top);
 }
 
 namespace {
@@ -1527,7 +1570,8 @@ int attention(const uint16_t* q, int64_t rows, int64_t heads, int64_t ld_q, int6
     if (!aligned(out, 16) || !aligned(blocks, 4)) return fail(H3MI_EALIGN, "kv_attention: out must be 16-byte aligned, blocks 4-byte");
     const int64_t n = seqs->n, dim = cache->dim;
     if (!sizes_ok(n, rows, heads, cache->heads, dim, seqs->blocks, top)) return fail(H3MI_EINVAL, "kv_attention: too many rows for one call");
-    const Plan p = plan_of(n, rows, heads, cache->heads, dim, seqs->blocks, top);
+    constexpr bool kFour = std::is_same_v<C, KvCache4>;
+    const Plan p = plan_of(kFour, n, rows, heads, cache->heads, dim, seqs->blocks, top);
     const int64_t part_rows = p.part_rows(), need = part_rows * (dim * 4 + 8);
     const int64_t rest = (p.items - p.whole) * p.splits;
     if (p.items > (1 << 30) || rest > (1 << 30)) return fail(H3MI_EINVAL, "kv_attention: too many rows for one call");
@@ -1549,7 +1593,7 @@ int attention(const uint16_t* q, int64_t rows, int64_t heads, int64_t ld_q, int6
     Partial part = {static_cast<float*>(workspace), nullptr, p.shares ? p.shares + static_cast<int>(n) : p.splits, static_cast<int>(p.rows)};
     const Items items = {static_cast<int>(p.tiles), static_cast<int>(p.heads), p.pack, static_cast<int>(p.rows),
                          p.pack == 1 ? 0u : static_cast<uint32_t>(((uint64_t{1} << 32) + p.pack - 1) / p.pack), static_cast<int>(p.items),
-                         static_cast<int>(p.whole), static_cast<int>(p.whole / 8), static_cast<int>((rest + 7) / 8), p.flat, causal != 0};
+                         static_cast<int>(p.whole), static_cast<int>(p.whole / 8), static_cast<int>((rest + 7) / 8), p.flat, causal != 0, static_cast<int>(n)};
     if (need > 0) part.ml = reinterpret_cast<float2*>(part.o + (part_rows - p.spans) * dim);
     const C c = kv_cache(*cache);
     const KvSeqs s = kv_seqs(*seqs);
@@ -1585,8 +1629,8 @@ int attention(const uint16_t* q, int64_t rows, int64_t heads, int64_t ld_q, int6
     const bool few = p.splits <= kFewSplits;
     const int64_t a_group = few ? 1024 / dim : 4;
     if (!launchable((all + a_group - 1) / a_group, 1, 1, 256, &groups)) return fail(H3MI_EINVAL, "kv_attention: too many rows for one call");
-    const auto join = few ? (dim == 64 ? kv_join_kernel<64, true> : dim == 128 ? kv_join_kernel<128, true> : kv_join_kernel<256, true>)
-                          : (dim == 64 ? kv_join_kernel<64, false> : dim == 128 ? kv_join_kernel<128, false> : kv_join_kernel<256, false>);
+    const auto join = few ? (dim == 64 ? kv_join_kernel<64, true, kFour> : dim == 128 ? kv_join_kernel<128, true, kFour> : kv_join_kernel<256, true, kFour>)
+                          : (dim == 64 ? kv_join_kernel<64, false, kFour> : dim == 128 ? kv_join_kernel<128, false, kFour> : kv_join_kernel<256, false, kFour>);
     hipLaunchKernelGGL(join, dim3(static_cast<unsigned>(groups)), dim3(256), 0, st, part, qs, items,
                        static_cast<uint32_t>(all), out);
     return check_launch("kv_attention");

@@ -86,6 +86,7 @@ SIGNATURES = {
     "h3mi_kv_attention_bf16": [_P, _I, _I, _I, _I, _KC, _KS, _F, _C, _P, _I, _P, _P, _I, _P],
     "h3mi_kv_write_mx4": [_P, _P, _I, _I, _I, _I, _I, _KC4, _KS, _P],
     "h3mi_kv_read_mx4_bf16": [_P, _P, _P, _I, _KC4, _KS, _P],
+    "h3mi_kv_attention_mx4_workspace": [_I, _I, _I, _I, _I, _I, _I],
     "h3mi_kv_attention_mx4_bf16": [_P, _I, _I, _I, _I, _KC4, _KS, _F, _C, _P, _I, _P, _P, _I, _P],
     "h3mi_kv_extend": [_KP, _P, _P, _P, _I, _I, _I, _P, _P, _P, _P],
     "h3mi_kv_release": [_KP, _P, _P, _P, _I, _I, _P],
@@ -95,7 +96,8 @@ SIGNATURES = {
     "h3mi_debug_bf16_rne": [_P, _P, _I, _P],
     "h3mi_debug_buffer_lds_load": [_P, _I, _P, ctypes.c_int32, ctypes.c_int32, _P, _P],
 }
-_RESTYPE = {"h3mi_last_error": ctypes.c_char_p, "h3mi_kv_attention_workspace": _I, "h3mi_kv_select_workspace": _I}
+_RESTYPE = {"h3mi_last_error": ctypes.c_char_p, "h3mi_kv_attention_workspace": _I, "h3mi_kv_attention_mx4_workspace": _I,
+            "h3mi_kv_select_workspace": _I}
 
 
 class H3miError(RuntimeError):

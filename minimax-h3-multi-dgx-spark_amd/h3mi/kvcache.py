@@ -243,9 +243,10 @@ def kv_attention(q, cache, tables, lens, causal=False, counts=None, scale=None, 
         same_gpu(q, blocks=blocks)
     out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
     with torch.cuda.device(q.device):
-        need = lib.h3mi_kv_attention_workspace(s.n, rows, heads, c.heads, c.dim, s.blocks, top)
+        size, attend = ((lib.h3mi_kv_attention_mx4_workspace, lib.h3mi_kv_attention_mx4_bf16) if isinstance(cache, KVCache4) else
+                        (lib.h3mi_kv_attention_workspace, lib.h3mi_kv_attention_bf16))
+        need = size(s.n, rows, heads, c.heads, c.dim, s.blocks, top)
         work = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
-        attend = lib.h3mi_kv_attention_mx4_bf16 if isinstance(cache, KVCache4) else lib.h3mi_kv_attention_bf16
         check(attend(ptr(q), rows, heads, ld, bs, ctypes.byref(c), ctypes.byref(s), float(c.dim ** -0.5 if scale is None else scale),
                      int(bool(causal)), ptr(blocks), top, ptr(out), ptr(work), max(need, 0), stream_of(q)))
     return out

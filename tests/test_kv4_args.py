@@ -98,9 +98,9 @@ def test_null_structures(fn):
 
 
 def test_workspace():
-    """A call that splits its work refuses less than h3mi_kv_attention_workspace asks for, and one over what it reads or writes."""
+    """A call that splits its work refuses less than h3mi_kv_attention_mx4_workspace asks for, and one over what it reads or writes."""
     from h3mi import _lib
-    need = _lib.lib.h3mi_kv_attention_workspace(1, 1, 56, 56, 128, 309, 0)
+    need = _lib.lib.h3mi_kv_attention_mx4_workspace(1, 1, 56, 56, 128, 309, 0)
     assert need > 0
     cache, seqs = dict(heads=56, k=1 << 40, v=1 << 41, k_scale=1 << 42, v_scale=1 << 43), dict(n=1, blocks=309)
     kw = dict(rows=1, heads=56, ld=7168, bs=7168, p=1 << 44, out=1 << 45)
