@@ -155,8 +155,8 @@ def kv_write_(cache, k, v, tables, lens, counts=None):
     writes have to be distinct.
 
     4 bits: every 32 elements of a token have a power of two of their own, the least with which they fit, and are off by
-    half a step at most (a sixteenth of the largest of them, a seventh of it where that lies just above 5 steps): nothing
-    written before changes.  A NaN or an infinity makes its 32 elements read back as NaN.  The tokens that a call writes
+    half the distance of the values on either side, a fifth of the largest of them at most: nothing written before
+    changes.  A NaN or an infinity makes its 32 elements read back as NaN.  The tokens that a call writes
     have to be distinct."""
     done = _fast.kv_write_(cache, k, v, tables, lens, counts)
     if done is not None:
