@@ -1,4 +1,4 @@
-// Attention over the 8-bit key/value cache.
+// Attention over the key/value caches of 8 and of 4 bits.
 //
 // One pass over a sequence's blocks of 64 tokens with the running maximum m and sum l of
 // the softmax, in base 2:  x = (q . k) c_b, c_b = k_scale scale log2(e);  p = 2^(x - m);
@@ -17,6 +17,10 @@
 // those that the second product wants them in.  Rows of K are taken in the order that
 // makes the probabilities' registers whole runs of tokens; V is stored transposed, so that
 // its rows are runs of tokens too.  P never leaves the registers.
+//
+// In 4 bits a factor is a power of two and a value has two bits, so that their products are
+// exact in bf16 too and go into the MFMAs as they are: no factors of blocks, c = scale log2(e).
+// Values lie token by token there, and are transposed on their way, in pairs by permutes.
 //
 // Two kernels: tiles of 128 or 256 query rows of a head, bound by the MFMAs and the
 // softmax, and up to 64, 32 or 16 queries (of 64, 128, 256 elements) of a kv head's group,
@@ -1439,20 +1443,22 @@ struct Plan {
     int64_t part_rows() const { return shares ? heads * (shares + items / heads) * rows + spans : splits > 1 ? (items - whole) * splits * rows : 0; }
 };
 
-// How many pieces the blocks of `rest` items are split into over 4 bits: the least of what this makes of the launch, in steps of
-// a block (1 to 2 us).  A piece costs 3 beside its blocks, a join 4 and its bytes, 12 MB a step.  One sequence's items are alike
-// and go in rounds; of several, whose lengths are not known here, the lists are taken to be three quarters of the longest, the
-// pieces to be dealt out evenly, and the last one to come on top.  Against as many as fill one round: 1000 rows of 20 heads of 256
-// over 4000 tokens 182 -> 141 us, 3 sequences of 300 rows and up to 30000 tokens of 24 heads of 64 214 -> 145, of 150 rows and up
-// to 9000 of 56 of 128 231 -> 165; 200 rows of 40 heads over 9000 61.5 -> 62.0.
-int64_t four_splits(int64_t n, int64_t rest, int64_t slots, int64_t longest, int64_t item_bytes) {
+// How many pieces the blocks of `rest` items are split into over 4 bits: the least of what this makes of the launch, in us.  A block
+// takes a tile 1.0, 1.8 or 2.8 (64, 128, 256 elements), alone on its CU or with as many beside it as fit; a piece costs 4 beside its
+// blocks, a join 7 and its bytes.  One sequence's items are alike and go in rounds; of several, whose lengths are not known here,
+// the lists are taken to be six tenths of the longest, the pieces to be dealt out evenly, and the last one to come on top.  The
+// partial sums are at most what the memory-side cache holds.  Against as many pieces as fill one round: 1000 rows of 20 heads of
+// 256 over 4000 tokens 182 -> 141 us, 3 sequences of 300 rows and up to 30000 tokens of 24 heads of 64 214 -> 145, of 150 rows and
+// up to 9000 of 56 of 128 231 -> 165.
+int64_t four_splits(int64_t n, int64_t rest, int64_t slots, int64_t longest, int64_t dim, int64_t item_bytes) {
+    const double block = dim == 64 ? 1.0 : dim == 128 ? 1.8 : 2.8;
     int64_t best = 1;
     double least = 0.0;
-    for (int64_t s = 1; s <= kMaxSplits && (s == 1 || longest / s >= 4); ++s) {
-        const int64_t rounds = (rest * s + slots - 1) / slots, piece = (longest + s - 1) / s;
-        double cost = n == 1 ? static_cast<double>(rounds * (piece + 3))
-                             : static_cast<double>(rest) * (0.75 * longest + 3.0 * s) / slots * (rounds > 1) + piece + 3;
-        if (s > 1) cost += 4.0 + static_cast<double>(rest * s * item_bytes) / 12e6;
+    for (int64_t s = 1; s <= kMaxSplits && (s == 1 || (longest / s >= 4 && rest * s * item_bytes <= kMemoryCache)); ++s) {
+        const int64_t rounds = (rest * s + slots - 1) / slots;
+        const double piece = block * ((longest + s - 1) / s) + 4.0;
+        double cost = n == 1 ? rounds * piece : piece + (rounds > 1 ? rest * (0.6 * block * longest + 4.0 * s) / slots : 0.0);
+        if (s > 1) cost += 7.0 + rest * s * item_bytes / 7e6;
         if (s == 1 || cost < least) best = s, least = cost;
     }
     return best;
@@ -1502,7 +1508,7 @@ Plan plan_of(bool four, int64_t n, int64_t rows, int64_t heads, int64_t kv, int6
     int64_t splits = rest > 0 ? (longest >= 24 ? slots : cus) / rest : 1;
     if (splits > longest / 4) splits = longest / 4;
     if (splits > kMaxSplits) splits = kMaxSplits;
-    if (four && rest > 0) splits = four_splits(n, rest, slots, longest, p.rows * (dim * 4 + 8));
+    if (four && rest > 0) splits = four_splits(n, rest, slots, longest, dim, p.rows * (dim * 4 + 8));
     if (splits <= 1) p.whole = p.items / 8 * 8, splits = 1;
     p.splits = static_cast<int>(splits);
     return p;

@@ -14,13 +14,13 @@ CASES = {
     "64 elements, whole rounds and splits": (2, 900, 50, 10, 64, 40, 0, 32 * 10 * 128),
     "64 elements, lists": (2, 900, 60, 60, 64, 90, 40, 192 * 4 * 128),
     "64 elements, many splits": (3, 200, 2, 2, 64, 300, 0, 12 * 60 * 128),
-    "64 elements, more pieces than one round": (3, 271, 24, 24, 64, 500, 0, 216 * 20 * 128),
+    "64 elements, more pieces than one round": (3, 271, 24, 24, 64, 500, 0, 216 * 14 * 128),
     "128 elements, whole rounds and splits": (3, 700, 40, 8, 128, 60, 0, 208 * 2 * 128),
     "128 elements, lists": (3, 700, 40, 8, 128, 90, 30, 208 * 2 * 128),
     "128 elements, heads in common": (4, 100, 200, 40, 128, 30, 0, 128 * 4 * 128),
     "128 elements, whole rounds": (4, 300, 56, 56, 128, 7, 0, 0),
     "128 elements, 8 waves, more than a look-up": (3, 1100, 18, 18, 128, 1100, 0, 14 * 18 * 256),
-    "128 elements, 8 waves": (4, 1030, 18, 6, 128, 140, 0, 104 * 2 * 256),
+    "128 elements, 8 waves, more pieces than one round": (4, 1030, 18, 6, 128, 140, 0, 104 * 7 * 256),
     "256 elements": (2, 200, 30, 6, 256, 30, 0, 120 * 2 * 128),
     "256 elements, lists": (1, 1900, 20, 20, 256, 100, 40, 44 * 5 * 128),
     "256 elements, one sequence in rounds": (1, 1000, 20, 20, 256, 63, 0, 160 * 3 * 128),
