@@ -11,7 +11,8 @@
 // sines, one for each row and pair whatever the heads, are formed once for a workgroup's share of
 // the row's heads and kept in LDS.  A workgroup takes a few whole rows, or where there are few
 // rows a share of one's heads.  A thread takes 8 pairs of a head (4 interleaved ones): 16-byte
-// accesses whose lanes lie side by side.
+// accesses whose lanes lie side by side, or as many bytes as the turned part (or its half) divides
+// into.
 #include "kv.h"
 
 namespace h3mi {
@@ -40,8 +41,6 @@ constexpr int kRopeThreads = 256;
 constexpr int kRopeAhead = 4;   // units that a thread has in flight (2 and 8: 1% and 4% slower)
 constexpr int kRopeTokens = 16;
 
-enum RopeForm { kHalves, kPairs, kOne };
-
 // How rows go through the caches.  kCached: rows in place that the memory-side cache may hold.  kStore: new tensors, written past
 // the L2 (2401 rows of 112 heads, the memory-side cache full of others 31.5 us, 28.6 so; else 24.2 and 24.6).  kPast: rows that
 // are more than that cache holds beside others, read past it too (19200 in place 217 us, 191 so; 2401 of 48 heads of 4 sequences
@@ -49,16 +48,38 @@ enum RopeForm { kHalves, kPairs, kOne };
 enum RopeWay { kCached, kStore, kPast };
 constexpr int64_t kRopePast = kMemoryCache / 4 * 3;
 
-template <bool PAST>
-__device__ __forceinline__ void store_row(uint16_t* p, uint4 v) {
-    if constexpr (PAST) store_past(p, v);
-    else *reinterpret_cast<uint4*>(p) = v;
-}
-
-// What a thread holds of a unit: 8 elements and their partners 8 chunks on (kHalves), 8 elements (kPairs), two (kOne).
-template <RopeForm F>
-struct Unit {
-    uint4 a, b;
+// V neighbouring elements, one access.
+template <int V>
+struct Run {
+    uint32_t w[V == 1 ? 1 : V / 2];
+    template <bool PAST>
+    __device__ __forceinline__ void load(const uint16_t* p) {
+        if constexpr (V == 8) {
+            const uint4 x = load_row<PAST>(p);
+            w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+        } else if constexpr (V == 4) {
+            const uint2 x = *reinterpret_cast<const uint2*>(p);
+            w[0] = x.x, w[1] = x.y;
+        } else if constexpr (V == 2) {
+            w[0] = *reinterpret_cast<const uint32_t*>(p);
+        } else {
+            w[0] = *p;
+        }
+    }
+    template <bool PAST>
+    __device__ __forceinline__ void store(uint16_t* p) const {
+        if constexpr (V == 8) {
+            const uint4 x = make_uint4(w[0], w[1], w[2], w[3]);
+            if constexpr (PAST) store_past(p, x);
+            else *reinterpret_cast<uint4*>(p) = x;
+        } else if constexpr (V == 4) {
+            *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+        } else if constexpr (V == 2) {
+            *reinterpret_cast<uint32_t*>(p) = w[0];
+        } else {
+            *p = static_cast<uint16_t>(w[0]);
+        }
+    }
 };
 
 __device__ __forceinline__ void turn(float x, float y, float2 cs, float& u, float& v) {
@@ -66,38 +87,35 @@ __device__ __forceinline__ void turn(float x, float y, float2 cs, float& u, floa
     v = __builtin_fmaf(x, cs.y, y * cs.x);
 }
 
-// tab: (c, s) of the unit's first pair
-template <RopeForm F>
-__device__ __forceinline__ void turn(Unit<F>& x, const float2* tab) {
-    if constexpr (F == kHalves) {
-        uint32_t* const a = &x.a.x;
-        uint32_t* const b = &x.b.x;
+// A unit's pairs; tab: (c, s) of its first.  PAIRS: neighbours in a, else a and b.
+template <bool PAIRS, int V>
+__device__ __forceinline__ void turn(Run<V>& a, Run<V>& b, const float2* tab) {
+    if constexpr (PAIRS) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            float u0, v0, u1, v1;
-            turn(bf16_lo(a[j]), bf16_lo(b[j]), tab[2 * j], u0, v0);
-            turn(bf16_hi(a[j]), bf16_hi(b[j]), tab[2 * j + 1], u1, v1);
-            a[j] = bf16x2_bits(u0, u1);
-            b[j] = bf16x2_bits(v0, v1);
-        }
-    } else if constexpr (F == kPairs) {
-        uint32_t* const a = &x.a.x;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < V / 2; ++j) {
             float u, v;
-            turn(bf16_lo(a[j]), bf16_hi(a[j]), tab[j], u, v);
-            a[j] = bf16x2_bits(u, v);
+            turn(bf16_lo(a.w[j]), bf16_hi(a.w[j]), tab[j], u, v);
+            a.w[j] = bf16x2_bits(u, v);
         }
-    } else {
+    } else if constexpr (V == 1) {
         float u, v;
-        turn(bf16_f32(x.a.x), bf16_f32(x.b.x), tab[0], u, v);
-        x.a.x = bf16_bits(u);
-        x.b.x = bf16_bits(v);
+        turn(bf16_f32(a.w[0]), bf16_f32(b.w[0]), tab[0], u, v);
+        a.w[0] = bf16_bits(u), b.w[0] = bf16_bits(v);
+    } else {
+#pragma unroll
+        for (int j = 0; j < V / 2; ++j) {
+            float u0, v0, u1, v1;
+            turn(bf16_lo(a.w[j]), bf16_lo(b.w[j]), tab[2 * j], u0, v0);
+            turn(bf16_hi(a.w[j]), bf16_hi(b.w[j]), tab[2 * j + 1], u1, v1);
+            a.w[j] = bf16x2_bits(u0, u1);
+            b.w[j] = bf16x2_bits(v0, v1);
+        }
     }
 }
 
-template <RopeForm F, RopeWay W>
-__global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeCall c, int interleaved) {
+// A unit: V pairs of halves, V / 2 of neighbours, or as many elements that are copied.
+template <bool PAIRS, int V, RopeWay W>
+__global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeCall c) {
     extern __shared__ float2 tab[];  // [tokens, rot / 2]: (c, s)
     __shared__ bool real[kRopeTokens];  // rows that a position was given for
     const int half = c.rot / 2, t = threadIdx.x;
@@ -126,19 +144,11 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeCall c, int inte
     const int lanes = kRopeThreads / c.units, unit = t % c.units, lane = t / c.units;
     if (lane >= lanes) return;
     const bool turned = unit < c.turned;
-    // elements of the unit: a at `at`, b at `at + apart`
-    int at, apart = 0;
-    if (turned) {
-        at = F == kOne ? (interleaved ? 2 * unit : unit) : 8 * unit;
-        apart = F == kPairs ? 0 : F == kOne && interleaved ? 1 : half;
-    } else {
-        at = F == kOne ? c.rot + 2 * (unit - c.turned) : c.rot + 8 * (unit - c.turned) * (F == kHalves ? 2 : 1);
-        apart = F == kOne ? 1 : 8;
-    }
-    // (the last copied unit of kHalves may have 8 elements alone)
-    const bool two = F == kOne || (F == kHalves && at + apart < c.dim);
+    // its elements: a at `at`, and of halves b at `at + apart`
+    const int at = turned ? V * unit : c.rot + (PAIRS ? V : 2 * V) * (unit - c.turned), apart = turned ? half : V;
+    const bool two = !PAIRS && at + apart < c.dim;  // (the last copied unit may have V elements alone)
     for (int x0 = lane; x0 < tokens * mine; x0 += lanes * kRopeAhead) {
-        Unit<F> y[kRopeAhead];
+        Run<V> y[kRopeAhead], z[kRopeAhead];
         uint16_t* to[kRopeAhead];
         int tok[kRopeAhead];
 #pragma unroll
@@ -151,30 +161,20 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeCall c, int inte
             const uint32_t row = first + tok[j], i = row / c.rows, r = row - i * c.rows;
             if (c.in_place && !real[tok[j]]) continue;
             const bool of_q = h < c.q.heads;
-            const RopeRows& z = of_q ? c.q : c.k;
+            const RopeRows& rows = of_q ? c.q : c.k;
             const int64_t el = static_cast<int64_t>(of_q ? h : h - c.q.heads) * c.dim + at;
-            const uint16_t* const from = z.in + i * z.bs_in + r * z.ld_in + el;
-            to[j] = z.out + i * z.bs_out + r * z.ld_out + el;
+            const uint16_t* const from = rows.in + i * rows.bs_in + r * rows.ld_in + el;
+            to[j] = rows.out + i * rows.bs_out + r * rows.ld_out + el;
             if (!(turned && real[tok[j]])) tok[j] = -1;
-            if constexpr (F == kOne) {
-                y[j].a.x = from[0];
-                y[j].b.x = from[apart];
-            } else {
-                y[j].a = load_row<W == kPast>(from);
-                if (two) y[j].b = load_row<W == kPast>(from + apart);
-            }
+            y[j].template load<W == kPast>(from);
+            if (two) z[j].template load<W == kPast>(from + apart);
         }
 #pragma unroll
         for (int j = 0; j < kRopeAhead; ++j) {
             if (!to[j]) continue;
-            if (tok[j] >= 0) turn<F>(y[j], tab + tok[j] * half + unit * (F == kHalves ? 8 : F == kPairs ? 4 : 1));
-            if constexpr (F == kOne) {
-                to[j][0] = static_cast<uint16_t>(y[j].a.x);
-                to[j][apart] = static_cast<uint16_t>(y[j].b.x);
-            } else {
-                store_row<W != kCached>(to[j], y[j].a);
-                if (two) store_row<W != kCached>(to[j] + apart, y[j].b);
-            }
+            if (tok[j] >= 0) turn<PAIRS, V>(y[j], z[j], tab + tok[j] * half + unit * (PAIRS ? V / 2 : V));
+            y[j].template store<W != kCached>(to[j]);
+            if (two) z[j].template store<W != kCached>(to[j] + apart);
         }
     }
 }
@@ -250,7 +250,10 @@ extern "C" int h3mi_rope_bf16(const h3mi_rope_rows* q, const h3mi_rope_rows* k, 
         return fail(H3MI_EALIAS, "rope: q and k overlap");
     if (k && (k->in == k->out) != (q->in == q->out)) return fail(H3MI_EINVAL, "rope: q and k must both be in place, or neither");
 
-    const RopeForm form = interleaved ? (rot % 8 ? kOne : kPairs) : (rot % 16 ? kOne : kHalves);
+    // The widest accesses that the turned part fills, or each of its halves (2261 rows in place of 80 heads of 256, 128 of them
+    // turned: 20 us in 8; 120, in 4: 23; 124: in pairs, by 4, 28, else by 2 27; 126: pairs by 2 37, else singly 39, which is
+    // what all but the first took singly, 40 to 45).
+    const int64_t run = interleaved ? rot : rot / 2, V = run % 8 == 0 ? 8 : run % 4 == 0 ? 4 : run % 2 == 0 ? 2 : 1;
     RopeCall c = {};
     const auto side = [](const h3mi_rope_rows& x) { return RopeRows{x.in, x.out, static_cast<int>(x.heads), x.ld_in, x.bs_in, x.ld_out, x.bs_out}; };
     c.q = side(*q);
@@ -260,9 +263,9 @@ extern "C" int h3mi_rope_bf16(const h3mi_rope_rows* q, const h3mi_rope_rows* k, 
     c.dim = static_cast<int>(dim), c.rot = static_cast<int>(rot);
     c.amplitude = amplitude, c.sign = inverse ? -amplitude : amplitude;
     c.in_place = q->in == q->out;
-    c.turned = static_cast<int>(form == kHalves ? rot / 16 : form == kPairs ? rot / 8 : rot / 2);
+    c.turned = static_cast<int>(run / V);
     const int64_t rest = c.in_place ? 0 : dim - rot;
-    c.units = c.turned + static_cast<int>(form == kHalves ? (rest + 15) / 16 : form == kPairs ? rest / 8 : rest / 2);
+    c.units = c.turned + static_cast<int>(interleaved ? rest / V : (rest + 2 * V - 1) / (2 * V));
     // Rows until a thread has kRopeAhead units, as far as there are workgroups for every CU; else a share of a row's heads.
     const int64_t heads = q->heads + (k ? k->heads : 0), a_round = kRopeThreads / c.units, want = a_round * kRopeAhead, cus = cu_count();
     int64_t tokens = want / heads;
@@ -280,9 +283,12 @@ extern "C" int h3mi_rope_bf16(const h3mi_rope_rows* q, const h3mi_rope_rows* k, 
     if (groups * kRopeThreads >= (int64_t{1} << 32)) return fail(H3MI_EINVAL, "rope: too many rows for one call");
     const size_t lds = static_cast<size_t>(tokens) * (rot / 2) * 8;
     const RopeWay way = c.all * heads * dim * (c.in_place ? 2 : 4) > kRopePast ? kPast : c.in_place ? kCached : kStore;
-    const auto halves = way == kCached ? rope_kernel<kHalves, kCached> : way == kStore ? rope_kernel<kHalves, kStore> : rope_kernel<kHalves, kPast>;
-    const auto pairs = way == kCached ? rope_kernel<kPairs, kCached> : way == kStore ? rope_kernel<kPairs, kStore> : rope_kernel<kPairs, kPast>;
-    const auto fn = form == kHalves ? halves : form == kPairs ? pairs : rope_kernel<kOne, kCached>;
-    hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(groups)), dim3(kRopeThreads), lds, as_stream(stream), c, interleaved != 0);
+    const auto wide = interleaved ? (way == kCached ? rope_kernel<true, 8, kCached> : way == kStore ? rope_kernel<true, 8, kStore> : rope_kernel<true, 8, kPast>)
+                                  : (way == kCached ? rope_kernel<false, 8, kCached> : way == kStore ? rope_kernel<false, 8, kStore> : rope_kernel<false, 8, kPast>);
+    const auto fn = V == 8 ? wide
+                  : V == 4 ? (interleaved ? rope_kernel<true, 4, kCached> : rope_kernel<false, 4, kCached>)
+                  : V == 2 ? (interleaved ? rope_kernel<true, 2, kCached> : rope_kernel<false, 2, kCached>)
+                           : rope_kernel<false, 1, kCached>;
+    hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(groups)), dim3(kRopeThreads), lds, as_stream(stream), c);
     return check_launch("rope");
 }

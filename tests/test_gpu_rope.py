@@ -48,7 +48,7 @@ def _check(got, x, positions, freqs, interleaved, inverse, amplitude):
 
 
 @pytest.mark.parametrize("dim,rot", [(128, 128), (128, 64), (128, 32), (128, 96), (64, 64), (64, 16), (256, 256), (80, 80), (80, 48), (72, 16), (128, 126),
-                                     (128, 2), (64, 24), (40, 40), (8, 8), (8, 2), (512, 512), (512, 510), (104, 40)])
+                                     (128, 2), (64, 24), (40, 40), (8, 8), (8, 2), (512, 512), (512, 510), (104, 40), (128, 124), (64, 4), (72, 60)])
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("n,rows,hq,hk", [(1, 1, 3, 3), (3, 37, 5, 1), (2, 300, 2, 4)])
 def test_rope(dim, rot, interleaved, n, rows, hq, hk):
@@ -87,7 +87,8 @@ def test_far_positions(interleaved):
 
 
 @pytest.mark.parametrize("n,rows,hq,hk,dim,rot", [(1, 3001, 56, 56, 128, 128), (4, 701, 40, 8, 128, 64), (300, 1, 40, 8, 128, 128), (1, 9001, 1, 1, 64, 64),
-                                                  (1, 1, 600, 300, 256, 256), (2, 1500, 24, 24, 64, 32), (1, 5, 56, 56, 128, 126)])
+                                                  (1, 1, 600, 300, 256, 256), (2, 1500, 24, 24, 64, 32), (1, 5, 56, 56, 128, 126),
+                                                  (2, 1500, 24, 24, 64, 12)])
 @pytest.mark.parametrize("interleaved", [False, True])
 def test_every_split_of_the_rows(n, rows, hq, hk, dim, rot, interleaved):
     """Many rows to a workgroup, many workgroups to a row."""
