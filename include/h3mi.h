@@ -348,9 +348,10 @@ int h3mi_kv_read_mx4_bf16(uint16_t* k, uint16_t* v, const int32_t* starts, int64
 
 /* As h3mi_kv_attention_bf16, with a workspace of h3mi_kv_attention_mx4_workspace bytes.
  * Keys and values are exact in the products, whose sums are formed before the scale: queries
- * and keys whose product passes 2^127 have no finite score.  A value group that stands for no number
- * makes NaNs of its 32 elements of the rows that see its token, a key group of all of
- * theirs. */
+ * and keys whose product passes 2^127 have no finite score, and as a probability's weight may
+ * be 2^8, values of 2^119 over the number of tokens and more may have no finite sum.  A value
+ * group that stands for no number makes NaNs of its 32 elements of the rows that see its
+ * token, a key group of all of theirs. */
 int64_t h3mi_kv_attention_mx4_workspace(int64_t n, int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim,
                                         int64_t blocks, int64_t top);
 int h3mi_kv_attention_mx4_bf16(const uint16_t* q, int64_t rows, int64_t heads, int64_t ld_q, int64_t bs_q,

@@ -214,6 +214,29 @@ def test_attention_with_holes(rows, blocks, causal):
     _check(ref, q, tables, lens, counts, causal)
 
 
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("rows", [1, 40, 150])
+def test_every_code(dim, rows):
+    """Every scale code with every 4-bit value, read back and as the one token that a sequence's rows see, whose values are
+    then the result: exact where they are normal numbers (codes of 2 and more; what is written has no others)."""
+    h = _h()
+    ref = R4.Cache4(256, 1, dim)
+    ref.v[:] = np.tile(np.arange(0x10, 0x100, 0x22, dtype=np.uint8), dim // 16 + 1)[:dim // 2]
+    ref.k[:, :, 0] = ref.v[:, :, 0]
+    ref.ks[:] = np.arange(256, dtype=np.uint8)[:, None, None, None]
+    ref.vs[:] = ref.ks
+    assert set(np.concatenate([ref.v & 15, ref.v >> 4], None)) == set(range(16))
+    cache, tables, lens = ref.to(), _i32(np.arange(256)[:, None]), _i32([1] * 256)
+    want = R4.values(ref.v[:, :, 0], ref.vs[:, :, :, 0])[:, None]
+    k, v = h.kv_read(cache, tables, lens, 1)
+    for x in (k, v):
+        assert np.array_equal(x.double().cpu().numpy(), want, equal_nan=True)
+    cache.k_scale.fill_(127)
+    out = h.kv_attention(_bf(np.ones((256, rows, 1, dim))), cache, tables, lens).double().cpu().numpy()
+    assert np.array_equal(out[2:], np.broadcast_to(want, out.shape)[2:], equal_nan=True)
+    assert (np.abs(out[:2] - want[:2]) <= 2.0 ** -126).all()
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.2, 1e-30, 30.0])
 @pytest.mark.parametrize("rows", [2, 140])
 def test_scales_and_views(rows, scale):
