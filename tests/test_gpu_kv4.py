@@ -352,6 +352,47 @@ def test_steep_factors():
         assert torch.equal(out, x.expand(1, rows, 1, 64))
 
 
+def test_pages_past_32_bits():
+    """A cache of more than 2^32 bytes of keys gives what a small one with the same pages gives."""
+    h = _h()
+    rng = np.random.default_rng(32)
+    heads, dim, blocks = 56, 128, 9
+    pages = 2 ** 32 // (heads * 64 * dim // 2) + 2 * blocks
+    small, far = h.kv_cache(2 * blocks, heads, dim, bits=4), h.kv_cache(pages, heads, dim, bits=4)
+    near = _i32(rng.permutation(2 * blocks).reshape(2, blocks))
+    tables, lens = near + (pages - 2 * blocks), _i32([blocks * 64, 400])
+    k, v = (torch.randn((2, 400, heads, dim), device=DEV, dtype=torch.bfloat16) for _ in range(2))
+    got = []
+    for cache, t in ((small, near), (far, tables)):
+        h.kv_write_(cache, k, v, t, lens)
+        got.append([*h.kv_read(cache, t, lens, blocks * 64)] + [h.kv_attention(k[:, :rows], cache, t, lens, True) for rows in (1, 40, 300)])
+    for x, y in zip(*got):
+        assert torch.equal(x, y)
+    assert torch.equal(small.k, far.k[pages - 2 * blocks:]) and torch.equal(small.v_scale, far.v_scale[pages - 2 * blocks:])
+
+
+def test_rows_past_32_bits():
+    """Of tensors of more than 2^32 bytes the last rows are what they are alone."""
+    h = _h()
+    rows, heads, dim, some = 300_000, 56, 128, 1280
+    blocks = -(-rows // 64)
+    x = torch.empty((1, rows, heads, dim), device=DEV, dtype=torch.bfloat16).normal_()
+    assert x.numel() * 2 > 2 ** 32
+    cache, tables, lens = h.kv_cache(blocks, heads, dim, bits=4), _i32(np.arange(blocks)[None]), _i32([rows])
+    h.kv_write_(cache, x, x, tables, lens)
+    assert torch.equal(cache.k, cache.v) and torch.equal(cache.k_scale, cache.v_scale)
+    k, _ = h.kv_read(cache, tables, lens, rows)
+    tail, _ = h.kv_read(cache, tables, lens, some, starts=_i32([rows - some]))
+    assert torch.equal(k[:, -some:], tail)
+    del k
+    alone = h.kv_cache(blocks, heads, dim, bits=4)
+    h.kv_write_(alone, x[:, -some:], x[:, -some:], tables, lens)
+    assert torch.equal(h.kv_read(alone, tables, lens, some, starts=_i32([rows - some]))[0], tail)
+    few = _i32([37])  # one block: a row's result is its own, whatever rows share its tile
+    out = h.kv_attention(x, cache, tables[:, :1].contiguous(), few)
+    assert torch.equal(out[:, -some:], h.kv_attention(x[:, -some:], cache, tables[:, :1].contiguous(), few))
+
+
 def test_other_streams_and_devices_tensors():
     """Calls on a side stream follow what it did before; a native call and the checked one give the same."""
     h = _h()

@@ -213,6 +213,20 @@ def test_captured_and_streams():
         assert all(torch.equal(a, b) and torch.equal(c, b) for a, b, c in zip(out, want, beside)), r
 
 
+def test_rows_past_32_bits():
+    """Of tensors of more than 2^32 bytes the last rows are turned as they are alone, in place and into new ones."""
+    h = _h()
+    rows, heads, some = 300_000, 56, 50
+    x = torch.empty((1, rows, heads, 128), device=DEV, dtype=torch.bfloat16).normal_()
+    assert x.numel() * 2 > 2 ** 32
+    freqs, _ = h.rotary_frequencies(128)
+    positions = torch.arange(rows, dtype=torch.int32, device=DEV)[None]
+    want = h.rotary(x[:, -some:], None, positions[:, -some:].contiguous(), freqs)[0]
+    assert torch.equal(h.rotary(x, None, positions, freqs)[0][:, -some:], want)
+    h.rotary_(x, None, positions, freqs)
+    assert torch.equal(x[:, -some:], want)
+
+
 def test_refusals():
     h = _h()
     freqs, _ = h.rotary_frequencies(64)
