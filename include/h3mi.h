@@ -404,7 +404,9 @@ typedef struct h3mi_rope_rows {
  * and so are rows with p < 0.  inverse is the transpose: what a gradient goes through.
  * k NULL: none.  dim a multiple of 8 up to 512, rot even, 2 to dim; pointers 16-byte
  * aligned, strides multiples of 8 and no shorter than a row.  q and k may be views of
- * one buffer whose rows do not overlap, but not of what else the call reads or writes. */
+ * one buffer, but not of what else the call reads or writes: with equal strides, one a
+ * multiple of the other, and no element in both, or with whole sequences (of equal
+ * bs), or what all sequences have of a token (of equal ld), apart. */
 int h3mi_rope_bf16(const h3mi_rope_rows* q, const h3mi_rope_rows* k, const int32_t* positions, const double* freqs,
                    int64_t n, int64_t rows, int64_t dim, int64_t rot, int interleaved, int inverse, float amplitude,
                    void* stream);

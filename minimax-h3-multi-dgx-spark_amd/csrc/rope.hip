@@ -204,18 +204,26 @@ int check_rows(const char* name, const h3mi_rope_rows& x, int64_t n, int64_t row
     return H3MI_OK;
 }
 
-// Whether rows of a and b share an element.  Rows of equal strides, as views of one projection's output, may lie between
-// each other's.
+// Whether runs of run_a elements every `step` of them meet runs of run_b that lie d behind.
+bool runs_meet(int64_t d, int64_t step, int64_t run_a, int64_t run_b) {
+    d %= step;
+    if (d < 0) d += step;
+    return d < run_a || d + run_b > step;
+}
+
+// Whether rows of a and b share an element; of one buffer they are known not to in views of a projection's output, and where
+// whole sequences, or what all sequences have of a token, lie apart.
 bool rows_meet(const uint16_t* a, int64_t ha, int64_t lda, int64_t bsa, const uint16_t* b, int64_t hb, int64_t ldb, int64_t bsb,
                int64_t n, int64_t rows, int64_t dim) {
     const h3mi_rope_rows x = {a, nullptr, ha, lda, bsa, 0, 0}, y = {b, nullptr, hb, ldb, bsb, 0, 0};
     if (!overlap(a, span_of(x, false, n, rows, dim), b, span_of(y, false, n, rows, dim))) return false;
-    if ((rows > 1 && lda != ldb) || (n > 1 && bsa != bsb) || (rows == 1 && n == 1)) return true;
-    const int64_t step = rows == 1 ? bsa : n == 1 || lda < bsa ? lda : bsa;
-    if (n > 1 && rows > 1 && (lda < bsa ? bsa : lda) % step) return true;
-    int64_t d = (reinterpret_cast<intptr_t>(b) - reinterpret_cast<intptr_t>(a)) / 2 % step;
-    if (d < 0) d += step;
-    return d < ha * dim || d + hb * dim > step;
+    const int64_t d = (reinterpret_cast<intptr_t>(b) - reinterpret_cast<intptr_t>(a)) / 2, ea = ha * dim, eb = hb * dim;
+    if (n > 1 && bsa == bsb && !runs_meet(d, bsa, (rows - 1) * lda + ea, (rows - 1) * ldb + eb)) return false;
+    if (rows > 1 && lda == ldb && !runs_meet(d, lda, (n - 1) * bsa + ea, (n - 1) * bsb + eb)) return false;
+    // equal strides, one a multiple of the other: rows between each other's
+    if (n == 1 || rows == 1 || lda != ldb || bsa != bsb) return true;
+    const int64_t step = lda < bsa ? lda : bsa;
+    return (lda + bsa - step) % step || runs_meet(d, step, ea, eb);
 }
 
 }  // namespace

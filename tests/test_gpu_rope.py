@@ -128,6 +128,28 @@ def test_sequences_between_each_other():
         _check(t, x.transpose(0, 1), positions, freqs, False, False, 1.0)
 
 
+@pytest.mark.parametrize("hq,hk", [(4, 4), (5, 2)])
+def test_q_and_k_of_one_buffer(hq, hk):
+    """All of a sequence's q rows before its k rows, all of a token's: in place, with heads of their own."""
+    h = _h()
+    rng = np.random.default_rng(16)
+    n, rows, dim = 3, 37, 128
+    freqs, _ = h.rotary_frequencies(dim, device="cpu")
+    positions = torch.from_numpy(rng.integers(-1, 9999, (n, rows))).to(torch.int32)
+    for tokens_first in (False, True):
+        a, b = (rows, n) if tokens_first else (n, rows)
+        x = _bf(rng, a, b * (hq + hk) * dim)
+        d = x.to(DEV)
+
+        def sides(t):
+            two = t[:, :b * hq * dim].unflatten(1, (b, hq, dim)), t[:, b * hq * dim:].unflatten(1, (b, hk, dim))
+            return [s.transpose(0, 1) for s in two] if tokens_first else two
+
+        h.rotary_(*sides(d), positions.to(DEV), freqs.to(DEV))
+        for got, was in zip(sides(d), sides(x)):
+            _check(got, was, positions, freqs, False, False, 1.0)
+
+
 def test_inverse_is_the_gradient():
     """<g, R x> = <R' g, x>, and differences of R along a direction; to the roundings of both sides."""
     h = _h()

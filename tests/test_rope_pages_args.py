@@ -52,6 +52,50 @@ def test_rope_rows_between_each_other():
             assert (rc, "both be in place" in m, "q and k overlap" in m) == ((1, True, False) if want else (3, False, True)), (strides, heads, m)
 
 
+def _apart(qs, ks, at, n, rows, qh=4, kh=4):
+    """(whether q and k in place, k `at` elements behind q, are taken for apart, whether they are), dim 128.  q's result goes
+    elsewhere and k's does not, which is refused once the rows have been looked at, so that nothing is launched."""
+    base = 1 << 24
+    sides = [dict(ld_in=ld, ld_out=ld, bs_in=bs, bs_out=bs) for ld, bs in (qs, ks)]
+    # the other order has the same rows: k's result beside q's rows
+    rc, m = _rope(dict(sides[0], heads=qh, in_=base, out=1 << 40), dict(sides[1], heads=kh, in_=base + 2 * at, out=base + 2 * at), n=n, rows=rows)
+    assert (rc, "both be in place" in m) == (1, True) or (rc == 3 and "q and k overlap" in m), (rc, m)
+    taken = set()
+    for (ld, bs), h, off in ((qs, qh, 0), (ks, kh, at)):
+        runs = {off + i * bs + r * ld + x for i in range(n) for r in range(rows) for x in range(0, 128 * h, 8)}
+        if taken & runs:
+            return rc == 1, False
+        taken |= runs
+    return rc == 1, True
+
+
+@pytest.mark.parametrize("n,rows", [(2, 5), (3, 4), (1, 5), (4, 1), (2, 2)])
+def test_rope_rows_of_one_buffer(n, rows):
+    """q and k of one buffer are taken as long as no element is in both: side by side in a row, all of a sequence's q rows before
+    its k rows, tokens before sequences, and with heads of their own."""
+    e, w = 512, 1024  # 4 heads, 8 heads
+    layouts = [
+        ((2 * e, 2 * e * rows), (2 * e, 2 * e * rows), e, 4, 4),              # [n, rows, 2, e]
+        ((e, 2 * e * rows), (e, 2 * e * rows), e * rows, 4, 4),               # [n, 2, rows, e]
+        ((e * n, e), (e * n, e), e * n * rows, 4, 4),                         # [2, rows, n, e]
+        ((2 * e * n, e), (2 * e * n, e), e * n, 4, 4),                        # [rows, 2, n, e]
+        ((w, (w + e) * rows), (e, (w + e) * rows), w * rows, 8, 4),           # [n, (rows of 8 heads, rows of 4)]
+        ((e, (w + e) * rows), (w, (w + e) * rows), e * rows, 4, 8),           # [n, (rows of 4, rows of 8)]
+        (((w + e) * n, w), ((w + e) * n, e), w * n, 8, 4),                    # [rows, (n of 8 heads, n of 4)]
+        ((e, 2 * e * rows + 64), (e, 2 * e * rows + 64), e * rows + 32, 4, 4),  # sequences with room between them
+    ]
+    for qs, ks, at, qh, kh in layouts:
+        for order in (1, -1):
+            a, b = ((qs, qh), (ks, kh)) if order == 1 else ((ks, kh), (qs, qh))
+            got = _apart(a[0], b[0], order * at, n, rows, a[1], b[1])
+            assert got == (True, True), (qs, ks, at, order, got)
+    # and never where an element is in both
+    for qs, ks, at, qh, kh in layouts:
+        for shift in (-8, 8, e // 2, -e // 2, e, -e):
+            taken, apart = _apart(qs, ks, at + shift, n, rows, qh, kh)
+            assert apart or not taken, (qs, ks, at, shift)
+
+
 def _pages(fn, pool=None, **kw):
     from h3mi import _lib
     p = {**dict(free=1 << 20, count=1 << 21, pages=100), **(pool or {})}
