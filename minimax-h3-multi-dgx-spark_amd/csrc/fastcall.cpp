@@ -96,6 +96,15 @@ const uint16_t* u16(const at::Tensor* t) { return t ? static_cast<const uint16_t
 uint16_t* mu16(const at::Tensor& t) { return static_cast<uint16_t*>(t.data_ptr()); }
 const float* f32(const at::Tensor* t) { return static_cast<const float*>(t->data_ptr()); }
 
+// The library has written into a caller's tensor: its version moves on, as after torch's own in-place operations, so that
+// autograd refuses what it saved of it and prequant.take sees the change.  (A tensor of inference mode has no version.)
+void wrote(const at::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+void wrote_all(PyObject* tensors) {
+    for (Py_ssize_t x = 0; x < PyTuple_GET_SIZE(tensors); ++x) wrote(THPVariable_Unpack(PyTuple_GET_ITEM(tensors, x)));
+}
+
 PyObject* raise_status(int status) {
     const char* msg = h3mi_last_error();
     PyObject* e = PyObject_CallFunction(g_error, "is", status, msg ? msg : "");
@@ -298,6 +307,7 @@ PyObject* norm_any(PyObject*, PyObject* const* v, Py_ssize_t n) {
         }
     }
     if (rc) return raise_status(rc);
+    if (GATE) wrote(*t.x);
     return quant ? pair(h, qs) : THPVariable_Wrap(h);
     H3MI_END
 }
@@ -317,6 +327,7 @@ PyObject* gate_(PyObject*, PyObject* const* v, Py_ssize_t n) {
         rc = h3mi_gate_bf16(mu16(*t.x), u16(t.o), u16(t.g), t.ri(), t.S, t.N, t.R, a.stream());
     }
     if (rc) return raise_status(rc);
+    wrote(*t.x);
     Py_INCREF(v[0]);
     return v[0];
     H3MI_END
@@ -367,7 +378,10 @@ PyObject* rms_rope_(PyObject*, PyObject* const* v, Py_ssize_t n) {
         rc = h3mi_rms_rope_split_half_bf16(mu16(*q.t), mu16(*k.t), u16(tab), u16(qw), u16(kw), q.S, q.H, q.D, q.ld, k.ld, rot,
                                            static_cast<float>(eps), H3MI_RSQRT_HW, nullptr, a.stream());
     }
-    return rc ? raise_status(rc) : PyTuple_Pack(2, v[0], v[1]);
+    if (rc) return raise_status(rc);
+    wrote(*q.t);
+    wrote(*k.t);
+    return PyTuple_Pack(2, v[0], v[1]);
     H3MI_END
 }
 
@@ -478,6 +492,7 @@ PyObject* kv_write_(PyObject*, PyObject* const* v, Py_ssize_t n) {
                      : h3mi_kv_write_i8(u16(k.t), u16(x.t), k.rows, k.ld, k.bs, x.ld, x.bs, &kv.c, &kv.s, a.stream());
     }
     if (rc) return raise_status(rc);
+    wrote_all(v[0]);
     Py_INCREF(v[0]);
     return v[0];
     H3MI_END
@@ -597,6 +612,11 @@ struct Pool {
         tables = i32(t), lens = i32(l);
     }
     static int32_t* i32(const at::Tensor* t) { return static_cast<int32_t*>(t->data_ptr()); }
+    static void wrote_to(PyObject* pool, PyObject* to, PyObject* lo) {
+        wrote_all(pool);
+        wrote(THPVariable_Unpack(to));
+        wrote(THPVariable_Unpack(lo));
+    }
 };
 
 // (pool, tables, lens, rows, counts) -> (granted, positions, slots)
@@ -620,6 +640,7 @@ PyObject* kv_extend_(PyObject*, PyObject* const* v, Py_ssize_t n) {
                             Pool::i32(&positions), static_cast<int64_t*>(slots.data_ptr()), a.stream());
     }
     if (rc) return raise_status(rc);
+    p.wrote_to(v[0], v[1], v[2]);
     PyObject *x = THPVariable_Wrap(granted), *y = x ? THPVariable_Wrap(positions) : nullptr, *z = y ? THPVariable_Wrap(slots) : nullptr;
     PyObject* r = z ? PyTuple_Pack(3, x, y, z) : nullptr;
     Py_XDECREF(x);
@@ -644,6 +665,7 @@ PyObject* kv_release_(PyObject*, PyObject* const* v, Py_ssize_t n) {
         rc = h3mi_kv_release(&p.p, p.tables, p.lens, keep ? Kv::i32(keep) : nullptr, p.n, p.blocks, a.stream());
     }
     if (rc) return raise_status(rc);
+    p.wrote_to(v[0], v[1], v[2]);
     Py_INCREF(v[0]);
     return v[0];
     H3MI_END
@@ -703,7 +725,11 @@ PyObject* rotary(PyObject*, PyObject* const* v, Py_ssize_t n) {
                             2 * freqs->numel(), interleaved, inverse, static_cast<float>(amplitude), a.stream());
     }
     if (rc) return raise_status(rc);
-    if (in_place) return PyTuple_Pack(2, v[0], v[1]);
+    if (in_place) {
+        wrote(*q.t);
+        if (two) wrote(*k.t);
+        return PyTuple_Pack(2, v[0], v[1]);
+    }
     if (two) return pair(qo, ko);
     PyObject* x = THPVariable_Wrap(qo);
     PyObject* r = x ? PyTuple_Pack(2, x, Py_None) : nullptr;

@@ -159,6 +159,15 @@ def ptr(t):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
 
 
+def wrote(*tensors):
+    """The library has written into the caller's tensors (None entries are skipped): their versions move on, as after torch's
+    own in-place operations, so that autograd refuses what it saved of them and prequant.take sees the change.  (A tensor of
+    inference mode has no version.)"""
+    for t in tensors:
+        if t is not None and not t.is_inference():
+            torch.autograd.graph.increment_version(t)
+
+
 def stream_of(t):
     """The current torch stream on t's device, as a hipStream_t."""
     import torch

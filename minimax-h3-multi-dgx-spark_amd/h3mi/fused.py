@@ -16,7 +16,7 @@ import ctypes
 
 import torch
 
-from ._lib import ORDER_DEFAULT, RSQRT_HW, _fast, check, lib, ptr, same_gpu, stream_of
+from ._lib import ORDER_DEFAULT, RSQRT_HW, _fast, check, lib, ptr, same_gpu, stream_of, wrote
 
 ORDER_NAMES = {"default": 0, "ref": 1, "w64": 2}
 
@@ -60,6 +60,7 @@ def norm_mod_ex(x, w, eps, ridx, s1, sh, order=ORDER_DEFAULT, rsqrt_mode=RSQRT_H
     r = _table(s1, n, "s1")
     if _table(sh, n, "sh") != r:
         raise ValueError("s1 and sh must have the same number of rows")
+    given = h
     if h is None:
         h = torch.empty_like(x)
     var = rstd = None
@@ -70,6 +71,7 @@ def norm_mod_ex(x, w, eps, ridx, s1, sh, order=ORDER_DEFAULT, rsqrt_mode=RSQRT_H
     check(lib.h3mi_norm_mod_bf16_ex(ptr(x), ptr(w), ptr(ridx), ptr(s1), ptr(sh), ptr(h), s, n, r, float(eps),
                                     int(ORDER_NAMES.get(order, order)), int(rsqrt_mode), ptr(var), ptr(rstd),
                                     stream_of(x)))
+    wrote(given)
     return (h, var, rstd) if stats else h
 
 
@@ -82,6 +84,7 @@ def gate_norm_mod_ex(x, o, g, w, eps, ridx, s1, sh, order=ORDER_DEFAULT, rsqrt_m
     r = _table(s1, n, "s1")
     if _table(sh, n, "sh") != r or _table(g, n, "g") != r:
         raise ValueError("g, s1 and sh must have the same number of rows")
+    given = h
     if h is None:
         h = torch.empty_like(x)
     var = rstd = None
@@ -92,6 +95,7 @@ def gate_norm_mod_ex(x, o, g, w, eps, ridx, s1, sh, order=ORDER_DEFAULT, rsqrt_m
     check(lib.h3mi_gate_norm_mod_bf16_ex(ptr(x), ptr(o), ptr(g), ptr(w), ptr(ridx), ptr(s1), ptr(sh), ptr(h),
                                          s, n, r, float(eps), int(ORDER_NAMES.get(order, order)), int(rsqrt_mode),
                                          ptr(var), ptr(rstd), stream_of(x)))
+    wrote(x, given)
     return (h, var, rstd) if stats else h
 
 
@@ -133,6 +137,7 @@ def gate_norm_mod_(x, o, g, w, eps, ridx, s1, sh):
     same_gpu(x, o=o, g=g, w=w, ridx=ridx, s1=s1, sh=sh)
     check(lib.h3mi_gate_norm_mod_bf16(ptr(x), ptr(o), ptr(g), ptr(w), ptr(ridx), ptr(s1), ptr(sh), ptr(h),
                                       s, n, r, float(eps), stream_of(x)))
+    wrote(x)
     return h
 
 
@@ -147,6 +152,7 @@ def gate_(x, o, g, ridx):
     r = _table(g, n, "g")
     same_gpu(x, o=o, g=g, ridx=ridx)
     check(lib.h3mi_gate_bf16(ptr(x), ptr(o), ptr(g), ptr(ridx), s, n, r, stream_of(x)))
+    wrote(x)
     return x
 
 
@@ -208,4 +214,5 @@ def gate_norm_mod_q_(x, o, g, w, eps, ridx, s1, sh, want_h=False):
     same_gpu(x, o=o, g=g, w=w, ridx=ridx, s1=s1, sh=sh)
     check(lib.h3mi_gate_norm_mod_quant_i8(ptr(x), ptr(o), ptr(g), ptr(w), ptr(ridx), ptr(s1), ptr(sh), ptr(h), ptr(q),
                                           ptr(qs), s, n, r, float(eps), stream_of(x)))
+    wrote(x)
     return (h, q, qs) if want_h else (q, qs)

@@ -31,7 +31,7 @@ import re
 
 import torch
 
-from ._lib import H3miError, _fast, check, lib, ptr, same_gpu, stream_of
+from ._lib import H3miError, _fast, check, lib, ptr, same_gpu, stream_of, wrote
 
 log = logging.getLogger("h3mi")
 
@@ -178,6 +178,7 @@ def int8_mm_scaled(xq, w, xs, ws, out=None, bias=None):
         raise ValueError("ws must be contiguous float32 with N elements")
     if bias is not None and (bias.dtype != torch.bfloat16 or bias.numel() != N or not bias.is_contiguous()):
         raise ValueError("bias must be contiguous bfloat16 with N elements")
+    given = out
     if out is None:
         out = torch.empty((M, N), dtype=torch.bfloat16, device=xq.device)
     elif out.dtype != torch.bfloat16 or out.shape != (M, N) or out.stride(1) != 1:
@@ -187,6 +188,7 @@ def int8_mm_scaled(xq, w, xs, ws, out=None, bias=None):
     def launch():
         check(lib.h3mi_w8a8_gemm_bf16(ptr(xq), ptr(w), ptr(xs), ptr(ws), ptr(bias), ptr(out),
                                       M, N, K, xq.stride(0), w.stride(0), out.stride(0), stream_of(xq)))
+        wrote(given)
 
     if _autotune() and M > 0 and N > 0:
         key = (N, K, -(-M // 4096))
@@ -209,6 +211,7 @@ def int8_mm_scaled(xq, w, xs, ws, out=None, bias=None):
 def int8_mm_i32(xq, w, out=None):
     """The int32 accumulators sum_k xq[m,k]*w[n,k] of the same GEMM ([M,N] int32)."""
     M, N, K = _check_operands(xq, w)
+    given = out
     if out is None:
         out = torch.empty((M, N), dtype=torch.int32, device=xq.device)
     elif out.dtype != torch.int32 or out.shape != (M, N) or out.stride(1) != 1:
@@ -216,4 +219,5 @@ def int8_mm_i32(xq, w, out=None):
     same_gpu(xq, out=out)
     check(lib.h3mi_w8a8_gemm_i32(ptr(xq), ptr(w), ptr(out), M, N, K, xq.stride(0), w.stride(0),
                                  out.stride(0), stream_of(xq)))
+    wrote(given)
     return out

@@ -30,7 +30,7 @@ import typing
 import torch
 from torch.autograd import forward_ad
 
-from ._lib import KvCache4C, KvCacheC, KvSeqsC, _fast, check, lib, ptr, same_gpu, stream_of
+from ._lib import KvCache4C, KvCacheC, KvSeqsC, _fast, check, lib, ptr, same_gpu, stream_of, wrote
 
 KV_BLOCK = 64   # tokens of a block, and of a page; in 8 bits one scale per block and head
 KV_TILE = 128   # query rows that share a selection
@@ -171,6 +171,7 @@ def kv_write_(cache, k, v, tables, lens, counts=None):
     with torch.cuda.device(k.device):
         write = lib.h3mi_kv_write_mx4 if isinstance(cache, KVCache4) else lib.h3mi_kv_write_i8
         check(write(ptr(k), ptr(v), rows, ldk, bsk, ldv, bsv, ctypes.byref(c), ctypes.byref(s), stream_of(k)))
+    wrote(*cache)
     return cache
 
 

@@ -20,7 +20,7 @@ import typing
 
 import torch
 
-from ._lib import KvPoolC, _fast, check, lib, ptr, same_gpu, stream_of
+from ._lib import KvPoolC, _fast, check, lib, ptr, same_gpu, stream_of, wrote
 from .kvcache import _ints
 
 
@@ -72,6 +72,7 @@ def kv_extend_(pool, tables, lens, rows, counts=None):
     with torch.cuda.device(tables.device):
         check(lib.h3mi_kv_extend(ctypes.byref(p), ptr(tables), ptr(lens), ptr(counts), n, blocks, rows, ptr(granted), ptr(positions),
                                  ptr(slots), stream_of(tables)))
+    wrote(*pool, tables, lens)
     return granted, positions, slots
 
 
@@ -89,4 +90,5 @@ def kv_release_(pool, tables, lens, keep=None):
     same_gpu(tables, keep=keep)
     with torch.cuda.device(tables.device):
         check(lib.h3mi_kv_release(ctypes.byref(p), ptr(tables), ptr(lens), ptr(keep), n, blocks, stream_of(tables)))
+    wrote(*pool, tables, lens)
     return pool

@@ -7,7 +7,7 @@ for an all-zero row.
 """
 import torch
 
-from ._lib import _fast, check, lib, ptr, same_gpu, stream_of
+from ._lib import _fast, check, lib, ptr, same_gpu, stream_of, wrote
 
 
 def quantize_rowwise(x, xq=None, xs=None):
@@ -21,6 +21,7 @@ def quantize_rowwise(x, xq=None, xs=None):
     if x.stride(1) != 1:
         raise ValueError("x must have unit column stride")
     M, K = x.shape
+    given = xq, xs
     if xq is None:
         xq = torch.empty((M, K), dtype=torch.int8, device=x.device)
     if xs is None:
@@ -31,6 +32,7 @@ def quantize_rowwise(x, xq=None, xs=None):
         raise ValueError("xs must be contiguous float32 with M elements")
     same_gpu(x, xq=xq, xs=xs)
     check(lib.h3mi_quant_rowwise_i8(ptr(x), ptr(xq), ptr(xs), M, K, x.stride(0), stream_of(x)))
+    wrote(*given)
     return xq, xs
 
 
@@ -61,6 +63,7 @@ def quantize_rowwise_convrot(x, act=None, group_size=256, xq=None, xs=None):
     if a == 1 and kin % 2:
         raise ValueError("swiglu input needs an even number of columns")
     K = kin // 2 if a == 1 else kin
+    given = xq, xs
     if xq is None:
         xq = torch.empty((M, K), dtype=torch.int8, device=x.device)
     if xs is None:
@@ -71,4 +74,5 @@ def quantize_rowwise_convrot(x, act=None, group_size=256, xq=None, xs=None):
         raise ValueError("xs must be contiguous float32 with M elements")
     same_gpu(x, xq=xq, xs=xs)
     check(lib.h3mi_quant_convrot_i8(ptr(x), ptr(xq), ptr(xs), M, K, x.stride(0), group_size, a, stream_of(x)))
+    wrote(*given)
     return xq, xs

@@ -21,7 +21,7 @@ import math
 import torch
 from torch.autograd import forward_ad
 
-from ._lib import RSQRT_HW, RSQRT_RN, RopeRowsC, _fast, check, lib, ptr, same_gpu, stream_of
+from ._lib import RSQRT_HW, RSQRT_RN, RopeRowsC, _fast, check, lib, ptr, same_gpu, stream_of, wrote
 
 _MODES = {"hw": RSQRT_HW, "rn": RSQRT_RN}
 
@@ -71,6 +71,7 @@ def rms_rope_split_half_(q, k, rope_freqs, qw, kw, epsilon=1e-6, rot_dim=None, r
     check(lib.h3mi_rms_rope_split_half_bf16(ptr(q3), ptr(k3), ptr(tab) if tab is not None else None, ptr(qw), ptr(kw),
                                             S, H, D, ldq, ldk, rot_dim, float(epsilon), _MODES[rsqrt],
                                             ptr(rstd_out) if rstd_out is not None else None, stream_of(q3)))
+    wrote(q, k, rstd_out)
     return q, k
 
 
@@ -150,6 +151,8 @@ def _rotary(q, k, positions, freqs, interleaved, inverse, amplitude, in_place):
     with torch.cuda.device(positions.device):
         check(lib.h3mi_rope_bf16(ctypes.byref(sides[0]), None if k is None else ctypes.byref(sides[1]), ptr(positions), ptr(freqs), n, rows,
                                  dim, 2 * freqs.numel(), int(bool(interleaved)), int(bool(inverse)), float(amplitude), stream_of(positions)))
+    if in_place:
+        wrote(q, k)
     return tuple(outs)
 
 
