@@ -88,14 +88,15 @@ def rotary_frequencies(rot_dim, base=10000.0, scaling=None, factor=1.0, window=8
     scaling, for contexts of `factor` (>= 1) times the `window` tokens that the frequencies were made for:
       "linear"  positions count for 1 / factor: all frequencies are divided by it
       "ntk"     the base grows by factor ** (rot_dim / (rot_dim - 2)): the slowest pair is divided by factor, the fastest stays
-      "yarn"    pairs that turn less than once in the window are divided by factor, those that turn 32 times and more stay,
-                and those between go from one to the other with their number (rounded outward to whole ones); the amplitude
-                is 1 + 0.1 ln factor (Peng et al., 2023)"""
+      "yarn"    pairs that turn once in the window or less are divided by factor, those that turn 32 times and more stay; in between
+                the share that stays falls evenly with a pair's index, from the last whole index of 32 turns or more to the first
+                of one or less.  The amplitude is 1 + 0.1 ln factor.  (Amplitude and both bounds: Peng et al., 2023.  Their share
+                falls evenly with the number of turns; by the index is how checkpoints with such configurations are run.)"""
     rot_dim, base, factor = int(rot_dim), float(base), float(factor)
     if rot_dim < 2 or rot_dim % 2:
         raise ValueError("rot_dim must be even and at least 2")
-    if not (base > 1.0 and math.isfinite(base)) or not (factor >= 1.0 and math.isfinite(factor)) or not window > 0:
-        raise ValueError("base must be above 1, factor at least 1 and window above 0")
+    if not (base > 1.0 and math.isfinite(base)) or not (factor >= 1.0 and math.isfinite(factor)) or not 0 < window < math.inf:
+        raise ValueError("base must be above 1, factor at least 1 and window above 0, all of them finite")
     if scaling not in (None, "linear", "ntk", "yarn"):
         raise ValueError("scaling must be None, 'linear', 'ntk' or 'yarn'")
     if scaling == "ntk" and rot_dim > 2:
@@ -107,8 +108,8 @@ def rotary_frequencies(rot_dim, base=10000.0, scaling=None, factor=1.0, window=8
     elif scaling == "yarn" and factor > 1.0:
         def at(turns):  # the pair, as a real number, that turns so often in the window
             return rot_dim * math.log(window / (2 * math.pi * turns)) / (2 * math.log(base))
-        lo, hi = max(math.floor(at(32.0)), 0), min(math.ceil(at(1.0)), rot_dim - 1)
-        keep = 1 - ((i - lo) / max(hi - lo, 0.001)).clamp(0, 1)
+        lo, hi = math.floor(at(32.0)), math.ceil(at(1.0))  # lo < hi: a pair of 32 turns is before one of a single turn
+        keep = 1 - ((i - lo) / (hi - lo)).clamp(0, 1)
         f, amplitude = f * (keep + (1 - keep) / factor), 1 + 0.1 * math.log(factor)
     return f.to(device), amplitude
 
