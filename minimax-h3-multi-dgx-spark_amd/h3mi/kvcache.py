@@ -74,6 +74,13 @@ def kv_cache(pages, heads, dim, device="cuda", bits=8):
 # other form.
 
 
+def _named(c):
+    """A cache's tensors as a plain tuple are taken for the cache that they are the tensors of, as the native calls do."""
+    if type(c) is tuple and len(c) in (4, 5):
+        return (KVCache4 if len(c) == 4 else KVCache)(*c)
+    return c
+
+
 def _cache4(c):
     k = c.k
     if k.dim() != 4 or k.shape[2] != KV_BLOCK or k.dtype != torch.uint8:
@@ -162,6 +169,7 @@ def kv_write_(cache, k, v, tables, lens, counts=None):
     if done is not None:
         return done
     _no_grad(k, v)
+    given, cache = cache, _named(cache)
     c = _cache(cache)
     s = _seqs(cache, tables, lens, counts)
     rows, ldk, bsk = _rows(k, cache, s.n, "k", c.heads)
@@ -172,7 +180,7 @@ def kv_write_(cache, k, v, tables, lens, counts=None):
         write = lib.h3mi_kv_write_mx4 if isinstance(cache, KVCache4) else lib.h3mi_kv_write_i8
         check(write(ptr(k), ptr(v), rows, ldk, bsk, ldv, bsv, ctypes.byref(c), ctypes.byref(s), stream_of(k)))
     wrote(*cache)
-    return cache
+    return given
 
 
 def kv_read(cache, tables, lens, length, starts=None):
@@ -180,6 +188,7 @@ def kv_read(cache, tables, lens, length, starts=None):
     got = _fast.kv_read(cache, tables, lens, length, starts)
     if got is not None:
         return got
+    cache = _named(cache)
     c = _cache(cache)
     s = _seqs(cache, tables, lens, None)
     _ints(starts, (s.n,), "starts")
@@ -207,6 +216,7 @@ def kv_select(q, cache, tables, lens, top, causal=False, counts=None):
     if out is not None:
         return out
     _no_grad(q)
+    cache = _named(cache)
     if isinstance(cache, KVCache4):
         raise ValueError("kv_select takes an 8-bit cache: one of 4 bits holds no sums of its blocks' keys")
     c = _cache(cache)
@@ -232,6 +242,7 @@ def kv_attention(q, cache, tables, lens, causal=False, counts=None, scale=None, 
     if out is not None:
         return out
     _no_grad(q)
+    cache = _named(cache)
     c = _cache(cache)
     s = _seqs(cache, tables, lens, counts)
     rows, ld, bs = _rows(q, cache, s.n, "q")

@@ -39,6 +39,8 @@ def kv_pool(pages, device="cuda"):
 
 
 def _pool(pool, tables, lens):
+    if type(pool) is tuple and len(pool) == 2:  # as the native calls do
+        pool = KVPool(*pool)
     if tables.dim() != 2:
         raise ValueError("tables must be [n, blocks]")
     n, blocks = tables.shape
