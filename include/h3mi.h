@@ -385,7 +385,8 @@ int h3mi_kv_extend(const h3mi_kv_pool* pool, int32_t* tables, int32_t* lens, con
 /* Drops tokens: sequence i keeps its first keep[i] (NULL: none; taken as 0 .. lens[i]).
  * The pages of blocks wholly behind go back onto the stack, in the order of sequences,
  * then blocks; their table entries become -1 and lens[i] becomes what was kept.  Entries
- * that are no page of the pool are passed over, and pages past a full stack dropped. */
+ * that are no page of the pool are passed over, and pages past a full stack dropped.  A
+ * page that two released tables hold goes back twice. */
 int h3mi_kv_release(const h3mi_kv_pool* pool, int32_t* tables, int32_t* lens, const int32_t* keep, int64_t n,
                     int64_t blocks, void* stream);
 

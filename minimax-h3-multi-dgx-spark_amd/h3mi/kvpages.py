@@ -82,8 +82,9 @@ def kv_release_(pool, tables, lens, keep=None):
     """Drops all but the first keep[i] (int32 [n]; default none) tokens of each sequence; returns the pool.
 
     The pages of blocks wholly behind go back to the pool, their entries in tables become -1 and lens what is kept (a
-    sequence shorter than keep[i] stays as it is).  A page that two sequences' tables share would go back twice: such
-    tables are not released."""
+    sequence shorter than keep[i] stays as it is).  A page that two released tables hold goes back twice, and later to two
+    sequences: of sequences that share pages one is their owner, released last, and the others' entries for them are set to
+    -1 before, which a release passes over."""
     done = _fast.kv_release_(pool, tables, lens, keep)
     if done is not None:
         return done

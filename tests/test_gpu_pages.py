@@ -134,6 +134,35 @@ def test_many_pages_come_back():
     _release(ref, *state, rng.integers(0, 30000, 40))
 
 
+def test_shared_prefix():
+    """Whole blocks that three sequences hold: the owner's pages stay out of the pool until it is released, and come back once."""
+    import h3mi
+    pool = h3mi.kv_pool(12)
+    tables, lens = torch.full((4, 4), -1, dtype=torch.int32, device=DEV), _i32([0, 0, 0, 0])
+    h3mi.kv_extend_(pool, tables, lens, 150, _i32([150, 0, 0, 0]))
+    shared = tables[0, :2].clone()
+    for i in (1, 2):
+        tables[i, :2] = shared
+        lens[i] = 128
+    granted, positions, slots = h3mi.kv_extend_(pool, tables, lens, 70, _i32([1, 22, 70, 0]))
+    assert granted.tolist() == [1, 22, 70, 0] and positions[:, 0].tolist() == [150, 128, 128, -1]
+    held = [set(row) - {-1} for row in tables.tolist()]
+    assert held[1] & held[0] == held[2] & held[0] == set(shared.tolist()) and slots[:3, 0].unique().numel() == 3
+
+    def free():
+        return pool.free[:int(pool.count)].tolist()
+
+    for i in (1, 2):  # one at a time: the others' tables stay out of the call
+        tables[i, :2] = -1
+        h3mi.kv_release_(pool, tables[i:i + 1], lens[i:i + 1])
+        assert not held[0] & set(free()) and (tables[i] == -1).all()
+        # what is handed out meanwhile is none of the owner's
+        h3mi.kv_extend_(pool, tables, lens, 200, _i32([0, 0, 0, 200 if i == 1 else 0]))
+        assert not held[0] & set(tables[3].tolist())
+    h3mi.kv_release_(pool, tables, lens)
+    assert sorted(free()) == list(range(12)) and lens.tolist() == [0] * 4
+
+
 @pytest.mark.parametrize("n,rows", [(5, 3), (300, 40)])
 def test_captured(n, rows):
     """A captured step, replayed with other counts, beside the CPU's."""
