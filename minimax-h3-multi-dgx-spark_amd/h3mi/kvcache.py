@@ -161,9 +161,10 @@ def kv_write_(cache, k, v, tables, lens, counts=None):
     an infinity makes its block read back as NaN until the block's first token is written again.  The pages that a call
     writes have to be distinct.
 
-    4 bits: every 32 elements of a token have a power of two of their own, the least with which they fit, and are off by
-    half the distance of the values on either side, a fifth of the largest of them at most: nothing written before
-    changes.  A NaN or an infinity makes its 32 elements read back as NaN.  The tokens that a call writes
+    4 bits: every 32 elements of a token have a power of two of their own, the least of 2^-125 to 2^125 with which they fit, and
+    are off by half the distance of the values on either side: a fifth of the largest of them at most, where that is above
+    3.5 2^-125.  (Below, the power stays, 2^-127 and less become 0; above 7 2^125, the last quarter of bf16's range, values become 6 2^125, up to a
+    quarter less.)  Nothing written before changes.  A NaN or an infinity makes its 32 elements read back as NaN.  The tokens that a call writes
     have to be distinct."""
     done = _fast.kv_write_(cache, k, v, tables, lens, counts)
     if done is not None:

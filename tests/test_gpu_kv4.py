@@ -96,6 +96,28 @@ def test_every_bf16_beside_every_largest():
         assert (np.abs(got[ok] - src[ok]) <= np.where(a <= 7, most, np.abs(src[ok]) / 4)).all()
 
 
+def test_how_far_a_value_is_off():
+    """A fifth of its group's largest, from 3.5 2^-125 up to 7 2^125, and what it is outside."""
+    h = _h()
+    rng = np.random.default_rng(17)
+    tops = _round(np.exp2(rng.uniform(-133, 128, 4000)))
+    edge = _round(np.array([a * 2.0 ** e for e in (-133, -127, -126, -125, -124, 0, 124, 125) for a in (1, 1.25, 1.75, 3.5, 3.515625, 5, 7)]))
+    tops = np.concatenate([tops[np.isfinite(tops) & (tops > 0)], edge])
+    x = _round(tops[:, None] * rng.uniform(-1, 1, (len(tops), 32)))
+    x[np.arange(len(tops)), rng.integers(0, 32, len(tops))] = tops
+    x = np.concatenate([x, np.zeros((-len(x) % 4, 32))]).reshape(1, -1, 1, 128)
+    n = x.shape[1]
+    tables = np.arange(-(-n // 64), dtype=np.int32)[None]
+    cache = h.kv_cache(tables.size, 1, 128, bits=4)
+    h.kv_write_(cache, _bf(x), _bf(x), _i32(tables), _i32([n]))
+    src = _bf(x).double().cpu().numpy().reshape(-1, 32)
+    for got in h.kv_read(cache, _i32(tables), _i32([n]), n):
+        off = np.abs(got.double().cpu().numpy().reshape(-1, 32) - src)
+        top = np.abs(src).max(1, keepdims=True)
+        most = np.where(top <= 3.5 * 2.0 ** -125, np.where(np.abs(src) <= 2.0 ** -127, np.abs(src), 2.0 ** -126), np.where(top <= 7 * 2.0 ** 125, top / 5, top / 4))
+        assert (off <= most).all()
+
+
 def test_write_of_views_and_without_counts():
     h = _h()
     rng = np.random.default_rng(5)
