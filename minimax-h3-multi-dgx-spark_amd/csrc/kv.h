@@ -116,7 +116,6 @@ typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void store_past(void* p, uint4 v) {
     __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v), static_cast<u32x4*>(p));
 }
-__device__ __forceinline__ void store_past(void* p, uint32_t v) { __builtin_nontemporal_store(v, static_cast<uint32_t*>(p)); }
 __device__ __forceinline__ void store_past(void* p, uint2 v) {
     __builtin_nontemporal_store(__builtin_bit_cast(u32x2, v), static_cast<u32x2*>(p));
 }
