@@ -173,6 +173,40 @@ def test_inverse_is_the_gradient():
         assert ((d - want).abs() <= slack).all()
 
 
+@pytest.mark.parametrize("dim,rot", [(128, 128), (128, 64), (64, 60), (256, 126)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_inverse_is_the_transpose_pair_by_pair(dim, rot, interleaved):
+    """<g, R x> = <R' g, x> over every pair of elements, within the roundings of its four results; a rotation the wrong way round,
+    or none, passes it in few pairs."""
+    h = _h()
+    rng = np.random.default_rng(dim + rot)
+    freqs, amplitude = h.rotary_frequencies(rot, scaling="yarn", factor=16.0)
+    positions = torch.from_numpy(rng.integers(1, 99999, (2, 50))).to(torch.int32).to(DEV)
+    x, g = (_bf(rng, 2, 50, 3, dim).to(DEV) for _ in range(2))
+
+    def pairs(t):
+        t = t[..., :rot].double()
+        return t.unflatten(-1, (-1, 2)) if interleaved else t.unflatten(-1, (2, -1)).transpose(-1, -2)
+
+    y = pairs(h.rotary(x, None, positions, freqs, interleaved, False, amplitude)[0])
+    u, w = pairs(x), pairs(g)
+
+    def within(b):
+        b = pairs(b)
+        # each result is off by half a step at most, 2^-8 of it, and by what 32 bits add, less than a hundredth of that beside
+        # the larger of the pair's elements
+        most = 2.0 ** -8 * ((w * y).abs() + (b * u).abs()).sum(-1) + 2.0 ** -15 * amplitude * w.abs().sum(-1) * u.abs().sum(-1)
+        return ((w * y).sum(-1) - (b * u).sum(-1)).abs() <= most
+
+    turned = h.rotary(g, None, positions, freqs, interleaved, True, amplitude)[0]
+    assert within(turned).all()
+    # the slow pairs of a short turn hardly move: the first half of them
+    for wrong in (h.rotary(g, None, positions, freqs, interleaved, False, amplitude)[0], h.rotary(g, None, torch.zeros_like(positions), freqs, interleaved, True, amplitude)[0]):
+        assert within(wrong)[..., :rot // 4].double().mean() < 0.1
+    if rot < dim:
+        assert torch.equal(turned[..., rot:], g[..., rot:])
+
+
 def test_special_values_stay_in_their_pairs():
     h = _h()
     rng = np.random.default_rng(8)
