@@ -346,7 +346,8 @@ int h3mi_kv_write_mx4(const uint16_t* k, const uint16_t* v, int64_t rows, int64_
 int h3mi_kv_read_mx4_bf16(uint16_t* k, uint16_t* v, const int32_t* starts, int64_t length,
                           const h3mi_kv_cache4* cache, const h3mi_kv_seqs* seqs, void* stream);
 
-/* As h3mi_kv_attention_bf16, with a workspace of h3mi_kv_attention_mx4_workspace bytes.
+/* As h3mi_kv_attention_bf16, with a workspace of h3mi_kv_attention_mx4_workspace bytes, 256 MiB
+ * at most (hundreds of rows of several sequences over long tables come near that).
  * Keys and values are exact in the products, whose sums are formed before the scale: queries
  * and keys whose product passes 2^127 have no finite score, and as a probability's weight may
  * be 2^8, values of 2^119 over the number of tokens and more may have no finite sum.  A value

@@ -8,8 +8,12 @@
 // a term of the exponent, p v_scale = 2^(x - m + log2 v_scale), which costs nothing per
 // score; l takes the sum times 1 / v_scale.  Scores and sums are fp32; a probability is
 // rounded once, to the bf16 that the second product multiplies.  That is off by 2^-8 of it at
-// most, as the output's own rounding is: outputs are 1.8e-3 off (rms) where probabilities in
-// 32 bits leave 1.7e-3, and a second MFMA for the remainder would add half of all products.
+// most, as the output's own rounding is: outputs are 1.8e-3 off (rms) where a few tokens outweigh
+// the rest, 2.4e-3 where thousands weigh alike, and 1.7e-3 is what the output's rounding leaves
+// with probabilities in 32 bits.  A second MFMA for the remainder would add half of all products
+// of a tile.  Of few queries, which memory bounds, it costs (4 bits, 16 queries) 2% at 128 and 256
+// elements and 8 to 10% at 64, with 32 queries of 128 21% (8 x 20 rows 61.6 us, 74.5 so); left
+// out there too, so that a row's result is as good whatever rows it comes with.
 //
 // Both products are formed transposed, S^T = K Q^T and O^T = V^T P^T: a query is then a
 // column, whose scores lie in the registers of two (four) lanes, so that the maximum needs
@@ -330,8 +334,8 @@ struct Items {
     __device__ __forceinline__ int row_of(int x) const { return pack == 1 ? x : static_cast<int>(__umulhi(static_cast<uint32_t>(x), per_pack)); }
     // Of causal items those of a head's last rows, the longest, come first: first of all in a flat launch.  MIX: where items are
     // dealt out in runs those of a head's sequences are consecutive, not those of a sequence's heads, so that the XCDs' shares are
-    // alike however uneven the sequences are (8 of 1176 rows and up to 10228 tokens 1800 -> 1086 us, 16 of 2560 rows over
-    // themselves of 256 elements 2122 -> 1514).
+    // alike however uneven the sequences are (over 4 bits 8 of 1176 rows and up to 10228 tokens 1800 -> 1086 us, 16 of 2560 rows over
+    // themselves of 256 elements 2122 -> 1514; over 8 bits it was not tried).
     template <bool MIX>
     __device__ __forceinline__ void place(int item, int& seq, int& head, int& tile) const {
         const int all = count / tiles, nh = flat ? item % all : item / tiles;
@@ -741,7 +745,8 @@ __device__ __forceinline__ void wave_order() {
 // of each lane's.  Each load's lanes then lie on whole cache lines, which no other load touches (but keys of 256 elements):
 // where two did, the second waited in the L1 for the first's line (43% of cycles).  Scales are loaded once a wave, in order, and
 // go through LDS to the lanes that want them.  A query of 56 heads over 19721 tokens (150 MB) 33.2 us with neighbouring tokens
-// in a lane, 30.4 so, the join's 4.6 among them; 16 sequences of up to 32768 tokens of 8 heads 58.9 and 53.2, 5.7 TB/s.
+// in a lane, 30.4 so, the join's 4.6 among them; 16 sequences of up to 32768 tokens of 8 heads, one draw of lengths, 58.9 and
+// 53.2 (eight draws, 244593 to 380465 tokens, 266 to 414 MB: 53 to 73 us, 5.0 to 5.7 TB/s).
 template <int D>
 struct FourFew {
     static constexpr int kRun = D >= 128 ? 32 : 16;       // neighbouring elements of a key
@@ -1449,7 +1454,10 @@ struct Plan {
 // the lists are taken to be six tenths of the longest, the pieces to be dealt out evenly, and the last one to come on top.  The
 // partial sums are at most what the memory-side cache holds.  Against as many pieces as fill one round: 1000 rows of 20 heads of
 // 256 over 4000 tokens 182 -> 141 us, 3 sequences of 300 rows and up to 30000 tokens of 24 heads of 64 214 -> 145, of 150 rows and
-// up to 9000 of 56 of 128 231 -> 165.
+// up to 9000 of 56 of 128 231 -> 165.  Sequences that are equally long, and lists, are taken for uneven too, and get more pieces
+// than they need (2 of 19721 tokens, 56 heads of 128: 450 rows in 8 pieces 673 us and 239 MB of partial sums, unsplit 576; 800 rows
+// in 10 970, in 3 962, unsplit 1054; 2401 rows in 13 2543, in 4 2535, unsplit 2673; 600 rows over lists of 100 blocks in 10 256,
+// in 4 259, unsplit 345).
 int64_t four_splits(int64_t n, int64_t rest, int64_t slots, int64_t longest, int64_t dim, int64_t item_bytes) {
     const double block = dim == 64 ? 1.0 : dim == 128 ? 1.8 : 2.8;
     int64_t best = 1;

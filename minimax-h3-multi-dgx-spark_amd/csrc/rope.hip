@@ -260,7 +260,8 @@ extern "C" int h3mi_rope_bf16(const h3mi_rope_rows* q, const h3mi_rope_rows* k, 
 
     // The widest accesses that the turned part fills, or each of its halves (2261 rows in place of 80 heads of 256, 128 of them
     // turned: 20 us in 8; 120, in 4: 23; 124: in pairs, by 4, 28, else by 2 27; 126: pairs by 2 37, else singly 39, which is
-    // what all but the first took singly, 40 to 45).
+    // what all but the first took singly, 40 to 45.  Into new tensors, whose copied elements go by the same width, 128 takes 38 to
+    // 43, 120 43 to 50, 124 62, 126 85 to 93; at a copy's rate all would take 38).
     const int64_t run = interleaved ? rot : rot / 2, V = run % 8 == 0 ? 8 : run % 4 == 0 ? 4 : run % 2 == 0 ? 2 : 1;
     RopeCall c = {};
     const auto side = [](const h3mi_rope_rows& x) { return RopeRows{x.in, x.out, static_cast<int>(x.heads), x.ld_in, x.bs_in, x.ld_out, x.bs_out}; };
